@@ -326,6 +326,104 @@ int moe355_merge_host_f32(const float* acc, const float* host_src, size_t n, int
  */
 int moe355_h2d_async(void* dst, const void* src, size_t bytes, void* stream);
 
+/*
+ * Rows in 8 bits, weights in 4 bits. Both hold one power-of-two scale per 32
+ * consecutive values of a row, a byte b that stands for 2^(b - 127).
+ *   rows     e4m3 codes [T, Hp] and scales [T, Hp/32], Hp = H rounded up to 128; the
+ *            scale is the smallest that brings the block's largest finite magnitude
+ *            to at most 448, a block of zeros has scale 0, infinities and NaN become
+ *            NaN codes, columns H.. are zeros
+ *   weights  e2m1 codes, two per byte, the even column in the low half; a scale of
+ *            255 stands for NaN; laid out once by moe355_mx_pack
+ * The reference has no such formats (its quantised experts are int8 on the host,
+ * reframework/moe/fused.py:140-197).
+ */
+
+/* dtype of moe355_mx_pack's source: codes and scales instead of weights. */
+#define MOE355_MX_CODES (-1)
+
+/* Scores of the routing by groups, and how a group is scored: by its best expert,
+ * or by the sum of its best two. */
+#define MOE355_SCORE_SOFTMAX 0
+#define MOE355_SCORE_SIGMOID 1
+#define MOE355_GROUP_MAX 0
+#define MOE355_GROUP_TOP2 1
+#define MOE355_MAX_GROUPS 64
+#define MOE355_MAX_GROUPED_TOPK 64
+
+/* Codes and scales (above) of x [T,H]; H a multiple of 32. */
+int moe355_mx_quantize(const void* x, int T, int H, int dtype, void* codes, void* scales,
+                       void* stream);
+
+/*
+ * moe355_add_rmsnorm that also writes the normed rows as codes and scales (bit for
+ * bit moe355_mx_quantize of normed_out); H a multiple of 32. Extends
+ * RMSNorm.forward_add_residual (reframework/layers/norm.py:27-53), which knows
+ * no 8-bit rows.
+ */
+int moe355_add_rmsnorm_mxfp8(const void* x, const void* residual, void* residual_out,
+                             const void* weight, const void* bias, int weight_dtype, float eps,
+                             int T, int H, int dtype, void* normed_out, void* codes, void* scales,
+                             void* stream);
+
+/*
+ * Routing by groups on fp32 logits [T,E] (torch_fused_topk,
+ * reframework/moe/fused.py:32-46, has softmax and no groups):
+ *   s = softmax(logits) or sigmoid(logits); c = s + bias (bias may be NULL);
+ *   the num_groups consecutive groups of E / num_groups experts are scored by
+ *   group_score of c, the topk_groups best are kept, and of their experts the K of
+ *   largest c are chosen, descending;
+ *   w = s of the chosen, divided by their sum + 1e-20 when renormalize, times scale.
+ * The ids are those of exact arithmetic on the given logits; ties go to the lower
+ * group and expert, a NaN choice ranks last. topk_w [T,out_ld] fp32, topk_ids
+ * [T,out_ld] int32 or int64; columns K.. are left as they are.
+ */
+int moe355_grouped_topk(const float* logits, const float* bias, int T, int E, int K, int scoring,
+                        int num_groups, int topk_groups, int group_score, int renormalize,
+                        float scale, float* topk_w, void* topk_ids, int ids_int64, int out_ld,
+                        void* stream);
+
+/* logits_out [T,E] fp32 = x . gate^T summed in fp32, rounded to dtype if
+ * round_logits: the F.linear of FusedMoE.route (reframework/moe/moe_layer.py:324)
+ * for moe355_grouped_topk to select from. */
+int moe355_router_logits(const void* x, const void* gate, int T, int H, int E, int dtype,
+                         int round_logits, float* logits_out, void* stream);
+
+/* Bytes of the codes and scales of one laid-out 4-bit matrix [rows, cols]; gate_up:
+ * rows 0 .. rows/2 - 1 are gate rows, the others up rows (a w1). rows (each half) and
+ * cols multiples of 32. */
+int moe355_mx_matrix_bytes(int rows, int cols, int gate_up, size_t* codes, size_t* scales);
+
+/*
+ * Lays one matrix out for moe355_mx_fused_experts: from codes [rows, cols/2] and
+ * scales [rows, cols/32] (dtype MOE355_MX_CODES), or from weights [rows, cols], each
+ * block rounded with the smallest scale that keeps it within 6 (a block with an
+ * infinity or NaN becomes NaN; src_scales is unused).
+ */
+int moe355_mx_pack(const void* src, const void* src_scales, int rows, int cols, int gate_up,
+                   int dtype, void* codes, void* scales, void* stream);
+
+/* Workspace of a moe355_mx_fused_experts call. */
+int moe355_mx_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes);
+
+/*
+ * moe355_fused_experts on 4-bit weights and 8-bit rows (the products of
+ * fused_experts, reframework/moe/fused.py:49-87):
+ *   x in 8 bits (quantised here when x_scales is NULL: x is then [T,H] of dtype;
+ *   else x holds codes [T,Hp]), g, u = x . w1[e]^T, h = act(g) * u in 8 bits,
+ *   y = h . w2[e]^T, out[t] = sum_k topk_w[t,k] * y.
+ * w1, w1_scales, w2, w2_scales: the laid-out matrices of the E experts one after the
+ * other. H and I multiples of 32. Products are summed in fp32; for dtype bf16 by the
+ * scaled MFMA, which keeps about 14 bits of a product below the largest one it
+ * adds in a step of 128 columns, for the others exactly. Slots whose id lies outside
+ * [0,E) or whose weight is 0 add nothing. out as in moe355_combine.
+ */
+int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
+                            const void* w1_scales, const void* w2, const void* w2_scales,
+                            const float* topk_w, const void* topk_ids, int ids_int64, int T, int H,
+                            int I, int E, int K, int dtype, int act, void* out, int accumulate_f32,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

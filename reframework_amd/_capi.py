@@ -26,6 +26,9 @@ HEADER_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__fil
 
 F32, BF16, F16 = 0, 1, 2
 ACT_CODES = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+SCORE_CODES = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORE_CODES = {"max": 0, "top2": 1}
+MX_CODES = -1
 PATH_MFMA_TILED, PATH_MFMA_SKINNY, PATH_SIMT, PATH_MFMA_TILED128 = 0, 1, 2, 4
 MAX_EXPERTS = 256
 STATIC_SCRATCH_BYTES = 64 << 20
@@ -98,6 +101,17 @@ _SIGNATURES: Dict[str, Tuple[object, List[object]]] = {
     "moe355_copy_to_host": (_I, [_P, _P, _Z, _P]),
     "moe355_copy_to_host_multi": (_I, [_P, _I, _P, _P, _P, _P]),
     "moe355_merge_host_f32": (_I, [_P, _P, _Z, _I, _P, _P]),
+    "moe355_mx_quantize": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "moe355_add_rmsnorm_mxfp8": (_I, [_P, _P, _P, _P, _P, _I, ctypes.c_float, _I, _I, _I, _P, _P,
+                                      _P, _P]),
+    "moe355_grouped_topk": (_I, [_P, _P, _I, _I, _I, _I, _I, _I, _I, _I, ctypes.c_float, _P, _P,
+                                 _I, _I, _P]),
+    "moe355_router_logits": (_I, [_P, _P, _I, _I, _I, _I, _I, _P, _P]),
+    "moe355_mx_matrix_bytes": (_I, [_I, _I, _I, ctypes.POINTER(_Z), ctypes.POINTER(_Z)]),
+    "moe355_mx_pack": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
+    "moe355_mx_workspace_bytes": (_I, [_I, _I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
+    "moe355_mx_fused_experts": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
+                                     _I, _P, _I, _P, _Z, _P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -406,6 +420,108 @@ def fused_experts_static(x: torch.Tensor, w1_ptrs: Sequence[int], w2_ptrs: Seque
     _check("moe355_fused_experts_static", lib().moe355_fused_experts_static(
         _ptr(x), t1, t2, _ptr(topk_w), _ptr(topk_ids), int(topk_ids.dtype == torch.int64), mp,
         mlen, T, H, I, E, K, dtype_code(x.dtype), act, _ptr(out), int(accumulate_f32), s))
+
+
+# Entry points of the 8-bit and 4-bit formats and of the routing by groups. Each runs
+# with its tensors' device current: a launch goes to the current device.
+def _call(device: torch.device, name: str, *args) -> None:
+    fn = getattr(lib(), name)
+    if device.index is None or device.index == torch.cuda.current_device():
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args)
+    _check(name, rc)
+
+
+def mx_quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                stream: Optional[int] = None) -> None:
+    T, H = x.shape
+    s = stream if stream is not None else stream_handle(x.device)
+    _call(x.device, "moe355_mx_quantize", _ptr(x), T, H, dtype_code(x.dtype), _ptr(codes),
+          _ptr(scales), s)
+
+
+def add_rmsnorm_mxfp8(x: torch.Tensor, residual: Optional[torch.Tensor],
+                      residual_out: Optional[torch.Tensor], weight: torch.Tensor,
+                      bias: Optional[torch.Tensor], eps: float, normed_out: torch.Tensor,
+                      codes: torch.Tensor, scales: torch.Tensor,
+                      stream: Optional[int] = None) -> None:
+    T, H = x.shape
+    s = stream if stream is not None else stream_handle(x.device)
+    _call(x.device, "moe355_add_rmsnorm_mxfp8", _ptr(x), _ptr(residual), _ptr(residual_out),
+          _ptr(weight), _ptr(bias), dtype_code(weight.dtype), float(eps), T, H,
+          dtype_code(x.dtype), _ptr(normed_out), _ptr(codes), _ptr(scales), s)
+
+
+def grouped_topk(logits: torch.Tensor, bias: Optional[torch.Tensor], K: int, scoring: int,
+                 num_groups: int, topk_groups: int, group_score: int, renormalize: bool,
+                 scale: float, topk_w: torch.Tensor, topk_ids: torch.Tensor,
+                 stream: Optional[int] = None) -> None:
+    """topk_w / topk_ids [T, ld] with ld >= K; columns K.. are left as they are."""
+    T, E = logits.shape
+    s = stream if stream is not None else stream_handle(logits.device)
+    _call(logits.device, "moe355_grouped_topk", _ptr(logits), _ptr(bias), T, E, K, scoring,
+          num_groups, topk_groups, group_score, int(renormalize), float(scale), _ptr(topk_w),
+          _ptr(topk_ids), int(topk_ids.dtype == torch.int64), topk_w.shape[1], s)
+
+
+def router_logits(x: torch.Tensor, gate: torch.Tensor, round_logits: bool,
+                  logits_out: torch.Tensor, stream: Optional[int] = None) -> None:
+    T, H = x.shape
+    s = stream if stream is not None else stream_handle(x.device)
+    _call(x.device, "moe355_router_logits", _ptr(x), _ptr(gate), T, H, gate.shape[0],
+          dtype_code(x.dtype), int(round_logits), _ptr(logits_out), s)
+
+
+def mx_matrix_bytes(rows: int, cols: int, gate_up: bool) -> Tuple[int, int]:
+    codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
+    _check("moe355_mx_matrix_bytes", lib().moe355_mx_matrix_bytes(
+        rows, cols, int(gate_up), ctypes.byref(codes), ctypes.byref(scales)))
+    return codes.value, scales.value
+
+
+def mx_pack(src: torch.Tensor, src_scales: Optional[torch.Tensor], rows: int, cols: int,
+            gate_up: bool, codes: torch.Tensor, scales: torch.Tensor,
+            stream: Optional[int] = None) -> None:
+    """One expert's matrix; ``src_scales`` given: ``src`` holds codes."""
+    s = stream if stream is not None else stream_handle(src.device)
+    dtype = MX_CODES if src_scales is not None else dtype_code(src.dtype)
+    _call(src.device, "moe355_mx_pack", _ptr(src), _ptr(src_scales), rows, cols, int(gate_up),
+          dtype, _ptr(codes), _ptr(scales), s)
+
+
+_MX_WORKSPACES: "OrderedDict[Tuple[int, ...], int]" = OrderedDict()
+
+
+def mx_workspace_bytes(T: int, H: int, I: int, E: int, K: int, dtype: int,
+                       device: torch.device) -> int:
+    """Workspace of an mx_fused_experts call. It depends on the sizes and the device's
+    CU count, so it is cached."""
+    key = (T, H, I, E, K, dtype, device.index)
+    n = _MX_WORKSPACES.get(key)
+    if n is None:
+        v = ctypes.c_size_t()
+        _call(device, "moe355_mx_workspace_bytes", T, H, I, E, K, dtype, ctypes.byref(v))
+        n = int(v.value)
+        with _lock:
+            _MX_WORKSPACES[key] = n
+            if len(_MX_WORKSPACES) > 1024:
+                _MX_WORKSPACES.popitem(last=False)
+    return n
+
+
+def mx_fused_experts(x: torch.Tensor, x_scales: Optional[torch.Tensor], H: int, I: int, E: int,
+                     w1: torch.Tensor, w1_scales: torch.Tensor, w2: torch.Tensor,
+                     w2_scales: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor,
+                     dtype: int, act: int, out: torch.Tensor, accumulate_f32: bool,
+                     workspace: torch.Tensor, stream: Optional[int] = None) -> None:
+    T, K = topk_ids.shape
+    s = stream if stream is not None else stream_handle(x.device)
+    _call(x.device, "moe355_mx_fused_experts", _ptr(x), _ptr(x_scales), _ptr(w1), _ptr(w1_scales),
+          _ptr(w2), _ptr(w2_scales), _ptr(topk_w), _ptr(topk_ids),
+          int(topk_ids.dtype == torch.int64), T, H, I, E, K, dtype, act, _ptr(out),
+          int(accumulate_f32), _ptr(workspace), workspace.numel(), s)
 
 
 def cast_f32(src: torch.Tensor, dst: torch.Tensor, stream: Optional[int] = None) -> None:

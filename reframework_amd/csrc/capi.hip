@@ -9,6 +9,7 @@
 
 #include <mutex>
 
+#include "capi_detail.h"
 #include "common.h"
 
 using namespace moe355;
@@ -18,9 +19,9 @@ using namespace moe355;
 // process ends; see static_scratch for how host code reaches it.
 static __device__ __align__(256) unsigned char scratch[MOE355_STATIC_SCRATCH_BYTES];
 
-namespace {
+namespace moe355 {
 
-thread_local char g_err[512] = "";
+static thread_local char g_err[512] = "";
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -34,6 +35,10 @@ int check_hip(hipError_t e, const char* what) {
   if (e == hipSuccess) return MOE355_OK;
   return fail(MOE355_EHIP, "%s: %s", what, hipGetErrorString(e));
 }
+
+}  // namespace moe355
+
+namespace {
 
 constexpr int kMaxDevices = 64;
 
@@ -49,21 +54,6 @@ constexpr double kStreamSmallBytes = 24e6, kStreamReadBytes = 500e6;
 // above), while the general one falls from 6.3 TB/s at 12 rows to 4.9 at 64.
 constexpr int kMidRows = 64, kMidRowsLarge = 40;
 constexpr double kMidLargeBytes = 3e9;
-
-size_t align256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
-
-bool valid_dtype(int d) { return d == MOE355_F32 || d == MOE355_BF16 || d == MOE355_F16; }
-
-int elem_size(int d) { return d == MOE355_F32 ? 4 : 2; }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
-
-template <typename T>
-T* at(void* ws, size_t off) {
-  return reinterpret_cast<T*>(static_cast<char*>(ws) + off);
-}
 
 int check_plan(const moe355_plan* p) {
   if (!p) return fail(MOE355_EINVAL, "plan is NULL");

@@ -1,0 +1,290 @@
+// extern "C" entry points of the 8-bit and 4-bit formats (mx.h) and of the routing
+// by groups: argument checks, the plan of the expert FFN, and dispatch.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "capi_detail.h"
+#include "mx.h"
+
+using namespace moe355;
+
+namespace {
+
+bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
+
+// The stages of one expert call and where their data lies in the workspace.
+struct MxPlan {
+  int rows, n_blocks, tile_rows, max_tiles, down_splits, down_steps;
+  int Hp, Ip;
+  size_t block_counts, offsets, slot_to_row, row_src, tile_map, xq, xq_scales, inter,
+      inter_scales, y, bytes;
+};
+
+int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
+  if (T < 0) return fail(MOE355_EINVAL, "bad T=%d", T);
+  if (H <= 0 || I <= 0) return fail(MOE355_EINVAL, "bad sizes H=%d I=%d", H, I);
+  if (bad_blocks(H) || bad_blocks(I))
+    return fail(MOE355_EUNSUPPORTED, "H=%d and I=%d must be multiples of %d", H, I, kMxBlock);
+  if (H > (1 << 20) || I > (1 << 20)) return fail(MOE355_EUNSUPPORTED, "H=%d or I=%d over 2^20", H, I);
+  if (E < 1 || E > MOE355_MAX_EXPERTS)
+    return fail(MOE355_EUNSUPPORTED, "E=%d outside [1, %d]", E, MOE355_MAX_EXPERTS);
+  if (K < 1 || K > E) return fail(MOE355_EINVAL, "top-k K=%d outside [1, E=%d]", K, E);
+  if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  const long long R = static_cast<long long>(T) * K;
+  if (R > INT_MAX / 2) return fail(MOE355_EUNSUPPORTED, "T*K=%lld too large", R);
+
+  *p = MxPlan{};
+  p->rows = static_cast<int>(R);
+  p->Hp = mx_pad(H);
+  p->Ip = mx_pad(I);
+  p->n_blocks = R <= kPermuteSingleMax ? 1 : static_cast<int>((R + kPermuteChunk - 1) / kPermuteChunk);
+  const int active = static_cast<int>(std::max<long long>(1, std::min<long long>(R, E)));
+  const long long avg = R / active;
+  p->tile_rows = avg <= 12 ? 16 : avg <= 28 ? 32 : 64;
+  p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
+  // Columns of the down projection over workgroups, until there are 512 of them.
+  const int steps = p->Ip / kMxStep;
+  const long long groups = static_cast<long long>(p->Hp / kMxSuper) * std::max(p->max_tiles, 1);
+  int s = 1;
+  while (s < 8 && groups * s < 512 && steps >= 8 * s) s *= 2;
+  p->down_splits = s;
+  p->down_steps = (steps + s - 1) / s;
+
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off = align256(off + bytes);
+    return at;
+  };
+  p->block_counts = take(static_cast<size_t>(p->n_blocks) * E * 4);
+  p->offsets = take(static_cast<size_t>(E + 1) * 4);
+  p->slot_to_row = take(static_cast<size_t>(R) * 4);
+  p->row_src = take(static_cast<size_t>(R) * 4);
+  p->tile_map = take((2 + 2 * static_cast<size_t>(p->max_tiles)) * 4);
+  p->xq = take(static_cast<size_t>(T) * p->Hp);
+  p->xq_scales = take(static_cast<size_t>(T) * p->Hp / kMxBlock);
+  p->inter = take(static_cast<size_t>(R) * p->Ip);
+  p->inter_scales = take(static_cast<size_t>(R) * p->Ip / kMxBlock);
+  p->y = take(static_cast<size_t>(p->down_splits) * R * H * 4);
+  p->bytes = off;
+  return MOE355_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int moe355_mx_quantize(const void* x, int T, int H, int dtype, void* codes, void* scales,
+                       void* stream) {
+  if (T < 0) return fail(MOE355_EINVAL, "bad T=%d", T);
+  if (bad_blocks(H)) return fail(MOE355_EUNSUPPORTED, "H=%d must be a multiple of %d", H, kMxBlock);
+  if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  if (T == 0) return MOE355_OK;
+  if (!x || !codes || !scales) return fail(MOE355_EINVAL, "NULL tensor argument");
+  if (!aligned16(x) || !aligned16(codes)) return fail(MOE355_EINVAL, "x/codes not 16-byte aligned");
+  const MxQuantArgs a{x, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), T, H, mx_pad(H)};
+  return check_hip(launch_mx_quantize(a, dtype, as_stream(stream)), "mx_quantize launch");
+}
+
+int moe355_add_rmsnorm_mxfp8(const void* x, const void* residual, void* residual_out,
+                             const void* weight, const void* bias, int weight_dtype, float eps,
+                             int T, int H, int dtype, void* normed_out, void* codes, void* scales,
+                             void* stream) {
+  if (T < 0 || H <= 0) return fail(MOE355_EINVAL, "bad sizes T=%d H=%d", T, H);
+  if (!valid_dtype(dtype) || !valid_dtype(weight_dtype))
+    return fail(MOE355_EINVAL, "unknown dtype %d / weight dtype %d", dtype, weight_dtype);
+  if (bad_blocks(H) || H > norm_max_hidden(dtype))
+    return fail(MOE355_EUNSUPPORTED, "norm with 8-bit rows needs H %% %d == 0 and H <= %d", kMxBlock,
+                norm_max_hidden(dtype));
+  if (!(eps >= 0.0f)) return fail(MOE355_EINVAL, "eps must be >= 0");
+  if (T == 0) return MOE355_OK;
+  if (!x || !weight || !normed_out || !codes || !scales)
+    return fail(MOE355_EINVAL, "NULL tensor argument");
+  if (residual && !residual_out) return fail(MOE355_EINVAL, "residual given without residual_out");
+  if (!aligned16(x) || !aligned16(normed_out) || !aligned16(codes) ||
+      (residual && (!aligned16(residual) || !aligned16(residual_out))))
+    return fail(MOE355_EINVAL, "x/residual/out/codes not 16-byte aligned");
+  if (!aligned16(weight) || (bias && !aligned16(bias)))
+    return fail(MOE355_EINVAL, "norm weight/bias not 16-byte aligned");
+  NormArgs a{};
+  a.x = x; a.residual = residual; a.residual_out = residual_out; a.weight = weight;
+  a.bias = bias; a.out = normed_out;
+  a.T = T; a.H = H; a.weight_dtype = weight_dtype; a.eps = eps;
+  a.codes = static_cast<uint8_t*>(codes);
+  a.scales = static_cast<uint8_t*>(scales);
+  a.Hp = mx_pad(H);
+  return check_hip(launch_add_rmsnorm(a, dtype, as_stream(stream)), "add_rmsnorm_mxfp8 launch");
+}
+
+int moe355_grouped_topk(const float* logits, const float* bias, int T, int E, int K, int scoring,
+                        int num_groups, int topk_groups, int group_score, int renormalize,
+                        float scale, float* topk_w, void* topk_ids, int ids_int64, int out_ld,
+                        void* stream) {
+  if (T < 0) return fail(MOE355_EINVAL, "bad T=%d", T);
+  if (E < 1 || E > MOE355_MAX_EXPERTS)
+    return fail(MOE355_EUNSUPPORTED, "E=%d outside [1, %d]", E, MOE355_MAX_EXPERTS);
+  if (scoring != MOE355_SCORE_SOFTMAX && scoring != MOE355_SCORE_SIGMOID)
+    return fail(MOE355_EINVAL, "unknown scoring %d", scoring);
+  if (group_score != MOE355_GROUP_MAX && group_score != MOE355_GROUP_TOP2)
+    return fail(MOE355_EINVAL, "unknown group score %d", group_score);
+  if (num_groups < 1 || E % num_groups)
+    return fail(MOE355_EINVAL, "%d groups do not divide E=%d experts", num_groups, E);
+  if (num_groups > MOE355_MAX_GROUPS)
+    return fail(MOE355_EUNSUPPORTED, "%d groups, at most %d", num_groups, MOE355_MAX_GROUPS);
+  if (topk_groups < 1 || topk_groups > num_groups)
+    return fail(MOE355_EINVAL, "topk_groups=%d outside [1, %d]", topk_groups, num_groups);
+  if (K < 1 || K > topk_groups * (E / num_groups))
+    return fail(MOE355_EINVAL, "top-k K=%d outside [1, %d], the experts of %d groups", K,
+                topk_groups * (E / num_groups), topk_groups);
+  if (K > MOE355_MAX_GROUPED_TOPK)
+    return fail(MOE355_EUNSUPPORTED, "top-k K=%d over %d", K, MOE355_MAX_GROUPED_TOPK);
+  if (!std::isfinite(scale)) return fail(MOE355_EINVAL, "scale must be finite");
+  if (out_ld < K) return fail(MOE355_EINVAL, "output row stride %d < K=%d", out_ld, K);
+  if (T == 0) return MOE355_OK;
+  if (!logits || !topk_w || !topk_ids) return fail(MOE355_EINVAL, "NULL tensor argument");
+  GroupTopkArgs a{};
+  a.logits = logits; a.bias = bias; a.topk_w = topk_w; a.topk_ids = topk_ids;
+  a.T = T; a.E = E; a.K = K; a.G = num_groups; a.KG = topk_groups;
+  a.sigmoid = scoring == MOE355_SCORE_SIGMOID;
+  a.top2 = group_score == MOE355_GROUP_TOP2;
+  a.renormalize = renormalize != 0; a.ids_int64 = ids_int64 != 0; a.out_ld = out_ld;
+  a.scale = scale;
+  return check_hip(launch_group_topk(a, as_stream(stream)), "grouped_topk launch");
+}
+
+int moe355_router_logits(const void* x, const void* gate, int T, int H, int E, int dtype,
+                         int round_logits, float* logits_out, void* stream) {
+  if (T < 0 || H <= 0) return fail(MOE355_EINVAL, "bad sizes T=%d H=%d", T, H);
+  if (E < 1 || E > MOE355_MAX_EXPERTS)
+    return fail(MOE355_EUNSUPPORTED, "E=%d outside [1, %d]", E, MOE355_MAX_EXPERTS);
+  if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  const int vec = 16 / elem_size(dtype);
+  if (H % vec) return fail(MOE355_EUNSUPPORTED, "router needs H %% %d == 0", vec);
+  if (T == 0) return MOE355_OK;
+  if (!x || !gate || !logits_out) return fail(MOE355_EINVAL, "NULL tensor argument");
+  if (!aligned16(x) || !aligned16(gate)) return fail(MOE355_EINVAL, "x/gate not 16-byte aligned");
+  RouterArgs a{};
+  a.x = x; a.gate = gate; a.logits_out = logits_out;
+  a.T = T; a.H = H; a.E = E; a.K = 0; a.round_logits = round_logits != 0;
+  return check_hip(launch_router_logits(a, dtype, as_stream(stream)), "router_logits launch");
+}
+
+int moe355_mx_matrix_bytes(int rows, int cols, int gate_up, size_t* codes, size_t* scales) {
+  if (!codes || !scales) return fail(MOE355_EINVAL, "NULL result");
+  if (rows <= 0 || (gate_up && rows % 2)) return fail(MOE355_EINVAL, "bad rows=%d", rows);
+  if (bad_blocks(cols) || bad_blocks(gate_up ? rows / 2 : rows) || rows > (1 << 21) || cols > (1 << 20))
+    return fail(MOE355_EUNSUPPORTED, "a 4-bit matrix of %d x %d: sizes must be multiples of %d", rows,
+                cols, kMxBlock);
+  const int rows_p = gate_up ? 2 * mx_pad(rows / 2) : mx_pad(rows);
+  *codes = mx_code_bytes(rows_p, mx_pad(cols));
+  *scales = mx_scale_bytes(rows_p, mx_pad(cols));
+  return MOE355_OK;
+}
+
+int moe355_mx_pack(const void* src, const void* src_scales, int rows, int cols, int gate_up,
+                   int dtype, void* codes, void* scales, void* stream) {
+  size_t nc, ns;
+  if (int rc = moe355_mx_matrix_bytes(rows, cols, gate_up, &nc, &ns)) return rc;
+  const bool is_codes = dtype == MOE355_MX_CODES;
+  if (!is_codes && !valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  if (!src || !codes || !scales || (is_codes && !src_scales))
+    return fail(MOE355_EINVAL, "NULL tensor argument");
+  if (!aligned16(codes) || (is_codes && !aligned16(src)) ||
+      (!is_codes && reinterpret_cast<uintptr_t>(src) % elem_size(dtype)))
+    return fail(MOE355_EINVAL, "src/codes not aligned");
+  MxPackArgs a{};
+  a.src = src; a.scales = static_cast<const uint8_t*>(src_scales);
+  a.codes_out = static_cast<uint8_t*>(codes); a.scales_out = static_cast<uint8_t*>(scales);
+  a.rows = rows; a.cols = cols;
+  a.rows_p = gate_up ? 2 * mx_pad(rows / 2) : mx_pad(rows);
+  a.cols_p = mx_pad(cols);
+  a.gate_up = gate_up != 0;
+  return check_hip(launch_mx_pack(a, is_codes ? -1 : dtype, as_stream(stream)), "mx_pack launch");
+}
+
+int moe355_mx_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes) {
+  if (!bytes) return fail(MOE355_EINVAL, "NULL result");
+  MxPlan p;
+  if (int rc = mx_plan(T, H, I, E, K, dtype, &p)) return rc;
+  *bytes = p.bytes;
+  return MOE355_OK;
+}
+
+int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
+                            const void* w1_scales, const void* w2, const void* w2_scales,
+                            const float* topk_w, const void* topk_ids, int ids_int64, int T, int H,
+                            int I, int E, int K, int dtype, int act, void* out, int accumulate_f32,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  MxPlan p;
+  if (int rc = mx_plan(T, H, I, E, K, dtype, &p)) return rc;
+  if (act < MOE355_ACT_SILU || act > MOE355_ACT_GELU_TANH)
+    return fail(MOE355_EINVAL, "unknown activation %d", act);
+  if (T == 0) return MOE355_OK;
+  if (!x || !w1 || !w1_scales || !w2 || !w2_scales || !topk_w || !topk_ids || !out)
+    return fail(MOE355_EINVAL, "NULL tensor argument");
+  if (!aligned16(x) || !aligned16(w1) || !aligned16(w1_scales) || !aligned16(w2) ||
+      !aligned16(w2_scales) || !aligned16(out) ||
+      (x_scales && reinterpret_cast<uintptr_t>(x_scales) % 4))
+    return fail(MOE355_EINVAL, "x/w1/w2/scales/out not 16-byte aligned");
+  if (!workspace || workspace_bytes < p.bytes)
+    return fail(MOE355_EWORKSPACE, "workspace of %zu bytes, the call needs %zu", workspace_bytes,
+                p.bytes);
+  if (!aligned16(workspace)) return fail(MOE355_EINVAL, "workspace not 16-byte aligned");
+  hipStream_t s = as_stream(stream);
+
+  const uint8_t* xq = static_cast<const uint8_t*>(x);
+  const uint8_t* xs = static_cast<const uint8_t*>(x_scales);
+  if (!x_scales) {
+    const MxQuantArgs qa{x, at<uint8_t>(workspace, p.xq), at<uint8_t>(workspace, p.xq_scales), T, H, p.Hp};
+    if (int rc = check_hip(launch_mx_quantize(qa, dtype, s), "mx_quantize launch")) return rc;
+    xq = qa.codes;
+    xs = qa.scales;
+  }
+
+  PermuteArgs pa{};
+  pa.ids = topk_ids;
+  pa.block_counts = at<int32_t>(workspace, p.block_counts);
+  pa.offsets = at<int32_t>(workspace, p.offsets);
+  pa.slot_to_row = at<int32_t>(workspace, p.slot_to_row);
+  pa.row_src = at<int32_t>(workspace, p.row_src);
+  pa.tile_map = at<int32_t>(workspace, p.tile_map);
+  pa.R = p.rows; pa.K = K; pa.E = E; pa.n_blocks = p.n_blocks;
+  pa.tile_rows = p.tile_rows; pa.max_tiles = p.max_tiles;
+  pa.ids_int64 = ids_int64 != 0;
+  pa.weights = topk_w;
+  if (int rc = check_hip(launch_permute(pa, s), "permute launch")) return rc;
+
+  MxFfnArgs f{};
+  f.row_src = pa.row_src; f.tile_map = pa.tile_map; f.offsets = pa.offsets;
+  f.max_tiles = p.max_tiles; f.tile_rows = p.tile_rows;
+  f.R = p.rows; f.H = H; f.Ip = p.Ip; f.act = act;
+  // A bf16 result keeps 8 bits, below which the scaled MFMA's alignment of products
+  // does not show; results of more bits take the exact products.
+  f.exact = dtype != MOE355_BF16;
+  f.out_codes = at<uint8_t>(workspace, p.inter);
+  f.out_scales = at<uint8_t>(workspace, p.inter_scales);
+  f.y = at<float>(workspace, p.y);
+
+  f.x = xq; f.x_scales = xs;
+  f.w = static_cast<const uint8_t*>(w1); f.w_scales = static_cast<const uint32_t*>(w1_scales);
+  f.w_stride = mx_code_bytes(2 * p.Ip, p.Hp); f.ws_stride = mx_scale_bytes(2 * p.Ip, p.Hp) / 4;
+  f.Kp = p.Hp; f.n_super = 2 * p.Ip / kMxSuper;
+  f.splits = 1; f.steps_per_split = p.Hp / kMxStep;
+  if (int rc = check_hip(launch_mx_gate_up(f, s), "mx gate_up launch")) return rc;
+
+  f.x = f.out_codes; f.x_scales = f.out_scales;
+  f.w = static_cast<const uint8_t*>(w2); f.w_scales = static_cast<const uint32_t*>(w2_scales);
+  f.w_stride = mx_code_bytes(p.Hp, p.Ip); f.ws_stride = mx_scale_bytes(p.Hp, p.Ip) / 4;
+  f.Kp = p.Ip; f.n_super = p.Hp / kMxSuper;
+  f.splits = p.down_splits; f.steps_per_split = p.down_steps;
+  if (int rc = check_hip(launch_mx_down(f, s), "mx down launch")) return rc;
+
+  CombineArgs c{};
+  c.y = f.y; c.topk_w = topk_w; c.slot_to_row = pa.slot_to_row; c.out = out;
+  c.T = T; c.K = K; c.H = H; c.R = p.rows; c.splits = p.down_splits;
+  c.accumulate = accumulate_f32 != 0;
+  return check_hip(launch_combine(c, dtype, s), "combine launch");
+}
+
+}  // extern "C"

@@ -265,6 +265,20 @@ struct NormArgs {
   void* out;            // [T,H] normed
   int T, H, weight_dtype;
   float eps;
+  uint8_t* codes;       // [T,Hp] the normed row in 8 bits (mx.h), or nullptr
+  uint8_t* scales;      // [T,Hp/32]
+  int Hp;
+};
+
+// Selection of experts by groups from router logits (group_topk.hip).
+struct GroupTopkArgs {
+  const float* logits;  // [T,E]
+  const float* bias;    // [E] added to the scores for the choice alone, or nullptr
+  float* topk_w;        // [T,out_ld]
+  void* topk_ids;       // [T,out_ld] int32 or int64
+  int T, E, K, G, KG;   // G groups, of which the best KG are kept
+  int sigmoid, top2, renormalize, ids_int64, out_ld;
+  float scale;
 };
 
 struct CombineArgs {
@@ -287,6 +301,9 @@ hipError_t launch_router(const RouterArgs& a, int dtype, hipStream_t s);
 hipError_t launch_add_rmsnorm(const NormArgs& a, int dtype, hipStream_t s);
 int norm_max_hidden(int dtype);
 hipError_t launch_topk_from_logits(const RouterArgs& a, hipStream_t s);
+hipError_t launch_group_topk(const GroupTopkArgs& a, hipStream_t s);
+// Router logits alone, [T,E] fp32 in a.logits_out, for any E.
+hipError_t launch_router_logits(const RouterArgs& a, int dtype, hipStream_t s);
 hipError_t launch_permute(const PermuteArgs& a, hipStream_t s);
 hipError_t launch_gate_up_tiled(const FfnArgs& a, int dtype, hipStream_t s);
 hipError_t launch_down_tiled(const FfnArgs& a, int dtype, hipStream_t s);

@@ -1,0 +1,110 @@
+// Formats with one power-of-two scale per 32 consecutive values of a row: 8 bits
+// (e4m3 codes) for tokens and intermediates, 4 bits (e2m1 codes, two per byte, the
+// even column in the low half) for expert weights. A scale is a byte b that
+// stands for 2^(b - 127); in weights 255 stands for NaN.
+//
+// Rows of 8 bits are padded to whole 128-value steps with codes of 0, so that the
+// matrix kernels never see a partial step.
+//
+// 4-bit matrices are laid out once, in the order in which the kernels stream them.
+// A tile is 16 rows x 128 columns, 1 KB: lane 16 q + r of a wave holds row r,
+// columns 32 q .. 32 q + 31 (one block, 16 bytes), which is the operand of
+// v_mfma_scale_f32_16x16x128_f8f6f4 as it stands, so one load instruction fetches
+// one tile from 1 KB of consecutive bytes and no lane moves data afterwards.
+// Four groups of 16 rows make a supergroup, whose four tiles of a 128-column step
+// follow each other (4 KB), then the next step's; its scales are one dword per lane
+// and step, byte g for group g, so that a wave working on a supergroup loads all of
+// a step's scales at once and the instruction picks its byte. A gate|up matrix is
+// interleaved by groups (gate 0, up 0, gate 1, up 1, ..): a supergroup then
+// holds one 32-value block of the intermediate. Rows and columns are padded to
+// multiples of 128 with zeros.
+#pragma once
+
+#include "common.h"
+
+namespace moe355 {
+
+constexpr int kMxBlock = 32;    // values per scale
+constexpr int kMxStep = 128;    // columns per matrix instruction
+constexpr int kMxSuper = 64;    // rows per supergroup
+constexpr int kMxTileBytes = 1024;
+
+__host__ __device__ constexpr int mx_pad(int n) { return (n + kMxStep - 1) / kMxStep * kMxStep; }
+
+// Bytes of the codes and scales of a 4-bit matrix of [rows, cols], both padded.
+__host__ __device__ constexpr size_t mx_code_bytes(int rows, int cols) {
+  return static_cast<size_t>(rows) * cols / 2;
+}
+__host__ __device__ constexpr size_t mx_scale_bytes(int rows, int cols) {
+  return static_cast<size_t>(rows) * cols / kMxBlock;
+}
+
+// Scale byte of a block whose largest finite magnitude is amax: the smallest power
+// of two with amax <= 448 * 2^e (448 = 1.75 * 2^8 is the largest e4m3 value), so
+// that no value is clipped; 0 for a block of zeros.
+__device__ __forceinline__ int mx8_scale(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  return max(static_cast<int>(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0), 0);
+}
+
+// 2^(127 - b), the factor that brings a block's values to the range of the codes.
+__device__ __forceinline__ float mx_inverse(int b) {
+  return __uint_as_float(static_cast<uint32_t>(254 - b) << 23);
+}
+
+// Magnitude that counts for a block's scale: 0 for infinities and NaN, whose
+// codes become NaN whatever the scale is.
+__device__ __forceinline__ float mx_finite_abs(float v) {
+  const float a = fabsf(v);
+  return a < INFINITY ? a : 0.f;
+}
+
+// Four e4m3 codes, rounded to nearest even; infinities and NaN become NaN.
+__device__ __forceinline__ uint32_t mx8_codes(float a, float b, float c, float d) {
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true));
+}
+
+struct MxQuantArgs {
+  const void* x;    // [T, H]
+  uint8_t* codes;   // [T, Hp]
+  uint8_t* scales;  // [T, Hp / 32]
+  int T, H, Hp;
+};
+
+struct MxPackArgs {
+  const void* src;        // codes [rows, cols / 2], or weights [rows, cols] to be rounded
+  const uint8_t* scales;  // [rows, cols / 32] of codes
+  uint8_t* codes_out;
+  uint8_t* scales_out;
+  int rows, cols;         // of the source
+  int rows_p, cols_p;     // padded (both halves of a gate|up matrix each)
+  int gate_up;            // rows 0 .. rows / 2 - 1 gate, the others up
+};
+
+struct MxFfnArgs {
+  const uint8_t* x;         // token rows in 8 bits, [*, Kp]
+  const uint8_t* x_scales;  // [*, Kp / 32]
+  const int32_t* row_src;   // gate_up: x row of each permuted row
+  const int32_t* tile_map;  // [2 + 2 * max_tiles]
+  const int32_t* offsets;   // [E + 1]
+  const uint8_t* w;         // 4-bit matrices, w_stride bytes apart
+  const uint32_t* w_scales; // dwords, ws_stride apart
+  size_t w_stride, ws_stride;
+  int Kp, n_super;          // padded columns, supergroups of rows
+  int max_tiles, tile_rows, splits, steps_per_split;
+  int R, H;                 // down: rows and features of y
+  float* y;                 // down: [splits, R, H]
+  uint8_t* out_codes;       // gate_up: [R, Ip]
+  uint8_t* out_scales;      // [R, Ip / 32]
+  int Ip, act;
+  int exact;                // multiply in bf16 (exactly) instead of the scaled MFMA
+};
+
+hipError_t launch_mx_gate_up(const MxFfnArgs& a, hipStream_t s);
+hipError_t launch_mx_down(const MxFfnArgs& a, hipStream_t s);
+hipError_t launch_mx_quantize(const MxQuantArgs& a, int dtype, hipStream_t s);
+// dtype -1: src holds codes.
+hipError_t launch_mx_pack(const MxPackArgs& a, int dtype, hipStream_t s);
+
+}  // namespace moe355

@@ -14,6 +14,7 @@
 
 #include "common.h"
 #include "dma_pipe.h"
+#include "mx.h"
 
 namespace moe355 {
 namespace {
@@ -87,7 +88,11 @@ struct ParamChunk {
 // (CPT of them at most). Every load of a phase is issued before any is used:
 // phase 1 reads x and the residual, phase 2 (after the sum of squares) the
 // weight and bias, so each phase costs one memory round trip.
-template <typename T, typename W, int CPT>
+// kQ8: the row that goes to out, as it is rounded there, also in 8 bits, from
+// registers: a block of 32 values lies in 32 / N neighbouring lanes (H is a
+// multiple of 32), whose maximum gives its scale. Quantising the rounded row makes
+// it bit for bit what quantising `out` in a launch of its own gives.
+template <typename T, typename W, int CPT, bool kQ8>
 __global__ __launch_bounds__(kThreads) void add_rmsnorm_kernel(const NormArgs a) {
   constexpr int N = Vec16<T>::N;  // elements per 16-byte chunk
   const int t = blockIdx.x, tid = threadIdx.x;
@@ -155,8 +160,31 @@ __global__ __launch_bounds__(kThreads) void add_rmsnorm_kernel(const NormArgs a)
       o[i] = r[c][i] * inv * wv[i];
       if (a.bias) o[i] += bv[i];
     }
-    *reinterpret_cast<u32x4*>(static_cast<T*>(a.out) + row + static_cast<size_t>(ch) * N) =
-        pack16<T>(o);
+    const u32x4 packed = pack16<T>(o);
+    *reinterpret_cast<u32x4*>(static_cast<T*>(a.out) + row + static_cast<size_t>(ch) * N) = packed;
+    if constexpr (kQ8) {
+      Vec16<T>::unpack(packed, o);
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) amax = fmaxf(amax, mx_finite_abs(o[i]));
+#pragma unroll
+      for (int l = 1; l < kMxBlock / N; l <<= 1) amax = fmaxf(amax, __shfl_xor(amax, l, kWave));
+      const int b = mx8_scale(amax);
+      const float f = mx_inverse(b);
+      uint32_t* q = reinterpret_cast<uint32_t*>(a.codes + static_cast<size_t>(t) * a.Hp + ch * N);
+#pragma unroll
+      for (int i = 0; i < N; i += 4)
+        q[i / 4] = mx8_codes(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+      if (tid % (kMxBlock / N) == 0)
+        a.scales[static_cast<size_t>(t) * (a.Hp / kMxBlock) + ch * N / kMxBlock] =
+            static_cast<uint8_t>(b);
+    }
+  }
+  if constexpr (kQ8) {  // the padding of the row's last step
+    const int pad = a.Hp - a.H;  // < 128
+    if (tid < pad) a.codes[static_cast<size_t>(t) * a.Hp + a.H + tid] = 0;
+    if (tid < pad / kMxBlock)
+      a.scales[static_cast<size_t>(t) * (a.Hp / kMxBlock) + a.H / kMxBlock + tid] = 0;
   }
 }
 
@@ -634,26 +662,26 @@ hipError_t launch_norm_router_t(const NormArgs& a, const RouterArgs& ra, hipStre
   return launch_norm_router_tw<T, float>(a, ra, s);
 }
 
-template <typename T, typename W>
+template <typename T, typename W, bool kQ8>
 hipError_t launch_norm_tw(const NormArgs& a, hipStream_t s) {
   const int per_thread = (a.H / Vec16<T>::N + kThreads - 1) / kThreads;
   const dim3 grid(a.T), block(kThreads);
   if (per_thread <= 1)
-    add_rmsnorm_kernel<T, W, 1><<<grid, block, 0, s>>>(a);
+    add_rmsnorm_kernel<T, W, 1, kQ8><<<grid, block, 0, s>>>(a);
   else if (per_thread <= 2)
-    add_rmsnorm_kernel<T, W, 2><<<grid, block, 0, s>>>(a);
+    add_rmsnorm_kernel<T, W, 2, kQ8><<<grid, block, 0, s>>>(a);
   else if (per_thread <= 4)
-    add_rmsnorm_kernel<T, W, 4><<<grid, block, 0, s>>>(a);
+    add_rmsnorm_kernel<T, W, 4, kQ8><<<grid, block, 0, s>>>(a);
   else
-    add_rmsnorm_kernel<T, W, kMaxChunks><<<grid, block, 0, s>>>(a);
+    add_rmsnorm_kernel<T, W, kMaxChunks, kQ8><<<grid, block, 0, s>>>(a);
   return hipGetLastError();
 }
 
-template <typename T>
+template <typename T, bool kQ8>
 hipError_t launch_norm_t(const NormArgs& a, hipStream_t s) {
-  if (a.weight_dtype == MOE355_BF16) return launch_norm_tw<T, bf16>(a, s);
-  if (a.weight_dtype == MOE355_F16) return launch_norm_tw<T, f16>(a, s);
-  return launch_norm_tw<T, float>(a, s);
+  if (a.weight_dtype == MOE355_BF16) return launch_norm_tw<T, bf16, kQ8>(a, s);
+  if (a.weight_dtype == MOE355_F16) return launch_norm_tw<T, f16, kQ8>(a, s);
+  return launch_norm_tw<T, float, kQ8>(a, s);
 }
 
 }  // namespace
@@ -697,9 +725,14 @@ hipError_t launch_add_rmsnorm_router_mfma(const NormArgs& a, const RouterArgs& r
 
 hipError_t launch_add_rmsnorm(const NormArgs& a, int dtype, hipStream_t s) {
   if (a.T == 0) return hipSuccess;
-  if (dtype == MOE355_BF16) return launch_norm_t<bf16>(a, s);
-  if (dtype == MOE355_F16) return launch_norm_t<f16>(a, s);
-  return launch_norm_t<float>(a, s);
+  if (a.codes) {
+    if (dtype == MOE355_BF16) return launch_norm_t<bf16, true>(a, s);
+    if (dtype == MOE355_F16) return launch_norm_t<f16, true>(a, s);
+    return launch_norm_t<float, true>(a, s);
+  }
+  if (dtype == MOE355_BF16) return launch_norm_t<bf16, false>(a, s);
+  if (dtype == MOE355_F16) return launch_norm_t<f16, false>(a, s);
+  return launch_norm_t<float, false>(a, s);
 }
 
 }  // namespace moe355

@@ -91,6 +91,7 @@ __global__ __launch_bounds__(kThreads) void router_kernel(const RouterArgs a) {
     }
     __syncthreads();
   }
+  if (a.K == 0) return;  // logits alone
 
   for (int t = wave; t < ntok; t += kThreads / kWave)
     wave_topk(lg[t], a.E, a.K, a.renormalize, a.entropy_k_min,
@@ -133,7 +134,9 @@ struct Mfma16R<f16> {
 // (now 8.5 and 12.3 us at 4096 tokens, H = 4096 and 2048).
 // The fp32 VALU router re-reads the gate per 8 tokens and spends E*H FMAs per
 // token on the VALU: at 4096 tokens, 64 experts and H = 2048 it took 54 us.
-template <typename T, int NG>
+// kLogits: the logits of 16 NG experts from 16 NG blockIdx.y on and no selection, so
+// that any number of experts runs here.
+template <typename T, int NG, bool kLogits = false>
 __global__ __launch_bounds__(kThreads) void router_mfma_kernel(const RouterArgs a) {
   constexpr int kTok = 16, EP = 16 * NG, kRows = kTok + EP;
   constexpr int kLoads = kRows / 8;  // direct-to-LDS loads per batch
@@ -153,6 +156,7 @@ __global__ __launch_bounds__(kThreads) void router_mfma_kernel(const RouterArgs 
   Part& part = *reinterpret_cast<Part*>(&stage[0][0][0]);
   Lg& lg = *reinterpret_cast<Lg*>(&stage[0][0][0] + sizeof(Part));
   const int t0 = blockIdx.x * kTok;
+  const int eb = kLogits ? blockIdx.y * EP : 0;  // first expert
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int r = lane & 15, kq = lane >> 4;
@@ -164,12 +168,13 @@ __global__ __launch_bounds__(kThreads) void router_mfma_kernel(const RouterArgs 
   // and gate rows past E load the last row again (never read back).
   const __amdgpu_buffer_rsrc_t xsrc =
       pipe::lds_rsrc(static_cast<const T*>(a.x) + static_cast<size_t>(t0) * a.H + wave * hq);
-  const __amdgpu_buffer_rsrc_t gsrc = pipe::lds_rsrc(static_cast<const T*>(a.gate) + wave * hq);
+  const __amdgpu_buffer_rsrc_t gsrc = pipe::lds_rsrc(
+      static_cast<const T*>(a.gate) + static_cast<size_t>(eb) * a.H + wave * hq);
   uint32_t voff[kLoads];
 #pragma unroll
   for (int q = 0; q < kLoads; ++q) {
     const int row = 8 * q + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
-    const int src = row < kTok ? min(t0 + row, a.T - 1) - t0 : min(row - kTok, a.E - 1);
+    const int src = row < kTok ? min(t0 + row, a.T - 1) - t0 : min(row - kTok, a.E - 1 - eb);
     voff[q] = static_cast<uint32_t>(src) * pitch + c * 16;
   }
   auto issue = [&](int b) {
@@ -219,14 +224,15 @@ __global__ __launch_bounds__(kThreads) void router_mfma_kernel(const RouterArgs 
   __syncthreads();
   for (int i = tid; i < kTok * EP; i += kThreads) {
     const int t = i / EP, e = i % EP;
-    if (t0 + t < a.T && e < a.E) {
+    if (t0 + t < a.T && eb + e < a.E) {
       float l = (part[0][t][e] + part[1][t][e]) + (part[2][t][e] + part[3][t][e]);
       if (a.round_logits) l = to_f32(from_f32<T>(l));
-      if (a.bias) l += a.bias[e];
-      lg[t][e] = l;
-      if (a.logits_out) a.logits_out[static_cast<size_t>(t0 + t) * a.E + e] = l;
+      if (a.bias) l += a.bias[eb + e];
+      if (!kLogits) lg[t][e] = l;
+      if (a.logits_out) a.logits_out[static_cast<size_t>(t0 + t) * a.E + eb + e] = l;
     }
   }
+  if constexpr (kLogits) return;
   __syncthreads();
   // 16 lanes per token (tid = 16 t + sub).
   const int tt = tid / 16;
@@ -353,6 +359,38 @@ hipError_t launch_router_t(const RouterArgs& a, hipStream_t s) {
   else
     router_kernel<T, 1, 8><<<dim3(a.T), block, 0, s>>>(a);
   return hipGetLastError();
+}
+
+// The logits alone, by the kernels above: few tokens over (token, 8 experts)
+// workgroups, more on MFMA where the types and H allow it, else on the VALU.
+template <typename T>
+hipError_t launch_logits_t(const RouterArgs& a, hipStream_t s) {
+  const dim3 block(kThreads);
+  if (a.T < 256) {
+    router_logits_kernel<T, 8><<<dim3(a.T, (a.E + 7) / 8), block, 0, s>>>(a);
+    return hipGetLastError();
+  }
+  if constexpr (!std::is_same<T, float>::value) {
+    if (a.H % 256 == 0) {
+      const unsigned nt = (a.T + 15) / 16;
+      if (a.E <= 16)
+        router_mfma_kernel<T, 1, true><<<dim3(nt), block, 0, s>>>(a);
+      else if (a.E <= 32)
+        router_mfma_kernel<T, 2, true><<<dim3(nt), block, 0, s>>>(a);
+      else
+        router_mfma_kernel<T, 4, true><<<dim3(nt, (a.E + 63) / 64), block, 0, s>>>(a);
+      return hipGetLastError();
+    }
+  }
+  router_kernel<T, 4, 16><<<dim3((a.T + 3) / 4), block, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_router_logits(const RouterArgs& a, int dtype, hipStream_t s) {
+  if (a.T == 0) return hipSuccess;
+  if (dtype == MOE355_BF16) return launch_logits_t<bf16>(a, s);
+  if (dtype == MOE355_F16) return launch_logits_t<f16>(a, s);
+  return launch_logits_t<float>(a, s);
 }
 
 hipError_t launch_router(const RouterArgs& a, int dtype, hipStream_t s) {

@@ -7,7 +7,8 @@ computed in fp32 (``x / sqrt(mean(x^2) + eps) * weight (+ bias)``) and rounded
 once to the input dtype; ``forward_add_residual`` first forms
 ``residual = x + residual`` in the input dtype and returns
 ``(rmsnorm(residual), residual)``. Parameters may be stored in fp32 or the
-activation dtype.
+activation dtype. ``forward_mxfp8`` and ``forward_add_residual_mxfp8`` also leave
+the normed rows in 8 bits (mx.Mxfp8Rows), for expert products that take them.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ import torch.nn as nn
 
 from reframework_amd import _capi
 from reframework_amd.layers.base import BaseOP
+from reframework_amd.mx import BLOCK, Mxfp8Rows
 
 
 class RMSNorm(BaseOP):
@@ -68,6 +70,42 @@ class RMSNorm(BaseOP):
         out = torch.empty_like(x)
         self._run(x, residual, out, new_res)
         return out, new_res
+
+    def _run_mxfp8(self, x: torch.Tensor, residual: Optional[torch.Tensor], out: torch.Tensor,
+                   residual_out: Optional[torch.Tensor]) -> Mxfp8Rows:
+        w, b = self._params(x)
+        H = self.size
+        if H % BLOCK:
+            raise ValueError(f"8-bit rows need a size of whole blocks of {BLOCK}, not {H}")
+        x2 = x.reshape(-1, H)
+        q = Mxfp8Rows.empty(x2.shape[0], H, x.device)
+        _capi.add_rmsnorm_mxfp8(x2, None if residual is None else residual.reshape(-1, H),
+                                None if residual_out is None else residual_out.reshape(-1, H),
+                                w, b, self.eps, out.reshape(-1, H), q.padded_codes,
+                                q.padded_scales)
+        return q
+
+    def forward_mxfp8(self, x: torch.Tensor) -> Tuple[torch.Tensor, Mxfp8Rows]:
+        """(normed, normed in 8 bits), in one launch; the latter is
+        ``quantize_mxfp8(normed)`` bit for bit, one row per row of ``x``."""
+        x = x.contiguous()
+        out = torch.empty_like(x)
+        return out, self._run_mxfp8(x, None, out, None)
+
+    def forward_add_residual_mxfp8(
+            self, x: torch.Tensor,
+            residual: torch.Tensor) -> Tuple[torch.Tensor, Mxfp8Rows, torch.Tensor]:
+        """forward_add_residual that also returns the normed rows in 8 bits:
+        (normed, normed in 8 bits, new_residual), in one launch."""
+        x = x.contiguous()
+        residual = residual.to(x.dtype).contiguous()
+        if residual.shape != x.shape or residual.device != x.device:
+            raise ValueError(f"residual {tuple(residual.shape)} on {residual.device} does not match "
+                             f"x {tuple(x.shape)} on {x.device}")
+        new_res = torch.empty_like(x)
+        out = torch.empty_like(x)
+        q = self._run_mxfp8(x, residual, out, new_res)
+        return out, q, new_res
 
 
 __all__ = ["RMSNorm"]

@@ -1,7 +1,8 @@
 """MoE: routing, grouped expert compute and the host-offload expert cache.
 
 Import surface of the reference's ``reframework.moe`` (reframework/moe/
-__init__.py:8-18).
+__init__.py:8-18), and what it lacks: routing by groups (grouped_topk) and experts on
+4-bit weights (Mxfp4Experts, fused_experts_mxfp4).
 """
 
 import importlib
@@ -11,11 +12,12 @@ import torch
 
 from reframework_amd import _capi
 from reframework_amd.moe import fused as _fused
-from reframework_amd.moe.fused import fused_experts, torch_fused_topk
+from reframework_amd.moe.fused import (fused_experts, fused_experts_mxfp4, grouped_topk,
+                                       torch_fused_topk)
 from reframework_amd.moe.moe_layer import CpuShuttle, FusedMoE
 from reframework_amd.moe.offload_cache import (ExpertOffloadCache, ExpertPool, OffloadStats,
                                                Prediction)
-
+from reframework_amd.mx import Mxfp4Experts, Mxfp8Rows, quantize_mxfp8
 
 
 def available() -> bool:
@@ -80,7 +82,12 @@ __all__ = [
     "available",
     "install",
     "torch_fused_topk",
+    "grouped_topk",
     "fused_experts",
+    "fused_experts_mxfp4",
+    "Mxfp4Experts",
+    "Mxfp8Rows",
+    "quantize_mxfp8",
     "FusedMoE",
     "CpuShuttle",
     "ExpertOffloadCache",

@@ -13,6 +13,10 @@ Same call surface as the reference's module (reframework/moe/fused.py):
     topk_weights, topk_ids, active, activation)`` -> fp32 [M,H] on the host:
     the split's CPU half on int8 banks (fused.py:140-197), run by
     libmoe355_host.
+  * ``grouped_topk(gating_output, topk, renormalize, ...)``: routing with softmax or
+    sigmoid scores, a bias for the choice and groups of experts (not in the reference).
+  * ``fused_experts_mxfp4(hidden_states, experts, ...)``: fused_experts on 4-bit
+    weights and 8-bit rows (mx.Mxfp4Experts, mx.Mxfp8Rows; not in the reference).
 
 The reference loops over experts in Python (gather, two torch.mm, activation,
 scale, index_add_). Here one C call runs the whole thing on the current HIP
@@ -33,6 +37,7 @@ import torch
 
 from reframework_amd import _capi
 from reframework_amd.layers import activation_code
+from reframework_amd.mx import Mxfp4Experts, Mxfp8Rows, _aligned
 
 Bank = Union[torch.Tensor, Sequence[torch.Tensor]]
 
@@ -87,6 +92,59 @@ def torch_fused_topk(
     _capi.topk_from_logits(logits, topk, renormalize, w, ids)
     shape = tuple(gating_output.shape[:-1]) + (topk,)
     return w.reshape(shape), ids.long().reshape(shape)
+
+
+def grouped_topk(
+    gating_output: torch.Tensor,  # [..., E] router logits
+    topk: int,
+    renormalize: bool = True,
+    scoring: str = "softmax",
+    bias: Optional[torch.Tensor] = None,  # [E], for the choice alone
+    num_groups: int = 1,
+    topk_groups: int = 1,
+    group_score: str = "max",
+    scale: float = 1.0,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Routing by groups: (weights fp32 [..., topk], ids int64 [..., topk]).
+
+    Scores ``s`` are the ``"softmax"`` or ``"sigmoid"`` of the logits, ``c = s + bias``
+    the choice. The ``num_groups`` runs of consecutive experts are scored by their best
+    ``c`` (``"max"``) or the sum of their best two (``"top2"``); the ``topk_groups`` best
+    groups stay, and of their experts the ``topk`` of largest ``c`` are chosen, in
+    descending order. The weights are their ``s``, over their sum if ``renormalize``,
+    times ``scale``. The ids are those of exact arithmetic on the fp32 logits and bias;
+    ties go to the lower group and the lower expert, a NaN ranks last. At most 64
+    groups and a topk of 64."""
+    require_gpu(gating_output, "gating_output")
+    E = gating_output.shape[-1]
+    logits = gating_output.detach().reshape(-1, E).float().contiguous()
+    w = torch.empty((logits.shape[0], topk), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((logits.shape[0], topk), dtype=torch.int64, device=logits.device)
+    run_grouped_topk(logits, bias, renormalize, scoring, num_groups, topk_groups, group_score,
+                     scale, topk, w, ids)
+    if gating_output.dim() == 2:
+        return w, ids
+    shape = tuple(gating_output.shape[:-1]) + (topk,)
+    return w.reshape(shape), ids.reshape(shape)
+
+
+def run_grouped_topk(logits: torch.Tensor, bias: Optional[torch.Tensor], renormalize: bool,
+                     scoring: str, num_groups: int, topk_groups: int, group_score: str,
+                     scale: float, topk: int, w: torch.Tensor, ids: torch.Tensor) -> None:
+    """grouped_topk of fp32 ``logits`` [T, E] into the first ``topk`` columns of ``w``
+    and ``ids`` [T, ld] (fp32; int32 or int64)."""
+    for what, name, known in (("scoring", scoring, _capi.SCORE_CODES),
+                              ("group score", group_score, _capi.GROUP_SCORE_CODES)):
+        if name not in known:
+            raise ValueError(f"unknown {what} {name!r}; known: {tuple(known)}")
+    E = logits.shape[1]
+    if bias is not None:
+        if bias.numel() != E or bias.device != logits.device:
+            raise ValueError(f"bias {tuple(bias.shape)} on {bias.device} does not match {E} experts "
+                             f"on {logits.device}")
+        bias = bias.detach().reshape(E).float().contiguous()
+    _capi.grouped_topk(logits, bias, topk, _capi.SCORE_CODES[scoring], num_groups, topk_groups,
+                       _capi.GROUP_SCORE_CODES[group_score], renormalize, scale, w, ids)
 
 
 def run_experts(
@@ -162,6 +220,75 @@ def fused_experts(
     w = topk_weights.reshape(M, -1).float().contiguous()
     out = run_experts(x, w1_ptrs, w2_ptrs, I, w, ids, act)
     return out if out.dtype == hidden_states.dtype else out.to(hidden_states.dtype)
+
+
+def fused_experts_mxfp4(
+    hidden_states: Union[torch.Tensor, Mxfp8Rows],  # [M, H]
+    experts: Mxfp4Experts,
+    topk_weights: torch.Tensor,  # [M, K] fp32
+    topk_ids: torch.Tensor,  # [M, K] int64 (or int32)
+    activation: str = "silu",
+    out: Optional[torch.Tensor] = None,
+    accumulate_f32: bool = False,
+    out_dtype: Optional[torch.dtype] = None,
+) -> torch.Tensor:
+    """fused_experts on 4-bit weights: ``[M, H]``, summed over the K slots.
+
+    Tokens go through gate|up in 8 bits (``hidden_states`` quantised first unless they
+    are Mxfp8Rows, e.g. of RMSNorm.forward_add_residual_mxfp8) and the gated activation
+    through down in 8 bits. The result is of ``out_dtype``: the tokens' type, bfloat16
+    for Mxfp8Rows. A bfloat16 result takes the scaled MFMA, whose products keep about
+    14 bits below the largest they are added to; float16 and float32 results take exact
+    products. Slots whose id lies outside the experts or whose weight is 0 add nothing.
+    With ``accumulate_f32`` the result is added to the fp32 ``out``."""
+    act = activation_code(activation)
+    rows = hidden_states if isinstance(hidden_states, Mxfp8Rows) else None
+    if rows is None:
+        require_gpu(hidden_states, "hidden_states")
+        if hidden_states.dim() != 2:
+            raise ValueError(f"hidden_states are [M, H], not {tuple(hidden_states.shape)}")
+        M, H = hidden_states.shape
+        x = _aligned(hidden_states.detach().contiguous())
+        _capi.dtype_code(x.dtype)
+        if out_dtype not in (None, x.dtype):
+            raise ValueError(f"out_dtype {out_dtype} differs from the tokens' {x.dtype}")
+        dtype, x_scales = x.dtype, None
+    else:
+        M, H = len(rows), rows.size
+        x, x_scales = rows.padded_codes, rows.padded_scales
+        dtype = out_dtype or torch.bfloat16
+    dev = x.device
+    E, I = experts.num_experts, experts.intermediate_size
+    if H != experts.hidden_size:
+        raise ValueError(f"hidden size {H} does not match the experts' {experts.hidden_size}")
+    b = experts._buffers
+    if b["w1"].device != dev or topk_weights.device != dev or topk_ids.device != dev:
+        raise ValueError(f"experts on {b['w1'].device}, weights on {topk_weights.device} and ids on "
+                         f"{topk_ids.device} must be on the tokens' {dev}")
+    if topk_ids.numel() != topk_weights.numel() or (M and topk_ids.numel() % M):
+        raise ValueError(f"topk_ids {tuple(topk_ids.shape)} and topk_weights "
+                         f"{tuple(topk_weights.shape)} are not [{M}, K]")
+    out_type = torch.float32 if accumulate_f32 else dtype
+    if out is None:
+        if accumulate_f32:
+            raise ValueError("accumulate_f32 adds to an fp32 out")
+        out = torch.empty((M, H), dtype=out_type, device=dev)
+    elif out.dtype != out_type or tuple(out.shape) != (M, H) or out.device != dev or \
+            not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {out_type} [{M}, {H}] on {dev}")
+    if M == 0:
+        return out
+    ids = topk_ids if topk_ids.dtype in (torch.int32, torch.int64) else topk_ids.long()
+    ids = ids.reshape(M, -1).contiguous()
+    w = topk_weights.detach().reshape(M, -1).float().contiguous()
+    code = _capi.dtype_code(dtype)
+    # From the caching allocator on the current stream, not from a buffer that calls
+    # share: captured graphs then have workspaces of their own.
+    ws = torch.empty(_capi.mx_workspace_bytes(M, H, I, E, ids.shape[1], code, dev),
+                     dtype=torch.uint8, device=dev)
+    _capi.mx_fused_experts(x, x_scales, H, I, E, b["w1"], b["w1_scales"], b["w2"], b["w2_scales"],
+                           w, ids, code, act, out, accumulate_f32, ws)
+    return out
 
 
 def fused_experts_masked(
@@ -262,5 +389,6 @@ def fused_experts_cpu_int8(
     return out
 
 
-__all__ = ["torch_fused_topk", "fused_experts", "fused_experts_masked", "fused_experts_cpu_int8",
-           "run_experts", "bank_pointers", "require_gpu"]
+__all__ = ["torch_fused_topk", "grouped_topk", "fused_experts", "fused_experts_mxfp4",
+           "fused_experts_masked", "fused_experts_cpu_int8", "run_experts", "run_grouped_topk",
+           "bank_pointers", "require_gpu"]

@@ -1,0 +1,153 @@
+"""GPU routing by groups against 64-bit arithmetic.
+
+Bars: the ids are those of exact arithmetic, ties to the lower. A weight is a score
+(exp within 2 units of 2^-23, two roundings of 2^-24, for softmax a sum of positive
+terms of the same errors) over a sum of scores: at most 2^-20 relative in all.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import _mx_ref as ref
+from _helpers import banner
+from reframework_amd import _capi
+from reframework_amd.moe import grouped_topk, torch_fused_topk
+
+pytestmark = pytest.mark.gpu
+TOL = 2.0 ** -20
+
+
+def _check(logits, K, dev, bias=None, **kw):
+    w, ids = grouped_topk(torch.from_numpy(logits).to(dev), K,
+                          bias=None if bias is None else torch.from_numpy(bias).to(dev), **kw)
+    rw, rids = ref.grouped_topk(logits, K, bias=bias, **kw)
+    assert w.dtype == torch.float32 and ids.dtype == torch.int64
+    assert np.array_equal(ids.cpu().numpy(), rids)
+    got = ref.to64(w)
+    assert np.array_equal(np.isnan(got), np.isnan(rw))
+    fin = ~np.isnan(rw)
+    assert np.all(np.abs(got - rw)[fin] <= TOL * np.abs(rw)[fin] + 1e-30)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("T,E,K,G,KG,score", [
+    (1, 1, 1, 1, 1, "max"), (5, 8, 2, 1, 1, "max"), (33, 64, 6, 8, 3, "max"),
+    (19, 160, 6, 8, 3, "max"), (130, 256, 8, 8, 4, "top2"), (7, 60, 4, 12, 5, "top2"),
+    (9, 96, 12, 3, 2, "top2"), (4, 256, 64, 2, 1, "max"), (6, 64, 3, 64, 5, "top2"),
+    (3, 256, 5, 64, 2, "max"), (11, 255, 9, 17, 2, "top2"), (8, 34, 2, 17, 1, "top2"),
+])
+def test_matches_64_bit(T, E, K, G, KG, score, with_bias, scoring, dev):
+    banner(f"grouped_topk T={T} E={E} K={K} G={G}/{KG} {score} {scoring} bias={with_bias}")
+    rng = np.random.default_rng(E * 7 + T)
+    logits = (rng.normal(size=(T, E)) * 1.5).astype(np.float32)
+    bias = (rng.normal(size=E) * 0.1).astype(np.float32) if with_bias else None
+    for renorm, scale in ((True, 1.0), (False, 2.5)):
+        _check(logits, K, dev, bias=bias, renormalize=renorm, scoring=scoring, num_groups=G,
+               topk_groups=KG, group_score=score, scale=scale)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("G,KG,score", [(1, 1, "max"), (8, 3, "max"), (8, 3, "top2")])
+def test_ties_and_near_ties(G, KG, score, scoring, dev):
+    """Rounded logits (equal ones are common), a bias of few distinct values, and
+    choices whose distance is below a step of 32 bits."""
+    banner(f"grouped_topk ties {scoring} G={G} {score}")
+    rng = np.random.default_rng(11)
+    E, T = 64, 200
+    logits = np.round(rng.normal(size=(T, E)) * 4).astype(np.float32) / 4
+    for bias in (None, np.zeros(E, np.float32), (rng.integers(0, 3, E) / 8).astype(np.float32)):
+        _check(logits, 6, dev, bias=bias, scoring=scoring, num_groups=G, topk_groups=KG,
+               group_score=score)
+    # distances of some 1e-9: every choice is left to 64 bits
+    close = (1.0 + rng.integers(0, 40, (T, E)) * 2.0 ** -23).astype(np.float32)
+    _check(close, 6, dev, bias=np.full(E, 0.25, np.float32), scoring=scoring, num_groups=G,
+           topk_groups=KG, group_score=score)
+    # a bias that outweighs the scores: their bits are below its last one
+    _check(logits, 6, dev, bias=np.full(E, 3.0e4, np.float32), scoring=scoring, num_groups=G,
+           topk_groups=KG, group_score=score)
+    # saturated scores
+    _check((logits * 30).astype(np.float32), 6, dev, bias=np.zeros(E, np.float32),
+           scoring="sigmoid", num_groups=G, topk_groups=KG, group_score=score)
+
+
+def test_nan_and_infinities_keep_ids_in_range(dev):
+    banner("grouped_topk NaN / infinities")
+    rng = np.random.default_rng(3)
+    E = 32
+    logits = rng.normal(size=(12, E)).astype(np.float32)
+    logits[0, :] = np.nan
+    logits[1, 5] = np.nan
+    logits[2, 3:9] = -np.inf
+    logits[3, :] = -np.inf
+    logits[4, 7] = np.inf
+    logits[5, 8:] = np.nan
+    logits[6, 8:] = np.finfo(np.float32).min
+    logits[7, ::2] = -np.inf
+    bias = (rng.normal(size=E) * 0.1).astype(np.float32)
+    for b in (None, bias):
+        for scoring in ("sigmoid", "softmax"):
+            for G, KG, score in ((1, 1, "max"), (4, 2, "max"), (4, 2, "top2")):
+                w, ids = grouped_topk(torch.from_numpy(logits).to(dev), 9, scoring=scoring,
+                                      bias=None if b is None else torch.from_numpy(b).to(dev),
+                                      num_groups=G, topk_groups=KG, group_score=score)
+                got = ids.cpu().numpy()
+                assert got.min() >= 0 and got.max() < E
+                assert all(len(set(r)) == 9 for r in got.tolist())
+        rows = [1, 2, 6, 7, 8, 9, 10, 11]
+        _check(logits[rows], 9, dev, bias=b, scoring="sigmoid", num_groups=4, topk_groups=2)
+
+
+def test_strides_types_and_empty(dev):
+    banner("grouped_topk layouts")
+    g = torch.Generator().manual_seed(0)
+    big = torch.randn(3, 5, 128, generator=g)
+    w, ids = grouped_topk(big.to(dev)[:, :, ::2], 4, num_groups=4, topk_groups=2)
+    rw, rids = ref.grouped_topk(big[:, :, ::2].reshape(15, 64).numpy(), 4, num_groups=4,
+                                topk_groups=2)
+    assert ids.shape == (3, 5, 4) and np.array_equal(ids.cpu().numpy().reshape(15, 4), rids)
+    # 16-bit logits are widened exactly
+    h = torch.randn(9, 64, generator=g).bfloat16()
+    w, ids = grouped_topk(h.to(dev), 4, scoring="sigmoid", num_groups=4, topk_groups=2)
+    assert np.array_equal(ids.cpu().numpy(),
+                          ref.grouped_topk(h.float().numpy(), 4, scoring="sigmoid", num_groups=4,
+                                           topk_groups=2)[1])
+    w, ids = grouped_topk(torch.empty((0, 64), device=dev), 4)
+    assert w.shape == (0, 4) and ids.shape == (0, 4)
+    # columns past K, and int32 ids
+    lg = torch.randn(10, 64, generator=g).to(dev)
+    wl = torch.full((10, 7), -1.0, device=dev)
+    il = torch.full((10, 7), -5, dtype=torch.int32, device=dev)
+    _capi.grouped_topk(lg, None, 4, 1, 8, 3, 0, True, 1.0, wl, il)
+    w, ids = grouped_topk(lg, 4, scoring="sigmoid", num_groups=8, topk_groups=3)
+    assert torch.equal(wl[:, :4], w) and torch.equal(il[:, :4].long(), ids)
+    assert bool((wl[:, 4:] == -1).all()) and bool((il[:, 4:] == -5).all())
+
+
+def test_plain_softmax_agrees_with_torch_fused_topk(dev):
+    banner("grouped_topk == torch_fused_topk")
+    lg = torch.randn(65, 64, generator=torch.Generator().manual_seed(1)).to(dev)
+    w, ids = grouped_topk(lg, 6, renormalize=False)
+    w2, ids2 = torch_fused_topk(lg, 6, False)
+    assert torch.equal(ids, ids2)
+    assert float((w - w2).abs().max()) <= 2 * TOL
+
+
+@pytest.mark.parametrize("T,E", [(1, 8), (255, 160), (300, 8), (300, 24), (515, 256), (257, 64)])
+@pytest.mark.parametrize("dt,H", [(torch.bfloat16, 512), (torch.float16, 264), (torch.float32, 256)])
+def test_router_logits(T, E, dt, H, dev):
+    """fp32 sums of H products: H * 2^-24 of their absolute sum bounds any order."""
+    banner(f"router_logits T={T} E={E} H={H} {dt}")
+    g = torch.Generator().manual_seed(T + E)
+    x, gate = torch.randn(T, H, generator=g).to(dt), (torch.randn(E, H, generator=g) * 0.1).to(dt)
+    out = torch.full((T, E), float("nan"), device=dev)
+    _capi.router_logits(x.to(dev), gate.to(dev), False, out)
+    r = ref.to64(x) @ ref.to64(gate).T
+    bound = np.abs(ref.to64(x)) @ np.abs(ref.to64(gate)).T * H * 2.0 ** -24
+    assert np.all(np.abs(ref.to64(out) - r) <= bound)
+    _capi.router_logits(x.to(dev), gate.to(dev), True, out)
+    rnd = out.to(dt).float()
+    assert torch.equal(rnd, out)
