@@ -13,9 +13,13 @@ namespace {
 
 bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 
+// Average rows per active expert up to which the weights are streamed past tiles of
+// at most 64 rows, and up to which tiles of 128 rows run; above, 256 rows.
+constexpr int kMxStreamRows = 40, kMxTile128Rows = 192;
+
 // The stages of one expert call and where their data lies in the workspace.
 struct MxPlan {
-  int rows, n_blocks, tile_rows, max_tiles, down_splits, down_steps;
+  int rows, n_blocks, tiled, tile_rows, max_tiles, down_splits, down_steps;
   int Hp, Ip;
   size_t block_counts, offsets, slot_to_row, row_src, tile_map, xq, xq_scales, inter,
       inter_scales, y, bytes;
@@ -41,13 +45,35 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   p->n_blocks = R <= kPermuteSingleMax ? 1 : static_cast<int>((R + kPermuteChunk - 1) / kPermuteChunk);
   const int active = static_cast<int>(std::max<long long>(1, std::min<long long>(R, E)));
   const long long avg = R / active;
-  p->tile_rows = avg <= 12 ? 16 : avg <= 28 ? 32 : 64;
+  // The tiled kernels address token rows by 32-bit byte offsets whose bit 31 marks
+  // padding.
+  p->tiled = avg > kMxStreamRows && static_cast<long long>(T) * p->Hp < (1ll << 31);
+  p->tile_rows = p->tiled ? (avg > kMxTile128Rows ? 256 : 128) : avg <= 12 ? 16 : avg <= 28 ? 32 : 64;
   p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
-  // Columns of the down projection over workgroups, until there are 512 of them.
   const int steps = p->Ip / kMxStep;
-  const long long groups = static_cast<long long>(p->Hp / kMxSuper) * std::max(p->max_tiles, 1);
   int s = 1;
-  while (s < 8 && groups * s < 512 && steps >= 8 * s) s *= 2;
+  if (p->tiled) {
+    // The columns of the down projection are cut where that leaves its last round of
+    // workgroups shorter: a round takes a workgroup's steps and about 8 more to start
+    // and end, a further plane of y is written and read once.
+    const double est = std::min<double>(p->max_tiles, active * std::max(1.0, static_cast<double>(R) / active / p->tile_rows + 0.5));
+    const long long items = static_cast<long long>((p->Hp + 255) / 256) * static_cast<long long>(est + 0.5);
+    const int cus = device_cu_count();
+    double best = 0.0;
+    for (int c = 1; c <= 4 && steps >= 8 * c; c *= 2) {
+      const double rounds = static_cast<double>((items * c + cus - 1) / cus);
+      const double cost = rounds * ((steps + c - 1) / c + 8.0) * (p->tile_rows / 256.0) +
+                          (c - 1) * static_cast<double>(R) * H * 1.8e-6;
+      if (c == 1 || cost < 0.97 * best) {
+        best = cost;
+        s = c;
+      }
+    }
+  } else {
+    // Columns of the down projection over workgroups, until there are 512 of them.
+    const long long groups = static_cast<long long>(p->Hp / kMxSuper) * std::max(p->max_tiles, 1);
+    while (s < 8 && groups * s < 512 && steps >= 8 * s) s *= 2;
+  }
   p->down_splits = s;
   p->down_steps = (steps + s - 1) / s;
 
@@ -271,14 +297,14 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
   f.w_stride = mx_code_bytes(2 * p.Ip, p.Hp); f.ws_stride = mx_scale_bytes(2 * p.Ip, p.Hp) / 4;
   f.Kp = p.Hp; f.n_super = 2 * p.Ip / kMxSuper;
   f.splits = 1; f.steps_per_split = p.Hp / kMxStep;
-  if (int rc = check_hip(launch_mx_gate_up(f, s), "mx gate_up launch")) return rc;
+  if (int rc = check_hip(p.tiled ? launch_mx_gate_up_tiled(f, s) : launch_mx_gate_up(f, s), "mx gate_up launch")) return rc;
 
   f.x = f.out_codes; f.x_scales = f.out_scales;
   f.w = static_cast<const uint8_t*>(w2); f.w_scales = static_cast<const uint32_t*>(w2_scales);
   f.w_stride = mx_code_bytes(p.Hp, p.Ip); f.ws_stride = mx_scale_bytes(p.Hp, p.Ip) / 4;
   f.Kp = p.Ip; f.n_super = p.Hp / kMxSuper;
   f.splits = p.down_splits; f.steps_per_split = p.down_steps;
-  if (int rc = check_hip(launch_mx_down(f, s), "mx down launch")) return rc;
+  if (int rc = check_hip(p.tiled ? launch_mx_down_tiled(f, s) : launch_mx_down(f, s), "mx down launch")) return rc;
 
   CombineArgs c{};
   c.y = f.y; c.topk_w = topk_w; c.slot_to_row = pa.slot_to_row; c.out = out;

@@ -15,8 +15,11 @@
 // follow each other (4 KB), then the next step's; its scales are one dword per lane
 // and step, byte g for group g, so that a wave working on a supergroup loads all of
 // a step's scales at once and the instruction picks its byte. A gate|up matrix is
-// interleaved by groups (gate 0, up 0, gate 1, up 1, ..): a supergroup then
-// holds one 32-value block of the intermediate. Rows and columns are padded to
+// interleaved so that a supergroup holds one 32-value block of the intermediate: its
+// groups are gate, up, gate, up, and row r of the first (second) pair is feature
+// 8 (r / 4) + r % 4 (+ 4) of the block. The matrix core leaves rows 4 q .. 4 q + 3 of
+// every group in lane q of a token, which so has features 8 q .. 8 q + 7, gate and
+// up, and stores their codes as 8 consecutive bytes. Rows and columns are padded to
 // multiples of 128 with zeros.
 #pragma once
 
@@ -103,6 +106,8 @@ struct MxFfnArgs {
 
 hipError_t launch_mx_gate_up(const MxFfnArgs& a, hipStream_t s);
 hipError_t launch_mx_down(const MxFfnArgs& a, hipStream_t s);
+hipError_t launch_mx_gate_up_tiled(const MxFfnArgs& a, hipStream_t s);
+hipError_t launch_mx_down_tiled(const MxFfnArgs& a, hipStream_t s);
 hipError_t launch_mx_quantize(const MxQuantArgs& a, int dtype, hipStream_t s);
 // dtype -1: src holds codes.
 hipError_t launch_mx_pack(const MxPackArgs& a, int dtype, hipStream_t s);

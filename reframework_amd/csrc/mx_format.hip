@@ -66,7 +66,8 @@ __global__ __launch_bounds__(kThreads) void mx_pack_kernel(const MxPackArgs a) {
   int row;
   bool in;
   if (a.gate_up) {
-    const int half = a.rows / 2, f = (group >> 1) * 16 + r;
+    const int half = a.rows / 2;
+    const int f = (group >> 2) * kMxBlock + 8 * (r >> 2) + 4 * ((group >> 1) & 1) + (r & 3);
     in = f < half;
     row = (group & 1) * half + f;
   } else {

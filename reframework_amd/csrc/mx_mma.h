@@ -1,0 +1,75 @@
+// The matrix products of 4-bit weights and 8-bit tokens and the epilogue of gate|up,
+// shared by the weight-streaming (ffn_mx.hip) and the tiled kernels
+// (ffn_mx_tiled.hip). Included inside their anonymous namespaces.
+#pragma once
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// One 16-row tile times 16 tokens over 128 columns on the scaled MFMA: the
+// instruction applies the blocks' scales. It aligns a step's products to their
+// largest and keeps about 14 bits below it (measured: an error of 5e-6 of the
+// result's typical size for normal data, far below the rounding of a bf16 result);
+// sums over the steps are in fp32.
+template <int g>
+__device__ __forceinline__ f32x4 mma_scaled(u32x4 w, uint32_t ws, const u32x4* x, uint32_t xs, f32x4 c) {
+  const i32x8 a = {static_cast<int>(w[0]), static_cast<int>(w[1]), static_cast<int>(w[2]),
+                   static_cast<int>(w[3]), 0, 0, 0, 0};
+  const i32x8 b = {static_cast<int>(x[0][0]), static_cast<int>(x[0][1]), static_cast<int>(x[0][2]),
+                   static_cast<int>(x[0][3]), static_cast<int>(x[1][0]), static_cast<int>(x[1][1]),
+                   static_cast<int>(x[1][2]), static_cast<int>(x[1][3])};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, /*A e2m1*/ 4, /*B e4m3*/ 0, g,
+                                                          static_cast<int>(ws), 0,
+                                                          static_cast<int>(xs));
+}
+
+// The same product in bf16, which holds every code times its scale exactly (4
+// significant bits at most), summed in fp32: for results of more bits than bf16.
+// Lane (r, q) multiplies columns 32 q + 8 j .. + 7 in the j-th of four MFMAs (the
+// order of columns is free as long as both operands share it).
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ bf16x8 join(bf16x2 a, bf16x2 b, bf16x2 c, bf16x2 d) {
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+__device__ __forceinline__ bf16x8 weights_bf16(uint32_t w, float s) {
+  return join(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0),
+              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1),
+              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2),
+              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+}
+
+__device__ __forceinline__ bf16x8 tokens_bf16(uint32_t lo, uint32_t hi, float s) {
+  return join(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false),
+              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true),
+              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false),
+              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
+}
+
+// The gated activation of one supergroup for one token, in 8 bits: lane q holds
+// features 8 q .. 8 q + 7 of the block (v: gate, up of the lower four, then of the
+// upper four), whose maximum is over the token's four lanes.
+template <bool kExact>
+__device__ __forceinline__ void store_block(const MxFfnArgs& a, const f32x4* v, int sg, int row,
+                                            int row_end, int q) {
+  float h[8], amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float g = v[i / 4 * 2][i % 4], u = v[i / 4 * 2 + 1][i % 4];
+    h[i] = (kExact ? gate_act(a.act, g) : gate_act_fast(a.act, g)) * u;
+    amax = fmaxf(amax, mx_finite_abs(h[i]));
+  }
+  amax = fmaxf(amax, __shfl_xor(amax, 16, kWave));
+  amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
+  const int b = mx8_scale(amax);
+  const float f = mx_inverse(b);
+  if (row < row_end) {
+    *reinterpret_cast<u32x2*>(a.out_codes + static_cast<size_t>(row) * a.Ip + sg * kMxBlock + 8 * q) =
+        u32x2{mx8_codes(h[0] * f, h[1] * f, h[2] * f, h[3] * f),
+              mx8_codes(h[4] * f, h[5] * f, h[6] * f, h[7] * f)};
+    if (q == 0)
+      a.out_scales[static_cast<size_t>(row) * (a.Ip / kMxBlock) + sg] = static_cast<uint8_t>(b);
+  }
+}

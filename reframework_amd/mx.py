@@ -222,8 +222,8 @@ class Mxfp4Experts(torch.nn.Module):
         s = self._buffers[name + "_scales"].reshape(E, rows_p // 64, cols_p // STEP, 4, 16, 4)
         c = c.permute(0, 1, 3, 5, 2, 4, 6).reshape(E, rows_p, cols_p // 2)
         s = s.permute(0, 1, 5, 4, 2, 3).reshape(E, rows_p, cols_p // BLOCK)
-        if gate_up:  # groups of 16 rows alternate between gate and up
-            c, s = (t.reshape(E, rows_p // 32, 2, 16, -1).transpose(1, 2)
+        if gate_up:  # per block: (four feature runs of 4), gate / up, (feature 8 q + 4 j + i)
+            c, s = (t.reshape(E, rows_p // 64, 2, 2, 4, 4, -1).permute(0, 3, 1, 4, 2, 5, 6)
                     .reshape(E, 2, rows_p // 2, -1)[:, :, :rows // 2].reshape(E, rows, -1)
                     for t in (c, s))
         return (c[:, :rows, :cols // 2].contiguous(), s[:, :rows, :cols // BLOCK].contiguous())
