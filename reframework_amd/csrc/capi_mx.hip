@@ -14,12 +14,16 @@ namespace {
 bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 
 // Average rows per active expert up to which the weights are streamed past tiles of
-// at most 64 rows, and up to which tiles of 128 rows run; above, 256 rows.
-constexpr int kMxStreamRows = 40, kMxTile128Rows = 192;
+// at most 64 rows (ffn_mx.hip), and up to which the tiled kernels (ffn_mx_tiled.hip)
+// take tiles of 64 rows; above, 256. gate|up + down us of 64 / 256-row tiles, 8
+// experts of H 4096, I 14336: 128 rows 280 / 385, 160 rows 369 / 380, 192 rows 396 / 385,
+// 256 rows 468 / 425; 64 experts of H 2048, I 1408: 128 rows 92 / 122, 192 rows 132 / 131,
+// 256 rows 170 / 143, 512 rows 403 / 298.
+constexpr int kMxStreamRows = 24, kMxTile64Rows = 176;
 
 // The stages of one expert call and where their data lies in the workspace.
 struct MxPlan {
-  int rows, n_blocks, tiled, tile_rows, max_tiles, down_splits, down_steps;
+  int rows, n_blocks, tiled, tile_rows, max_tiles, down_splits, down_steps, y16;
   int Hp, Ip;
   size_t block_counts, offsets, slot_to_row, row_src, tile_map, xq, xq_scales, inter,
       inter_scales, y, bytes;
@@ -48,24 +52,32 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   // The tiled kernels address token rows by 32-bit byte offsets whose bit 31 marks
   // padding.
   p->tiled = avg > kMxStreamRows && static_cast<long long>(T) * p->Hp < (1ll << 31);
-  p->tile_rows = p->tiled ? (avg > kMxTile128Rows ? 256 : 128) : avg <= 12 ? 16 : avg <= 28 ? 32 : 64;
+  p->tile_rows = p->tiled ? (avg > kMxTile64Rows ? 256 : 64) : avg <= 12 ? 16 : avg <= 28 ? 32 : 64;
   p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
+  // A bf16 call of several slots per token keeps their results in bf16 until they are
+  // weighed and added: half the bytes, and a rounding that the sum over the slots
+  // makes smaller than the result's own.
+  const bool narrow = p->tiled && dtype == MOE355_BF16 && K > 1;
   const int steps = p->Ip / kMxStep;
   int s = 1;
   if (p->tiled) {
-    // The columns of the down projection are cut where that leaves its last round of
-    // workgroups shorter: a round takes a workgroup's steps and about 8 more to start
-    // and end, a further plane of y is written and read once.
-    const double est = std::min<double>(p->max_tiles, active * std::max(1.0, static_cast<double>(R) / active / p->tile_rows + 0.5));
+    // The columns of the down projection are cut where that shortens its rounds of
+    // workgroups by more than the planes of y cost: a step of a CU takes 1.25 us on
+    // 256-row tiles and 0.85 on 64-row ones, an item 3 steps more, y 5 TB/s (us with 1 /
+    // 2 / 4 parts: 8 experts of I 14336 at 49 rows 92 / 54 / 53, at 1085 rows 444 / 434 / 498;
+    // 12 of H 1280, I 3328 at 83 rows 20.8 / 14.7 / 16.0).
+    const double fill = static_cast<double>(R) / active / p->tile_rows;
+    const double est = std::min<double>(p->max_tiles, active * (fill < 0.8 ? 1.0 : fill + 0.5));
     const long long items = static_cast<long long>((p->Hp + 255) / 256) * static_cast<long long>(est + 0.5);
     const int cus = device_cu_count();
     double best = 0.0;
-    for (int c = 1; c <= 4 && steps >= 8 * c; c *= 2) {
+    for (int c = 1; c <= 4 && steps >= 4 * c; c *= 2) {
       const double rounds = static_cast<double>((items * c + cus - 1) / cus);
-      const double cost = rounds * ((steps + c - 1) / c + 8.0) * (p->tile_rows / 256.0) +
-                          (c - 1) * static_cast<double>(R) * H * 1.8e-6;
-      if (c == 1 || cost < 0.97 * best) {
-        best = cost;
+      const double y_bytes = c == 1 && narrow ? 4.0 : 8.0 * c;
+      const double us = rounds * ((steps + c - 1) / c + 3.0) * (p->tile_rows == 256 ? 1.25 : 0.85) +
+                        static_cast<double>(R) * H * y_bytes / 5e6;
+      if (c == 1 || us < 0.97 * best) {
+        best = us;
         s = c;
       }
     }
@@ -75,6 +87,7 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
     while (s < 8 && groups * s < 512 && steps >= 8 * s) s *= 2;
   }
   p->down_splits = s;
+  p->y16 = narrow && s == 1;
   p->down_steps = (steps + s - 1) / s;
 
   size_t off = 0;
@@ -92,7 +105,7 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   p->xq_scales = take(static_cast<size_t>(T) * p->Hp / kMxBlock);
   p->inter = take(static_cast<size_t>(R) * p->Ip);
   p->inter_scales = take(static_cast<size_t>(R) * p->Ip / kMxBlock);
-  p->y = take(static_cast<size_t>(p->down_splits) * R * H * 4);
+  p->y = take(static_cast<size_t>(p->down_splits) * R * H * (p->y16 ? 2 : 4));
   p->bytes = off;
   return MOE355_OK;
 }
@@ -279,6 +292,7 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
   pa.tile_rows = p.tile_rows; pa.max_tiles = p.max_tiles;
   pa.ids_int64 = ids_int64 != 0;
   pa.weights = topk_w;
+  pa.full_tiles = 1;
   if (int rc = check_hip(launch_permute(pa, s), "permute launch")) return rc;
 
   MxFfnArgs f{};
@@ -290,7 +304,8 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
   f.exact = dtype != MOE355_BF16;
   f.out_codes = at<uint8_t>(workspace, p.inter);
   f.out_scales = at<uint8_t>(workspace, p.inter_scales);
-  f.y = at<float>(workspace, p.y);
+  f.y = at<void>(workspace, p.y);
+  f.y16 = p.y16;
 
   f.x = xq; f.x_scales = xs;
   f.w = static_cast<const uint8_t*>(w1); f.w_scales = static_cast<const uint32_t*>(w1_scales);
@@ -310,6 +325,7 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
   c.y = f.y; c.topk_w = topk_w; c.slot_to_row = pa.slot_to_row; c.out = out;
   c.T = T; c.K = K; c.H = H; c.R = p.rows; c.splits = p.down_splits;
   c.accumulate = accumulate_f32 != 0;
+  c.y16 = p.y16;
   return check_hip(launch_combine(c, dtype, s), "combine launch");
 }
 

@@ -213,6 +213,7 @@ struct PermuteArgs {
   int ids_int64, map_len;  // map_len 0: no map
   int32_t map[kMaxExperts];
   const float* weights;    // [R] routing weights, or nullptr: a slot of weight 0 is dropped
+  int full_tiles;          // 256-row tiles lie 256 rows apart too (not tile_height)
 };
 
 // Local expert of routed slot `slot`, or -1 when the slot is dropped (an id

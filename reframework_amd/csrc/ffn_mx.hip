@@ -112,16 +112,18 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
   __syncthreads();
   if constexpr (kGateUp) {
     // Token tile m by wave m % 4.
-    for (int m = wave; m < MT; m += kWaves) {
-      f32x4 v[4];
+    by_activation(a.act, [&](auto act) {
+      for (int m = wave; m < MT; m += kWaves) {
+        f32x4 v[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        v[g] = red[0][m][g][lane];
+        for (int g = 0; g < 4; ++g) {
+          v[g] = red[0][m][g][lane];
 #pragma unroll
-        for (int k = 1; k < kWaves; ++k) v[g] += red[k][m][g][lane];
+          for (int k = 1; k < kWaves; ++k) v[g] += red[k][m][g][lane];
+        }
+        store_block<act.value, kExact>(a, v, sg, row0 + 16 * m + (lane & 15), row_end, q);
       }
-      store_block<kExact>(a, v, sg, row0 + 16 * m + (lane & 15), row_end, q);
-    }
+    });
   } else {
     // Group g by wave g.
     const int g = wave, col = sg * kMxSuper + 16 * g + 4 * q;
@@ -132,7 +134,8 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
       for (int k = 1; k < kWaves; ++k) v += red[k][m][g][lane];
       const int r = row0 + 16 * m + (lane & 15);
       if (r < row_end && col < a.H)
-        *reinterpret_cast<f32x4*>(a.y + (static_cast<size_t>(split) * a.R + r) * a.H + col) = v;
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + (static_cast<size_t>(split) * a.R + r) * a.H +
+                                  col) = v;
     }
   }
 }

@@ -1,13 +1,19 @@
 // Grouped expert FFN on 4-bit weights and 8-bit tokens (formats: mx.h) for many tokens
-// per expert: a workgroup multiplies BM token rows of one expert by 256 packed weight
-// rows (4 supergroups: 128 features of gate and up), 128 columns a step.
+// per expert: an item multiplies BM token rows of one expert by 256 packed weight rows
+// (4 supergroups: 128 features of gate and up), 128 columns a step.
 //
 // Tokens (128 bytes a row and step), weights (64) and both scales go straight to
-// LDS, kStages steps deep. Token rows are stored with their 16-byte chunks XORed by
+// LDS, several steps deep. Token rows are stored with their 16-byte chunks XORed by
 // half the row number, which leaves the fragment reads without bank conflicts;
-// weight tiles lie in fragment order already. A wave owns 64 tokens x 128 weight
-// rows: per step it reads 8 KB of each operand for 32 instructions of 32 cycles, so
-// that LDS is read at half of its rate while the matrix cores are busy.
+// weight tiles lie in fragment order already.
+//
+// Eight waves, two per SIMD, work in turns: while the first four multiply a step, the
+// others read theirs from LDS, and a barrier swaps them, so that the matrix cores
+// always have a wave with its operands in registers.
+//
+// A workgroup runs several items, whose steps follow each other in one stream of
+// loads: the first steps of an item are on their way while the item before it is
+// multiplied and stored.
 #include <climits>
 
 #include "dma_pipe.h"
@@ -19,24 +25,27 @@ namespace {
 #include "mx_mma.h"
 
 constexpr int kBN = 256;
-constexpr int kWaveM = 64, kWaveN = 128;
-constexpr int kMT = kWaveM / 16, kNT = kWaveN / 16;
+constexpr int kWaves = 8, kThreads = kWaves * kWave;
+constexpr int kMaxItems = 32;  // items of a workgroup
 
-template <int BM>
+// BM token rows, WM waves over them and 8 / WM over the weight rows; kPerCu workgroups
+// share a CU.
+template <int BM, int WM, int kPerCu>
 struct Shape {
-  static constexpr int kWaves = BM / kWaveM * (kBN / kWaveN);
-  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kMT = BM / WM / 16, kNT = kBN / (kWaves / WM) / 16;  // 16 x 16 tiles of a wave
   static constexpr int kTokBytes = BM * kMxStep;          // codes of the tokens
   static constexpr int kWgtBytes = kBN * kMxStep / 2;     // codes of the weights
   static constexpr int kTokScale = BM * 4;                // a dword per row
   static constexpr int kWgtScale = kBN / kMxSuper * kWave * 4;
   static constexpr int kStage = kTokBytes + kWgtBytes + kTokScale + kWgtScale;
-  static constexpr int kStages = 160 * 1024 / kStage;
-  // direct-to-LDS loads of a wave per step: 1 KB of codes, 256 bytes of scales each
+  static constexpr int kStages = (160 * 1024 / kPerCu - kMaxItems * 16) / kStage;
+  // direct-to-LDS loads of a wave per step: 1 KB of codes each, and 256 bytes of
+  // scales (the weights' four by waves 0-3, the tokens' by the others, some twice)
   static constexpr int kTokLoads = kTokBytes / 1024 / kWaves;
   static constexpr int kWgtLoads = kWgtBytes / 1024 / kWaves;
-  static constexpr int kScaleLoads = BM == 256 ? 1 : 2;
-  static constexpr int kLoads = kTokLoads + kWgtLoads + kScaleLoads;
+  static constexpr int kLoads = kTokLoads + kWgtLoads + 1;
+  static_assert(kNT % 4 == 0 && kMT >= 1 && kTokLoads >= 1 && kWgtLoads >= 1, "whole supergroups");
+  static_assert(kStages >= 3 && (kStages - 1) * kLoads < 64, "pipeline");
 };
 
 __device__ __forceinline__ void dma4_rsrc(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t soff,
@@ -44,81 +53,111 @@ __device__ __forceinline__ void dma4_rsrc(__amdgpu_buffer_rsrc_t r, uint32_t off
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (pipe::lds_void*)(dst), 4, off, soff, 0, 0);
 }
 
-template <bool kGateUp, int BM, bool kExact>
-__global__ __launch_bounds__(Shape<BM>::kThreads) void mx_tiled_kernel(const MxFfnArgs a) {
-  typedef Shape<BM> S;
-  static_assert(S::kStages >= 3 && (S::kStages - 1) * S::kLoads < 64, "pipeline");
+// Item L: weight tile `wt` of the token rows [row0, row_end) of expert e, split z of
+// the columns. The token tiles of an expert vary fastest, so that neighbours (on one
+// XCD) share their weights.
+struct Item {
+  int e_split, row0, row_end, wt;  // e_split: expert + 256 * split
+};
+
+template <int BM>
+__device__ __forceinline__ Item decode_item(const MxFfnArgs& a, int L, int nw, int per_split) {
+  const int split = L / per_split, rem = L - split * per_split;
+  const int t0 = rem / nw;
+  const int e = a.tile_map[2 + 2 * t0];
+  const int eb = a.offsets[e], ee = a.offsets[e + 1];
+  const int b = t0 - (a.tile_map[3 + 2 * t0] - eb) / BM;  // the expert's first tile
+  const int ne = (ee - eb + BM - 1) / BM;
+  const int r2 = rem - b * nw, wt = r2 / ne;
+  const int row0 = eb + (r2 - wt * ne) * BM;
+  return Item{e + 256 * split, row0, min(row0 + BM, ee), wt};
+}
+
+template <bool kGateUp, int BM, int WM, int kPerCu, bool kExact>
+__global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const MxFfnArgs a) {
+  typedef Shape<BM, WM, kPerCu> S;
+  constexpr int kMT = S::kMT, kNT = S::kNT;
   __shared__ __attribute__((aligned(1024))) uint8_t stage[S::kStages][S::kStage];
+  __shared__ Item items[kMaxItems];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int q = lane >> 4, r = lane & 15;
 
-  // Item: weight tile wt of token tile tt, the token tiles of an expert varying
-  // fastest, so that neighbours (on one XCD) share their weights.
+  // This workgroup's items: one of every gridDim.x, the workgroups of an XCD taking
+  // neighbouring ones.
   const int nw = (a.n_super * kMxSuper + kBN - 1) / kBN;
-  const int n_tiles = a.tile_map[0];
-  const int per_split = n_tiles * nw, total = per_split * a.splits;
-  if (static_cast<int>(blockIdx.x) >= total) return;
-  const int item = xcd_remap(blockIdx.x, total);
-  const int split = item / per_split, rem = item - split * per_split;
-  const int t0 = rem / nw;
-  const int e = a.tile_map[2 + 2 * t0];
-  const int eb = a.offsets[e], ee = a.offsets[e + 1];
-  const int height = tile_height(ee - eb, a.tile_rows);
-  const int b = t0 - (a.tile_map[3 + 2 * t0] - eb) / height;
-  const int ne = (ee - eb + a.tile_rows - 1) / a.tile_rows;
-  const int r2 = rem - b * nw;
-  const int wt = r2 / ne;
-  const int row0 = a.tile_map[3 + 2 * (b + r2 - wt * ne)];
-  const int row_end = min(row0 + height, ee);
-
-  const int steps = a.Kp / kMxStep;
-  const int sbeg = min(split * a.steps_per_split, steps);
-  const int n = min(sbeg + a.steps_per_split, steps) - sbeg;
-
-  // Sources. Rows past the tile's last load zeros (an offset that is out of range).
-  const size_t first = kGateUp ? 0 : row0;
-  const __amdgpu_buffer_rsrc_t xsrc = pipe::lds_rsrc(a.x + first * a.Kp);
-  const __amdgpu_buffer_rsrc_t xssrc = pipe::lds_rsrc(a.x_scales + first * (a.Kp / kMxBlock));
-  const int sg0 = wt * (kBN / kMxSuper);
-  const __amdgpu_buffer_rsrc_t wsrc =
-      pipe::lds_rsrc(a.w + e * a.w_stride + static_cast<size_t>(sg0) * steps * 4 * kMxTileBytes);
-  const __amdgpu_buffer_rsrc_t wssrc =
-      pipe::lds_rsrc(a.w_scales + e * a.ws_stride + static_cast<size_t>(sg0) * steps * kWave);
-  auto token = [&](int row) {  // row of x of tile row `row`, or -1
-    const int p = row0 + row;
-    return p >= row_end ? -1 : kGateUp ? a.row_src[p] : row;
+  const int per_split = a.tile_map[0] * nw, total = per_split * a.splits;
+  const int G = gridDim.x, pid = blockIdx.x;
+  const int rounds = total / G, tail = total - rounds * G;
+  const int n_items = rounds + (pid < tail ? 1 : 0);
+  if (n_items == 0) return;
+  if (wave == 0 && lane < n_items)
+    items[lane] = decode_item<BM>(a, lane * G + xcd_remap(pid, lane < rounds ? G : tail), nw, per_split);
+  __syncthreads();
+  auto item_at = [&](int j) {
+    const Item* p = &items[j];
+    return Item{__builtin_amdgcn_readfirstlane(p->e_split), __builtin_amdgcn_readfirstlane(p->row0),
+                __builtin_amdgcn_readfirstlane(p->row_end), __builtin_amdgcn_readfirstlane(p->wt)};
   };
-  // The last weight tile of a matrix of an odd number of 128 rows reads its last
-  // supergroup twice; those results are not stored.
-  auto super = [&](int s) { return min(s, a.n_super - 1 - sg0); };
-  uint32_t xoff[S::kTokLoads], woff[S::kWgtLoads], soff[S::kScaleLoads];
-#pragma unroll
-  for (int i = 0; i < S::kTokLoads; ++i) {
-    const int row = 8 * (wave * S::kTokLoads + i) + (lane >> 3);
-    const int src = token(row);
-    xoff[i] = src < 0 ? pipe::kPadOffset
-                      : static_cast<uint32_t>(src) * a.Kp + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
-  }
-#pragma unroll
-  for (int i = 0; i < S::kWgtLoads; ++i) {
-    const int c = wave * S::kWgtLoads + i;  // tile c % 4 of supergroup c / 4
-    woff[i] = static_cast<uint32_t>(super(c >> 2)) * steps * 4 * kMxTileBytes +
-              (c & 3) * kMxTileBytes + lane * 16;
-  }
-  // Scale loads: the weights' four, then the tokens' (64 rows each). With 8 waves
-  // one each; with 4 waves one of each kind, the tokens' two loaded twice.
-  const bool first_is_token = S::kScaleLoads == 1 && wave >= 4;
-  const int tok64 = S::kScaleLoads == 1 ? wave & 3 : wave & 1;
-  const int ssrc = token(64 * tok64 + lane);
-  const uint32_t tok_scale = ssrc < 0 ? pipe::kPadOffset : static_cast<uint32_t>(ssrc) * (a.Kp / kMxBlock);
-  const uint32_t wgt_scale = (static_cast<uint32_t>(super(wave & 3)) * steps * kWave + lane) * 4;
-  soff[0] = first_is_token ? tok_scale : wgt_scale;
-  if (S::kScaleLoads == 2) soff[S::kScaleLoads - 1] = tok_scale;
+  const int steps = a.Kp / kMxStep;
+  auto first_step = [&](const Item& it) { return (it.e_split >> 8) * a.steps_per_split; };
+  auto n_steps = [&](const Item& it) {
+    return min(first_step(it) + a.steps_per_split, steps) - first_step(it);
+  };
 
-  auto issue = [&](int st) {
-    uint8_t* s = stage[st % S::kStages];
-    const int k = sbeg + st;
+  // Token rows whose codes (kTokLoads of them) and scales this lane loads, as rows of
+  // x; -1 past the tile's last row.
+  const int tok64 = (wave & 3) % (BM / 64);  // 64 tokens whose scales waves 4-7 load
+  int src[S::kTokLoads + 1];
+  auto load_rows = [&](const Item& it) {
+#pragma unroll
+    for (int i = 0; i <= S::kTokLoads; ++i) {
+      const int row = i < S::kTokLoads ? 8 * (wave * S::kTokLoads + i) + (lane >> 3) : 64 * tok64 + lane;
+      const int p = it.row0 + row;
+      src[i] = p >= it.row_end ? -1 : kGateUp ? a.row_src[p] : row;
+    }
+  };
+
+  // The item whose steps are being loaded: sources, and this lane's offsets.
+  __amdgpu_buffer_rsrc_t xsrc, xssrc, wsrc, wssrc;
+  uint32_t xoff[S::kTokLoads], woff[S::kWgtLoads], soff;
+  int load_item = 0, load_step, load_end, loaded = 0;  // loaded: steps of all items
+  auto begin_loads = [&](const Item& it) {
+    const int e = it.e_split & 255;
+    const int sg0 = it.wt * (kBN / kMxSuper);
+    // down: rows are counted from the tile's first, so that offsets stay small
+    const size_t first = kGateUp ? 0 : it.row0;
+    xsrc = pipe::lds_rsrc(a.x + first * a.Kp);
+    xssrc = pipe::lds_rsrc(a.x_scales + first * (a.Kp / kMxBlock));
+    wsrc = pipe::lds_rsrc(a.w + e * a.w_stride + static_cast<size_t>(sg0) * steps * 4 * kMxTileBytes);
+    wssrc = pipe::lds_rsrc(a.w_scales + e * a.ws_stride + static_cast<size_t>(sg0) * steps * kWave);
+    // The last weight tile of a matrix of an odd number of 128 rows reads its last
+    // supergroup again; those results are not stored.
+    const int last = a.n_super - 1 - sg0;
+#pragma unroll
+    for (int i = 0; i < S::kTokLoads; ++i) {
+      const int row = 8 * (wave * S::kTokLoads + i) + (lane >> 3);
+      xoff[i] = src[i] < 0 ? pipe::kPadOffset  // out of range: zeros
+                           : static_cast<uint32_t>(src[i]) * a.Kp + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kWgtLoads; ++i) {
+      const int c = wave * S::kWgtLoads + i;  // tile c % 4 of supergroup c / 4
+      woff[i] = static_cast<uint32_t>(min(c >> 2, last)) * steps * 4 * kMxTileBytes +
+                (c & 3) * kMxTileBytes + lane * 16;
+    }
+    soff = wave < 4 ? (static_cast<uint32_t>(min(wave, last)) * steps * kWave + lane) * 4
+           : src[S::kTokLoads] < 0 ? pipe::kPadOffset
+                                   : static_cast<uint32_t>(src[S::kTokLoads]) * (a.Kp / kMxBlock);
+    load_step = first_step(it);
+    load_end = load_step + n_steps(it);
+    if (load_item + 1 < n_items) load_rows(item_at(load_item + 1));
+  };
+  // Loads the next step of the stream, if there is one.
+  auto load = [&]() {
+    if (load_item >= n_items) return;
+    uint8_t* s = stage[loaded % S::kStages];
+    const int k = load_step;
 #pragma unroll
     for (int i = 0; i < S::kTokLoads; ++i)
       pipe::dma16_rsrc(xsrc, xoff[i], k * kMxStep, s + (wave * S::kTokLoads + i) * 1024);
@@ -127,124 +166,183 @@ __global__ __launch_bounds__(Shape<BM>::kThreads) void mx_tiled_kernel(const MxF
       pipe::dma16_rsrc(wsrc, woff[i], k * 4 * kMxTileBytes,
                        s + S::kTokBytes + (wave * S::kWgtLoads + i) * 1024);
     uint8_t* ts = s + S::kTokBytes + S::kWgtBytes;
-    uint8_t* ws = ts + S::kTokScale;
-    if (first_is_token)
-      dma4_rsrc(xssrc, soff[0], k * (kMxStep / kMxBlock), ts + tok64 * 256);
+    if (wave < 4)
+      dma4_rsrc(wssrc, soff, k * kWave * 4, ts + S::kTokScale + wave * 256);
     else
-      dma4_rsrc(wssrc, soff[0], k * kWave * 4, ws + (wave & 3) * 256);
-    if (S::kScaleLoads == 2)
-      dma4_rsrc(xssrc, soff[S::kScaleLoads - 1], k * (kMxStep / kMxBlock), ts + tok64 * 256);
+      dma4_rsrc(xssrc, soff, k * (kMxStep / kMxBlock), ts + tok64 * 256);
+    ++loaded;
+    if (++load_step == load_end && ++load_item < n_items) begin_loads(item_at(load_item));
+  };
+  // Waits until this wave's loads of step `step` of the stream have landed; of the
+  // steps after it kStages - 2 may be in flight (fewer at the end of the stream, where
+  // it waits for all).
+  auto landed = [&](int step) {
+    if (loaded >= step + S::kStages - 1)
+      pipe::wait_vmcnt<(S::kStages - 2) * S::kLoads>();
+    else
+      pipe::wait_vmcnt<0>();
+  };
+  // All waves; nothing moves across it.
+  auto turn = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  const int wm = wave >> 1, wn = wave & 1;  // this wave's 64 tokens and 128 weight rows
-  f32x4 acc[kMT][kNT];
+  load_rows(item_at(0));
+  begin_loads(item_at(0));
 #pragma unroll
-  for (int m = 0; m < kMT; ++m)
+  for (int i = 0; i < S::kStages - 1; ++i) load();
+  landed(0);
+  turn();
+  // Half-step 2 s: the first waves read step s of the stream, the second multiply step
+  // s - 1; the next half-step the other way round. Before half-step 2 s every wave
+  // has seen its loads of step s land; the buffer of step s - 1 was last read in
+  // half-step 2 s - 1 and is filled again from half-step 2 s on.
+  const bool second = wave >= 4;
+  if (second) turn();
+  int done = 0;  // steps of the stream
+  const int wm = wave % WM, wn = wave / WM;  // this wave's tokens and weight rows
+  for (int j = 0; j < n_items; ++j) {
+    const Item it = item_at(j);
+    const int n = n_steps(it);
+    f32x4 acc[kMT][kNT];
 #pragma unroll
-    for (int g = 0; g < kNT; ++g) acc[m][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-
+    for (int m = 0; m < kMT; ++m)
 #pragma unroll
-  for (int st = 0; st < S::kStages - 1; ++st)
-    if (st < n) issue(st);
-  for (int st = 0; st < n; ++st) {
-    // All but the newest kStages - 2 steps have landed, for every wave; and every wave
-    // has read step st - 1, whose buffer the next load overwrites.
-    pipe::wait_lgkm0();
-    if (st + S::kStages - 1 <= n)
-      pipe::dma_barrier<(S::kStages - 2) * S::kLoads>();
-    else
-      pipe::dma_barrier<0>();
-    if (st + S::kStages - 1 < n) issue(st + S::kStages - 1);
-    const uint8_t* s = stage[st % S::kStages];
-    const uint8_t* wtile = s + S::kTokBytes + wn * (kNT * kMxTileBytes) + lane * 16;
-    const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (wm * kWaveM + r) * 4;
-    const uint8_t* ws = s + S::kTokBytes + S::kWgtBytes + S::kTokScale + wn * 512 + lane * 4;
-    u32x4 w[kNT];
+      for (int g = 0; g < kNT; ++g) acc[m][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // A wave has every WM-th 16 rows of the tile, so that the waves share the rows of
+    // one that is not full; mt of its kMT hold any.
+    const int mt = min((it.row_end - it.row0 + 16 * (WM - 1 - wm) + 15) / (16 * WM), kMT);
+    auto run_steps = [&](auto full) {
+      constexpr bool kFull = decltype(full)::value;
+      for (int st = 0; st < n; ++st, ++done) {
+        const uint8_t* s = stage[done % S::kStages];
+        const uint8_t* wtile = s + S::kTokBytes + wn * (kNT * kMxTileBytes) + lane * 16;
+        const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
+        const uint8_t* ws = s + S::kTokBytes + S::kWgtBytes + S::kTokScale + wn * (kNT / 4 * 256) + lane * 4;
+        u32x4 w[kNT];
+        uint32_t wsc[kNT / 4];
 #pragma unroll
-    for (int g = 0; g < kNT; ++g) w[g] = *reinterpret_cast<const u32x4*>(wtile + g * kMxTileBytes);
-    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(ws);
-    const uint32_t w1 = *reinterpret_cast<const uint32_t*>(ws + 256);
-    u32x4 x[kMT][2];
-    uint32_t xs[kMT];
+        for (int g = 0; g < kNT; ++g) w[g] = *reinterpret_cast<const u32x4*>(wtile + g * kMxTileBytes);
 #pragma unroll
-    for (int m = 0; m < kMT; ++m) {
-      const int row = wm * kWaveM + 16 * m + r, sw = (row >> 1) & 7;
-      const uint8_t* p = s + row * kMxStep;
-      x[m][0] = *reinterpret_cast<const u32x4*>(p + (((kExact ? 2 * q : q) ^ sw) << 4));
-      x[m][1] = *reinterpret_cast<const u32x4*>(p + (((kExact ? 2 * q + 1 : 4 + q) ^ sw) << 4));
-      xs[m] = *reinterpret_cast<const uint32_t*>(ts + 64 * m) >> (8 * q);
-    }
-    if constexpr (kExact) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bf16x8 wb[kNT];
-#pragma unroll
-        for (int g = 0; g < kNT; ++g)
-          wb[g] = weights_bf16(w[g][j], scale_of(((g < 4 ? w0 : w1) >> (8 * (g & 3))) & 0xffu));
+        for (int h = 0; h < kNT / 4; ++h) wsc[h] = *reinterpret_cast<const uint32_t*>(ws + 256 * h);
+        u32x4 x[kMT][2];
+        uint32_t xs[kMT];
 #pragma unroll
         for (int m = 0; m < kMT; ++m) {
-          const bf16x8 t = tokens_bf16(x[m][j / 2][2 * (j % 2)], x[m][j / 2][2 * (j % 2) + 1],
-                                       scale_of(xs[m] & 0xffu));
-#pragma unroll
-          for (int g = 0; g < kNT; ++g)
-            acc[m][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[g], t, acc[m][g], 0, 0, 0);
+          if (!kFull && m >= mt) continue;
+          const int row = 16 * (wm + WM * m) + r, sw = (row >> 1) & 7;
+          const uint8_t* p = s + row * kMxStep;
+          x[m][0] = *reinterpret_cast<const u32x4*>(p + (((kExact ? 2 * q : q) ^ sw) << 4));
+          x[m][1] = *reinterpret_cast<const u32x4*>(p + (((kExact ? 2 * q + 1 : 4 + q) ^ sw) << 4));
+          xs[m] = *reinterpret_cast<const uint32_t*>(ts + 64 * WM * m) >> (8 * q);
         }
+        load();
+        if (second) landed(done + 1);
+        pipe::wait_lgkm0();
+        turn();
+        if constexpr (kExact) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            bf16x8 wb[kNT];
+#pragma unroll
+            for (int g = 0; g < kNT; ++g)
+              wb[g] = weights_bf16(w[g][i], scale_of((wsc[g / 4] >> (8 * (g & 3))) & 0xffu));
+#pragma unroll
+            for (int m = 0; m < kMT; ++m) {
+              if (!kFull && m >= mt) continue;
+              const bf16x8 t = tokens_bf16(x[m][i / 2][2 * (i % 2)], x[m][i / 2][2 * (i % 2) + 1],
+                                           scale_of(xs[m] & 0xffu));
+#pragma unroll
+              for (int g = 0; g < kNT; ++g)
+                acc[m][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[g], t, acc[m][g], 0, 0, 0);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int m = 0; m < kMT; ++m) {
+            if (!kFull && m >= mt) continue;
+#pragma unroll
+            for (int h = 0; h < kNT / 4; ++h) {
+              acc[m][4 * h + 0] = mma_scaled<0>(w[4 * h + 0], wsc[h], x[m], xs[m], acc[m][4 * h + 0]);
+              acc[m][4 * h + 1] = mma_scaled<1>(w[4 * h + 1], wsc[h], x[m], xs[m], acc[m][4 * h + 1]);
+              acc[m][4 * h + 2] = mma_scaled<2>(w[4 * h + 2], wsc[h], x[m], xs[m], acc[m][4 * h + 2]);
+              acc[m][4 * h + 3] = mma_scaled<3>(w[4 * h + 3], wsc[h], x[m], xs[m], acc[m][4 * h + 3]);
+            }
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (!second) landed(done + 1);
+        turn();
       }
+    };
+    if (it.row_end - it.row0 > BM - 16 * WM)
+      run_steps(std::true_type());
+    else
+      run_steps(std::false_type());
+
+    const int row1 = it.row0 + 16 * wm + r;
+    if constexpr (kGateUp) {
+      by_activation(a.act, [&](auto act) {
+#pragma unroll
+        for (int m = 0; m < kMT; ++m) {
+          if (m >= mt) continue;
+#pragma unroll
+          for (int h = 0; h < kNT / 4; ++h)
+            store_block<act.value, kExact>(a, &acc[m][4 * h],
+                                           it.wt * (kBN / kMxSuper) + wn * (kNT / 4) + h,
+                                           row1 + 16 * WM * m, it.row_end, q);
+        }
+      });
     } else {
 #pragma unroll
       for (int m = 0; m < kMT; ++m) {
-        acc[m][0] = mma_scaled<0>(w[0], w0, x[m], xs[m], acc[m][0]);
-        acc[m][1] = mma_scaled<1>(w[1], w0, x[m], xs[m], acc[m][1]);
-        acc[m][2] = mma_scaled<2>(w[2], w0, x[m], xs[m], acc[m][2]);
-        acc[m][3] = mma_scaled<3>(w[3], w0, x[m], xs[m], acc[m][3]);
-        acc[m][4] = mma_scaled<0>(w[4], w1, x[m], xs[m], acc[m][4]);
-        acc[m][5] = mma_scaled<1>(w[5], w1, x[m], xs[m], acc[m][5]);
-        acc[m][6] = mma_scaled<2>(w[6], w1, x[m], xs[m], acc[m][6]);
-        acc[m][7] = mma_scaled<3>(w[7], w1, x[m], xs[m], acc[m][7]);
+        const int row = row1 + 16 * WM * m;
+        const size_t at = (static_cast<size_t>(it.e_split >> 8) * a.R + row) * a.H;
+#pragma unroll
+        for (int g = 0; g < kNT; ++g) {
+          const int col = it.wt * kBN + (wn * kNT + g) * 16 + 4 * q;
+          if (row >= it.row_end || col >= a.H) continue;
+          const f32x4 v = acc[m][g];
+          if (!kExact && a.y16)
+            store4<bf16>(static_cast<bf16*>(a.y) + at + col, v[0], v[1], v[2], v[3]);
+          else
+            *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at + col) = v;
+        }
       }
     }
   }
-
-#pragma unroll
-  for (int m = 0; m < kMT; ++m) {
-    const int row = row0 + wm * kWaveM + 16 * m + r;
-    if constexpr (kGateUp) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        store_block<kExact>(a, &acc[m][4 * h], sg0 + 2 * wn + h, row, row_end, q);
-    } else {
-      float* y = a.y + (static_cast<size_t>(split) * a.R + row) * a.H;
-#pragma unroll
-      for (int g = 0; g < kNT; ++g) {
-        const int col = wt * kBN + wn * kWaveN + 16 * g + 4 * q;
-        if (row < row_end && col < a.H) *reinterpret_cast<f32x4*>(y + col) = acc[m][g];
-      }
-    }
-  }
+  if (!second) turn();
 }
 
-template <bool kGateUp, int BM>
+template <bool kGateUp, int BM, int WM, int kPerCu>
 hipError_t launch_t(const MxFfnArgs& a, hipStream_t s) {
   if (a.max_tiles == 0) return hipSuccess;
   const int nw = (a.n_super * kMxSuper + kBN - 1) / kBN;
-  const long long grid = static_cast<long long>(a.max_tiles) * nw * a.splits;
-  if (grid > INT_MAX) return hipErrorInvalidValue;
-  const dim3 g(static_cast<unsigned>(grid)), block(Shape<BM>::kThreads);
+  const long long total = static_cast<long long>(a.max_tiles) * nw * a.splits;
+  if (total > INT_MAX) return hipErrorInvalidValue;
+  long long grid = static_cast<long long>(device_cu_count()) * kPerCu;
+  grid = total < grid ? total : grid * ((total + grid * kMaxItems - 1) / (grid * kMaxItems));
+  const dim3 g(static_cast<unsigned>(grid)), block(kThreads);
   if (a.exact)
-    mx_tiled_kernel<kGateUp, BM, true><<<g, block, 0, s>>>(a);
+    mx_tiled_kernel<kGateUp, BM, WM, kPerCu, true><<<g, block, 0, s>>>(a);
   else
-    mx_tiled_kernel<kGateUp, BM, false><<<g, block, 0, s>>>(a);
+    mx_tiled_kernel<kGateUp, BM, WM, kPerCu, false><<<g, block, 0, s>>>(a);
   return hipGetLastError();
+}
+
+template <bool kGateUp>
+hipError_t launch(const MxFfnArgs& a, hipStream_t s) {
+  return a.tile_rows == 256 ? launch_t<kGateUp, 256, 4, 1>(a, s) : launch_t<kGateUp, 64, 2, 2>(a, s);
 }
 
 }  // namespace
 
-hipError_t launch_mx_gate_up_tiled(const MxFfnArgs& a, hipStream_t s) {
-  return a.tile_rows == 256 ? launch_t<true, 256>(a, s) : launch_t<true, 128>(a, s);
-}
+hipError_t launch_mx_gate_up_tiled(const MxFfnArgs& a, hipStream_t s) { return launch<true>(a, s); }
 
-hipError_t launch_mx_down_tiled(const MxFfnArgs& a, hipStream_t s) {
-  return a.tile_rows == 256 ? launch_t<false, 256>(a, s) : launch_t<false, 128>(a, s);
-}
+hipError_t launch_mx_down_tiled(const MxFfnArgs& a, hipStream_t s) { return launch<false>(a, s); }
 
 }  // namespace moe355

@@ -50,16 +50,23 @@ __device__ __forceinline__ bf16x8 tokens_bf16(uint32_t lo, uint32_t hi, float s)
 
 // The gated activation of one supergroup for one token, in 8 bits: lane q holds
 // features 8 q .. 8 q + 7 of the block (v: gate, up of the lower four, then of the
-// upper four), whose maximum is over the token's four lanes.
-template <bool kExact>
+// upper four), whose maximum is over the token's four lanes. It runs while the
+// matrix cores wait, so instructions count: infinities and NaN cost a branch that is
+// seldom taken instead of a test per value.
+template <int kAct, bool kExact>
 __device__ __forceinline__ void store_block(const MxFfnArgs& a, const f32x4* v, int sg, int row,
                                             int row_end, int q) {
   float h[8], amax = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float g = v[i / 4 * 2][i % 4], u = v[i / 4 * 2 + 1][i % 4];
-    h[i] = (kExact ? gate_act(a.act, g) : gate_act_fast(a.act, g)) * u;
-    amax = fmaxf(amax, mx_finite_abs(h[i]));
+    h[i] = (kExact ? gate_act(kAct, g) : gate_act_fast(kAct, g)) * u;
+    amax = fmaxf(amax, fabsf(h[i]));  // ignores NaN
+  }
+  if (amax == INFINITY) {
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_finite_abs(h[i]));
   }
   amax = fmaxf(amax, __shfl_xor(amax, 16, kWave));
   amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
@@ -72,4 +79,15 @@ __device__ __forceinline__ void store_block(const MxFfnArgs& a, const f32x4* v, 
     if (q == 0)
       a.out_scales[static_cast<size_t>(row) * (a.Ip / kMxBlock) + sg] = static_cast<uint8_t>(b);
   }
+}
+
+// f(activation as a compile-time constant).
+template <typename F>
+__device__ __forceinline__ void by_activation(int act, F f) {
+  if (act == MOE355_ACT_SILU)
+    f(std::integral_constant<int, MOE355_ACT_SILU>());
+  else if (act == MOE355_ACT_GELU)
+    f(std::integral_constant<int, MOE355_ACT_GELU>());
+  else
+    f(std::integral_constant<int, MOE355_ACT_GELU_TANH>());
 }

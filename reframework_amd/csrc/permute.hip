@@ -114,7 +114,8 @@ __device__ __forceinline__ void write_tile(const PermuteArgs& a, const int* star
   const int e = order[lo];
   a.tile_map[2 + 2 * j] = e;
   a.tile_map[3 + 2 * j] =
-      start[e] + (j - place_start[lo]) * tile_height(start[e + 1] - start[e], a.tile_rows);
+      start[e] + (j - place_start[lo]) *
+                     (a.full_tiles ? a.tile_rows : tile_height(start[e + 1] - start[e], a.tile_rows));
 }
 
 // All slots fit one block (up to kPermuteSingleMax), one thread each: a chain of
