@@ -13,13 +13,15 @@ namespace {
 
 bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 
-// Average rows per active expert up to which the weights are streamed past tiles of
-// at most 64 rows (ffn_mx.hip), and up to which the tiled kernels (ffn_mx_tiled.hip)
-// take tiles of 64 rows; above, 256. gate|up + down us of 64 / 256-row tiles, 8
-// experts of H 4096, I 14336: 128 rows 280 / 385, 160 rows 369 / 380, 192 rows 396 / 385,
-// 256 rows 468 / 425; 64 experts of H 2048, I 1408: 128 rows 92 / 122, 192 rows 132 / 131,
-// 256 rows 170 / 143, 512 rows 403 / 298.
-constexpr int kMxStreamRows = 24, kMxTile64Rows = 176;
+// Average rows per active expert up to which the weights are streamed past 16-row
+// tiles (ffn_mx.hip), and up to which the tiled kernels (ffn_mx_tiled.hip) take tiles
+// of 64 rows; above, 256 (exact products: 64). gate|up + down us, streaming / 64 rows: 8
+// experts of H 4096, I 14336 at 8 rows 117 / 132, 12 rows 125 / 136 (and with more than 16
+// rows for one expert in ten, some 137), 16 rows 131 / 136, 20 rows 262 / 145; 64 experts
+// of H 2048, I 1408 at 8 rows 51 / 53, 12 rows 52 / 53, 20 rows 110 / 55. 64 / 256 rows: the
+// former at 128 rows 280 / 385, 160 rows 369 / 380, 192 rows 396 / 385, 256 rows 468 / 425; the
+// latter at 128 rows 92 / 122, 192 rows 132 / 131, 256 rows 170 / 143, 512 rows 403 / 298.
+constexpr int kMxStreamRows = 10, kMxTile64Rows = 176;
 
 // The stages of one expert call and where their data lies in the workspace.
 struct MxPlan {
@@ -49,15 +51,14 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   p->n_blocks = R <= kPermuteSingleMax ? 1 : static_cast<int>((R + kPermuteChunk - 1) / kPermuteChunk);
   const int active = static_cast<int>(std::max<long long>(1, std::min<long long>(R, E)));
   const long long avg = R / active;
-  // The tiled kernels address token rows by 32-bit byte offsets whose bit 31 marks
-  // padding.
-  p->tiled = avg > kMxStreamRows && static_cast<long long>(T) * p->Hp < (1ll << 31);
-  p->tile_rows = p->tiled ? (avg > kMxTile64Rows ? 256 : 64) : avg <= 12 ? 16 : avg <= 28 ? 32 : 64;
+  p->tiled = avg > kMxStreamRows;
+  const bool exact = dtype != MOE355_BF16;
+  p->tile_rows = !p->tiled ? kMxStreamTile : avg > kMxTile64Rows && !exact ? 256 : 64;
   p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
   // A bf16 call of several slots per token keeps their results in bf16 until they are
   // weighed and added: half the bytes, and a rounding that the sum over the slots
   // makes smaller than the result's own.
-  const bool narrow = p->tiled && dtype == MOE355_BF16 && K > 1;
+  const bool narrow = p->tiled && !exact && K > 1;
   const int steps = p->Ip / kMxStep;
   int s = 1;
   if (p->tiled) {
@@ -108,6 +109,80 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   p->y = take(static_cast<size_t>(p->down_splits) * R * H * (p->y16 ? 2 : 4));
   p->bytes = off;
   return MOE355_OK;
+}
+
+// The tiled kernels address token rows by 32-bit byte offsets whose bit 31 marks
+// padding: a call of more 8-bit bytes than that runs in parts.
+int max_tokens(int H) { return INT_MAX / mx_pad(H); }
+
+struct MxCall {
+  const void* x;
+  const uint8_t* x_scales;  // nullptr: x is to be quantised
+  const uint8_t *w1, *w2;
+  const uint32_t *w1_scales, *w2_scales;
+  const float* topk_w;
+  const void* topk_ids;
+  void* out;
+  int ids_int64, accumulate, T, H, E, K, dtype, act;
+};
+
+int mx_run(const MxPlan& p, const MxCall& a, void* workspace, hipStream_t s) {
+  PermuteArgs pa{};
+  pa.ids = a.topk_ids;
+  pa.block_counts = at<int32_t>(workspace, p.block_counts);
+  pa.offsets = at<int32_t>(workspace, p.offsets);
+  pa.slot_to_row = at<int32_t>(workspace, p.slot_to_row);
+  pa.row_src = at<int32_t>(workspace, p.row_src);
+  pa.tile_map = at<int32_t>(workspace, p.tile_map);
+  pa.R = p.rows; pa.K = a.K; pa.E = a.E; pa.n_blocks = p.n_blocks;
+  pa.tile_rows = p.tile_rows; pa.max_tiles = p.max_tiles;
+  pa.ids_int64 = a.ids_int64;
+  pa.weights = a.topk_w;
+  pa.full_tiles = 1;
+  MxQuantArgs qa{};
+  qa.T = a.T; qa.H = a.H; qa.Hp = p.Hp;
+  if (!a.x_scales) {
+    qa.x = a.x;
+    qa.codes = at<uint8_t>(workspace, p.xq);
+    qa.scales = at<uint8_t>(workspace, p.xq_scales);
+  }
+  if (int rc = check_hip(launch_mx_prepare(pa, qa, a.dtype, s), "mx prepare launch")) return rc;
+
+  MxFfnArgs f{};
+  f.row_src = pa.row_src; f.tile_map = pa.tile_map; f.offsets = pa.offsets;
+  f.max_tiles = p.max_tiles; f.tile_rows = p.tile_rows;
+  f.R = p.rows; f.H = a.H; f.Ip = p.Ip; f.act = a.act;
+  // A bf16 result keeps 8 bits, below which the scaled MFMA's alignment of products
+  // does not show; results of more bits take the exact products.
+  f.exact = a.dtype != MOE355_BF16;
+  f.out_codes = at<uint8_t>(workspace, p.inter);
+  f.out_scales = at<uint8_t>(workspace, p.inter_scales);
+  f.y = at<void>(workspace, p.y);
+  f.y16 = p.y16;
+
+  f.x = a.x_scales ? static_cast<const uint8_t*>(a.x) : qa.codes;
+  f.x_scales = a.x_scales ? a.x_scales : qa.scales;
+  f.w = a.w1; f.w_scales = a.w1_scales;
+  f.w_stride = mx_code_bytes(2 * p.Ip, p.Hp); f.ws_stride = mx_scale_bytes(2 * p.Ip, p.Hp) / 4;
+  f.Kp = p.Hp; f.n_super = 2 * p.Ip / kMxSuper;
+  f.splits = 1; f.steps_per_split = p.Hp / kMxStep;
+  if (int rc = check_hip(p.tiled ? launch_mx_gate_up_tiled(f, s) : launch_mx_gate_up(f, s), "mx gate_up launch"))
+    return rc;
+
+  f.x = f.out_codes; f.x_scales = f.out_scales;
+  f.w = a.w2; f.w_scales = a.w2_scales;
+  f.w_stride = mx_code_bytes(p.Hp, p.Ip); f.ws_stride = mx_scale_bytes(p.Hp, p.Ip) / 4;
+  f.Kp = p.Ip; f.n_super = p.Hp / kMxSuper;
+  f.splits = p.down_splits; f.steps_per_split = p.down_steps;
+  if (int rc = check_hip(p.tiled ? launch_mx_down_tiled(f, s) : launch_mx_down(f, s), "mx down launch"))
+    return rc;
+
+  CombineArgs c{};
+  c.y = f.y; c.topk_w = a.topk_w; c.slot_to_row = pa.slot_to_row; c.out = a.out;
+  c.T = a.T; c.K = a.K; c.H = a.H; c.R = p.rows; c.splits = p.down_splits;
+  c.accumulate = a.accumulate;
+  c.y16 = p.y16;
+  return check_hip(launch_combine(c, a.dtype, s), "combine launch");
 }
 
 }  // namespace
@@ -246,6 +321,8 @@ int moe355_mx_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size
   if (!bytes) return fail(MOE355_EINVAL, "NULL result");
   MxPlan p;
   if (int rc = mx_plan(T, H, I, E, K, dtype, &p)) return rc;
+  if (T > max_tokens(H))
+    if (int rc = mx_plan(max_tokens(H), H, I, E, K, dtype, &p)) return rc;
   *bytes = p.bytes;
   return MOE355_OK;
 }
@@ -266,67 +343,31 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
       !aligned16(w2_scales) || !aligned16(out) ||
       (x_scales && reinterpret_cast<uintptr_t>(x_scales) % 4))
     return fail(MOE355_EINVAL, "x/w1/w2/scales/out not 16-byte aligned");
+  if (T > max_tokens(H))
+    if (int rc = mx_plan(max_tokens(H), H, I, E, K, dtype, &p)) return rc;
   if (!workspace || workspace_bytes < p.bytes)
     return fail(MOE355_EWORKSPACE, "workspace of %zu bytes, the call needs %zu", workspace_bytes,
                 p.bytes);
   if (!aligned16(workspace)) return fail(MOE355_EINVAL, "workspace not 16-byte aligned");
-  hipStream_t s = as_stream(stream);
-
-  const uint8_t* xq = static_cast<const uint8_t*>(x);
-  const uint8_t* xs = static_cast<const uint8_t*>(x_scales);
-  if (!x_scales) {
-    const MxQuantArgs qa{x, at<uint8_t>(workspace, p.xq), at<uint8_t>(workspace, p.xq_scales), T, H, p.Hp};
-    if (int rc = check_hip(launch_mx_quantize(qa, dtype, s), "mx_quantize launch")) return rc;
-    xq = qa.codes;
-    xs = qa.scales;
+  const size_t x_row = x_scales ? p.Hp : static_cast<size_t>(H) * elem_size(dtype);
+  const size_t out_row = static_cast<size_t>(H) * (accumulate_f32 ? 4 : elem_size(dtype));
+  for (int t = 0; t < T; t += max_tokens(H)) {
+    const int n = std::min(T - t, max_tokens(H));
+    if (n != T)
+      if (int rc = mx_plan(n, H, I, E, K, dtype, &p)) return rc;
+    MxCall c{};
+    c.x = static_cast<const char*>(x) + t * x_row;
+    c.x_scales = x_scales ? static_cast<const uint8_t*>(x_scales) + t * static_cast<size_t>(p.Hp / kMxBlock) : nullptr;
+    c.w1 = static_cast<const uint8_t*>(w1); c.w1_scales = static_cast<const uint32_t*>(w1_scales);
+    c.w2 = static_cast<const uint8_t*>(w2); c.w2_scales = static_cast<const uint32_t*>(w2_scales);
+    c.topk_w = topk_w + static_cast<size_t>(t) * K;
+    c.topk_ids = static_cast<const char*>(topk_ids) + static_cast<size_t>(t) * K * (ids_int64 ? 8 : 4);
+    c.out = static_cast<char*>(out) + t * out_row;
+    c.ids_int64 = ids_int64 != 0; c.accumulate = accumulate_f32 != 0;
+    c.T = n; c.H = H; c.E = E; c.K = K; c.dtype = dtype; c.act = act;
+    if (int rc = mx_run(p, c, workspace, as_stream(stream))) return rc;
   }
-
-  PermuteArgs pa{};
-  pa.ids = topk_ids;
-  pa.block_counts = at<int32_t>(workspace, p.block_counts);
-  pa.offsets = at<int32_t>(workspace, p.offsets);
-  pa.slot_to_row = at<int32_t>(workspace, p.slot_to_row);
-  pa.row_src = at<int32_t>(workspace, p.row_src);
-  pa.tile_map = at<int32_t>(workspace, p.tile_map);
-  pa.R = p.rows; pa.K = K; pa.E = E; pa.n_blocks = p.n_blocks;
-  pa.tile_rows = p.tile_rows; pa.max_tiles = p.max_tiles;
-  pa.ids_int64 = ids_int64 != 0;
-  pa.weights = topk_w;
-  pa.full_tiles = 1;
-  if (int rc = check_hip(launch_permute(pa, s), "permute launch")) return rc;
-
-  MxFfnArgs f{};
-  f.row_src = pa.row_src; f.tile_map = pa.tile_map; f.offsets = pa.offsets;
-  f.max_tiles = p.max_tiles; f.tile_rows = p.tile_rows;
-  f.R = p.rows; f.H = H; f.Ip = p.Ip; f.act = act;
-  // A bf16 result keeps 8 bits, below which the scaled MFMA's alignment of products
-  // does not show; results of more bits take the exact products.
-  f.exact = dtype != MOE355_BF16;
-  f.out_codes = at<uint8_t>(workspace, p.inter);
-  f.out_scales = at<uint8_t>(workspace, p.inter_scales);
-  f.y = at<void>(workspace, p.y);
-  f.y16 = p.y16;
-
-  f.x = xq; f.x_scales = xs;
-  f.w = static_cast<const uint8_t*>(w1); f.w_scales = static_cast<const uint32_t*>(w1_scales);
-  f.w_stride = mx_code_bytes(2 * p.Ip, p.Hp); f.ws_stride = mx_scale_bytes(2 * p.Ip, p.Hp) / 4;
-  f.Kp = p.Hp; f.n_super = 2 * p.Ip / kMxSuper;
-  f.splits = 1; f.steps_per_split = p.Hp / kMxStep;
-  if (int rc = check_hip(p.tiled ? launch_mx_gate_up_tiled(f, s) : launch_mx_gate_up(f, s), "mx gate_up launch")) return rc;
-
-  f.x = f.out_codes; f.x_scales = f.out_scales;
-  f.w = static_cast<const uint8_t*>(w2); f.w_scales = static_cast<const uint32_t*>(w2_scales);
-  f.w_stride = mx_code_bytes(p.Hp, p.Ip); f.ws_stride = mx_scale_bytes(p.Hp, p.Ip) / 4;
-  f.Kp = p.Ip; f.n_super = p.Hp / kMxSuper;
-  f.splits = p.down_splits; f.steps_per_split = p.down_steps;
-  if (int rc = check_hip(p.tiled ? launch_mx_down_tiled(f, s) : launch_mx_down(f, s), "mx down launch")) return rc;
-
-  CombineArgs c{};
-  c.y = f.y; c.topk_w = topk_w; c.slot_to_row = pa.slot_to_row; c.out = out;
-  c.T = T; c.K = K; c.H = H; c.R = p.rows; c.splits = p.down_splits;
-  c.accumulate = accumulate_f32 != 0;
-  c.y16 = p.y16;
-  return check_hip(launch_combine(c, dtype, s), "combine launch");
+  return MOE355_OK;
 }
 
 }  // extern "C"

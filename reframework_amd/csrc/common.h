@@ -306,6 +306,8 @@ hipError_t launch_group_topk(const GroupTopkArgs& a, hipStream_t s);
 // Router logits alone, [T,E] fp32 in a.logits_out, for any E.
 hipError_t launch_router_logits(const RouterArgs& a, int dtype, hipStream_t s);
 hipError_t launch_permute(const PermuteArgs& a, hipStream_t s);
+// Its second launch, above kPermuteSingleMax slots.
+hipError_t launch_permute_scatter(const PermuteArgs& a, hipStream_t s);
 hipError_t launch_gate_up_tiled(const FfnArgs& a, int dtype, hipStream_t s);
 hipError_t launch_down_tiled(const FfnArgs& a, int dtype, hipStream_t s);
 hipError_t launch_gate_up_skinny(const FfnArgs& a, int dtype, hipStream_t s);

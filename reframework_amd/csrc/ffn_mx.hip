@@ -1,9 +1,14 @@
-// Grouped expert FFN on 4-bit weights and 8-bit tokens (formats: mx.h):
+// Grouped expert FFN on 4-bit weights and 8-bit tokens (formats: mx.h) for few tokens
+// per expert:
 //   g, u = deq(x) . deq(w1)^T;  h = act(g) * u in 8 bits;  y = deq(h) . deq(w2)^T
-// A workgroup owns one supergroup (64 packed rows) of one expert and a tile of up
-// to 16 MT of its tokens; its four waves split the columns and add their sums in
-// LDS in a fixed order. Weights sit on the M side of the product, tokens on the N
-// side, so a lane ends with 4 consecutive features of one token per group.
+// Then the weights, read once, bound it. A workgroup owns one supergroup (64 packed
+// rows) of one expert and a tile of up to 16 of its tokens; its four waves split the
+// columns, two steps of 4 KB each in flight, and add their sums in LDS in a fixed
+// order. Weights sit on the M side of the product, tokens on the N side, so a lane
+// ends with 4 consecutive features of one token per group.
+// Weights of 8 experts of H 4096, I 14336 stream at 6.7 and 6.0 TB/s (gate|up and down, 8
+// rows each: 75 and 42 us), of 64 experts of H 2048, I 1408 at 6.2 and 5.1, of two
+// experts of the former for one token at 5.6 and 5.2 (22 and 12 us).
 #include "dma_pipe.h"
 #include "mx.h"
 
@@ -14,17 +19,17 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 #include "mx_mma.h"
 
-template <bool kGateUp, int MT, bool kExact>
+template <bool kGateUp, bool kExact>
 __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
-  constexpr int D = MT == 1 ? 4 : 2;  // steps in flight per wave
-  __shared__ f32x4 red[kWaves][MT][4][kWave];
+  constexpr int D = 2;  // steps in flight per wave (4 need more registers and gain nothing)
+  __shared__ f32x4 red[kWaves][4][kWave];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int ttile = blockIdx.x, sg = blockIdx.y, split = blockIdx.z;
   if (ttile >= a.tile_map[0]) return;
   const int e = a.tile_map[2 + 2 * ttile];
   const int row0 = a.tile_map[3 + 2 * ttile];
-  const int row_end = min(row0 + 16 * MT, a.offsets[e + 1]);
+  const int row_end = min(row0 + kMxStreamTile, a.offsets[e + 1]);
 
   const int steps = a.Kp / kMxStep;
   const int sbeg = min(split * a.steps_per_split, steps);
@@ -35,61 +40,47 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
   const uint8_t* w = a.w + e * a.w_stride + (static_cast<size_t>(sg) * steps + s0) * 4 * kMxTileBytes +
                      lane * 16;
   const uint32_t* ws = a.w_scales + e * a.ws_stride + (static_cast<size_t>(sg) * steps + s0) * kWave + lane;
-  const int q = lane >> 4;
-  const uint8_t* xp[MT];
-  const uint8_t* xsp[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    // rows past the tile's last read its first; their results are not stored
-    const int r = row0 + 16 * m + (lane & 15);
-    const size_t src = kGateUp ? a.row_src[r < row_end ? r : row0] : (r < row_end ? r : row0);
-    xp[m] = a.x + src * a.Kp + s0 * kMxStep + (kExact ? 32 * q : 16 * q);
-    xsp[m] = a.x_scales + src * (a.Kp / kMxBlock) + s0 * (kMxStep / kMxBlock);
-  }
+  const int q = lane >> 4, row = row0 + (lane & 15);
+  // rows past the tile's last read its first; their results are not stored
+  const int p = row < row_end ? row : row0;
+  const size_t src = kGateUp ? a.row_src[p] : p;
+  const uint8_t* xp = a.x + src * a.Kp + s0 * kMxStep + (kExact ? 32 * q : 16 * q);
+  const uint8_t* xsp = a.x_scales + src * (a.Kp / kMxBlock) + s0 * (kMxStep / kMxBlock);
 
-  u32x4 wr[D][4], xr[D][MT][2];
-  uint32_t wsr[D], xsr[D][MT];
+  u32x4 wr[D][4], xr[D][2];
+  uint32_t wsr[D], xsr[D];
   auto issue = [&](int slot, int st) {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
       wr[slot][g] = __builtin_nontemporal_load(
           reinterpret_cast<const u32x4*>(w + static_cast<size_t>(st) * 4 * kMxTileBytes + g * kMxTileBytes));
     wsr[slot] = ws[st * kWave];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const u32x4* p = reinterpret_cast<const u32x4*>(xp[m] + st * kMxStep);
-      xr[slot][m][0] = p[0];
-      xr[slot][m][1] = p[kExact ? 1 : 4];
-      xsr[slot][m] = *reinterpret_cast<const uint32_t*>(xsp[m] + st * (kMxStep / kMxBlock));
-    }
+    const u32x4* x = reinterpret_cast<const u32x4*>(xp + st * kMxStep);
+    xr[slot][0] = x[0];
+    xr[slot][1] = x[kExact ? 1 : 4];
+    xsr[slot] = *reinterpret_cast<const uint32_t*>(xsp + st * (kMxStep / kMxBlock));
   };
-  f32x4 acc[MT][4];
+  f32x4 acc[4];
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) acc[m][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int g = 0; g < 4; ++g) acc[g] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto consume = [&](int slot) {
-    const uint32_t s = wsr[slot];
+    const uint32_t s = wsr[slot], xs = xsr[slot] >> (8 * q);
+    const u32x4* x = xr[slot];
+    if constexpr (kExact) {
+      const float xf = scale_of(xs & 0xffu);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const uint32_t xs = xsr[slot][m] >> (8 * q);
-      const u32x4* x = xr[slot][m];
-      if constexpr (kExact) {
-        const float xf = scale_of(xs & 0xffu);
+      for (int j = 0; j < 4; ++j) {
+        const bf16x8 t = tokens_bf16(x[j / 2][2 * (j % 2)], x[j / 2][2 * (j % 2) + 1], xf);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bf16x8 t = tokens_bf16(x[j / 2][2 * (j % 2)], x[j / 2][2 * (j % 2) + 1], xf);
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            acc[m][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                weights_bf16(wr[slot][g][j], scale_of((s >> (8 * g)) & 0xffu)), t, acc[m][g], 0, 0, 0);
-        }
-      } else {
-        acc[m][0] = mma_scaled<0>(wr[slot][0], s, x, xs, acc[m][0]);
-        acc[m][1] = mma_scaled<1>(wr[slot][1], s, x, xs, acc[m][1]);
-        acc[m][2] = mma_scaled<2>(wr[slot][2], s, x, xs, acc[m][2]);
-        acc[m][3] = mma_scaled<3>(wr[slot][3], s, x, xs, acc[m][3]);
+        for (int g = 0; g < 4; ++g)
+          acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              weights_bf16(wr[slot][g][j], scale_of((s >> (8 * g)) & 0xffu)), t, acc[g], 0, 0, 0);
       }
+    } else {
+      acc[0] = mma_scaled<0>(wr[slot][0], s, x, xs, acc[0]);
+      acc[1] = mma_scaled<1>(wr[slot][1], s, x, xs, acc[1]);
+      acc[2] = mma_scaled<2>(wr[slot][2], s, x, xs, acc[2]);
+      acc[3] = mma_scaled<3>(wr[slot][3], s, x, xs, acc[3]);
     }
   };
 #pragma unroll
@@ -106,37 +97,29 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
   }
 
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) red[wave][m][g][lane] = acc[m][g];
+  for (int g = 0; g < 4; ++g) red[wave][g][lane] = acc[g];
   __syncthreads();
   if constexpr (kGateUp) {
-    // Token tile m by wave m % 4.
+    if (wave != 0) return;
+    f32x4 v[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      v[g] = red[0][g][lane];
+#pragma unroll
+      for (int k = 1; k < kWaves; ++k) v[g] += red[k][g][lane];
+    }
     by_activation(a.act, [&](auto act) {
-      for (int m = wave; m < MT; m += kWaves) {
-        f32x4 v[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          v[g] = red[0][m][g][lane];
-#pragma unroll
-          for (int k = 1; k < kWaves; ++k) v[g] += red[k][m][g][lane];
-        }
-        store_block<act.value, kExact>(a, v, sg, row0 + 16 * m + (lane & 15), row_end, q);
-      }
+      store_block<act.value, kExact>(a, v, sg, row, row_end, q);
     });
   } else {
     // Group g by wave g.
     const int g = wave, col = sg * kMxSuper + 16 * g + 4 * q;
+    f32x4 v = red[0][g][lane];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      f32x4 v = red[0][m][g][lane];
-#pragma unroll
-      for (int k = 1; k < kWaves; ++k) v += red[k][m][g][lane];
-      const int r = row0 + 16 * m + (lane & 15);
-      if (r < row_end && col < a.H)
-        *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + (static_cast<size_t>(split) * a.R + r) * a.H +
-                                  col) = v;
-    }
+    for (int k = 1; k < kWaves; ++k) v += red[k][g][lane];
+    if (row < row_end && col < a.H)
+      *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + (static_cast<size_t>(split) * a.R + row) * a.H +
+                                col) = v;
   }
 }
 
@@ -144,12 +127,7 @@ template <bool kGateUp, bool kExact>
 hipError_t launch_t(const MxFfnArgs& a, hipStream_t s) {
   if (a.max_tiles == 0) return hipSuccess;
   const dim3 grid(a.max_tiles, a.n_super, a.splits), block(kThreads);
-  if (a.tile_rows == 16)
-    mx_ffn_kernel<kGateUp, 1, kExact><<<grid, block, 0, s>>>(a);
-  else if (a.tile_rows == 32)
-    mx_ffn_kernel<kGateUp, 2, kExact><<<grid, block, 0, s>>>(a);
-  else
-    mx_ffn_kernel<kGateUp, 4, kExact><<<grid, block, 0, s>>>(a);
+  mx_ffn_kernel<kGateUp, kExact><<<grid, block, 0, s>>>(a);
   return hipGetLastError();
 }
 

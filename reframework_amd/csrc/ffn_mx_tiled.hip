@@ -318,7 +318,7 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
   if (!second) turn();
 }
 
-template <bool kGateUp, int BM, int WM, int kPerCu>
+template <bool kGateUp, int BM, int WM, int kPerCu, bool kExact>
 hipError_t launch_t(const MxFfnArgs& a, hipStream_t s) {
   if (a.max_tiles == 0) return hipSuccess;
   const int nw = (a.n_super * kMxSuper + kBN - 1) / kBN;
@@ -326,17 +326,17 @@ hipError_t launch_t(const MxFfnArgs& a, hipStream_t s) {
   if (total > INT_MAX) return hipErrorInvalidValue;
   long long grid = static_cast<long long>(device_cu_count()) * kPerCu;
   grid = total < grid ? total : grid * ((total + grid * kMaxItems - 1) / (grid * kMaxItems));
-  const dim3 g(static_cast<unsigned>(grid)), block(kThreads);
-  if (a.exact)
-    mx_tiled_kernel<kGateUp, BM, WM, kPerCu, true><<<g, block, 0, s>>>(a);
-  else
-    mx_tiled_kernel<kGateUp, BM, WM, kPerCu, false><<<g, block, 0, s>>>(a);
+  mx_tiled_kernel<kGateUp, BM, WM, kPerCu, kExact>
+      <<<dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s>>>(a);
   return hipGetLastError();
 }
 
+// Exact products need more registers than a wave of the 256-row tile has left.
 template <bool kGateUp>
 hipError_t launch(const MxFfnArgs& a, hipStream_t s) {
-  return a.tile_rows == 256 ? launch_t<kGateUp, 256, 4, 1>(a, s) : launch_t<kGateUp, 64, 2, 2>(a, s);
+  if (a.exact) return a.tile_rows == 64 ? launch_t<kGateUp, 64, 2, 2, true>(a, s) : hipErrorInvalidValue;
+  return a.tile_rows == 256 ? launch_t<kGateUp, 256, 4, 1, false>(a, s)
+                            : launch_t<kGateUp, 64, 2, 2, false>(a, s);
 }
 
 }  // namespace

@@ -31,6 +31,7 @@ constexpr int kMxBlock = 32;    // values per scale
 constexpr int kMxStep = 128;    // columns per matrix instruction
 constexpr int kMxSuper = 64;    // rows per supergroup
 constexpr int kMxTileBytes = 1024;
+constexpr int kMxStreamTile = 16;  // token rows of a tile of the weight-streaming kernels
 
 __host__ __device__ constexpr int mx_pad(int n) { return (n + kMxStep - 1) / kMxStep * kMxStep; }
 
@@ -109,6 +110,10 @@ hipError_t launch_mx_gate_up(const MxFfnArgs& a, hipStream_t s);
 hipError_t launch_mx_down(const MxFfnArgs& a, hipStream_t s);
 hipError_t launch_mx_gate_up_tiled(const MxFfnArgs& a, hipStream_t s);
 hipError_t launch_mx_down_tiled(const MxFfnArgs& a, hipStream_t s);
+// The first launch of an expert call: the routed slots grouped by expert (all of the
+// permute up to kPermuteSingleMax slots, its counts above) by the first workgroups,
+// x quantised by the others (x.x NULL: it is in 8 bits already).
+hipError_t launch_mx_prepare(const PermuteArgs& p, const MxQuantArgs& x, int dtype, hipStream_t s);
 hipError_t launch_mx_quantize(const MxQuantArgs& a, int dtype, hipStream_t s);
 // dtype -1: src holds codes.
 hipError_t launch_mx_pack(const MxPackArgs& a, int dtype, hipStream_t s);

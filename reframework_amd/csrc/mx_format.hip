@@ -1,18 +1,23 @@
-// Conversions into the formats of mx.h: token rows to 8 bits, and expert weights
+// Conversions into the formats of mx.h: token rows to 8 bits (alone, or in the first
+// launch of an expert call beside the grouping of its slots), and expert weights
 // (codes of a checkpoint, or 16/32-bit weights) to the 4-bit tile order.
+#include <climits>
+
 #include "mx.h"
 
 namespace moe355 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kRows = kMxStreamTile;
+#include "group_slots.h"
+#include "permute_body.h"
 
-// One thread per 8 consecutive values (4 threads per block); bound by reading T * H
-// elements and writing half (16 bits) or a quarter of their bytes.
+// Thread i of a launch quantises 8 consecutive values (4 threads per block of 32); bound
+// by reading T * H elements and writing half (16 bits) or a quarter of their bytes.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const MxQuantArgs a) {
+__device__ __forceinline__ void quantize8(const MxQuantArgs& a, size_t i) {
   const int per_row = a.Hp / 8;
-  const size_t i = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (i >= static_cast<size_t>(a.T) * per_row) return;  // whole blocks: per_row % 16 == 0
   const int t = static_cast<int>(i / per_row), c = static_cast<int>(i % per_row) * 8;
   float v[8];
@@ -36,6 +41,34 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const MxQuantArgs
             mx8_codes(v[4] * f, v[5] * f, v[6] * f, v[7] * f)};
   if ((threadIdx.x & 3) == 0)
     a.scales[static_cast<size_t>(t) * (a.Hp / kMxBlock) + c / kMxBlock] = static_cast<uint8_t>(b);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const MxQuantArgs a) {
+  quantize8<T>(a, static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x);
+}
+
+// The first launch of an expert call. Its first workgroups group the slots: one wave
+// up to 64 slots on 16-row tiles, one workgroup of a thread per slot up to
+// kPermuteSingleMax, above it the permute's counts; the others quantise x. Two
+// launches in a row took some 4 us longer.
+enum class Group { kWave, kOne, kCount };
+
+template <typename T, Group kGroup>
+__global__ __launch_bounds__(kGroup == Group::kOne ? kOneThreads : kThreads) void mx_prepare_kernel(
+    const PermuteArgs p, const MxQuantArgs x) {
+  const int n_group = kGroup == Group::kCount ? p.n_blocks : 1, b = blockIdx.x;
+  if (b >= n_group) {
+    quantize8<T>(x, static_cast<size_t>(b - n_group) * blockDim.x + threadIdx.x);
+  } else if constexpr (kGroup == Group::kCount) {
+    permute_count(p, b);
+  } else if constexpr (kGroup == Group::kOne) {
+    permute_one(p);
+  } else if (threadIdx.x < kWave) {
+    __shared__ int meta[4], rowsrc[kWave], estart[kGroupExpertsPerLane * kWave];
+    __shared__ unsigned long long emask[kGroupExpertsPerLane * kWave];
+    group_slots(p, 0, true, meta, rowsrc, emask, estart);
+  }
 }
 
 // e2m1 code of v (|v| <= 6): the values 0, 0.5, 1, 1.5, 2, 3, 4, 6, ties to the even
@@ -122,7 +155,27 @@ hipError_t launch_quantize_t(const MxQuantArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <typename T>
+hipError_t launch_prepare_t(const PermuteArgs& p, const MxQuantArgs& x, hipStream_t s) {
+  const size_t n = x.x ? static_cast<size_t>(x.T) * (x.Hp / 8) : 0;
+  const auto blocks = [n](int threads) { return static_cast<unsigned>((n + threads - 1) / threads); };
+  if (p.R <= kWave && p.tile_rows == kRows)
+    mx_prepare_kernel<T, Group::kWave><<<dim3(1 + blocks(kThreads)), dim3(kThreads), 0, s>>>(p, x);
+  else if (p.n_blocks == 1)
+    mx_prepare_kernel<T, Group::kOne><<<dim3(1 + blocks(kOneThreads)), dim3(kOneThreads), 0, s>>>(p, x);
+  else
+    mx_prepare_kernel<T, Group::kCount><<<dim3(p.n_blocks + blocks(kThreads)), dim3(kThreads), 0, s>>>(p, x);
+  hipError_t err = hipGetLastError();
+  return err != hipSuccess || p.n_blocks == 1 ? err : launch_permute_scatter(p, s);
+}
+
 }  // namespace
+
+hipError_t launch_mx_prepare(const PermuteArgs& p, const MxQuantArgs& x, int dtype, hipStream_t s) {
+  if (dtype == MOE355_BF16) return launch_prepare_t<bf16>(p, x, s);
+  if (dtype == MOE355_F16) return launch_prepare_t<f16>(p, x, s);
+  return launch_prepare_t<float>(p, x, s);
+}
 
 hipError_t launch_mx_quantize(const MxQuantArgs& a, int dtype, hipStream_t s) {
   if (a.T == 0) return hipSuccess;
