@@ -423,15 +423,21 @@ def fused_experts_static(x: torch.Tensor, w1_ptrs: Sequence[int], w2_ptrs: Seque
 
 
 # Entry points of the 8-bit and 4-bit formats and of the routing by groups. Each runs
-# with its tensors' device current: a launch goes to the current device.
+# with its tensors' device current: a launch goes to the current device. At decode
+# sizes a call is bound by its host time, so these look nothing up twice.
+_get_device = torch._C._cuda_getDevice
+
+
 def _call(device: torch.device, name: str, *args) -> None:
-    fn = getattr(lib(), name)
-    if device.index is None or device.index == torch.cuda.current_device():
+    fn = getattr(_lib or lib(), name)
+    index = device.index
+    if index is None or index == _get_device():
         rc = fn(*args)
     else:
         with torch.cuda.device(device):
             rc = fn(*args)
-    _check(name, rc)
+    if rc != 0:
+        _check(name, rc)
 
 
 def mx_quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -442,16 +448,19 @@ def mx_quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
           _ptr(scales), s)
 
 
-def add_rmsnorm_mxfp8(x: torch.Tensor, residual: Optional[torch.Tensor],
+def add_rmsnorm_mxfp8(T: int, H: int, x: torch.Tensor, residual: Optional[torch.Tensor],
                       residual_out: Optional[torch.Tensor], weight: torch.Tensor,
                       bias: Optional[torch.Tensor], eps: float, normed_out: torch.Tensor,
                       codes: torch.Tensor, scales: torch.Tensor,
                       stream: Optional[int] = None) -> None:
-    T, H = x.shape
-    s = stream if stream is not None else stream_handle(x.device)
-    _call(x.device, "moe355_add_rmsnorm_mxfp8", _ptr(x), _ptr(residual), _ptr(residual_out),
-          _ptr(weight), _ptr(bias), dtype_code(weight.dtype), float(eps), T, H,
-          dtype_code(x.dtype), _ptr(normed_out), _ptr(codes), _ptr(scales), s)
+    """x and its companions hold T rows of H, in any shape."""
+    device = x.device
+    _call(device, "moe355_add_rmsnorm_mxfp8", x.data_ptr(),
+          None if residual is None else residual.data_ptr(),
+          None if residual_out is None else residual_out.data_ptr(), weight.data_ptr(),
+          None if bias is None else bias.data_ptr(), dtype_code(weight.dtype), eps, T, H,
+          dtype_code(x.dtype), normed_out.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+          stream if stream is not None else stream_handle(device))
 
 
 def grouped_topk(logits: torch.Tensor, bias: Optional[torch.Tensor], K: int, scoring: int,
@@ -460,10 +469,12 @@ def grouped_topk(logits: torch.Tensor, bias: Optional[torch.Tensor], K: int, sco
                  stream: Optional[int] = None) -> None:
     """topk_w / topk_ids [T, ld] with ld >= K; columns K.. are left as they are."""
     T, E = logits.shape
-    s = stream if stream is not None else stream_handle(logits.device)
-    _call(logits.device, "moe355_grouped_topk", _ptr(logits), _ptr(bias), T, E, K, scoring,
-          num_groups, topk_groups, group_score, int(renormalize), float(scale), _ptr(topk_w),
-          _ptr(topk_ids), int(topk_ids.dtype == torch.int64), topk_w.shape[1], s)
+    device = logits.device
+    _call(device, "moe355_grouped_topk", logits.data_ptr(),
+          None if bias is None else bias.data_ptr(), T, E, K, scoring, num_groups, topk_groups,
+          group_score, int(renormalize), scale, topk_w.data_ptr(), topk_ids.data_ptr(),
+          int(topk_ids.dtype == torch.int64), topk_w.shape[1],
+          stream if stream is not None else stream_handle(device))
 
 
 def router_logits(x: torch.Tensor, gate: torch.Tensor, round_logits: bool,

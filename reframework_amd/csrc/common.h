@@ -279,6 +279,7 @@ struct GroupTopkArgs {
   void* topk_ids;       // [T,out_ld] int32 or int64
   int T, E, K, G, KG;   // G groups, of which the best KG are kept
   int sigmoid, top2, renormalize, ids_int64, out_ld;
+  int vec;               // groups of whole 16 bytes, aligned (set by the launcher)
   float scale;
 };
 

@@ -59,14 +59,17 @@ struct Key<double> {
   }
 };
 
+// v of the lane that the DPP control names; kDead, which a maximum ignores, in lanes
+// without a source (as its identity lets the compiler fold the move into v_max_i32).
 template <int kCtrl, int kRowMask = 0xf>
 __device__ __forceinline__ int dpp_key(int v) {
-  return __builtin_amdgcn_update_dpp(v, v, kCtrl, kRowMask, 0xf, false);
+  return __builtin_amdgcn_update_dpp(INT_MIN, v, kCtrl, kRowMask, 0xf, false);
 }
 
 template <int kCtrl, int kRowMask = 0xf>
 __device__ __forceinline__ long long dpp_key(long long v) {
-  const unsigned lo = dpp_key<kCtrl, kRowMask>(static_cast<int>(v));
+  // lanes without a source get INT_MIN : 0, which is kDead
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRowMask, 0xf, false);
   const unsigned hi = dpp_key<kCtrl, kRowMask>(static_cast<int>(v >> 32));
   return static_cast<long long>((static_cast<unsigned long long>(hi) << 32) | lo);
 }
@@ -92,11 +95,29 @@ __device__ __forceinline__ I wave_max_key(I v) {
   return lane_key(v, kWave - 1);
 }
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
+// exp(v) for the choice: 32 bits on the transcendental unit (about 2^-23 of the result
+// per unit of |v|, which the test for near values covers), or exactly enough.
+__device__ __forceinline__ float exp_of(float v) {
+  return __builtin_amdgcn_exp2f(v * 1.4426950408889634f);
+}
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
+__device__ __forceinline__ float inverse_of(float v) { return __builtin_amdgcn_rcpf(v); }
+__device__ __forceinline__ double inverse_of(double v) { return 1.0 / v; }
 
-template <typename F>
-__device__ __forceinline__ F wave_sum_of(F v) {
+// Sum over the wave, the same in every lane.
+__device__ __forceinline__ float wave_sum_of(float v) {
+  const auto add = [](float x, int moved) { return x + __int_as_float(moved); };
+  const auto bits = [](float x) { return __float_as_int(x); };
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x111, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x112, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x114, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x118, 0xf, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x142, 0xa, 0xf, false));
+  v = add(v, __builtin_amdgcn_update_dpp(0, bits(v), 0x143, 0xc, 0xf, false));
+  return __int_as_float(__builtin_amdgcn_readlane(bits(v), kWave - 1));
+}
+
+__device__ __forceinline__ double wave_sum_of(double v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
   return v;
@@ -108,21 +129,34 @@ struct Place {
   int width;     // lanes of a group
 };
 
-// The choice of one token, lane k < K of the wave getting the k-th expert. F float
-// returns whether 32 bits leave it open (`exact`: the choice is made on the logits
-// themselves, which leave nothing open); then nothing else is valid.
+// Largest two of b1 >= b2 over runs of `width` lanes (a power of two up to 64), in all
+// of them.
+template <typename I>
+__device__ __forceinline__ void top2_of_group(I& b1, I& b2, int width) {
+  const auto merge = [&](I x1, I x2) {
+    const I lo = min(b1, x1);
+    b1 = max(b1, x1);
+    b2 = max(max(b2, x2), lo);
+  };
+  if (width >= 2) merge(dpp_key<0xb1>(b1), dpp_key<0xb1>(b2));      // quad_perm 1 0 3 2
+  if (width >= 4) merge(dpp_key<0x4e>(b1), dpp_key<0x4e>(b2));      // quad_perm 2 3 0 1
+  if (width >= 8) merge(dpp_key<0x141>(b1), dpp_key<0x141>(b2));    // row_half_mirror
+  if (width >= 16) merge(dpp_key<0x140>(b1), dpp_key<0x140>(b2));   // row_mirror
+  for (int o = 16; o < width; o <<= 1) merge(__shfl_xor(b1, o, kWave), __shfl_xor(b2, o, kWave));
+}
+
+// The choice of one token into chosen[0..K) (LDS). F float returns whether 32 bits
+// leave it open (`exact`: the choice is made on the logits themselves, which leave
+// nothing open); then nothing else is valid.
 template <typename F, int NV>
 __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, const float (&l)[NV],
                                        const float (&bias)[NV], bool exact, float m, int lane,
                                        int* chosen) {
   typedef Key<F> KF;
   typedef typename KF::type I;
-  // Error of c in 32 bits, relative to the largest score plus |c|: some 2^-22
-  // from the score (the exponential, the sum, a division), 2^-24 from the sum
-  // with the bias. Twice that separates two values; 1e-6 leaves a margin.
-  F top = 1;
+  F top = 1;  // a score is at most this
   I key[NV];
-  unsigned idx = 0;  // the lane's experts, 4 bits each, in the order of key[]
+  int idx[NV];
   {
     F c[NV], sum = 0;
     if (exact) {
@@ -131,7 +165,7 @@ __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, c
     } else if (a.sigmoid) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        c[i] = F(1) / (F(1) + exp_of(-static_cast<F>(l[i]))) + static_cast<F>(bias[i]);
+        c[i] = inverse_of(F(1) + exp_of(-static_cast<F>(l[i]))) + static_cast<F>(bias[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -145,144 +179,426 @@ __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, c
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       key[i] = i < p.n ? KF::of(c[i]) : KF::kDead;
-      idx |= static_cast<unsigned>(i) << (4 * i);
+      idx[i] = i;
     }
   }
-  // Insertion sort, largest first, the lower expert first among equals.
+  // Insertion sort, largest first, the lower expert first among equals; then the
+  // experts' places in one register, 4 bits each.
 #pragma unroll
   for (int i = 1; i < NV; ++i)
 #pragma unroll
     for (int j = i; j > 0; --j) {
       const bool swap = key[j] > key[j - 1];
       const I hi = swap ? key[j] : key[j - 1], lo = swap ? key[j - 1] : key[j];
+      const int ih = swap ? idx[j] : idx[j - 1], il = swap ? idx[j - 1] : idx[j];
       key[j - 1] = hi;
       key[j] = lo;
-      const unsigned pair = (idx >> (4 * (j - 1))) & 0xffu;
-      const unsigned turned = ((pair >> 4) | (pair << 4)) & 0xffu;
-      idx ^= swap ? (pair ^ turned) << (4 * (j - 1)) : 0u;
+      idx[j - 1] = ih;
+      idx[j] = il;
     }
+  unsigned list = 0;
+#pragma unroll
+  for (int i = NV - 1; i >= 0; --i) list = (list << 4) | static_cast<unsigned>(idx[i]);
 
-  bool open = false;
-  auto near = [&](I hi, I lo) {  // hi >= lo
-    if (sizeof(F) != sizeof(float) || exact || lo <= KF::kDead + 1) return false;
+  // Whether hi >= lo lie too near each other for 32 bits. The error of c, relative to
+  // the largest score plus |c|, is below 4e-7 from the score (exp_of, where |v|
+  // exp(-|v|) <= 0.37 bounds what its error grows by, the sum, a reciprocal) and 6e-8
+  // from the sum with the bias; twice that, and twice again for a sum of two.
+  auto near = [&](I hi, I lo, F eps) {
     const F x = KF::value(hi), y = KF::value(lo);
-    return !(x - y > F(1e-6) * (top + fabs(x)));  // infinite ones too
+    return lo > KF::kDead + 1 && !(x - y > eps * (top + fabs(x)));  // infinite ones too
   };
+  constexpr bool kTest = sizeof(F) == sizeof(float);
+  bool open = false;
   if (a.KG < a.G) {
     I b1 = key[0], b2 = NV > 1 ? key[NV > 1 ? 1 : 0] : KF::kDead;
-    for (int o = 1; o < p.width; o <<= 1) {
-      const I x1 = __shfl_xor(b1, o, kWave), x2 = __shfl_xor(b2, o, kWave);
-      const I lo = b1 > x1 ? x1 : b1;
-      b2 = max(max(b2, x2), lo);
-      b1 = max(b1, x1);
-    }
-    // A group's score as a key; a sum with a NaN, and of a single expert, as its best.
+    top2_of_group(b1, b2, p.width);
+    // A group's score as a key; with a NaN, and of a single expert, its best.
     I score = b1;
     if (a.top2 && b1 > KF::kDead + 1 && b2 > KF::kDead + 1)
       score = KF::of(KF::value(b1) + KF::value(b2));
     if (p.group >= a.G) score = KF::kDead;
     int rank = 0;
-    I worst = 0, best_out = KF::kDead;  // of the kept, and of the others
     for (int g = 0; g < a.G; ++g) {
       const I other = lane_key(score, g * p.width);
       rank += other > score || (other == score && g < p.group) ? 1 : 0;
     }
     const bool kept = p.group < a.G && rank < a.KG;
-    if (sizeof(F) == sizeof(float) && !exact) {
-      worst = ~wave_max_key(kept ? ~score : KF::kDead);
-      best_out = wave_max_key(!kept && p.group < a.G ? score : KF::kDead);
-      // sums of two are of twice the error
-      if (near(worst, best_out) ||
-          (a.top2 && best_out > KF::kDead + 1 &&
-           !(KF::value(worst) - KF::value(best_out) > F(4e-6) * (top + fabs(KF::value(worst))))))
-        open = true;
+    if (kTest && !exact) {
+      const I worst = ~wave_max_key(kept ? ~score : KF::kDead);
+      const I best_out = wave_max_key(!kept && p.group < a.G ? score : KF::kDead);
+      open = near(worst, best_out, a.top2 ? F(2e-6) : F(1e-6));
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) key[i] = kept ? key[i] : KF::kDead;
   }
 
-  I before = 0;
-  int mine = 0;
+  I mine = KF::kDead, best = KF::kDead;  // lane k: the k-th value; the one after the last
   for (int k = 0; k <= a.K; ++k) {
-    const I best = wave_max_key(key[0]);
-    if (k > 0) open = open || near(before, best);
-    before = best;
+    best = wave_max_key(key[0]);
     if (k == a.K) break;
-    const int win = __builtin_ctzll(__ballot(key[0] == best));
-    const int e = __builtin_amdgcn_readlane(p.e0 + static_cast<int>(idx & 15u), win);
-    mine = lane == k ? e : mine;
-    const bool here = lane == win;
+    if (kTest) mine = lane == k ? best : mine;
+    if (lane == static_cast<int>(__builtin_ctzll(__ballot(key[0] == best)))) {
+      chosen[k] = p.e0 + static_cast<int>(list & 15u);
+      list >>= 4;
 #pragma unroll
-    for (int i = 0; i + 1 < NV; ++i) key[i] = here ? key[i + 1] : key[i];
-    key[NV - 1] = here ? KF::kDead : key[NV - 1];
-    idx = here ? idx >> 4 : idx;
+      for (int i = 0; i + 1 < NV; ++i) key[i] = key[i + 1];
+      key[NV - 1] = KF::kDead;
+    }
   }
-  *chosen = mine;
+  if (kTest && !exact) {
+    const I down = __shfl_down(mine, 1, kWave);
+    const I next = lane == a.K - 1 ? best : down;
+    open = open || __ballot(lane < a.K && near(mine, next, F(1e-6))) != 0;
+  }
   return open;
+}
+
+// This wave's place among the experts: `lanes` lanes in all, `width` per group.
+template <int NV>
+__device__ __forceinline__ Place place_of(const GroupTopkArgs& a, int lane, int width) {
+  Place p;
+  p.width = width;
+  p.group = lane / width;
+  const int first = (lane % width) * NV, S = a.E / a.G;
+  p.n = p.group < a.G ? min(max(S - first, 0), NV) : 0;
+  p.e0 = p.group * S + first;
+  return p;
+}
+
+// This lane's logits and biases, 16 bytes a load where groups are whole ones (`vec`): with
+// 4 bytes a load every instruction of a wave would touch a line per lane.
+template <int NV>
+__device__ __forceinline__ void load_experts(const float* src, const Place& p, bool vec, float (&v)[NV]) {
+  if (NV % 4 == 0 && vec) {
+#pragma unroll
+    for (int i = 0; i < NV; i += 4) {
+      const f32x4 x = i < p.n ? *reinterpret_cast<const f32x4*>(src + p.e0 + i) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 4 && i + j < NV; ++j) v[i + j] = x[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = i < p.n ? src[p.e0 + i] : 0.f;
+  }
+}
+
+template <int NV>
+__device__ __forceinline__ void load_token(const GroupTopkArgs& a, const Place& p, const float* row,
+                                           float (&l)[NV], float (&bias)[NV]) {
+  load_experts<NV>(row, p, a.vec, l);
+  if (a.bias) {
+    load_experts<NV>(a.bias, p, a.vec, bias);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) bias[i] = 0.f;
+  }
+}
+
+__device__ __forceinline__ bool by_logit(const GroupTopkArgs& a) {
+  return !a.bias && (!a.top2 || a.KG == a.G);
+}
+
+// The k-th weight and id of token t.
+__device__ __forceinline__ void store_choice(const GroupTopkArgs& a, int t, int k, float w, int e) {
+  const size_t at = static_cast<size_t>(t) * a.out_ld + k;
+  a.topk_w[at] = w;
+  if (a.ids_int64)
+    static_cast<int64_t*>(a.topk_ids)[at] = e;
+  else
+    static_cast<int32_t*>(a.topk_ids)[at] = e;
 }
 
 template <int NV>
 __global__ __launch_bounds__(kThreads) void group_topk_kernel(const GroupTopkArgs a, int width) {
+  __shared__ int chosen[kThreads / kWave][MOE355_MAX_GROUPED_TOPK];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int t = blockIdx.x * (kThreads / kWave) + wave;
   if (t >= a.T) return;
-  const int S = a.E / a.G;
-  Place p;
-  p.width = width;
-  p.group = lane / width;
-  const int first = (lane % width) * NV;
-  p.n = p.group < a.G ? min(max(S - first, 0), NV) : 0;
-  p.e0 = p.group * S + first;
-
+  const Place p = place_of<NV>(a, lane, width);
   const float* row = a.logits + static_cast<size_t>(t) * a.E;
   float l[NV], bias[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    l[i] = i < p.n ? row[p.e0 + i] : 0.f;
-    bias[i] = a.bias && i < p.n ? a.bias[p.e0 + i] : 0.f;
-  }
+  load_token<NV>(a, p, row, l, bias);
   int mk = Key<float>::of(-INFINITY);
 #pragma unroll
   for (int i = 0; i < NV; ++i) mk = i < p.n ? max(mk, Key<float>::of(l[i])) : mk;
   const float m = Key<float>::value(wave_max_key(mk));
 
-  const bool exact = !a.bias && (!a.top2 || a.KG == a.G);
-  int e = 0;
-  if (select<float, NV>(a, p, l, bias, exact, m, lane, &e))
-    select<double, NV>(a, p, l, bias, exact, m, lane, &e);
+  if (select<float, NV>(a, p, l, bias, by_logit(a), m, lane, chosen[wave]))
+    select<double, NV>(a, p, l, bias, by_logit(a), m, lane, chosen[wave]);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 
   // Lane k finishes the k-th weight from its logit.
-  float w = 0.f;
+  float w;
+  const int e = lane < a.K ? chosen[wave][lane] : 0;
   const float x = row[e];
   if (a.sigmoid) {
     w = 1.0f / (1.0f + expf(-x));
   } else {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) s += i < p.n ? expf(l[i] - m) : 0.f;
-    w = expf(x - m) / wave_sum(s);
+    for (int i = 0; i < NV; ++i) s += i < p.n ? exp_of(l[i] - m) : 0.f;
+    w = expf(x - m) / wave_sum_of(s);
   }
   w = lane < a.K ? w : 0.f;
-  if (a.renormalize) w /= wave_sum(w) + 1e-20f;
+  if (a.renormalize) w /= wave_sum_of(w) + 1e-20f;
   w *= a.scale;
-  if (lane < a.K) {
-    const size_t at = static_cast<size_t>(t) * a.out_ld + lane;
-    a.topk_w[at] = w;
-    if (a.ids_int64)
-      static_cast<int64_t*>(a.topk_ids)[at] = e;
-    else
-      static_cast<int32_t*>(a.topk_ids)[at] = e;
+  if (lane < a.K) store_choice(a, t, lane, w, e);
+}
+
+// ---------------------------------------------------------------- many tokens
+// The kernel above is bound by its instructions (621 of a wave per token at 256
+// experts of 8 groups, top-8; this one's 261). For many tokens a row of 16 lanes takes a token, four
+// to a wave, so that the maxima over lanes are four DPP rotations for four tokens;
+// and a key carries its place i among its lane's experts in its last 4 bits (as 15 -
+// i), so that a comparison of the sort is one maximum and one minimum. Keys are then
+// cut to 2^-19 of the value: choices nearer than that are left to `select`, as
+// are those within the error of 32 bits. Logits whose last 4 bits are 0 (16-bit
+// values) lose nothing.
+constexpr int kRow = 16;
+constexpr int kRowTopk = 8;  // largest K
+
+__device__ __forceinline__ int row_max_key(int v) {
+  v = max(v, dpp_key<0x121>(v));  // row_ror 1, 2, 4, 8
+  v = max(v, dpp_key<0x122>(v));
+  v = max(v, dpp_key<0x124>(v));
+  return max(v, dpp_key<0x128>(v));
+}
+
+__device__ __forceinline__ float row_sum(float v) {
+  const auto moved = [](float x, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl.value, 0xf, 0xf, false));
+  };
+  v += moved(v, std::integral_constant<int, 0x121>());
+  v += moved(v, std::integral_constant<int, 0x122>());
+  v += moved(v, std::integral_constant<int, 0x124>());
+  return v + moved(v, std::integral_constant<int, 0x128>());
+}
+
+// key of the lane `kLanes` further in the row.
+template <int kLanes>
+__device__ __forceinline__ int row_ahead(int v) {
+  return __builtin_amdgcn_update_dpp(v, v, 0x120 + (kRow - kLanes), 0xf, 0xf, false);
+}
+
+template <int kFrom, int kTo, typename F>
+__device__ __forceinline__ void unroll(F f) {
+  if constexpr (kFrom < kTo) {
+    f(std::integral_constant<int, kFrom>());
+    unroll<kFrom + 1, kTo>(f);
   }
 }
 
+// NV experts per lane of a row (4 NW), NW per lane of the wave that a token left open
+// is chosen by.
+template <int NW>
+__global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTopkArgs a, int width) {
+  constexpr int NV = 4 * NW;
+  constexpr int kList = NV < kRowTopk + 1 ? NV : kRowTopk + 1;  // of a lane that can be chosen
+  typedef Key<float> KF;
+  __shared__ int chosen[kThreads / kWave][MOE355_MAX_GROUPED_TOPK];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int sub = lane & (kRow - 1);
+  const int t0 = (blockIdx.x * (kThreads / kWave) + wave) * (kWave / kRow);
+  if (t0 >= a.T) return;
+  const int t = min(t0 + lane / kRow, a.T - 1);  // rows past the last repeat it
+  const int wr = width / 4;                      // lanes of a group
+  const Place p = place_of<NV>(a, sub, wr);
+  const float* row = a.logits + static_cast<size_t>(t) * a.E;
+  float l[NV], bias[NV];
+  load_token<NV>(a, p, row, l, bias);
+
+  const bool exact = by_logit(a);
+  int mk = KF::of(-INFINITY), bits = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    mk = i < p.n ? max(mk, KF::of(l[i])) : mk;
+    bits |= __float_as_int(l[i]);
+  }
+  const float m = KF::value(row_max_key(mk));
+  float top = 1.f, sum = 0.f;
+  int key[NV];
+  {
+    float c[NV];
+    if (exact && a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) c[i] = l[i];
+    } else if (a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) c[i] = inverse_of(1.f + exp_of(-l[i])) + bias[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        c[i] = exp_of(l[i] - m);
+        sum += i < p.n ? c[i] : 0.f;
+      }
+      sum = row_sum(sum);
+      top = 1.f / sum;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) c[i] = exact ? l[i] : c[i] * top + bias[i];
+    }
+    if (exact) top = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      key[i] = i < p.n ? max(KF::of(c[i]), INT_MIN + 16) & ~15 | (15 - i) : KF::kDead;
+  }
+  // The value of a key and whether two lie too near each other: 2^-19 of each from
+  // its cut, and what `select` allows.
+  const auto cut = [](int k) { return KF::value(k & ~15); };
+  const bool lossless = exact && row_max_key(bits & 15) == 0;
+  const auto near = [&](int hi, int lo, float eps) {
+    const float x = cut(hi), y = cut(lo);
+    return lo >= INT_MIN + 32 && !(x - y > eps * (top + fabsf(x)));
+  };
+
+  // Largest first (odd-even merge sort of the NV keys).
+  unroll<0, 4>([&](auto lp) {
+    constexpr int P = 1 << decltype(lp)::value;
+    if constexpr (P < NV) {
+      unroll<0, decltype(lp)::value + 1>([&](auto lk) {
+        constexpr int K2 = P >> decltype(lk)::value;
+#pragma unroll
+        for (int j = K2 % P; j + K2 < NV; j += 2 * K2)
+#pragma unroll
+          for (int i = 0; i < K2; ++i)
+            if (i + j + K2 < NV && (i + j) / (2 * P) == (i + j + K2) / (2 * P)) {
+              const int hi = max(key[i + j], key[i + j + K2]);
+              key[i + j + K2] = min(key[i + j], key[i + j + K2]);
+              key[i + j] = hi;
+            }
+      });
+    }
+  });
+
+  bool open = false;
+  if (a.KG < a.G) {
+    int b1 = key[0], b2 = key[1];
+    top2_of_group(b1, b2, wr);
+    int score = b1;
+    if (a.top2) score = b2 >= INT_MIN + 32 ? KF::of(cut(b1) + cut(b2)) : b1;
+    if (!a.top2) score = b1 & ~15;
+    if (p.group >= a.G) score = KF::kDead;
+    int rank = 0, above = INT_MAX, below = KF::kDead;  // next scores on both sides
+    unroll<1, kRow>([&](auto d) {
+      constexpr int D = decltype(d)::value;
+      if (D % wr) return;
+      const int other = row_ahead<D>(score);
+      const bool first = sub + D >= kRow;  // `other` is of a lower group
+      const bool over = other > score || (other == score && first);
+      rank += over ? 1 : 0;
+      above = over ? min(above, other) : above;
+      below = over ? below : max(below, other);
+    });
+    const bool kept = p.group < a.G && rank < a.KG;
+    // The last kept group and the first one left out lie next to each other.
+    const float eps = a.top2 ? 1.2e-5f : 6e-6f;
+    const int mine = score;
+    if (!lossless || a.top2)
+      open = (kept && rank == a.KG - 1 && below >= INT_MIN + 32 &&
+              !(KF::value(mine) - KF::value(below) > eps * (top + fabsf(KF::value(mine)))));
+#pragma unroll
+    for (int i = 0; i < kList; ++i) key[i] = kept ? key[i] : KF::kDead;
+  }
+
+  // Of equal values the first lane of the row is chosen, and in it the first place.
+  int* const list = chosen[wave] + (lane & ~(kRow - 1)) / kRow * kRowTopk;
+  int mine = KF::kDead, next = KF::kDead;  // lane k: the k-th value, and the one after it
+  unroll<0, kRowTopk + 1>([&](auto kc) {
+    constexpr int k = decltype(kc)::value;
+    if (k > a.K) return;
+    const int head = key[0] & ~15, best = row_max_key(head);
+    next = sub == k - 1 ? best : next;
+    if constexpr (k < kRowTopk) {
+      if (k == a.K) return;
+      mine = sub == k ? best : mine;
+      const unsigned long long at = __ballot(head == best);
+      const unsigned half = lane < 32 ? static_cast<unsigned>(at) : static_cast<unsigned>(at >> 32);
+      if (sub == __builtin_ctz(half >> (lane & 16))) {
+        list[k] = p.e0 + 15 - (key[0] & 15);
+        // What is left of the lane's list can be chosen kRowTopk - k times more.
+        constexpr int kLeft = NV < kRowTopk + 1 - k ? NV : kRowTopk + 1 - k;
+#pragma unroll
+        for (int i = 0; i + 1 < kLeft; ++i) key[i] = key[i + 1];
+        key[kLeft - 1] = KF::kDead;
+      }
+    }
+  });
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  int e = sub < a.K ? list[sub] : 0;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  float x = row[e];
+  if (!lossless) {
+    // What is chosen from what is not lies apart even as cut; the order of what is
+    // chosen, where the cut values are near, by the whole ones.
+    float c = x;
+    if (!exact) {
+      c = a.sigmoid ? inverse_of(1.f + exp_of(-x)) : exp_of(x - m) * top;
+      if (a.bias) c += a.bias[e];
+    }
+    const float after = __int_as_float(row_ahead<1>(__float_as_int(c)));
+    const int e_after = row_ahead<1>(e);
+    const bool ordered = exact ? c > after || (c == after && e < e_after)
+                               : c - after > 1e-6f * (top + fabsf(c));
+    open = open || (sub < a.K && near(mine, next, 6e-6f) && (sub == a.K - 1 || !ordered));
+  }
+
+  // Tokens left open, one after the other by the whole wave.
+  const unsigned long long left = __ballot(open);
+  for (int r = 0; r < kWave / kRow; ++r) {
+    if (!((left >> (kRow * r)) & 0xffffull) || t0 + r >= a.T) continue;
+    const Place pw = place_of<NW>(a, lane, width);
+    float lw[NW], bw[NW];
+    load_token<NW>(a, pw, a.logits + static_cast<size_t>(t0 + r) * a.E, lw, bw);
+    const float mw = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), kRow * r));
+    if (select<float, NW>(a, pw, lw, bw, exact, mw, lane, chosen[wave]))
+      select<double, NW>(a, pw, lw, bw, exact, mw, lane, chosen[wave]);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (lane / kRow == r && sub < a.K) {
+      e = chosen[wave][sub];
+      x = row[e];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+
+  float w = a.sigmoid ? 1.0f / (1.0f + expf(-x)) : expf(x - m) / sum;
+  w = sub < a.K ? w : 0.f;
+  if (a.renormalize) w /= row_sum(w) + 1e-20f;
+  w *= a.scale;
+  if (sub < a.K && t0 + lane / kRow < a.T) store_choice(a, t, sub, w, e);
+}
+
+// Tokens from which four to a wave are faster (256 experts of 8 groups with a bias, one /
+// four to a wave, us a call: 4096 tokens 10.3 / 11.8, 8192 13.1 / 13.0, 16384 19.3 / 16.7,
+// 32768 32 / 23; below, the longer chain of a wave's instructions shows).
+constexpr int kRowTokens = 8192;
+
 }  // namespace
 
-hipError_t launch_group_topk(const GroupTopkArgs& a, hipStream_t s) {
-  if (a.T == 0) return hipSuccess;
+hipError_t launch_group_topk(const GroupTopkArgs& args, hipStream_t s) {
+  if (args.T == 0) return hipSuccess;
+  GroupTopkArgs a = args;
+  const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  a.vec = a.E / a.G % 4 == 0 && aligned(a.logits) && aligned(a.bias);
   // Lanes of a group: 64 over the groups, rounded up to a power of two (G <= 64).
   int slots = 1;
   while (slots < a.G) slots *= 2;
   const int width = kWave / slots, per = (a.E / a.G + width - 1) / width;
+  if (a.T >= kRowTokens && slots <= kRow && per <= 4 && a.K <= kRowTopk) {
+    const int tokens = kThreads / kRow;
+    const dim3 rows((a.T + tokens - 1) / tokens), threads(kThreads);
+    if (per <= 1)
+      group_topk_rows_kernel<1><<<rows, threads, 0, s>>>(a, width);
+    else if (per <= 2)
+      group_topk_rows_kernel<2><<<rows, threads, 0, s>>>(a, width);
+    else
+      group_topk_rows_kernel<4><<<rows, threads, 0, s>>>(a, width);
+    return hipGetLastError();
+  }
   const int tokens = kThreads / kWave;
   const dim3 grid((a.T + tokens - 1) / tokens), block(kThreads);
   if (per <= 1)

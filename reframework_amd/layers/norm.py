@@ -73,16 +73,16 @@ class RMSNorm(BaseOP):
 
     def _run_mxfp8(self, x: torch.Tensor, residual: Optional[torch.Tensor], out: torch.Tensor,
                    residual_out: Optional[torch.Tensor]) -> Mxfp8Rows:
-        w, b = self._params(x)
         H = self.size
+        if x.shape[-1] != H:
+            raise ValueError(f"input rows of {x.shape[-1]} do not match the norm's size {H}")
         if H % BLOCK:
             raise ValueError(f"8-bit rows need a size of whole blocks of {BLOCK}, not {H}")
-        x2 = x.reshape(-1, H)
-        q = Mxfp8Rows.empty(x2.shape[0], H, x.device)
-        _capi.add_rmsnorm_mxfp8(x2, None if residual is None else residual.reshape(-1, H),
-                                None if residual_out is None else residual_out.reshape(-1, H),
-                                w, b, self.eps, out.reshape(-1, H), q.padded_codes,
-                                q.padded_scales)
+        w, b = self._params(x)
+        T = x.numel() // H
+        q = Mxfp8Rows.empty(T, H, x.device)
+        _capi.add_rmsnorm_mxfp8(T, H, x, residual, residual_out, w, b, self.eps, out,
+                                q.padded_codes, q.padded_scales)
         return q
 
     def forward_mxfp8(self, x: torch.Tensor) -> Tuple[torch.Tensor, Mxfp8Rows]:
@@ -98,7 +98,9 @@ class RMSNorm(BaseOP):
         """forward_add_residual that also returns the normed rows in 8 bits:
         (normed, normed in 8 bits, new_residual), in one launch."""
         x = x.contiguous()
-        residual = residual.to(x.dtype).contiguous()
+        if residual.dtype != x.dtype:
+            residual = residual.to(x.dtype)
+        residual = residual.contiguous()
         if residual.shape != x.shape or residual.device != x.device:
             raise ValueError(f"residual {tuple(residual.shape)} on {residual.device} does not match "
                              f"x {tuple(x.shape)} on {x.device}")

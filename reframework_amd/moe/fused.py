@@ -116,35 +116,43 @@ def grouped_topk(
     ties go to the lower group and the lower expert, a NaN ranks last. At most 64
     groups and a topk of 64."""
     require_gpu(gating_output, "gating_output")
-    E = gating_output.shape[-1]
-    logits = gating_output.detach().reshape(-1, E).float().contiguous()
-    w = torch.empty((logits.shape[0], topk), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((logits.shape[0], topk), dtype=torch.int64, device=logits.device)
+    shape = gating_output.shape
+    logits = gating_output
+    if logits.dim() != 2:
+        logits = logits.reshape(-1, shape[-1])
+    if logits.dtype != torch.float32:
+        logits = logits.float()
+    logits = logits.contiguous()
+    T, device = logits.shape[0], logits.device
+    w = torch.empty((T, topk), dtype=torch.float32, device=device)
+    ids = torch.empty((T, topk), dtype=torch.int64, device=device)
     run_grouped_topk(logits, bias, renormalize, scoring, num_groups, topk_groups, group_score,
                      scale, topk, w, ids)
-    if gating_output.dim() == 2:
+    if len(shape) == 2:
         return w, ids
-    shape = tuple(gating_output.shape[:-1]) + (topk,)
-    return w.reshape(shape), ids.reshape(shape)
+    return w.reshape(shape[:-1] + (topk,)), ids.reshape(shape[:-1] + (topk,))
 
 
 def run_grouped_topk(logits: torch.Tensor, bias: Optional[torch.Tensor], renormalize: bool,
                      scoring: str, num_groups: int, topk_groups: int, group_score: str,
                      scale: float, topk: int, w: torch.Tensor, ids: torch.Tensor) -> None:
-    """grouped_topk of fp32 ``logits`` [T, E] into the first ``topk`` columns of ``w``
-    and ``ids`` [T, ld] (fp32; int32 or int64)."""
-    for what, name, known in (("scoring", scoring, _capi.SCORE_CODES),
-                              ("group score", group_score, _capi.GROUP_SCORE_CODES)):
-        if name not in known:
-            raise ValueError(f"unknown {what} {name!r}; known: {tuple(known)}")
-    E = logits.shape[1]
+    """grouped_topk of contiguous fp32 ``logits`` [T, E] into the first ``topk`` columns
+    of ``w`` and ``ids`` [T, ld] (fp32; int32 or int64)."""
+    sc, gs = _capi.SCORE_CODES.get(scoring), _capi.GROUP_SCORE_CODES.get(group_score)
+    if sc is None:
+        raise ValueError(f"unknown scoring {scoring!r}; known: {tuple(_capi.SCORE_CODES)}")
+    if gs is None:
+        raise ValueError(f"unknown group score {group_score!r}; known: "
+                         f"{tuple(_capi.GROUP_SCORE_CODES)}")
     if bias is not None:
-        if bias.numel() != E or bias.device != logits.device:
-            raise ValueError(f"bias {tuple(bias.shape)} on {bias.device} does not match {E} experts "
-                             f"on {logits.device}")
-        bias = bias.detach().reshape(E).float().contiguous()
-    _capi.grouped_topk(logits, bias, topk, _capi.SCORE_CODES[scoring], num_groups, topk_groups,
-                       _capi.GROUP_SCORE_CODES[group_score], renormalize, scale, w, ids)
+        if bias.numel() != logits.shape[1] or bias.device != logits.device:
+            raise ValueError(f"bias {tuple(bias.shape)} on {bias.device} does not match "
+                             f"{logits.shape[1]} experts on {logits.device}")
+        if bias.dtype != torch.float32:
+            bias = bias.float()
+        bias = bias.contiguous()
+    _capi.grouped_topk(logits, bias, topk, sc, num_groups, topk_groups, gs, renormalize, scale, w,
+                       ids)
 
 
 def run_experts(

@@ -104,23 +104,20 @@ def grouped_topk(logits, K, renormalize=True, scoring="softmax", bias=None, num_
         c = x.copy()
     else:
         c = s + (0.0 if bias is None else bias.astype(np.float64))
-    w, ids = np.empty((T, K)), np.empty((T, K), np.int64)
     S = E // num_groups
-
-    def key(v):  # ascending sort order: largest first, NaN last
-        return (1, 0.0) if math.isnan(v) else (0, -v)
-
-    for t in range(T):
-        groups = []
-        for g in range(num_groups):
-            best = sorted((float(v) for v in c[t, g * S:(g + 1) * S]), key=key)
-            two = group_score == "top2" and S > 1 and not math.isnan(best[0]) and \
-                not math.isnan(best[1])
-            groups.append(best[0] + best[1] if two else best[0])
-        kept = sorted(range(num_groups), key=lambda g: (key(groups[g]), g))[:topk_groups]
-        cand = [e for e in range(E) if e // S in kept]
-        ids[t] = sorted(cand, key=lambda e: (key(float(c[t, e])), e))[:K]
-        w[t] = s[t, ids[t]]
+    # stable ascending sorts of -c: largest first, the lower index first, NaN last
+    best = -np.sort(-c.reshape(T, num_groups, S), axis=2)
+    group = best[:, :, 0]
+    if group_score == "top2" and S > 1:
+        two = best[:, :, 0] + best[:, :, 1]
+        group = np.where(np.isnan(two), group, two)
+    kept = np.zeros((T, num_groups), bool)
+    np.put_along_axis(kept, np.argsort(-group, axis=1, kind="stable")[:, :topk_groups], True, 1)
+    order = np.argsort(-c, axis=1, kind="stable")
+    on = np.take_along_axis(np.repeat(kept, S, axis=1), order, 1)
+    first = on & (np.cumsum(on, axis=1) <= K)
+    ids = order[first].reshape(T, K)
+    w = np.take_along_axis(s, ids, 1)
     if renormalize:
         w = w / (w.sum(1, keepdims=True) + 1e-20)
     return w * scale, ids

@@ -39,6 +39,10 @@ def _check(logits, K, dev, bias=None, **kw):
     (19, 160, 6, 8, 3, "max"), (130, 256, 8, 8, 4, "top2"), (7, 60, 4, 12, 5, "top2"),
     (9, 96, 12, 3, 2, "top2"), (4, 256, 64, 2, 1, "max"), (6, 64, 3, 64, 5, "top2"),
     (3, 256, 5, 64, 2, "max"), (11, 255, 9, 17, 2, "top2"), (8, 34, 2, 17, 1, "top2"),
+    (5, 64, 64, 1, 1, "max"), (8195, 256, 8, 8, 4, "top2"), (8193, 8, 2, 1, 1, "max"),
+    (8194, 64, 6, 1, 1, "max"), (8192, 160, 6, 8, 3, "max"), (8197, 96, 8, 16, 5, "top2"),
+    (8196, 60, 4, 12, 5, "top2"), (8192, 255, 7, 5, 2, "top2"), (8192, 64, 1, 2, 1, "max"),
+    (8192, 64, 9, 4, 2, "max"), (8192, 255, 3, 17, 2, "top2"), (8192, 4, 4, 1, 1, "max"),
 ])
 def test_matches_64_bit(T, E, K, G, KG, score, with_bias, scoring, dev):
     banner(f"grouped_topk T={T} E={E} K={K} G={G}/{KG} {score} {scoring} bias={with_bias}")
@@ -52,12 +56,13 @@ def test_matches_64_bit(T, E, K, G, KG, score, with_bias, scoring, dev):
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("G,KG,score", [(1, 1, "max"), (8, 3, "max"), (8, 3, "top2")])
-def test_ties_and_near_ties(G, KG, score, scoring, dev):
+@pytest.mark.parametrize("T", [200, 8194])
+def test_ties_and_near_ties(T, G, KG, score, scoring, dev):
     """Rounded logits (equal ones are common), a bias of few distinct values, and
     choices whose distance is below a step of 32 bits."""
-    banner(f"grouped_topk ties {scoring} G={G} {score}")
+    banner(f"grouped_topk ties T={T} {scoring} G={G} {score}")
     rng = np.random.default_rng(11)
-    E, T = 64, 200
+    E = 64
     logits = np.round(rng.normal(size=(T, E)) * 4).astype(np.float32) / 4
     for bias in (None, np.zeros(E, np.float32), (rng.integers(0, 3, E) / 8).astype(np.float32)):
         _check(logits, 6, dev, bias=bias, scoring=scoring, num_groups=G, topk_groups=KG,
@@ -69,15 +74,19 @@ def test_ties_and_near_ties(G, KG, score, scoring, dev):
     # a bias that outweighs the scores: their bits are below its last one
     _check(logits, 6, dev, bias=np.full(E, 3.0e4, np.float32), scoring=scoring, num_groups=G,
            topk_groups=KG, group_score=score)
+    # logits whose last bits decide, and so do equal ones
+    low = (1.0 + rng.integers(0, 6, (T, E)) * 2.0 ** -23).astype(np.float32) * np.float32(-3)
+    _check(low, 6, dev, scoring=scoring, num_groups=G, topk_groups=KG, group_score=score)
     # saturated scores
     _check((logits * 30).astype(np.float32), 6, dev, bias=np.zeros(E, np.float32),
            scoring="sigmoid", num_groups=G, topk_groups=KG, group_score=score)
 
 
-def test_nan_and_infinities_keep_ids_in_range(dev):
-    banner("grouped_topk NaN / infinities")
+@pytest.mark.parametrize("copies", [1, 700])
+def test_nan_and_infinities_keep_ids_in_range(copies, dev):
+    banner(f"grouped_topk NaN / infinities x {copies}")
     rng = np.random.default_rng(3)
-    E = 32
+    E, K = 32, 8
     logits = rng.normal(size=(12, E)).astype(np.float32)
     logits[0, :] = np.nan
     logits[1, 5] = np.nan
@@ -87,18 +96,20 @@ def test_nan_and_infinities_keep_ids_in_range(dev):
     logits[5, 8:] = np.nan
     logits[6, 8:] = np.finfo(np.float32).min
     logits[7, ::2] = -np.inf
+    logits = np.tile(logits, (copies, 1))
     bias = (rng.normal(size=E) * 0.1).astype(np.float32)
     for b in (None, bias):
         for scoring in ("sigmoid", "softmax"):
             for G, KG, score in ((1, 1, "max"), (4, 2, "max"), (4, 2, "top2")):
-                w, ids = grouped_topk(torch.from_numpy(logits).to(dev), 9, scoring=scoring,
+                w, ids = grouped_topk(torch.from_numpy(logits).to(dev), K, scoring=scoring,
                                       bias=None if b is None else torch.from_numpy(b).to(dev),
                                       num_groups=G, topk_groups=KG, group_score=score)
                 got = ids.cpu().numpy()
                 assert got.min() >= 0 and got.max() < E
-                assert all(len(set(r)) == 9 for r in got.tolist())
-        rows = [1, 2, 6, 7, 8, 9, 10, 11]
-        _check(logits[rows], 9, dev, bias=b, scoring="sigmoid", num_groups=4, topk_groups=2)
+                assert all(len(set(r)) == K for r in got.tolist())
+        rows = [r for r in range(len(logits)) if r % 12 in (1, 2, 6, 7, 8, 9, 10, 11)]
+        rows = rows if copies == 1 else (rows * 2)[:8200]
+        _check(logits[rows], K, dev, bias=b, scoring="sigmoid", num_groups=4, topk_groups=2)
 
 
 def test_strides_types_and_empty(dev):
