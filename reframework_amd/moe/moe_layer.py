@@ -38,6 +38,11 @@ expert-sized pieces and folded into the routed call as extra experts that
 every token reaches with weight 1; otherwise it runs as a second call into the
 same fp32 accumulator.
 
+Optional routing by groups (``scoring``, ``num_expert_groups``, ``topk_groups``,
+``group_score``, ``expert_bias``, ``routed_scale``; fused.grouped_topk) and 4-bit
+experts (``quantize_experts``: mx.Mxfp4Experts in place of the expert parameters,
+tokens in 8 bits) are not in the reference either.
+
 All device compute is in libmoe355: the router kernel (GEMV + softmax +
 top-k) and one fused_experts call per forward (or per chunk). A CPU tensor is
 an error, not a slower path; host compute happens only in the split forward,
@@ -49,15 +54,17 @@ from __future__ import annotations
 import logging
 import time
 from collections import deque
-from typing import Deque, Dict, List, Optional, Tuple
+from typing import Deque, Dict, List, Optional, Tuple, Union
 
 import numpy as np
 import torch
 
 from reframework_amd import _capi, env
 from reframework_amd.layers import BaseOP, activation_code
-from reframework_amd.moe.fused import require_gpu, run_experts
+from reframework_amd.moe.fused import (fused_experts_mxfp4, require_gpu, run_experts,
+                                       run_grouped_topk)
 from reframework_amd.moe.offload_cache import ExpertOffloadCache, Prediction
+from reframework_amd.mx import Mxfp4Experts, Mxfp8Rows
 
 logger = logging.getLogger(__name__)
 
@@ -106,8 +113,23 @@ class FusedMoE(BaseOP):
         dtype: torch.dtype = torch.float16,
         n_shared_experts: int = 0,
         shared_intermediate_size: Optional[int] = None,
+        scoring: str = "softmax",
+        num_expert_groups: int = 1,
+        topk_groups: int = 1,
+        group_score: str = "max",
+        expert_bias: bool = False,
+        routed_scale: float = 1.0,
     ) -> None:
         super().__init__()
+        if scoring not in _capi.SCORE_CODES:
+            raise ValueError(f"unknown scoring {scoring!r}; known: {tuple(_capi.SCORE_CODES)}")
+        if group_score not in _capi.GROUP_SCORE_CODES:
+            raise ValueError(f"unknown group score {group_score!r}; known: "
+                             f"{tuple(_capi.GROUP_SCORE_CODES)}")
+        if num_expert_groups < 1 or num_experts % num_expert_groups:
+            raise ValueError(f"{num_expert_groups} groups do not divide {num_experts} experts")
+        if not 1 <= topk_groups <= num_expert_groups:
+            raise ValueError(f"topk_groups {topk_groups} outside [1, {num_expert_groups}]")
         self.num_experts = num_experts
         self.top_k = top_k
         self.hidden_size = hidden_size
@@ -115,7 +137,17 @@ class FusedMoE(BaseOP):
         self.activation = activation
         self.renormalize = renormalize
         self.dtype = dtype
+        self.scoring = scoring
+        self.num_expert_groups = int(num_expert_groups)
+        self.topk_groups = int(topk_groups)
+        self.group_score = group_score
+        self.routed_scale = float(routed_scale)
+        # Routing that the softmax router does not do runs as logits + grouped_topk.
+        self._grouped = scoring != "softmax" or topk_groups < num_expert_groups or expert_bias or \
+            routed_scale != 1.0
         self.gate = torch.nn.Parameter(torch.empty(num_experts, hidden_size, dtype=dtype))
+        self.expert_bias = torch.nn.Parameter(torch.zeros(num_experts, dtype=torch.float32)) \
+            if expert_bias else None
         self.experts_w1 = torch.nn.ParameterList([
             torch.nn.Parameter(torch.empty(2 * intermediate_size, hidden_size, dtype=dtype))
             for _ in range(num_experts)
@@ -144,6 +176,10 @@ class FusedMoE(BaseOP):
             torch.nn.Parameter(torch.empty(hidden_size, piece, dtype=dtype))
             for _ in range(n_pieces)
         ])
+        # 4-bit experts in place of the parameters above (quantize_experts): the routed
+        # ones with the folded shared ones behind them, and the others
+        self.experts_mxfp4: Optional[Mxfp4Experts] = None
+        self.shared_mxfp4: Optional[Mxfp4Experts] = None
         self._checked_tables: set = set()
         self._shared_cols = None  # cached (key, weights [T,K+n], ids [T,K+n]); see _route32
         self._logits = None  # cached (key, fp32 [T,E] router logits buffer); see _logits_buffer
@@ -162,7 +198,11 @@ class FusedMoE(BaseOP):
         (num_experts, num_experts_per_tok, hidden_size, moe_inter,
         moe_activation, moe_renormalize, dtype; optional entropy_adaptive_k,
         entropy_k_min), honouring RE_ENTROPY_K / RE_ENTROPY_K_MIN. Optional
-        ``n_shared_experts`` / ``shared_intermediate_size`` add shared experts."""
+        ``n_shared_experts`` / ``shared_intermediate_size`` add shared experts, and
+        optional ``scoring_func``, ``n_group``, ``topk_group``, ``routed_scaling_factor``,
+        ``moe_expert_bias`` and ``moe_group_score`` set the routing by groups (a group is
+        scored by its best two experts where there is a bias and nothing else is said)."""
+        expert_bias = bool(getattr(cfg, "moe_expert_bias", False))
         moe = cls(
             num_experts=cfg.num_experts,
             top_k=cfg.num_experts_per_tok,
@@ -173,6 +213,12 @@ class FusedMoE(BaseOP):
             dtype=dtype or cfg.dtype,
             n_shared_experts=int(getattr(cfg, "n_shared_experts", 0) or 0),
             shared_intermediate_size=getattr(cfg, "shared_intermediate_size", None),
+            scoring=getattr(cfg, "scoring_func", None) or "softmax",
+            num_expert_groups=int(getattr(cfg, "n_group", None) or 1),
+            topk_groups=int(getattr(cfg, "topk_group", None) or 1),
+            group_score=getattr(cfg, "moe_group_score", None) or ("top2" if expert_bias else "max"),
+            expert_bias=expert_bias,
+            routed_scale=float(getattr(cfg, "routed_scaling_factor", None) or 1.0),
         )
         moe.entropy_adaptive_k = bool(getattr(cfg, "entropy_adaptive_k", False)) or env.get_entropy_k()
         moe.entropy_k_min = env.get_entropy_k_min(getattr(cfg, "entropy_k_min", 2))
@@ -193,6 +239,8 @@ class FusedMoE(BaseOP):
         ``host_from`` (another layer's cache with the same expert shapes)
         lends its staged host pool instead: this layer's experts are then
         that layer's weights."""
+        if self.experts_mxfp4 is not None:
+            raise RuntimeError("a layer of 4-bit experts is not offloaded")
         self._cache = ExpertOffloadCache(device=device, lru_capacity=lru_capacity, dtype=self.dtype,
                                          pool=pool)
         if host_from is not None:
@@ -234,6 +282,55 @@ class FusedMoE(BaseOP):
         self._cache.enable_host_experts(int8=env.get_moe_split_int8() if int8 is None else int8)
         self._cpu_split_enabled = True
 
+    def quantize_experts(self) -> None:
+        """Turn the expert parameters, shared ones included, into 4-bit experts
+        (mx.Mxfp4Experts, 4.25 bits per weight) and drop them; the layer, its gate and
+        its routing stay in the layer dtype, tokens reach the experts in 8 bits. On the
+        GPU, and not for an offloaded layer; hidden and intermediate sizes are
+        multiples of 32."""
+        if self.uses_offload:
+            raise RuntimeError("offloaded experts are not turned into 4-bit ones")
+        if self.experts_mxfp4 is not None:
+            return
+        w1, w2 = list(self.experts_w1), list(self.experts_w2)
+        if self._shared_folded:
+            w1 += list(self.shared_w1)
+            w2 += list(self.shared_w2)
+        routed = Mxfp4Experts.quantize(w1, w2)
+        if len(self.shared_w1) and not self._shared_folded:
+            self.shared_mxfp4 = Mxfp4Experts.quantize(list(self.shared_w1), list(self.shared_w2))
+        self.experts_mxfp4 = routed
+        for name in ("experts_w1", "experts_w2", "shared_w1", "shared_w2"):
+            setattr(self, name, torch.nn.ParameterList())
+        self._checked_tables.clear()
+
+    def _own_buffers(self) -> bool:
+        """Whether this call uses no buffer that another call does: graphs captured of a
+        layer of 4-bit experts may then be replayed on any streams."""
+        return self.experts_mxfp4 is not None and torch.cuda.is_current_stream_capturing()
+
+    def _experts_mxfp4(self, x: Union[torch.Tensor, Mxfp8Rows], w: torch.Tensor, ids: torch.Tensor,
+                       ) -> torch.Tensor:
+        """_experts on 4-bit weights, tokens in 8 bits or to be quantised."""
+        T, dev = ids.shape[0], ids.device
+        n = self.experts_mxfp4.num_experts - self.num_experts  # folded shared experts
+        if n and ids.shape[1] == self.top_k:
+            ids_x = torch.arange(self.num_experts, self.num_experts + n, dtype=ids.dtype, device=dev)
+            ids = torch.cat([ids, ids_x.expand(T, n)], dim=1)
+            w = torch.cat([w, torch.ones((T, n), dtype=torch.float32, device=dev)], dim=1)
+        if self.shared_mxfp4 is None:
+            return fused_experts_mxfp4(x, self.experts_mxfp4, w, ids, self.activation,
+                                       out_dtype=self.dtype)
+        acc = torch.zeros((T, self.hidden_size), dtype=torch.float32, device=dev)
+        fused_experts_mxfp4(x, self.experts_mxfp4, w, ids, self.activation, out=acc,
+                            accumulate_f32=True, out_dtype=self.dtype)
+        fused_experts_mxfp4(x, self.shared_mxfp4, torch.ones((T, 1), dtype=torch.float32, device=dev),
+                            torch.zeros((T, 1), dtype=torch.int32, device=dev), self.activation,
+                            out=acc, accumulate_f32=True, out_dtype=self.dtype)
+        out = torch.empty((T, self.hidden_size), dtype=self.dtype, device=dev)
+        _capi.cast_f32(acc, out)
+        return out
+
     def set_shuttle(self, shuttle: Optional[CpuShuttle]) -> None:
         self._shuttle = shuttle
 
@@ -266,7 +363,7 @@ class FusedMoE(BaseOP):
         gate = gate.to(self.dtype).contiguous()
         T = xd.shape[0]
         if with_shared_cols:
-            n = len(self.shared_w1)
+            n = self._n_folded
             # one pair per stream: forwards on different streams must not share
             key = (T, n, xd.device, _capi.stream_handle(xd.device))
             if self._shared_cols is None or self._shared_cols[0] != key:
@@ -279,13 +376,25 @@ class FusedMoE(BaseOP):
         else:
             w = torch.empty((T, self.top_k), dtype=torch.float32, device=xd.device)
             ids = torch.empty((T, self.top_k), dtype=torch.int32, device=xd.device)
+        if self._grouped:
+            if self.entropy_adaptive_k:
+                raise ValueError("entropy-adaptive routing does not go with routing by groups")
+            # in a buffer of this call's own: captured graphs do not share it
+            logits = torch.empty((T, self.num_experts), dtype=torch.float32, device=xd.device)
+            _capi.router_logits(xd, gate, True, logits)
+            run_grouped_topk(logits, self.expert_bias, self.renormalize, self.scoring,
+                             self.num_expert_groups, self.topk_groups, self.group_score,
+                             self.routed_scale, self.top_k, w, ids)
+            return w, ids
         kmin = 0
         if self.entropy_adaptive_k:
             if self.entropy_k_min < 1:
                 raise ValueError("entropy-adaptive routing needs entropy_k_min >= 1")
             kmin = min(int(self.entropy_k_min), self.top_k)
+        logits = self._logits_buffer(T, xd.device) if self.experts_mxfp4 is None else \
+            torch.empty((T, self.num_experts), dtype=torch.float32, device=xd.device)
         _capi.router_topk(xd, gate, None, self.top_k, self.renormalize, True, kmin, w, ids,
-                          logits_out=self._logits_buffer(T, xd.device))
+                          logits_out=logits)
         return w, ids
 
     def _logits_buffer(self, T: int, device: torch.device) -> torch.Tensor:
@@ -340,7 +449,14 @@ class FusedMoE(BaseOP):
 
     @property
     def _shared_folded(self) -> bool:
-        return len(self.shared_w1) > 0 and self._shared_piece == self.intermediate_size
+        return self._n_folded > 0
+
+    @property
+    def _n_folded(self) -> int:
+        """Shared experts that run as extra experts of the routed call."""
+        if self.experts_mxfp4 is not None:
+            return self.experts_mxfp4.num_experts - self.num_experts
+        return len(self.shared_w1) if self._shared_piece == self.intermediate_size else 0
 
     def _experts(self, xd: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, act: int,
                  w1p: List[int], w2p: List[int], expert_map: Optional[List[int]] = None,
@@ -396,10 +512,13 @@ class FusedMoE(BaseOP):
         xd = x2.to(self.dtype).contiguous()
         # resident layer with folded shared experts: route straight into the
         # [T, K+n] arrays the expert call takes
-        w, ids = self._route32(xd, with_shared_cols=not self.uses_offload and self._shared_folded)
+        w, ids = self._route32(xd, with_shared_cols=not self.uses_offload and self._shared_folded and
+                               not self._own_buffers())
         act = activation_code(self.activation)
 
-        if self.cpu_split:
+        if self.experts_mxfp4 is not None:
+            out = self._experts_mxfp4(xd, w, ids)
+        elif self.cpu_split:
             out = self._forward_split(M, xd, w, ids, act)
         elif self.uses_offload and env.get_chunk_size(0) > 0:
             out = self._forward_streaming(xd, w, ids, act)
@@ -423,6 +542,15 @@ class FusedMoE(BaseOP):
         require_gpu(x2)
         xd = x2.to(self.dtype).contiguous()
         res = residual.reshape(-1, self.hidden_size).to(self.dtype).contiguous()
+        if self.experts_mxfp4 is not None:
+            # the norm leaves its rows in 8 bits for the experts, the router takes them whole
+            normed, rows, new_res = norm.forward_add_residual_mxfp8(xd, res)
+            w, ids = self._route32(normed, with_shared_cols=self._shared_folded and
+                                   not self._own_buffers())
+            out = self._experts_mxfp4(rows, w, ids)
+            if out.dtype != x.dtype:
+                out = out.to(x.dtype)
+            return out.reshape(shape), new_res.reshape(shape).to(residual.dtype)
         T = xd.shape[0]
         normed = torch.empty_like(xd)
         new_res = torch.empty_like(xd)
@@ -432,8 +560,8 @@ class FusedMoE(BaseOP):
         if gate.device != xd.device:
             gate = gate.to(xd.device)
         nw, nb = norm._params(xd)
-        if self.entropy_adaptive_k:
-            # the entropy-adaptive router is not fused: norm, then the router
+        if self.entropy_adaptive_k or self._grouped:
+            # these routers are not fused: norm, then the router
             _capi.add_rmsnorm(xd, res, new_res, nw, nb, norm.eps, normed)
             w, ids = self._route32(normed)
         else:
@@ -658,10 +786,59 @@ class FusedMoE(BaseOP):
         return out
 
     # -------------------------------------------------------------- (de)serial
+    @staticmethod
+    def _bias_key(prefix: str) -> str:
+        return f"{prefix}.gate.e_score_correction_bias" if prefix else "gate.e_score_correction_bias"
+
+    def _load_mxfp4(self, state_dict: Dict[str, torch.Tensor], prefix: str) -> None:
+        """4-bit experts of a quantised layer's state dict, which a layer that is not
+        quantised yet takes over as they are; a quantised layer takes no expert weights."""
+        head = f"{prefix}." if prefix else ""
+        if self.experts_mxfp4 is not None and any(
+                k.startswith((head + "experts.", head + "shared_experts.")) for k in state_dict):
+            raise RuntimeError("the experts are in 4 bits already: load weights before "
+                               "quantize_experts()")
+        folded, found = self._n_folded, []
+        for name, count, width in (("experts_mxfp4", self.num_experts + folded,
+                                    self.intermediate_size),
+                                   ("shared_mxfp4", 1, self._shared_piece)):
+            keys = [f"{head}{name}.{k}" for k in ("w1", "w1_scales", "w2", "w2_scales")]
+            if not all(k in state_dict for k in keys):
+                continue
+            mx = getattr(self, name)
+            if mx is None:
+                if self.uses_offload or not len(self.experts_w1):
+                    raise RuntimeError("4-bit experts load into a resident layer")
+                mx = Mxfp4Experts(count, self.hidden_size, width, device=self.gate.device)
+            for key, buf in zip(keys, (mx.w1, mx.w1_scales, mx.w2, mx.w2_scales)):
+                if state_dict[key].shape != buf.shape:
+                    raise ValueError(f"{key}: {tuple(state_dict[key].shape)} does not match "
+                                     f"{tuple(buf.shape)}")
+                buf.copy_(state_dict[key])
+            found.append((name, mx))
+        if not found:
+            return
+        unfolded = self._shared_piece > 0 and self._shared_piece != self.intermediate_size
+        names = [name for name, _ in found]
+        if self.experts_mxfp4 is None and names != ["experts_mxfp4"] + ["shared_mxfp4"] * unfolded:
+            raise ValueError("the state dict holds 4-bit experts of only a part of this layer")
+        for name, mx in found:
+            setattr(self, name, mx)
+        for name in ("experts_w1", "experts_w2", "shared_w1", "shared_w2"):
+            setattr(self, name, torch.nn.ParameterList())
+        self._checked_tables.clear()
+
     def state_dict(self, *, prefix: str = "", result: Optional[dict] = None,
                    destination=None, keep_vars: bool = False) -> Dict[str, torch.Tensor]:
         result = destination if destination is not None else ({} if result is None else result)
         result[f"{prefix}.gate.weight" if prefix else "gate.weight"] = self.gate
+        if self.expert_bias is not None:
+            result[self._bias_key(prefix)] = self.expert_bias
+        for name in ("experts_mxfp4", "shared_mxfp4"):
+            mx = getattr(self, name)
+            if mx is not None:
+                for key, t in mx.named_buffers():
+                    result[f"{prefix}.{name}.{key}" if prefix else f"{name}.{key}"] = t
         I = self.intermediate_size
         for e in range(len(self.experts_w1)):
             p = f"{prefix}.experts.{e}" if prefix else f"experts.{e}"
@@ -683,6 +860,9 @@ class FusedMoE(BaseOP):
             g = f"{prefix}.gate.weight" if prefix else "gate.weight"
             if g in state_dict:
                 self.gate.copy_(state_dict[g].detach().to(dtype=self.dtype))
+            if self.expert_bias is not None and self._bias_key(prefix) in state_dict:
+                self.expert_bias.copy_(state_dict[self._bias_key(prefix)].detach())
+            self._load_mxfp4(state_dict, prefix)
             I = self.intermediate_size
             for e in range(len(self.experts_w1)):
                 p = f"{prefix}.experts.{e}" if prefix else f"experts.{e}"
