@@ -184,6 +184,68 @@ def test_experts(T, H, E, K, I, dt, dev):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("T,H,E,K,I,dt", [
+    (1024, 256, 2, 1, 8192, torch.bfloat16),   # 256-row tiles, more items than CUs
+    (620, 160, 8, 2, 4096, torch.bfloat16),    # 64-row tiles
+    (620, 160, 8, 2, 4096, torch.float16),
+    (700, 8192, 3, 2, 96, torch.bfloat16),     # down: one step of columns, many weight tiles
+])
+def test_several_items_per_workgroup(T, H, E, K, I, dt, dev):
+    """The loads of an item start while the one before it runs, with as few as one
+    step of columns each."""
+    banner(f"fused_experts_mxfp4 many items {dt} T={T} H={H} E={E} K={K} I={I}")
+    rng = np.random.default_rng(T)
+    w1, w2 = _random_codes(E, 2 * I, H, rng, 116, 119), _random_codes(E, H, I, rng)
+    x = torch.from_numpy(rng.normal(size=(T, H))).to(dt)
+    tw, ids = _routing(T, K, E, rng)
+    want = ref.experts(ref.to64(x), ref.dequant4(*w1), ref.dequant4(*w2), tw, ids)
+    got = fused_experts_mxfp4(x.to(dev), _experts(w1, w2, dev), torch.from_numpy(tw).to(dev),
+                              torch.from_numpy(ids).to(dev))
+    assert _rel(got, want) <= REL[dt]
+
+
+def test_more_items_than_a_launch_of_resident_workgroups_holds(dev):
+    """32 items for each of the workgroups that run at once are not enough here: the
+    launch has more. The same tokens in parts, whose launches do not, give the same
+    bits (a row's sums do not depend on the others)."""
+    banner("fused_experts_mxfp4 items past the workgroups' lists")
+    T, H, E, I = 8192, 65536, 2, 32
+    g = torch.Generator(device=dev).manual_seed(1)
+    w1 = torch.randn(E, 2 * I, H, generator=g, device=dev).bfloat16() * 0.01
+    w2 = torch.randn(E, H, I, generator=g, device=dev).bfloat16()
+    ex = Mxfp4Experts.quantize(w1, w2)
+    del w1, w2
+    x = torch.randn(T, H, generator=g, device=dev).bfloat16()
+    ids = torch.randint(0, E, (T, 1), generator=g, device=dev)
+    tw = torch.rand(T, 1, generator=g, device=dev) + 0.5
+    whole = fused_experts_mxfp4(x, ex, tw, ids)
+    assert bool(torch.isfinite(whole).all()) and float(whole.float().abs().max()) > 0
+    for t in range(0, T, 2048):
+        part = slice(t, t + 2048)
+        assert torch.equal(fused_experts_mxfp4(x[part], ex, tw[part], ids[part]), whole[part])
+
+
+def test_tokens_past_2_gb_run_in_parts(dev):
+    """8-bit tokens of more bytes than the kernels' offsets hold."""
+    banner("fused_experts_mxfp4 past 2 GB of tokens")
+    T, H, E, I = 40000, 65536, 2, 32
+    g = torch.Generator(device=dev).manual_seed(2)
+    ex = Mxfp4Experts.quantize(torch.randn(E, 2 * I, H, generator=g, device=dev) * 0.01,
+                               torch.randn(E, H, I, generator=g, device=dev))
+    codes = torch.randint(0, 120, (T, H), generator=g, device=dev, dtype=torch.uint8)
+    q = Mxfp8Rows(codes.view(torch.float8_e4m3fn),
+                  torch.randint(110, 120, (T, H // 32), generator=g, device=dev,
+                                dtype=torch.uint8).view(torch.float8_e8m0fnu), H)
+    ids = torch.randint(0, E, (T, 1), generator=g, device=dev)
+    tw = torch.rand(T, 1, generator=g, device=dev) + 0.5
+    whole = fused_experts_mxfp4(q, ex, tw, ids)
+    for t in (0, 16384, 32766, 32767, 32768, 39000):  # 32767 tokens of 64 KB fit below 2 GB
+        n = min(1000, T - t)
+        part = Mxfp8Rows(q.padded_codes[t:t + n], q.padded_scales[t:t + n], H)
+        got = fused_experts_mxfp4(part, ex, tw[t:t + n], ids[t:t + n])
+        assert torch.equal(got, whole[t:t + n])
+
+
 @pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_activations(activation, dt, dev):
