@@ -522,17 +522,18 @@ def mx_workspace_bytes(T: int, H: int, I: int, E: int, K: int, dtype: int,
     return n
 
 
-def mx_fused_experts(x: torch.Tensor, x_scales: Optional[torch.Tensor], H: int, I: int, E: int,
-                     w1: torch.Tensor, w1_scales: torch.Tensor, w2: torch.Tensor,
+def mx_fused_experts(x: torch.Tensor, x_scales: Optional[torch.Tensor], T: int, H: int, I: int,
+                     E: int, K: int, w1: torch.Tensor, w1_scales: torch.Tensor, w2: torch.Tensor,
                      w2_scales: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor,
                      dtype: int, act: int, out: torch.Tensor, accumulate_f32: bool,
                      workspace: torch.Tensor, stream: Optional[int] = None) -> None:
-    T, K = topk_ids.shape
-    s = stream if stream is not None else stream_handle(x.device)
-    _call(x.device, "moe355_mx_fused_experts", _ptr(x), _ptr(x_scales), _ptr(w1), _ptr(w1_scales),
-          _ptr(w2), _ptr(w2_scales), _ptr(topk_w), _ptr(topk_ids),
-          int(topk_ids.dtype == torch.int64), T, H, I, E, K, dtype, act, _ptr(out),
-          int(accumulate_f32), _ptr(workspace), workspace.numel(), s)
+    device = x.device
+    _call(device, "moe355_mx_fused_experts", x.data_ptr(),
+          None if x_scales is None else x_scales.data_ptr(), w1.data_ptr(), w1_scales.data_ptr(),
+          w2.data_ptr(), w2_scales.data_ptr(), topk_w.data_ptr(), topk_ids.data_ptr(),
+          int(topk_ids.dtype == torch.int64), T, H, I, E, K, dtype, act, out.data_ptr(),
+          int(accumulate_f32), workspace.data_ptr(), workspace.numel(),
+          stream if stream is not None else stream_handle(device))
 
 
 def cast_f32(src: torch.Tensor, dst: torch.Tensor, stream: Optional[int] = None) -> None:

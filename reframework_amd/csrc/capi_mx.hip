@@ -15,13 +15,15 @@ bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 
 // Average rows per active expert up to which the weights are streamed past 16-row
 // tiles (ffn_mx.hip), and up to which the tiled kernels (ffn_mx_tiled.hip) take tiles
-// of 64 rows; above, 256 (exact products: 64). gate|up + down us, streaming / 64 rows: 8
+// of 64 rows; above, 256 (exact products: 128). gate|up + down us, streaming / 64 rows: 8
 // experts of H 4096, I 14336 at 8 rows 117 / 132, 12 rows 125 / 136 (and with more than 16
 // rows for one expert in ten, some 137), 16 rows 131 / 136, 20 rows 262 / 145; 64 experts
 // of H 2048, I 1408 at 8 rows 51 / 53, 12 rows 52 / 53, 20 rows 110 / 55. 64 / 256 rows: the
 // former at 128 rows 280 / 385, 160 rows 369 / 380, 192 rows 396 / 385, 256 rows 468 / 425; the
-// latter at 128 rows 92 / 122, 192 rows 132 / 131, 256 rows 170 / 143, 512 rows 403 / 298.
-constexpr int kMxStreamRows = 10, kMxTile64Rows = 176;
+// latter at 128 rows 92 / 122, 192 rows 132 / 131, 256 rows 170 / 143, 512 rows 403 / 298. Exact products, 64 / 128 rows: the former at
+// 128 rows 444 / 488, 256 rows 827 / 728, 1024 rows 2710 / 2369; the latter at 128 rows 168 /
+// 161, 192 rows 253 / 287, 256 rows 341 / 300.
+constexpr int kMxStreamRows = 10, kMxTile64Rows = 176, kMxTile64RowsExact = 224;
 
 // The stages of one expert call and where their data lies in the workspace.
 struct MxPlan {
@@ -53,7 +55,9 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   const long long avg = R / active;
   p->tiled = avg > kMxStreamRows;
   const bool exact = dtype != MOE355_BF16;
-  p->tile_rows = !p->tiled ? kMxStreamTile : avg > kMxTile64Rows && !exact ? 256 : 64;
+  p->tile_rows = !p->tiled ? kMxStreamTile
+                 : exact   ? (avg > kMxTile64RowsExact ? 128 : 64)
+                           : (avg > kMxTile64Rows ? 256 : 64);
   p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
   // A bf16 call of several slots per token keeps their results in bf16 until they are
   // weighed and added: half the bytes, and a rounding that the sum over the slots
@@ -64,7 +68,7 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   if (p->tiled) {
     // The columns of the down projection are cut where that shortens its rounds of
     // workgroups by more than the planes of y cost: a step of a CU takes 1.25 us on
-    // 256-row tiles and 0.85 on 64-row ones, an item 3 steps more, y 5 TB/s (us with 1 /
+    // 256-row tiles (and 128-row ones of exact products) and 0.85 on 64-row ones, an item 3 steps more, y 5 TB/s (us with 1 /
     // 2 / 4 parts: 8 experts of I 14336 at 49 rows 92 / 54 / 53, at 1085 rows 444 / 434 / 498;
     // 12 of H 1280, I 3328 at 83 rows 20.8 / 14.7 / 16.0).
     const double fill = static_cast<double>(R) / active / p->tile_rows;
@@ -75,7 +79,7 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
     for (int c = 1; c <= 4 && steps >= 4 * c; c *= 2) {
       const double rounds = static_cast<double>((items * c + cus - 1) / cus);
       const double y_bytes = c == 1 && narrow ? 4.0 : 8.0 * c;
-      const double us = rounds * ((steps + c - 1) / c + 3.0) * (p->tile_rows == 256 ? 1.25 : 0.85) +
+      const double us = rounds * ((steps + c - 1) / c + 3.0) * (p->tile_rows > 64 ? 1.25 : 0.85) +
                         static_cast<double>(R) * H * y_bytes / 5e6;
       if (c == 1 || us < 0.97 * best) {
         best = us;

@@ -331,10 +331,13 @@ hipError_t launch_t(const MxFfnArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Exact products need more registers than a wave of the 256-row tile has left.
+// Exact products (four instructions and their conversions instead of one) leave no
+// registers for a 256-row tile.
 template <bool kGateUp>
 hipError_t launch(const MxFfnArgs& a, hipStream_t s) {
-  if (a.exact) return a.tile_rows == 64 ? launch_t<kGateUp, 64, 2, 2, true>(a, s) : hipErrorInvalidValue;
+  if (a.exact)
+    return a.tile_rows == 128 ? launch_t<kGateUp, 128, 2, 1, true>(a, s)
+                              : launch_t<kGateUp, 64, 2, 2, true>(a, s);
   return a.tile_rows == 256 ? launch_t<kGateUp, 256, 4, 1, false>(a, s)
                             : launch_t<kGateUp, 64, 2, 2, false>(a, s);
 }

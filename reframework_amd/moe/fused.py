@@ -250,30 +250,29 @@ def fused_experts_mxfp4(
     products. Slots whose id lies outside the experts or whose weight is 0 add nothing.
     With ``accumulate_f32`` the result is added to the fp32 ``out``."""
     act = activation_code(activation)
-    rows = hidden_states if isinstance(hidden_states, Mxfp8Rows) else None
-    if rows is None:
+    if isinstance(hidden_states, Mxfp8Rows):
+        x, x_scales = hidden_states.padded_codes, hidden_states.padded_scales
+        M, H = x.shape[0], hidden_states.size
+        dtype = out_dtype or torch.bfloat16
+    else:
         require_gpu(hidden_states, "hidden_states")
         if hidden_states.dim() != 2:
             raise ValueError(f"hidden_states are [M, H], not {tuple(hidden_states.shape)}")
         M, H = hidden_states.shape
-        x = _aligned(hidden_states.detach().contiguous())
-        _capi.dtype_code(x.dtype)
-        if out_dtype not in (None, x.dtype):
-            raise ValueError(f"out_dtype {out_dtype} differs from the tokens' {x.dtype}")
-        dtype, x_scales = x.dtype, None
-    else:
-        M, H = len(rows), rows.size
-        x, x_scales = rows.padded_codes, rows.padded_scales
-        dtype = out_dtype or torch.bfloat16
+        x, x_scales, dtype = _aligned(hidden_states.contiguous()), None, hidden_states.dtype
+        if out_dtype is not None and out_dtype != dtype:
+            raise ValueError(f"out_dtype {out_dtype} differs from the tokens' {dtype}")
+    code = _capi.dtype_code(dtype)
     dev = x.device
-    E, I = experts.num_experts, experts.intermediate_size
     if H != experts.hidden_size:
         raise ValueError(f"hidden size {H} does not match the experts' {experts.hidden_size}")
     b = experts._buffers
-    if b["w1"].device != dev or topk_weights.device != dev or topk_ids.device != dev:
-        raise ValueError(f"experts on {b['w1'].device}, weights on {topk_weights.device} and ids on "
+    w1 = b["w1"]
+    if w1.device != dev or topk_weights.device != dev or topk_ids.device != dev:
+        raise ValueError(f"experts on {w1.device}, weights on {topk_weights.device} and ids on "
                          f"{topk_ids.device} must be on the tokens' {dev}")
-    if topk_ids.numel() != topk_weights.numel() or (M and topk_ids.numel() % M):
+    slots = topk_ids.numel()
+    if slots != topk_weights.numel() or (M and slots % M):
         raise ValueError(f"topk_ids {tuple(topk_ids.shape)} and topk_weights "
                          f"{tuple(topk_weights.shape)} are not [{M}, K]")
     out_type = torch.float32 if accumulate_f32 else dtype
@@ -287,15 +286,15 @@ def fused_experts_mxfp4(
     if M == 0:
         return out
     ids = topk_ids if topk_ids.dtype in (torch.int32, torch.int64) else topk_ids.long()
-    ids = ids.reshape(M, -1).contiguous()
-    w = topk_weights.detach().reshape(M, -1).float().contiguous()
-    code = _capi.dtype_code(dtype)
+    w = topk_weights if topk_weights.dtype == torch.float32 else topk_weights.float()
+    E, I, K = experts.num_experts, experts.intermediate_size, slots // M
     # From the caching allocator on the current stream, not from a buffer that calls
     # share: captured graphs then have workspaces of their own.
-    ws = torch.empty(_capi.mx_workspace_bytes(M, H, I, E, ids.shape[1], code, dev),
-                     dtype=torch.uint8, device=dev)
-    _capi.mx_fused_experts(x, x_scales, H, I, E, b["w1"], b["w1_scales"], b["w2"], b["w2_scales"],
-                           w, ids, code, act, out, accumulate_f32, ws)
+    ws = torch.empty(_capi.mx_workspace_bytes(M, H, I, E, K, code, dev), dtype=torch.uint8,
+                     device=dev)
+    _capi.mx_fused_experts(x, x_scales, M, H, I, E, K, w1, b["w1_scales"], b["w2"],
+                           b["w2_scales"], w.contiguous(), ids.contiguous(), code, act, out,
+                           accumulate_f32, ws)
     return out
 
 

@@ -188,6 +188,7 @@ def test_experts(T, H, E, K, I, dt, dev):
     (1024, 256, 2, 1, 8192, torch.bfloat16),   # 256-row tiles, more items than CUs
     (620, 160, 8, 2, 4096, torch.bfloat16),    # 64-row tiles
     (620, 160, 8, 2, 4096, torch.float16),
+    (1024, 256, 2, 1, 8192, torch.float16),    # 128-row tiles
     (700, 8192, 3, 2, 96, torch.bfloat16),     # down: one step of columns, many weight tiles
 ])
 def test_several_items_per_workgroup(T, H, E, K, I, dt, dev):
