@@ -9,7 +9,9 @@
 //
 // Eight waves, two per SIMD, work in turns: while the first four multiply a step, the
 // others read theirs from LDS, and a barrier swaps them, so that the matrix cores
-// always have a wave with its operands in registers.
+// always have a wave with its operands in registers. Only gate_up's 64-row tiles, of
+// which two workgroups share a CU, do without turns: all waves read and multiply a step
+// between two barriers, and the other workgroup fills the gaps.
 //
 // A workgroup runs several items, whose steps follow each other in one stream of
 // loads: the first steps of an item are on their way while the item before it is
@@ -76,6 +78,10 @@ __device__ __forceinline__ Item decode_item(const MxFfnArgs& a, int L, int nw, i
 template <bool kGateUp, int BM, int WM, int kPerCu, bool kExact>
 __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const MxFfnArgs a) {
   typedef Shape<BM, WM, kPerCu> S;
+  // gate_up of 64-row tiles without turns, with: 13.1 / 15.4 us (8 x 128 rows,
+  // 2048 x 1408), 42 / 46 us (32 x 128, 1280 x 3328); 137 / 146 us (8 x 49, 4096 x 14336,
+  // exact). down, whose items are fewer and longer: 34 / 30, 170 / 112 us (scaled).
+  constexpr bool kTurns = !(kGateUp && kPerCu == 2);
   constexpr int kMT = S::kMT, kNT = S::kNT;
   __shared__ __attribute__((aligned(1024))) uint8_t stage[S::kStages][S::kStage];
   __shared__ Item items[kMaxItems];
@@ -195,14 +201,16 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
   begin_loads(item_at(0));
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) load();
-  landed(0);
-  turn();
   // Half-step 2 s: the first waves read step s of the stream, the second multiply step
   // s - 1; the next half-step the other way round. Before half-step 2 s every wave
   // has seen its loads of step s land; the buffer of step s - 1 was last read in
   // half-step 2 s - 1 and is filled again from half-step 2 s on.
   const bool second = wave >= 4;
-  if (second) turn();
+  if constexpr (kTurns) {
+    landed(0);
+    turn();
+    if (second) turn();
+  }
   int done = 0;  // steps of the stream
   const int wm = wave % WM, wn = wave / WM;  // this wave's tokens and weight rows
   for (int j = 0; j < n_items; ++j) {
@@ -219,6 +227,14 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
     auto run_steps = [&](auto full) {
       constexpr bool kFull = decltype(full)::value;
       for (int st = 0; st < n; ++st, ++done) {
+        if constexpr (!kTurns) {
+          // Every wave has read step `done` - 1, whose buffer is filled again, and has
+          // seen its loads of step `done` land.
+          landed(done);
+          pipe::wait_lgkm0();
+          turn();
+          load();
+        }
         const uint8_t* s = stage[done % S::kStages];
         const uint8_t* wtile = s + S::kTokBytes + wn * (kNT * kMxTileBytes) + lane * 16;
         const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
@@ -240,10 +256,12 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
           x[m][1] = *reinterpret_cast<const u32x4*>(p + (((kExact ? 2 * q + 1 : 4 + q) ^ sw) << 4));
           xs[m] = *reinterpret_cast<const uint32_t*>(ts + 64 * WM * m) >> (8 * q);
         }
-        load();
-        if (second) landed(done + 1);
-        pipe::wait_lgkm0();
-        turn();
+        if constexpr (kTurns) {
+          load();
+          if (second) landed(done + 1);
+          pipe::wait_lgkm0();
+          turn();
+        }
         if constexpr (kExact) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -274,9 +292,11 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
             }
           }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (!second) landed(done + 1);
-        turn();
+        if constexpr (kTurns) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (!second) landed(done + 1);
+          turn();
+        }
       }
     };
     if (it.row_end - it.row0 > BM - 16 * WM)
@@ -315,7 +335,7 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
       }
     }
   }
-  if (!second) turn();
+  if (kTurns && !second) turn();
 }
 
 template <bool kGateUp, int BM, int WM, int kPerCu, bool kExact>
