@@ -109,7 +109,15 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
       for (int k = 1; k < kWaves; ++k) v[g] += red[k][g][lane];
     }
     by_activation(a.act, [&](auto act) {
-      store_block<act.value, kExact>(a, v, sg, row, row_end, q);
+      float h[8];
+      uint32_t amax = gated_block<act.value, kExact>(v, h);
+      if (amax == kInfBits) amax = finite_max(h);
+      const int scale = mx8_scale(__uint_as_float(block_max(amax)));
+      if (row >= row_end) return;
+      *reinterpret_cast<u32x2*>(a.out_codes + static_cast<size_t>(row) * a.Ip + sg * kMxBlock + 8 * q) =
+          mx8_codes(h, scale);
+      if (q == 0)
+        a.out_scales[static_cast<size_t>(row) * (a.Ip / kMxBlock) + sg] = static_cast<uint8_t>(scale);
     });
   } else {
     // Group g by wave g.

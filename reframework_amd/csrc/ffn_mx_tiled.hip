@@ -304,28 +304,64 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
     else
       run_steps(std::false_type());
 
-    const int row1 = it.row0 + 16 * wm + r;
+    const int n_rows = it.row_end - it.row0, row1 = 16 * wm + r;
     if constexpr (kGateUp) {
+      // Stored relative to the tile's first row; an offset out of range stores nothing.
+      const auto codes = pipe::lds_rsrc(a.out_codes + static_cast<size_t>(it.row0) * a.Ip);
+      const auto scales = pipe::lds_rsrc(a.out_scales + static_cast<size_t>(it.row0) * (a.Ip / kMxBlock));
       by_activation(a.act, [&](auto act) {
+        // Two rows of blocks at once, which cover each other's latency (all at once
+        // do not fit the registers).
+        constexpr int kGroup = 2;
+        static_assert(kMT % kGroup == 0, "rows of blocks");
 #pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          if (m >= mt) continue;
+        for (int m0 = 0; m0 < kMT; m0 += kGroup) {
+          if (m0 >= mt) continue;
+          float h[kGroup][kNT / 4][8];
+          uint32_t amax[kGroup][kNT / 4], largest = 0;
 #pragma unroll
-          for (int h = 0; h < kNT / 4; ++h)
-            store_block<act.value, kExact>(a, &acc[m][4 * h],
-                                           it.wt * (kBN / kMxSuper) + wn * (kNT / 4) + h,
-                                           row1 + 16 * WM * m, it.row_end, q);
+          for (int m = 0; m < kGroup; ++m)
+#pragma unroll
+            for (int b = 0; b < kNT / 4; ++b) {
+              amax[m][b] = gated_block<act.value, kExact>(&acc[m0 + m][4 * b], h[m][b]);
+              largest = max(largest, amax[m][b]);
+            }
+          if (largest == kInfBits) {
+#pragma unroll
+            for (int m = 0; m < kGroup; ++m)
+#pragma unroll
+              for (int b = 0; b < kNT / 4; ++b) amax[m][b] = finite_max(h[m][b]);
+          }
+#pragma unroll
+          for (int m = 0; m < kGroup; ++m)
+#pragma unroll
+            for (int b = 0; b < kNT / 4; ++b) amax[m][b] = block_max(amax[m][b]);
+#pragma unroll
+          for (int m = 0; m < kGroup; ++m) {
+            const int row = row1 + 16 * WM * (m0 + m);
+#pragma unroll
+            for (int b = 0; b < kNT / 4; ++b) {
+              const int sg = it.wt * (kBN / kMxSuper) + wn * (kNT / 4) + b;
+              const int scale = mx8_scale(__uint_as_float(amax[m][b]));
+              __builtin_amdgcn_raw_buffer_store_b64(
+                  mx8_codes(h[m][b], scale), codes,
+                  row < n_rows ? row * a.Ip + sg * kMxBlock + 8 * q : pipe::kPadOffset, 0, 0);
+              __builtin_amdgcn_raw_buffer_store_b8(
+                  static_cast<uint8_t>(scale), scales,
+                  row < n_rows && q == 0 ? row * (a.Ip / kMxBlock) + sg : pipe::kPadOffset, 0, 0);
+            }
+          }
         }
       });
     } else {
 #pragma unroll
       for (int m = 0; m < kMT; ++m) {
         const int row = row1 + 16 * WM * m;
-        const size_t at = (static_cast<size_t>(it.e_split >> 8) * a.R + row) * a.H;
+        const size_t at = (static_cast<size_t>(it.e_split >> 8) * a.R + it.row0 + row) * a.H;
 #pragma unroll
         for (int g = 0; g < kNT; ++g) {
           const int col = it.wt * kBN + (wn * kNT + g) * 16 + 4 * q;
-          if (row >= it.row_end || col >= a.H) continue;
+          if (row >= n_rows || col >= a.H) continue;
           const f32x4 v = acc[m][g];
           if (!kExact && a.y16)
             store4<bf16>(static_cast<bf16*>(a.y) + at + col, v[0], v[1], v[2], v[3]);

@@ -35,10 +35,7 @@ __device__ __forceinline__ void quantize8(const MxQuantArgs& a, size_t i) {
   amax = fmaxf(amax, __shfl_xor(amax, 1, kWave));
   amax = fmaxf(amax, __shfl_xor(amax, 2, kWave));
   const int b = mx8_scale(amax);
-  const float f = mx_inverse(b);
-  *reinterpret_cast<u32x2*>(a.codes + static_cast<size_t>(t) * a.Hp + c) =
-      u32x2{mx8_codes(v[0] * f, v[1] * f, v[2] * f, v[3] * f),
-            mx8_codes(v[4] * f, v[5] * f, v[6] * f, v[7] * f)};
+  *reinterpret_cast<u32x2*>(a.codes + static_cast<size_t>(t) * a.Hp + c) = mx8_codes(v, b);
   if ((threadIdx.x & 3) == 0)
     a.scales[static_cast<size_t>(t) * (a.Hp / kMxBlock) + c / kMxBlock] = static_cast<uint8_t>(b);
 }

@@ -48,37 +48,38 @@ __device__ __forceinline__ bf16x8 tokens_bf16(uint32_t lo, uint32_t hi, float s)
               __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
 }
 
-// The gated activation of one supergroup for one token, in 8 bits: lane q holds
-// features 8 q .. 8 q + 7 of the block (v: gate, up of the lower four, then of the
-// upper four), whose maximum is over the token's four lanes. It runs while the
-// matrix cores wait, so instructions count: infinities and NaN cost a branch that is
-// seldom taken instead of a test per value.
+// The gated activation of one supergroup for one token, to be stored in 8 bits: lane q
+// holds features 8 q .. 8 q + 7 of the block (v: gate, up of the lower four, then of
+// the upper four). Returns the bits of their largest magnitude.
 template <int kAct, bool kExact>
-__device__ __forceinline__ void store_block(const MxFfnArgs& a, const f32x4* v, int sg, int row,
-                                            int row_end, int q) {
-  float h[8], amax = 0.f;
+__device__ __forceinline__ uint32_t gated_block(const f32x4* v, float* h) {
+  float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float g = v[i / 4 * 2][i % 4], u = v[i / 4 * 2 + 1][i % 4];
     h[i] = (kExact ? gate_act(kAct, g) : gate_act_fast(kAct, g)) * u;
     amax = fmaxf(amax, fabsf(h[i]));  // ignores NaN
   }
-  if (amax == INFINITY) {
-    amax = 0.f;
+  return __float_as_uint(amax);
+}
+
+// The same without infinities, which have no part in a block's scale. This and what
+// follows runs while the matrix cores wait, so instructions count: infinities cost a
+// branch that is seldom taken instead of a test per value.
+constexpr uint32_t kInfBits = 0x7f800000u;
+__device__ __forceinline__ uint32_t finite_max(const float* h) {
+  float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_finite_abs(h[i]));
-  }
-  amax = fmaxf(amax, __shfl_xor(amax, 16, kWave));
-  amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
-  const int b = mx8_scale(amax);
-  const float f = mx_inverse(b);
-  if (row < row_end) {
-    *reinterpret_cast<u32x2*>(a.out_codes + static_cast<size_t>(row) * a.Ip + sg * kMxBlock + 8 * q) =
-        u32x2{mx8_codes(h[0] * f, h[1] * f, h[2] * f, h[3] * f),
-              mx8_codes(h[4] * f, h[5] * f, h[6] * f, h[7] * f)};
-    if (q == 0)
-      a.out_scales[static_cast<size_t>(row) * (a.Ip / kMxBlock) + sg] = static_cast<uint8_t>(b);
-  }
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, mx_finite_abs(h[i]));
+  return __float_as_uint(amax);
+}
+
+// The largest of the token's four lanes (rows of 16 are exchanged without the LDS).
+__device__ __forceinline__ uint32_t block_max(uint32_t amax) {
+  const auto a = __builtin_amdgcn_permlane16_swap(amax, amax, false, false);
+  amax = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
+  return max(b[0], b[1]);
 }
 
 // f(activation as a compile-time constant).

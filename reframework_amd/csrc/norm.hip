@@ -170,11 +170,9 @@ __global__ __launch_bounds__(kThreads) void add_rmsnorm_kernel(const NormArgs a)
 #pragma unroll
       for (int l = 1; l < kMxBlock / N; l <<= 1) amax = fmaxf(amax, __shfl_xor(amax, l, kWave));
       const int b = mx8_scale(amax);
-      const float f = mx_inverse(b);
       uint32_t* q = reinterpret_cast<uint32_t*>(a.codes + static_cast<size_t>(t) * a.Hp + ch * N);
 #pragma unroll
-      for (int i = 0; i < N; i += 4)
-        q[i / 4] = mx8_codes(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+      for (int i = 0; i < N; i += 4) q[i / 4] = mx8_codes4(o + i, b);
       if (tid % (kMxBlock / N) == 0)
         a.scales[static_cast<size_t>(t) * (a.Hp / kMxBlock) + ch * N / kMxBlock] =
             static_cast<uint8_t>(b);
