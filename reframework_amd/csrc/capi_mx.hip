@@ -19,10 +19,11 @@ bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 // experts of H 4096, I 14336 at 8 rows 117 / 132, 12 rows 125 / 136 (and with more than 16
 // rows for one expert in ten, some 137), 16 rows 131 / 136, 20 rows 262 / 145; 64 experts
 // of H 2048, I 1408 at 8 rows 51 / 53, 12 rows 52 / 53, 20 rows 110 / 55. 64 / 256 rows: the
-// former at 128 rows 280 / 385, 160 rows 369 / 380, 192 rows 396 / 385, 256 rows 468 / 425; the
-// latter at 128 rows 92 / 122, 192 rows 132 / 131, 256 rows 170 / 143, 512 rows 403 / 298. Exact products, 64 / 128 rows: the former at
-// 128 rows 444 / 488, 256 rows 827 / 728, 1024 rows 2710 / 2369; the latter at 128 rows 168 /
-// 161, 192 rows 253 / 287, 256 rows 341 / 300.
+// former at 128 rows 253 / 266, 160 rows 373 / 294, 256 rows 475 / 335; the latter at 128
+// rows 91 / 109, 160 rows 128 / 120, 192 rows 126 / 131, 256 rows 166 / 138; 32 experts of
+// H 1280, I 3328 at 192 rows 96 / 122, 224 rows 125 / 118. Exact products, 64 / 128 rows: the
+// former at 128 rows 436 / 398, 192 rows 618 / 664, 256 rows 809 / 730; the latter at 192
+// rows 252 / 282, 256 rows 314 / 300.
 constexpr int kMxStreamRows = 10, kMxTile64Rows = 176, kMxTile64RowsExact = 224;
 
 // The stages of one expert call and where their data lies in the workspace.

@@ -90,9 +90,11 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
   const int q = lane >> 4, r = lane & 15;
 
   // This workgroup's items: one of every gridDim.x, the workgroups of an XCD taking
-  // neighbouring ones, each time one further: without that, experts of two tiles would
+  // neighbouring ones, each time some further: otherwise experts of two tiles would
   // give one workgroup all full tiles and the next all partial ones (64 experts of 350
-  // rows, 2048 x 1408: 141 us, without 153).
+  // rows, 2048 x 1408: 153 us, so 141). Grids of 256 or 512 and kShift more share no
+  // factor up to 16 with the number of tiles.
+  constexpr int kShift = 15;
   const int nw = (a.n_super * kMxSuper + kBN - 1) / kBN;
   const int per_split = a.tile_map[0] * nw, total = per_split * a.splits;
   const int G = gridDim.x, pid = blockIdx.x;
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
   if (n_items == 0) return;
   if (wave == 0 && lane < n_items) {
     const int n = lane < rounds ? G : tail;
-    items[lane] = decode_item<BM>(a, lane * G + (xcd_remap(pid, n) + lane) % n, nw, per_split);
+    items[lane] = decode_item<BM>(a, lane * G + (xcd_remap(pid, n) + kShift * lane) % n, nw, per_split);
   }
   __syncthreads();
   auto item_at = [&](int j) {
