@@ -425,7 +425,14 @@ def fused_experts_static(x: torch.Tensor, w1_ptrs: Sequence[int], w2_ptrs: Seque
 # Entry points of the 8-bit and 4-bit formats and of the routing by groups. Each runs
 # with its tensors' device current: a launch goes to the current device. At decode
 # sizes a call is bound by its host time, so these look nothing up twice.
-_get_device = torch._C._cuda_getDevice
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _rows(n: int) -> int:
+    """A row count as the C side takes it."""
+    if n > 0x7FFFFFFF:
+        raise ValueError(f"{n} rows, at most {0x7FFFFFFF}")
+    return n
 
 
 def _call(device: torch.device, name: str, *args) -> None:
@@ -444,7 +451,7 @@ def mx_quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                 stream: Optional[int] = None) -> None:
     T, H = x.shape
     s = stream if stream is not None else stream_handle(x.device)
-    _call(x.device, "moe355_mx_quantize", _ptr(x), T, H, dtype_code(x.dtype), _ptr(codes),
+    _call(x.device, "moe355_mx_quantize", _ptr(x), _rows(T), H, dtype_code(x.dtype), _ptr(codes),
           _ptr(scales), s)
 
 
@@ -458,7 +465,7 @@ def add_rmsnorm_mxfp8(T: int, H: int, x: torch.Tensor, residual: Optional[torch.
     _call(device, "moe355_add_rmsnorm_mxfp8", x.data_ptr(),
           None if residual is None else residual.data_ptr(),
           None if residual_out is None else residual_out.data_ptr(), weight.data_ptr(),
-          None if bias is None else bias.data_ptr(), dtype_code(weight.dtype), eps, T, H,
+          None if bias is None else bias.data_ptr(), dtype_code(weight.dtype), eps, _rows(T), H,
           dtype_code(x.dtype), normed_out.data_ptr(), codes.data_ptr(), scales.data_ptr(),
           stream if stream is not None else stream_handle(device))
 
@@ -471,7 +478,7 @@ def grouped_topk(logits: torch.Tensor, bias: Optional[torch.Tensor], K: int, sco
     T, E = logits.shape
     device = logits.device
     _call(device, "moe355_grouped_topk", logits.data_ptr(),
-          None if bias is None else bias.data_ptr(), T, E, K, scoring, num_groups, topk_groups,
+          None if bias is None else bias.data_ptr(), _rows(T), E, K, scoring, num_groups, topk_groups,
           group_score, int(renormalize), scale, topk_w.data_ptr(), topk_ids.data_ptr(),
           int(topk_ids.dtype == torch.int64), topk_w.shape[1],
           stream if stream is not None else stream_handle(device))
@@ -481,7 +488,7 @@ def router_logits(x: torch.Tensor, gate: torch.Tensor, round_logits: bool,
                   logits_out: torch.Tensor, stream: Optional[int] = None) -> None:
     T, H = x.shape
     s = stream if stream is not None else stream_handle(x.device)
-    _call(x.device, "moe355_router_logits", _ptr(x), _ptr(gate), T, H, gate.shape[0],
+    _call(x.device, "moe355_router_logits", _ptr(x), _ptr(gate), _rows(T), H, gate.shape[0],
           dtype_code(x.dtype), int(round_logits), _ptr(logits_out), s)
 
 
@@ -513,7 +520,7 @@ def mx_workspace_bytes(T: int, H: int, I: int, E: int, K: int, dtype: int,
     n = _MX_WORKSPACES.get(key)
     if n is None:
         v = ctypes.c_size_t()
-        _call(device, "moe355_mx_workspace_bytes", T, H, I, E, K, dtype, ctypes.byref(v))
+        _call(device, "moe355_mx_workspace_bytes", _rows(T), H, I, E, K, dtype, ctypes.byref(v))
         n = int(v.value)
         with _lock:
             _MX_WORKSPACES[key] = n

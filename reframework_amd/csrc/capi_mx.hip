@@ -120,6 +120,24 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
 // padding: a call of more 8-bit bytes than that runs in parts.
 int max_tokens(int H) { return INT_MAX / mx_pad(H); }
 
+// Bytes that a call of T tokens needs: those of its full parts or of its last one, whose
+// plan may cut the columns into more parts.
+int mx_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes) {
+  MxPlan p;
+  if (int rc = mx_plan(T, H, I, E, K, dtype, &p)) return rc;
+  if (T > max_tokens(H)) {
+    const int rest = T % max_tokens(H);
+    if (int rc = mx_plan(max_tokens(H), H, I, E, K, dtype, &p)) return rc;
+    *bytes = p.bytes;
+    if (rest == 0) return MOE355_OK;
+    if (int rc = mx_plan(rest, H, I, E, K, dtype, &p)) return rc;
+    *bytes = std::max(*bytes, p.bytes);
+    return MOE355_OK;
+  }
+  *bytes = p.bytes;
+  return MOE355_OK;
+}
+
 struct MxCall {
   const void* x;
   const uint8_t* x_scales;  // nullptr: x is to be quantised
@@ -202,8 +220,16 @@ int moe355_mx_quantize(const void* x, int T, int H, int dtype, void* codes, void
   if (T == 0) return MOE355_OK;
   if (!x || !codes || !scales) return fail(MOE355_EINVAL, "NULL tensor argument");
   if (!aligned16(x) || !aligned16(codes)) return fail(MOE355_EINVAL, "x/codes not 16-byte aligned");
-  const MxQuantArgs a{x, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), T, H, mx_pad(H)};
-  return check_hip(launch_mx_quantize(a, dtype, as_stream(stream)), "mx_quantize launch");
+  // In parts that a grid's 32 bits of threads hold.
+  for (int t = 0; t < T; t += max_tokens(H)) {
+    const size_t row = t, Hp = mx_pad(H);
+    const MxQuantArgs a{static_cast<const char*>(x) + row * H * elem_size(dtype),
+                        static_cast<uint8_t*>(codes) + row * Hp,
+                        static_cast<uint8_t*>(scales) + row * (Hp / kMxBlock),
+                        std::min(T - t, max_tokens(H)), H, mx_pad(H)};
+    if (int rc = check_hip(launch_mx_quantize(a, dtype, as_stream(stream)), "mx_quantize launch")) return rc;
+  }
+  return MOE355_OK;
 }
 
 int moe355_add_rmsnorm_mxfp8(const void* x, const void* residual, void* residual_out,
@@ -324,12 +350,7 @@ int moe355_mx_pack(const void* src, const void* src_scales, int rows, int cols, 
 
 int moe355_mx_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes) {
   if (!bytes) return fail(MOE355_EINVAL, "NULL result");
-  MxPlan p;
-  if (int rc = mx_plan(T, H, I, E, K, dtype, &p)) return rc;
-  if (T > max_tokens(H))
-    if (int rc = mx_plan(max_tokens(H), H, I, E, K, dtype, &p)) return rc;
-  *bytes = p.bytes;
-  return MOE355_OK;
+  return mx_bytes(T, H, I, E, K, dtype, bytes);
 }
 
 int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
@@ -337,8 +358,8 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
                             const float* topk_w, const void* topk_ids, int ids_int64, int T, int H,
                             int I, int E, int K, int dtype, int act, void* out, int accumulate_f32,
                             void* workspace, size_t workspace_bytes, void* stream) {
-  MxPlan p;
-  if (int rc = mx_plan(T, H, I, E, K, dtype, &p)) return rc;
+  size_t bytes;
+  if (int rc = mx_bytes(T, H, I, E, K, dtype, &bytes)) return rc;
   if (act < MOE355_ACT_SILU || act > MOE355_ACT_GELU_TANH)
     return fail(MOE355_EINVAL, "unknown activation %d", act);
   if (T == 0) return MOE355_OK;
@@ -348,18 +369,16 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
       !aligned16(w2_scales) || !aligned16(out) ||
       (x_scales && reinterpret_cast<uintptr_t>(x_scales) % 4))
     return fail(MOE355_EINVAL, "x/w1/w2/scales/out not 16-byte aligned");
-  if (T > max_tokens(H))
-    if (int rc = mx_plan(max_tokens(H), H, I, E, K, dtype, &p)) return rc;
-  if (!workspace || workspace_bytes < p.bytes)
+  if (!workspace || workspace_bytes < bytes)
     return fail(MOE355_EWORKSPACE, "workspace of %zu bytes, the call needs %zu", workspace_bytes,
-                p.bytes);
+                bytes);
   if (!aligned16(workspace)) return fail(MOE355_EINVAL, "workspace not 16-byte aligned");
-  const size_t x_row = x_scales ? p.Hp : static_cast<size_t>(H) * elem_size(dtype);
+  const size_t x_row = x_scales ? mx_pad(H) : static_cast<size_t>(H) * elem_size(dtype);
   const size_t out_row = static_cast<size_t>(H) * (accumulate_f32 ? 4 : elem_size(dtype));
   for (int t = 0; t < T; t += max_tokens(H)) {
     const int n = std::min(T - t, max_tokens(H));
-    if (n != T)
-      if (int rc = mx_plan(n, H, I, E, K, dtype, &p)) return rc;
+    MxPlan p;
+    if (int rc = mx_plan(n, H, I, E, K, dtype, &p)) return rc;
     MxCall c{};
     c.x = static_cast<const char*>(x) + t * x_row;
     c.x_scales = x_scales ? static_cast<const uint8_t*>(x_scales) + t * static_cast<size_t>(p.Hp / kMxBlock) : nullptr;

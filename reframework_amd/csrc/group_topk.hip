@@ -479,7 +479,7 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
     if (a.top2) score = b2 >= INT_MIN + 32 ? KF::of(cut(b1) + cut(b2)) : b1;
     if (!a.top2) score = b1 & ~15;
     if (p.group >= a.G) score = KF::kDead;
-    int rank = 0, above = INT_MAX, below = KF::kDead;  // next scores on both sides
+    int rank = 0, below = KF::kDead;  // groups above this one, the best score of the others
     unroll<1, kRow>([&](auto d) {
       constexpr int D = decltype(d)::value;
       if (D % wr) return;
@@ -487,7 +487,6 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
       const bool first = sub + D >= kRow;  // `other` is of a lower group
       const bool over = other > score || (other == score && first);
       rank += over ? 1 : 0;
-      above = over ? min(above, other) : above;
       below = over ? below : max(below, other);
     });
     const bool kept = p.group < a.G && rank < a.KG;
@@ -590,7 +589,7 @@ hipError_t launch_group_topk(const GroupTopkArgs& args, hipStream_t s) {
   const int width = kWave / slots, per = (a.E / a.G + width - 1) / width;
   if (a.T >= kRowTokens && slots <= kRow && per <= 4 && a.K <= kRowTopk) {
     const int tokens = kThreads / kRow;
-    const dim3 rows((a.T + tokens - 1) / tokens), threads(kThreads);
+    const dim3 rows((a.T - 1) / tokens + 1), threads(kThreads);
     if (per <= 1)
       group_topk_rows_kernel<1><<<rows, threads, 0, s>>>(a, width);
     else if (per <= 2)
@@ -600,7 +599,7 @@ hipError_t launch_group_topk(const GroupTopkArgs& args, hipStream_t s) {
     return hipGetLastError();
   }
   const int tokens = kThreads / kWave;
-  const dim3 grid((a.T + tokens - 1) / tokens), block(kThreads);
+  const dim3 grid((a.T - 1) / tokens + 1), block(kThreads);
   if (per <= 1)
     group_topk_kernel<1><<<grid, block, 0, s>>>(a, width);
   else if (per <= 2)

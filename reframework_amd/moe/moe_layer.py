@@ -130,6 +130,9 @@ class FusedMoE(BaseOP):
             raise ValueError(f"{num_expert_groups} groups do not divide {num_experts} experts")
         if not 1 <= topk_groups <= num_expert_groups:
             raise ValueError(f"topk_groups {topk_groups} outside [1, {num_expert_groups}]")
+        if num_expert_groups > 1 and top_k > topk_groups * (num_experts // num_expert_groups):
+            raise ValueError(f"top_k {top_k} is more than the experts of {topk_groups} of "
+                             f"{num_expert_groups} groups")
         self.num_experts = num_experts
         self.top_k = top_k
         self.hidden_size = hidden_size
@@ -811,9 +814,10 @@ class FusedMoE(BaseOP):
                     raise RuntimeError("4-bit experts load into a resident layer")
                 mx = Mxfp4Experts(count, self.hidden_size, width, device=self.gate.device)
             for key, buf in zip(keys, (mx.w1, mx.w1_scales, mx.w2, mx.w2_scales)):
-                if state_dict[key].shape != buf.shape:
-                    raise ValueError(f"{key}: {tuple(state_dict[key].shape)} does not match "
-                                     f"{tuple(buf.shape)}")
+                if state_dict[key].shape != buf.shape or state_dict[key].dtype != buf.dtype:
+                    raise ValueError(f"{key}: {state_dict[key].dtype} {tuple(state_dict[key].shape)} "
+                                     f"does not match {buf.dtype} {tuple(buf.shape)}")
+            for key, buf in zip(keys, (mx.w1, mx.w1_scales, mx.w2, mx.w2_scales)):
                 buf.copy_(state_dict[key])
             found.append((name, mx))
         if not found:

@@ -41,7 +41,8 @@ def _require_gpu(t: torch.Tensor, what: str) -> None:
 class Mxfp8Rows:
     """[T, size] values in 8 bits: ``codes`` (float8_e4m3fn, [T, size]) times
     ``scales`` (float8_e8m0fnu, [T, size / 32]). The kernels read the padded tensors
-    behind them, whose rows hold whole steps of 128 values."""
+    behind them, whose rows hold whole steps of 128 values: what lies past ``size`` must be
+    zeros (a NaN there would reach the results)."""
 
     __slots__ = ("padded_codes", "padded_scales", "size")
 

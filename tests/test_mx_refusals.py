@@ -138,6 +138,31 @@ def test_workspace_covers_every_stage(T, H, I, E, K):
         assert n >= least
 
 
+@pytest.mark.parametrize("H,I,E,K", [(1 << 20, 1 << 20, 4, 2), (1 << 20, 1 << 17, 1, 1), (1 << 19, 1 << 20, 8, 1),
+                                     (960000, 256, 256, 2)])
+def test_workspace_covers_the_last_part_of_a_call_of_several(H, I, E, K):
+    """Tokens past 2 GB of 8-bit codes run in parts, and the columns of a small last part
+    may be cut into more planes of fp32 results than those of a full one."""
+    part = 0x7FFFFFFF // padded(H)
+    cpu = torch.device("cpu")
+    for dtype in (0, 1, 2):
+        for rest in (0, 1, 3, 17, 200, 1381, part // 3, part // 2, part - 1):
+            whole = _capi.mx_workspace_bytes(part + rest, H, I, E, K, dtype, cpu)
+            assert whole >= _capi.mx_workspace_bytes(part, H, I, E, K, dtype, cpu)
+            assert whole >= _capi.mx_workspace_bytes(rest, H, I, E, K, dtype, cpu)
+
+
+def test_more_rows_than_the_interface_counts():
+    with pytest.raises(ValueError, match="rows"):
+        _capi.mx_workspace_bytes(1 << 32, 64, 64, 1, 1, 1, torch.device("cpu"))
+    big = torch.zeros(1, 1).expand(1 << 31, 1)
+    out = torch.zeros(1, 1)
+    with pytest.raises(ValueError, match="rows"):
+        _capi.grouped_topk(big, None, 1, 0, 1, 1, 0, False, 1.0, out, out, stream=0)
+    with pytest.raises(ValueError, match="rows"):
+        _capi.mx_quantize(big, out, out, stream=0)
+
+
 def _cpu_experts(E=2, H=64, I=32):
     return Mxfp4Experts(E, H, I)
 
