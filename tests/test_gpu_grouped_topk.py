@@ -162,3 +162,26 @@ def test_router_logits(T, E, dt, H, dev):
     _capi.router_logits(x.to(dev), gate.to(dev), True, out)
     rnd = out.to(dt).float()
     assert torch.equal(rnd, out)
+
+
+@pytest.mark.parametrize("T", [37, 8211])
+def test_starts_off_16_bytes_and_two_streams(T, dev):
+    """Logits, bias and results that start on 4 bytes, in two calls at once."""
+    banner(f"grouped_topk alignment T={T}")
+    g = torch.Generator().manual_seed(T)
+    E, K = 64, 6
+    kw = dict(scoring="sigmoid", num_groups=8, topk_groups=3, group_score="top2")
+    flat, bias = torch.randn(T * E + 1, generator=g).to(dev), (torch.randn(E + 1, generator=g) * 0.1).to(dev)
+    pairs = [(flat[1:].view(T, E), bias[1:]), (flat[:-1].view(T, E), bias[:-1])]
+    want = [ref.grouped_topk(l.cpu().numpy(), K, bias=b.cpu().numpy(), **kw) for l, b in pairs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s, (l, b) in zip(streams, pairs):
+            with torch.cuda.stream(s):
+                got.append(grouped_topk(l, K, bias=b, **kw))
+        torch.cuda.synchronize()
+        for (w, ids), (rw, rids) in zip(got, want):
+            assert np.array_equal(ids.cpu().numpy(), rids)
+            assert np.all(np.abs(ref.to64(w) - rw) <= TOL * np.abs(rw) + 1e-30)

@@ -446,3 +446,16 @@ def test_two_streams_at_once(dev):
                 got.append(fused_experts_mxfp4(x, ex, tw, ids))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("T", [3, 150, 900])
+def test_results_in_place_of_the_tokens(T, dev):
+    banner(f"fused_experts_mxfp4 in place T={T}")
+    rng = np.random.default_rng(T)
+    H, E, K, I = 288, 4, 2, 160
+    ex = _experts(_random_codes(E, 2 * I, H, rng), _random_codes(E, H, I, rng), dev)
+    tw, ids = _routing(T, K, E, rng)
+    tw, ids = torch.from_numpy(tw).to(dev), torch.from_numpy(ids).to(dev)
+    x = torch.from_numpy(rng.normal(size=(T, H))).bfloat16().to(dev)
+    want = fused_experts_mxfp4(x, ex, tw, ids)
+    assert fused_experts_mxfp4(x, ex, tw, ids, out=x) is x and torch.equal(x, want)
