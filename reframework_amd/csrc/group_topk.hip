@@ -544,7 +544,9 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
     open = open || (sub < a.K && near(mine, next, 6e-6f) && (sub == a.K - 1 || !ordered));
   }
 
-  // Tokens left open, one after the other by the whole wave.
+  // Tokens left open, one after the other by the whole wave: on the logits where those
+  // decide, else in 64 bits at once (32 bits first took 2 us longer, as in a launch of
+  // thousands of tokens one is open in 64 bits too).
   const unsigned long long left = __ballot(open);
   for (int r = 0; r < kWave / kRow; ++r) {
     if (!((left >> (kRow * r)) & 0xffffull) || t0 + r >= a.T) continue;
@@ -552,8 +554,10 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
     float lw[NW], bw[NW];
     load_token<NW>(a, pw, a.logits + static_cast<size_t>(t0 + r) * a.E, lw, bw);
     const float mw = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), kRow * r));
-    if (select<float, NW>(a, pw, lw, bw, exact, mw, lane, chosen[wave]))
-      select<double, NW>(a, pw, lw, bw, exact, mw, lane, chosen[wave]);
+    if (exact)
+      select<float, NW>(a, pw, lw, bw, true, mw, lane, chosen[wave]);
+    else
+      select<double, NW>(a, pw, lw, bw, false, mw, lane, chosen[wave]);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     if (lane / kRow == r && sub < a.K) {
@@ -572,9 +576,10 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
 }
 
 // Tokens from which four to a wave are faster (256 experts of 8 groups with a bias, one /
-// four to a wave, us a call: 4096 tokens 10.3 / 11.8, 8192 13.1 / 13.0, 16384 19.3 / 16.7,
-// 32768 32 / 23; below, the longer chain of a wave's instructions shows).
-constexpr int kRowTokens = 8192;
+// four to a wave, us a call in a graph: 1024 tokens 4.7 / 9.3, 4096 9.1 / 9.6, 6144 12.0 /
+// 10.8, 16384 19 / 13.8, 32768 32 / 20.8; below, the longer chain of a wave's
+// instructions shows).
+constexpr int kRowTokens = 6144;
 
 }  // namespace
 
