@@ -61,8 +61,9 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
                            : (avg > kMxTile64Rows ? 256 : 64);
   p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
   // A bf16 call of several slots per token keeps their results in bf16 until they are
-  // weighed and added: half the bytes, and a rounding that the sum over the slots
-  // makes smaller than the result's own.
+  // weighed and added, as the 16-bit experts do: half the bytes (4096 tokens of 6 slots,
+  // H 2048: 265 us instead of 286), and a rounding that is at most about as large as
+  // the result's own (error 0.0024 of the results' size instead of 0.0017).
   const bool narrow = p->tiled && !exact && K > 1;
   const int steps = p->Ip / kMxStep;
   int s = 1;
