@@ -75,6 +75,12 @@ __device__ __forceinline__ Item decode_item(const MxFfnArgs& a, int L, int nw, i
   return Item{e + 256 * split, row0, min(row0 + BM, ee), wt};
 }
 
+__device__ __forceinline__ u32x2 pack_bf16(f32x4 v) {
+  typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, bf16x4{from_f32<bf16>(v[0]), from_f32<bf16>(v[1]),
+                                          from_f32<bf16>(v[2]), from_f32<bf16>(v[3])});
+}
+
 template <bool kGateUp, int BM, int WM, int kPerCu, bool kExact>
 __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const MxFfnArgs a) {
   typedef Shape<BM, WM, kPerCu> S;
@@ -364,15 +370,27 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
       for (int m = 0; m < kMT; ++m) {
         const int row = row1 + 16 * WM * m;
         const size_t at = (static_cast<size_t>(it.e_split >> 8) * a.R + it.row0 + row) * a.H;
+        if (!kExact && a.y16) {
+          // Two column groups at once, exchanged between the lanes of a row so that each
+          // stores 16 bytes: 64 consecutive ones of a row instead of 32 (97 us to 87 for
+          // 64 experts of 384 rows, 2048 x 1408).
 #pragma unroll
-        for (int g = 0; g < kNT; ++g) {
-          const int col = it.wt * kBN + (wn * kNT + g) * 16 + 4 * q;
-          if (row >= n_rows || col >= a.H) continue;
-          const f32x4 v = acc[m][g];
-          if (!kExact && a.y16)
-            store4<bf16>(static_cast<bf16*>(a.y) + at + col, v[0], v[1], v[2], v[3]);
-          else
-            *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at + col) = v;
+          for (int g = 0; g < kNT; g += 2) {
+            const int col = it.wt * kBN + (wn * kNT + g + (q & 1)) * 16 + 8 * (q >> 1);
+            const u32x2 u = pack_bf16(acc[m][g]), v = pack_bf16(acc[m][g + 1]);
+            const auto lo = __builtin_amdgcn_permlane16_swap(u[0], v[0], false, false);
+            const auto hi = __builtin_amdgcn_permlane16_swap(u[1], v[1], false, false);
+            if (row < n_rows && col < a.H)
+              *reinterpret_cast<u32x4*>(static_cast<bf16*>(a.y) + at + col) =
+                  u32x4{lo[0], hi[0], lo[1], hi[1]};
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < kNT; ++g) {
+            const int col = it.wt * kBN + (wn * kNT + g) * 16 + 4 * q;
+            if (row < n_rows && col < a.H)
+              *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at + col) = acc[m][g];
+          }
         }
       }
     }
