@@ -78,7 +78,12 @@ class RMSNorm(BaseOP):
             raise ValueError(f"input rows of {x.shape[-1]} do not match the norm's size {H}")
         if H % BLOCK:
             raise ValueError(f"8-bit rows need a size of whole blocks of {BLOCK}, not {H}")
-        w, b = self._params(x)
+        w, b = self.weight, self.bias
+        dev = x.get_device()
+        if not x.is_cuda or w.get_device() != dev or not w.is_contiguous() or (
+                b is not None and (b.dtype != w.dtype or b.get_device() != dev or
+                                   not b.is_contiguous())):
+            w, b = self._params(x)
         T = x.numel() // H
         q = Mxfp8Rows.empty(T, H, x.device)
         _capi.add_rmsnorm_mxfp8(T, H, x, residual, residual_out, w, b, self.eps, out,
@@ -101,7 +106,7 @@ class RMSNorm(BaseOP):
         if residual.dtype != x.dtype:
             residual = residual.to(x.dtype)
         residual = residual.contiguous()
-        if residual.shape != x.shape or residual.device != x.device:
+        if residual.shape != x.shape or residual.get_device() != x.get_device():
             raise ValueError(f"residual {tuple(residual.shape)} on {residual.device} does not match "
                              f"x {tuple(x.shape)} on {x.device}")
         new_res = torch.empty_like(x)

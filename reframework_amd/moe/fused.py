@@ -124,8 +124,8 @@ def grouped_topk(
         logits = logits.float()
     logits = logits.contiguous()
     T, device = logits.shape[0], logits.device
-    w = torch.empty((T, topk), dtype=torch.float32, device=device)
-    ids = torch.empty((T, topk), dtype=torch.int64, device=device)
+    w = torch.empty(T, topk, dtype=torch.float32, device=device)
+    ids = torch.empty(T, topk, dtype=torch.int64, device=device)
     run_grouped_topk(logits, bias, renormalize, scoring, num_groups, topk_groups, group_score,
                      scale, topk, w, ids)
     if len(shape) == 2:
@@ -279,7 +279,7 @@ def fused_experts_mxfp4(
     if out is None:
         if accumulate_f32:
             raise ValueError("accumulate_f32 adds to an fp32 out")
-        out = torch.empty((M, H), dtype=out_type, device=dev)
+        out = torch.empty(M, H, dtype=out_type, device=dev)
     elif out.dtype != out_type or tuple(out.shape) != (M, H) or out.device != dev or \
             not out.is_contiguous():
         raise ValueError(f"out must be contiguous {out_type} [{M}, {H}] on {dev}")

@@ -65,8 +65,8 @@ class Mxfp8Rows:
         """Rows for a kernel to fill (the padding included)."""
         q = cls.__new__(cls)
         Hp = padded(size)
-        q.padded_codes = torch.empty((T, Hp), dtype=torch.float8_e4m3fn, device=device)
-        q.padded_scales = torch.empty((T, Hp // BLOCK), dtype=torch.float8_e8m0fnu, device=device)
+        q.padded_codes = torch.empty(T, Hp, dtype=torch.float8_e4m3fn, device=device)
+        q.padded_scales = torch.empty(T, Hp // BLOCK, dtype=torch.float8_e8m0fnu, device=device)
         q.size = size
         return q
 
