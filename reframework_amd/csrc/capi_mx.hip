@@ -31,7 +31,7 @@ struct MxPlan {
   int rows, n_blocks, tiled, tile_rows, max_tiles, down_splits, down_steps, y16;
   int Hp, Ip;
   size_t block_counts, offsets, slot_to_row, row_src, tile_map, xq, xq_scales, inter,
-      inter_scales, y, bytes;
+      inter_scales, y, y_scales, bytes;
 };
 
 int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
@@ -60,10 +60,10 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
                  : exact   ? (avg > kMxTile64RowsExact ? 128 : 64)
                            : (avg > kMxTile64Rows ? 256 : 64);
   p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
-  // A bf16 call of several slots per token keeps their results in bf16 until they are
-  // weighed and added, as the 16-bit experts do: half the bytes (4096 tokens of 6 slots,
-  // H 2048: 265 us instead of 286), and a rounding that is at most about as large as
-  // the result's own (error 0.0024 of the results' size instead of 0.0017).
+  // A bf16 call of several slots per token keeps their results in 16 bits until they are
+  // weighed and added: half the bytes (4096 tokens of 6 slots, H 2048: 259 us instead of
+  // 286). They are f16 with a scale per 64 columns, whose 11 bits leave the error of the
+  // bf16 sum as it is (0.0017 of the results' size; kept in bf16 it was 0.0024).
   const bool narrow = p->tiled && !exact && K > 1;
   const int steps = p->Ip / kMxStep;
   int s = 1;
@@ -113,6 +113,7 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   p->inter = take(static_cast<size_t>(R) * p->Ip);
   p->inter_scales = take(static_cast<size_t>(R) * p->Ip / kMxBlock);
   p->y = take(static_cast<size_t>(p->down_splits) * R * H * (p->y16 ? 2 : 4));
+  p->y_scales = take(p->y16 ? static_cast<size_t>(R) * (p->Hp / kMxSuper) : 0);
   p->bytes = off;
   return MOE355_OK;
 }
@@ -182,6 +183,7 @@ int mx_run(const MxPlan& p, const MxCall& a, void* workspace, hipStream_t s) {
   f.out_codes = at<uint8_t>(workspace, p.inter);
   f.out_scales = at<uint8_t>(workspace, p.inter_scales);
   f.y = at<void>(workspace, p.y);
+  f.y_scales = at<uint8_t>(workspace, p.y_scales);
   f.y16 = p.y16;
 
   f.x = a.x_scales ? static_cast<const uint8_t*>(a.x) : qa.codes;
@@ -206,6 +208,10 @@ int mx_run(const MxPlan& p, const MxCall& a, void* workspace, hipStream_t s) {
   c.T = a.T; c.K = a.K; c.H = a.H; c.R = p.rows; c.splits = p.down_splits;
   c.accumulate = a.accumulate;
   c.y16 = p.y16;
+  if (p.y16) {
+    c.y_scales = f.y_scales;
+    c.y_blocks = f.n_super;
+  }
   return check_hip(launch_combine(c, a.dtype, s), "combine launch");
 }
 

@@ -18,7 +18,9 @@ constexpr int kThreads = 256;
 // one or two 16-byte loads of fp32 partials.
 template <typename Y, int V>
 __device__ __forceinline__ void loadv(const Y* p, float* o) {
-  if constexpr (std::is_same<Y, float>::value) {
+  if constexpr (std::is_same<Y, Scaled16>::value) {
+    loadv<f16, V>(reinterpret_cast<const f16*>(p), o);
+  } else if constexpr (std::is_same<Y, float>::value) {
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
       const f32x4 v = *reinterpret_cast<const f32x4*>(p + i);
@@ -36,6 +38,14 @@ __device__ __forceinline__ void loadv(const Y* p, float* o) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = t[i];
   }
+}
+
+// What the values of row `row` from column h on are to be multiplied by.
+template <typename Y>
+__device__ __forceinline__ float scale_of(const CombineArgs& a, int row, int h) {
+  if constexpr (std::is_same<Y, Scaled16>::value)
+    return scaled16_value(a.y_scales[static_cast<size_t>(row) * a.y_blocks + h / kScaled16Block]);
+  return 1.f;
 }
 
 template <typename OutT, int V>
@@ -76,6 +86,7 @@ __global__ __launch_bounds__(NT) void combine_kernel(const CombineArgs a) {
     float part[KB][S][V];
 #pragma unroll
     for (int j = 0; j < KB; ++j) {
+      w[j] *= scale_of<Y>(a, row[j] < 0 ? 0 : row[j], h);
       const Y* yr = static_cast<const Y*>(a.y) + static_cast<size_t>(row[j] < 0 ? 0 : row[j]) * a.H + h;
 #pragma unroll
       for (int s = 0; s < S; ++s) loadv<Y, V>(yr + s * plane, part[j][s]);
@@ -137,10 +148,11 @@ __global__ __launch_bounds__(kThreads) void combine_tokens_kernel(const CombineA
 #pragma unroll
   for (int tt = 0; tt < TPB; ++tt)
 #pragma unroll
-    for (int j = 0; j < KM; ++j)
-      loadv<Y, V>(static_cast<const Y*>(a.y) +
-                      static_cast<size_t>(row[tt][j] < 0 ? 0 : row[tt][j]) * a.H + h,
-                  part[tt][j]);
+    for (int j = 0; j < KM; ++j) {
+      const int r = row[tt][j] < 0 ? 0 : row[tt][j];
+      loadv<Y, V>(static_cast<const Y*>(a.y) + static_cast<size_t>(r) * a.H + h, part[tt][j]);
+      w[tt][j] *= scale_of<Y>(a, r, h);
+    }
 #pragma unroll
   for (int tt = 0; tt < TPB; ++tt) {
     if (t0 + tt >= a.T) break;
@@ -194,7 +206,9 @@ hipError_t launch_combine_v(const CombineArgs& a, int dtype, hipStream_t s) {
   const dim3 grid(a.T, (a.H + NT * V - 1) / (NT * V)), block(NT);
   if (a.y16) {
     if (a.splits != 1 || dtype == MOE355_F32) return hipErrorInvalidValue;
-    if (dtype == MOE355_BF16)
+    if (a.y_scales)
+      combine_kernel<OutT, Scaled16, 1, V, NT><<<grid, block, 0, s>>>(a);
+    else if (dtype == MOE355_BF16)
       combine_kernel<OutT, bf16, 1, V, NT><<<grid, block, 0, s>>>(a);
     else
       combine_kernel<OutT, f16, 1, V, NT><<<grid, block, 0, s>>>(a);
@@ -222,6 +236,7 @@ hipError_t launch_combine_t(const CombineArgs& a, int dtype, hipStream_t s) {
   if (a.H % 8 == 0 && wide >= 2ll * device_cu_count()) {
     if (a.splits == 1 && a.K <= 8) {
       if (!a.y16) return launch_combine_tokens_k<OutT, float>(a, s);
+      if (a.y_scales) return launch_combine_tokens_k<OutT, Scaled16>(a, s);
       if (dtype == MOE355_BF16) return launch_combine_tokens_k<OutT, bf16>(a, s);
       if (dtype == MOE355_F16) return launch_combine_tokens_k<OutT, f16>(a, s);
       return hipErrorInvalidValue;

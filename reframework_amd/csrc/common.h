@@ -283,8 +283,27 @@ struct GroupTopkArgs {
   float scale;
 };
 
+// y in 16 bits with a scale per 64 columns: f16 values times 2^(b - 141), b >= 15 the byte of
+// the block (scaled16_byte).
+struct Scaled16 {
+  f16 v;
+};
+constexpr int kScaled16Block = 64;
+
+// The byte of a block whose largest finite magnitude has these bits, and the factor that
+// brings it to [2^14, 2^15), where f16 has all its bits for what lies up to 2^28 below.
+__device__ __forceinline__ int scaled16_byte(uint32_t amax) { return max(static_cast<int>(amax >> 23), 15); }
+__device__ __forceinline__ float scaled16_factor(int b) {
+  return __uint_as_float(static_cast<uint32_t>(268 - b) << 23);
+}
+__device__ __forceinline__ float scaled16_value(int b) {
+  return __uint_as_float(static_cast<uint32_t>(b - 14) << 23);
+}
+
 struct CombineArgs {
   const void* y;             // [S,R,H] fp32, or [R,H] in the layer dtype (y16)
+  const uint8_t* y_scales;   // y16 with these: Scaled16, bytes [R, y_blocks]
+  int y_blocks;
   const float* topk_w;       // [T,K]
   const int32_t* slot_to_row;  // [T*K]
   void* out;                 // [T,H]

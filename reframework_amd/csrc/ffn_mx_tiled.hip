@@ -82,10 +82,10 @@ __device__ __forceinline__ Item decode_item(const MxFfnArgs& a, int L, int nw, i
   return Item{e + 256 * split, row0, min(row0 + BM, ee), wt};
 }
 
-__device__ __forceinline__ u32x2 pack_bf16(f32x4 v) {
-  typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(u32x2, bf16x4{from_f32<bf16>(v[0]), from_f32<bf16>(v[1]),
-                                          from_f32<bf16>(v[2]), from_f32<bf16>(v[3])});
+__device__ __forceinline__ u32x2 pack_f16(f32x4 v) {
+  typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, f16x4{from_f32<f16>(v[0]), from_f32<f16>(v[1]),
+                                         from_f32<f16>(v[2]), from_f32<f16>(v[3])});
 }
 
 template <bool kGateUp, int BM, int WM, int kPerCu, bool kExact>
@@ -375,22 +375,51 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
     } else {
 #pragma unroll
       for (int m = 0; m < kMT; ++m) {
+        if (m >= mt) continue;
         const int row = row1 + 16 * WM * m;
         const size_t at = (static_cast<size_t>(it.e_split >> 8) * a.R + it.row0 + row) * a.H;
         if (!kExact && a.y16) {
-          // Two column groups at once, exchanged between the lanes of a row so that each
-          // stores 16 bytes: 64 consecutive ones of a row instead of 32 (97 us to 87 for
-          // 64 experts of 384 rows, 2048 x 1408).
+          // 16 bits with a scale per 64 columns (Scaled16). Two column groups are exchanged
+          // between the lanes of a row so that each stores 16 bytes: 64 consecutive ones
+          // of a row instead of 32 (97 us to 87 for 64 experts of 384 rows, 2048 x 1408).
+          int byte[kNT / 4];
+          float amax[kNT / 4], largest = 0.f;
 #pragma unroll
-          for (int g = 0; g < kNT; g += 2) {
-            const int col = it.wt * kBN + (wn * kNT + g + (q & 1)) * 16 + 8 * (q >> 1);
-            const u32x2 u = pack_bf16(acc[m][g]), v = pack_bf16(acc[m][g + 1]);
-            const auto lo = __builtin_amdgcn_permlane16_swap(u[0], v[0], false, false);
-            const auto hi = __builtin_amdgcn_permlane16_swap(u[1], v[1], false, false);
-            if (row < n_rows && col < a.H)
-              *reinterpret_cast<u32x4*>(static_cast<bf16*>(a.y) + at + col) =
-                  u32x4{lo[0], hi[0], lo[1], hi[1]};
+          for (int b = 0; b < kNT / 4; ++b) {
+            amax[b] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) amax[b] = fmaxf(amax[b], fabsf(acc[m][4 * b + i / 4][i % 4]));
+            largest = fmaxf(largest, amax[b]);
           }
+          if (largest == INFINITY) {
+#pragma unroll
+            for (int b = 0; b < kNT / 4; ++b) {
+              amax[b] = 0.f;
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                amax[b] = fmaxf(amax[b], mx_finite_abs(acc[m][4 * b + i / 4][i % 4]));
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < kNT / 4; ++b) {
+            const f32x4* v = &acc[m][4 * b];
+            byte[b] = scaled16_byte(block_max(__float_as_uint(amax[b])));
+            const float f = scaled16_factor(byte[b]);
+#pragma unroll
+            for (int g = 0; g < 4; g += 2) {
+              const u32x2 u = pack_f16(v[g] * f), w = pack_f16(v[g + 1] * f);
+              const auto lo = __builtin_amdgcn_permlane16_swap(u[0], w[0], false, false);
+              const auto hi = __builtin_amdgcn_permlane16_swap(u[1], w[1], false, false);
+              const int col = it.wt * kBN + (wn * kNT + 4 * b + g + (q & 1)) * 16 + 8 * (q >> 1);
+              if (row < n_rows && col < a.H)
+                *reinterpret_cast<u32x4*>(static_cast<f16*>(a.y) + at + col) =
+                    u32x4{lo[0], hi[0], lo[1], hi[1]};
+            }
+          }
+          const int block = it.wt * (kBN / kMxSuper) + wn * (kNT / 4) + q;
+          if (q < kNT / 4 && row < n_rows && block < a.n_super)
+            a.y_scales[static_cast<size_t>(it.row0 + row) * a.n_super + block] =
+                static_cast<uint8_t>(q ? byte[kNT / 4 - 1] : byte[0]);
         } else {
 #pragma unroll
           for (int g = 0; g < kNT; ++g) {

@@ -108,7 +108,8 @@ struct MxFfnArgs {
   int Kp, n_super;          // padded columns, supergroups of rows
   int max_tiles, tile_rows, splits, steps_per_split;
   int R, H;                 // down: rows and features of y
-  void* y;                  // down: fp32 [splits, R, H], or bf16 [R, H] (y16: one split)
+  void* y;                  // down: fp32 [splits, R, H], or Scaled16 [R, H] (y16: one split)
+  uint8_t* y_scales;        // [R, n_super]
   int y16;
   uint8_t* out_codes;       // gate_up: [R, Ip]
   uint8_t* out_scales;      // [R, Ip / 32]

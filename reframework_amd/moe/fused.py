@@ -246,8 +246,9 @@ def fused_experts_mxfp4(
     are Mxfp8Rows, e.g. of RMSNorm.forward_add_residual_mxfp8) and the gated activation
     through down in 8 bits. The result is of ``out_dtype``: the tokens' type, bfloat16
     for Mxfp8Rows. A bfloat16 result takes the scaled MFMA, whose products keep about
-    14 bits below the largest they are added to; float16 and float32 results take exact
-    products. Slots whose id lies outside the experts or whose weight is 0 add nothing.
+    14 bits below the largest they are added to, and the results of its slots may be
+    rounded to 11 bits (of values down to 2^-28 of the largest of 64 columns) before they
+    are added; float16 and float32 results take exact products and fp32 slots. Slots whose id lies outside the experts or whose weight is 0 add nothing.
     With ``accumulate_f32`` the result is added to the fp32 ``out``."""
     act = activation_code(activation)
     if isinstance(hidden_states, Mxfp8Rows):

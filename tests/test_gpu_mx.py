@@ -459,3 +459,33 @@ def test_results_in_place_of_the_tokens(T, dev):
     x = torch.from_numpy(rng.normal(size=(T, H))).bfloat16().to(dev)
     want = fused_experts_mxfp4(x, ex, tw, ids)
     assert fused_experts_mxfp4(x, ex, tw, ids, out=x) is x and torch.equal(x, want)
+
+
+@pytest.mark.parametrize("T,E", [(150, 2), (700, 3)])
+def test_slot_results_of_every_magnitude(T, E, dev):
+    """bf16 calls keep the slots' results in 16 bits with a scale per 64 columns: rows
+    from 2^-100 to 2^110, columns of one block 2^20 apart, an infinity beside them.
+    Each row and each column keeps the bar of the whole."""
+    banner(f"fused_experts_mxfp4 magnitudes T={T}")
+    rng = np.random.default_rng(T)
+    H, K, I = 288, 2, 384
+    (c1, s1), (c2, s2) = _random_codes(E, 2 * I, H, rng), _random_codes(E, H, I, rng)
+    s2 = (s2.astype(np.int64) + rng.integers(-10, 11, size=(1, H, 1))).astype(np.uint8)
+    shift = rng.integers(-50, 54, size=(T, 1))
+    x = torch.from_numpy(rng.normal(size=(T, H)) * np.exp2(shift)).bfloat16()
+    tw, ids = _routing(T, K, E, rng)
+    ex = _experts((c1, s1), (c2, s2), dev)
+    want = ref.experts(ref.to64(x), ref.dequant4(c1, s1), ref.dequant4(c2, s2), tw, ids)
+    args = ex, torch.from_numpy(tw).to(dev), torch.from_numpy(ids).to(dev)
+    got = ref.to64(fused_experts_mxfp4(x.to(dev), *args))
+    size = np.linalg.norm(want, axis=1, keepdims=True)
+    assert size.max() / size.min() > 2.0 ** 150
+    err, want = (got - want) / size, want / size
+    for axis in (0, 1):
+        assert np.all(np.linalg.norm(err, axis=axis) <= REL[torch.bfloat16] * np.linalg.norm(want, axis=axis))
+    # a row of w2 with a NaN scale spoils its column and no other of its block
+    s2[:, 70, 0] = 255
+    bad = ref.to64(fused_experts_mxfp4(x.to(dev), _experts((c1, s1), (c2, s2), dev), *args[1:]))
+    assert np.all(np.isnan(bad[:, 70]))
+    keep = np.arange(H) != 70
+    assert np.array_equal(bad[:, keep], got[:, keep])
