@@ -73,12 +73,12 @@ class Mxfp8Rows:
     @property
     def codes(self) -> torch.Tensor:
         c = self.padded_codes
-        return c if c.shape[1] == self.size else c[:, :self.size]
+        return c if c.shape[1] == self.size else c.narrow(1, 0, self.size)
 
     @property
     def scales(self) -> torch.Tensor:
         s = self.padded_scales
-        return s if s.shape[1] * BLOCK == self.size else s[:, :self.size // BLOCK]
+        return s if s.shape[1] * BLOCK == self.size else s.narrow(1, 0, self.size // BLOCK)
 
     @property
     def device(self) -> torch.device:
