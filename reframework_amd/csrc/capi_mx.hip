@@ -15,16 +15,23 @@ bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 
 // Average rows per active expert up to which the weights are streamed past 16-row
 // tiles (ffn_mx.hip), and up to which the tiled kernels (ffn_mx_tiled.hip) take tiles
-// of 64 rows; above, 256 (exact products: 128). gate|up + down us, streaming / 64 rows: 8
-// experts of H 4096, I 14336 at 8 rows 117 / 132, 12 rows 125 / 136 (and with more than 16
-// rows for one expert in ten, some 137), 16 rows 131 / 136, 20 rows 262 / 145; 64 experts
-// of H 2048, I 1408 at 8 rows 51 / 53, 12 rows 52 / 53, 20 rows 110 / 55. 64 / 256 rows: the
-// former at 128 rows 253 / 266, 160 rows 373 / 294, 256 rows 475 / 335; the latter at 128
-// rows 91 / 109, 160 rows 128 / 120, 192 rows 126 / 131, 256 rows 166 / 138; 32 experts of
-// H 1280, I 3328 at 192 rows 96 / 122, 224 rows 125 / 118. Exact products, 64 / 128 rows: the
-// former at 128 rows 436 / 398, 192 rows 618 / 664, 256 rows 809 / 730; the latter at 192
-// rows 252 / 282, 256 rows 314 / 300.
-constexpr int kMxStreamRows = 10, kMxTile64Rows = 176, kMxTile64RowsExact = 224;
+// of 64 rows; above, 256 (exact products: 128). gate|up + down us.
+// Streaming / 64 rows: 8 experts of H 4096, I 14336 at 8 rows 117 / 132, 12 rows 125 / 136
+// (and with more than 16 rows for one expert in ten, some 137), 16 rows 131 / 136, 20 rows
+// 262 / 145; 64 experts of H 2048, I 1408 at 8 rows 51 / 53, 12 rows 52 / 53, 20 rows 110 / 55.
+// 64 / 256 rows, whole calls of random routing: the taller tile costs more at the start
+// and end of an item, which few columns do not hide. 16 experts of H 7168, I 2048 at 60 rows
+// 134 / 121, 120 rows 171 / 148; 8 of H 4096, I 14336 at 60 rows 227 / 254, 75 rows 246 / 238,
+// 135 rows 346 / 294; 64 of H 2048, I 1408 (6 slots) at 105 rows 120 / 126, 135 rows 150 / 137;
+// 32 of H 1280, I 3328 (4 slots) at 180 rows 123 / 132, 200 rows 151 / 136; 16 of H 768, I
+// 1536 at 180 rows 41 / 51, 220 rows 44 / 55.
+// Exact products, 64 / 128 rows: the second at 160 rows 519 / 547, 230 rows 691 / 622, 420 rows
+// 1159 / 1088; the third at 160 rows 261 / 272, 230 rows 333 / 323, 420 rows 565 / 527; the fourth
+// at 230 rows 244 / 258, 300 rows 312 / 304.
+constexpr int kMxStreamRows = 10, kMxTile64RowsExact = 224;
+int tile64_rows(int steps, bool exact) {
+  return exact ? kMxTile64RowsExact : std::min(std::max(2000 / steps, 56), 224);
+}
 
 // The stages of one expert call and where their data lies in the workspace.
 struct MxPlan {
@@ -56,9 +63,10 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   const long long avg = R / active;
   p->tiled = avg > kMxStreamRows;
   const bool exact = dtype != MOE355_BF16;
-  p->tile_rows = !p->tiled ? kMxStreamTile
-                 : exact   ? (avg > kMxTile64RowsExact ? 128 : 64)
-                           : (avg > kMxTile64Rows ? 256 : 64);
+  p->tile_rows = !p->tiled                                      ? kMxStreamTile
+                 : avg <= tile64_rows(p->Hp / kMxStep, exact) ? 64
+                 : exact                                      ? 128
+                                                              : 256;
   p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
   // A bf16 call of several slots per token keeps their results in 16 bits until they are
   // weighed and added: half the bytes (4096 tokens of 6 slots, H 2048: 259 us instead of
