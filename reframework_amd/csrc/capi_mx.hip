@@ -15,11 +15,12 @@ bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 
 // Average rows per active expert up to which the weights are streamed past 16-row
 // tiles (ffn_mx.hip), and up to which the tiled kernels (ffn_mx_tiled.hip) take tiles
-// of 64 rows; above, 256 (exact products: 128). gate|up + down us.
-// Streaming / 64 rows: 8 experts of H 4096, I 14336 at 8 rows 117 / 132, 12 rows 125 / 136
-// (and with more than 16 rows for one expert in ten, some 137), 16 rows 131 / 136, 20 rows
-// 262 / 145; 64 experts of H 2048, I 1408 at 8 rows 51 / 53, 12 rows 52 / 53, 20 rows 110 / 55.
-// 64 / 256 rows, whole calls of random routing: the taller tile costs more at the start
+// of 64 rows; above, 256 (exact products: 128). Whole calls of random routing, us.
+// Streaming / 64 rows: 8 experts of H 4096, I 14336 at 8 rows 136 / 149, 12 rows 147 / 151, 14
+// rows 169 / 153, 20 rows 241 / 156; 64 of H 2048, I 1408 (6 slots) at 12 rows 72 / 78, 14 rows
+// 79 / 78; 8 of H 2048, I 8192 at 10 rows 52 / 56, 12 rows 60 / 57; 32 of H 1280, I 3328 (4 slots)
+// at 12 rows 58 / 69, 16 rows 70 / 70.
+// 64 / 256 rows: the taller tile costs more at the start
 // and end of an item, which few columns do not hide. 16 experts of H 7168, I 2048 at 60 rows
 // 134 / 121, 120 rows 171 / 148; 8 of H 4096, I 14336 at 60 rows 227 / 254, 75 rows 246 / 238,
 // 135 rows 346 / 294; 64 of H 2048, I 1408 (6 slots) at 105 rows 120 / 126, 135 rows 150 / 137;
@@ -28,7 +29,7 @@ bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 // Exact products, 64 / 128 rows: the second at 160 rows 519 / 547, 230 rows 691 / 622, 420 rows
 // 1159 / 1088; the third at 160 rows 261 / 272, 230 rows 333 / 323, 420 rows 565 / 527; the fourth
 // at 230 rows 244 / 258, 300 rows 312 / 304.
-constexpr int kMxStreamRows = 10, kMxTile64RowsExact = 224;
+constexpr int kMxStreamRows = 12, kMxTile64RowsExact = 224;
 int tile64_rows(int steps, bool exact) {
   return exact ? kMxTile64RowsExact : std::min(std::max(2000 / steps, 56), 224);
 }
