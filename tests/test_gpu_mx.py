@@ -489,3 +489,23 @@ def test_slot_results_of_every_magnitude(T, E, dev):
     assert np.all(np.isnan(bad[:, 70]))
     keep = np.arange(H) != 70
     assert np.array_equal(bad[:, keep], got[:, keep])
+
+
+@pytest.mark.parametrize("T,K", [(400, 10), (600, 10), (600, 8), (300, 3)])
+def test_many_slots_per_token(T, K, dev):
+    banner(f"fused_experts_mxfp4 T={T} K={K}")
+    rng = np.random.default_rng(T + K)
+    H, E, I = 96, 12, 64
+    w1, w2 = _random_codes(E, 2 * I, H, rng), _random_codes(E, H, I, rng)
+    x = torch.from_numpy(rng.normal(size=(T, H))).bfloat16()
+    tw, ids = _routing(T, K, E, rng)
+    tw[::7, 1] = 0.0  # dropped
+    want = ref.experts(ref.to64(x), ref.dequant4(*w1), ref.dequant4(*w2), tw, ids)
+    ex = _experts(w1, w2, dev)
+    args = x.to(dev), ex, torch.from_numpy(tw).to(dev), torch.from_numpy(ids).to(dev)
+    got = fused_experts_mxfp4(*args)
+    assert _rel(got, want) <= REL[torch.bfloat16]
+    acc = torch.ones((T, H), device=dev)
+    fused_experts_mxfp4(*args, out=acc, accumulate_f32=True)
+    assert _rel(acc, want + 1) <= REL[torch.bfloat16]
+    assert torch.equal(fused_experts_mxfp4(*args), got)
