@@ -16,8 +16,8 @@
 // Rates (random codes): 8 experts of 1024 rows, 4096 x 14336, 256-row tiles, gate|up 805 us
 // (2.39 PFLOP/s), down 345 (2.79), matrix cores 73 % busy at 1.73 to 1.88 GHz, so bound by
 // power; 64 experts of 384 rows, 2048 x 1408: 147 and 87 us, bound by the epilogues and
-// load latency of items of 16 and 11 steps; 8 of 49 rows, exact, 64-row tiles: 130 and 70 us,
-// 3.6 TB/s of weights. One barrier a step instead of two, with the groups half a step
+// load latency of items of 16 and 11 steps; 8 of 49 rows, exact, 64-row tiles: 126 and 68 us,
+// 3.8 TB/s of weights. One barrier a step instead of two, with the groups half a step
 // apart, takes 865 and 387 us in the first of these.
 //
 // A workgroup runs several items, whose steps follow each other in one stream of
@@ -281,6 +281,9 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
           pipe::wait_lgkm0();
           turn();
         }
+        // Conversions and products go before other waves' reads (8 experts of 49 rows,
+        // 4096 x 14336: gate|up 126 us, without 136; the scaled products do not care).
+        if constexpr (kExact) __builtin_amdgcn_s_setprio(1);
         if constexpr (kExact) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -311,6 +314,7 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
             }
           }
         }
+        if constexpr (kExact) __builtin_amdgcn_s_setprio(0);
         if constexpr (kTurns) {
           __builtin_amdgcn_sched_barrier(0);
           if (!second) landed(done + 1);
