@@ -441,6 +441,8 @@ __global__ __launch_bounds__(kThreads, 2 * kPerCu) void mx_tiled_kernel(const Mx
 template <bool kGateUp, int BM, int WM, int kPerCu, bool kExact>
 hipError_t launch_t(const MxFfnArgs& a, hipStream_t s) {
   if (a.max_tiles == 0) return hipSuccess;
+  // every part of the columns has steps: the stream of loads has no empty items
+  if ((a.splits - 1) * a.steps_per_split >= a.Kp / kMxStep) return hipErrorInvalidValue;
   const int nw = (a.n_super * kMxSuper + kBN - 1) / kBN;
   const long long total = static_cast<long long>(a.max_tiles) * nw * a.splits;
   if (total > INT_MAX) return hipErrorInvalidValue;

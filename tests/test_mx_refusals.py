@@ -226,3 +226,12 @@ def test_experts_move_as_a_module_and_keep_their_bytes():
     assert x.nbytes == 2 * (2 * 128 * 128 // 2 + 2 * 128 * 128 // 32 + 128 * 128 // 2 + 128 * 128 // 32)
     assert x.to(torch.float16).w1.dtype == torch.uint8
     assert set(x.state_dict()) == {"w1", "w1_scales", "w2", "w2_scales"}
+
+
+def test_column_parts_are_never_empty():
+    """What mx_plan does to the steps of down on 64- and 256-row tiles: parts c with at least
+    4 c steps."""
+    for steps in range(1, 8193):
+        for c in (1, 2, 4):
+            if c == 1 or steps >= 4 * c:
+                assert (c - 1) * -(-steps // c) < steps
