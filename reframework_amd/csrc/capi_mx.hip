@@ -16,10 +16,10 @@ bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 // Average rows per active expert up to which the weights are streamed past 16-row
 // tiles (ffn_mx.hip), and up to which the tiled kernels (ffn_mx_tiled.hip) take tiles
 // of 64 rows; above, 256 (exact products: 128). Whole calls of random routing, us.
-// Streaming / 64 rows: 8 experts of H 4096, I 14336 at 8 rows 136 / 149, 12 rows 147 / 151, 14
-// rows 169 / 153, 20 rows 241 / 156; 64 of H 2048, I 1408 (6 slots) at 12 rows 72 / 78, 14 rows
-// 79 / 78; 8 of H 2048, I 8192 at 10 rows 52 / 56, 12 rows 60 / 57; 32 of H 1280, I 3328 (4 slots)
-// at 12 rows 58 / 69, 16 rows 70 / 70.
+// Streaming (exact) / 64 rows (scaled): 8 experts of H 4096, I 14336 at 8 rows 138 / 149, 10 rows
+// 133 / 148, 12 rows 159 / 150, 14 rows 172 / 152, 20 rows 251 / 155; 64 of H 2048, I 1408 (6 slots)
+// at 12 rows 70 / 75, 14 rows 78 / 76; 8 of H 2048, I 8192 at 10 rows 51 / 56, 12 rows 56 / 56; 32
+// of H 1280, I 3328 (4 slots) at 12 rows 58 / 68, 16 rows 69 / 69.
 // 64 / 256 rows: the taller tile costs more at the start
 // and end of an item, which few columns do not hide. 16 experts of H 7168, I 2048 at 60 rows
 // 134 / 121, 120 rows 171 / 148; 8 of H 4096, I 14336 at 60 rows 227 / 254, 75 rows 246 / 238,
@@ -186,8 +186,8 @@ int mx_run(const MxPlan& p, const MxCall& a, void* workspace, hipStream_t s) {
   f.row_src = pa.row_src; f.tile_map = pa.tile_map; f.offsets = pa.offsets;
   f.max_tiles = p.max_tiles; f.tile_rows = p.tile_rows;
   f.R = p.rows; f.H = a.H; f.Ip = p.Ip; f.act = a.act;
-  // A bf16 result keeps 8 bits, below which the scaled MFMA's alignment of products
-  // does not show; results of more bits take the exact products.
+  // Tiled calls of a bf16 result take the scaled MFMA (mx_mma.h says what that costs the
+  // result and saves in time); the others, and all streaming ones, exact products.
   f.exact = a.dtype != MOE355_BF16;
   f.out_codes = at<uint8_t>(workspace, p.inter);
   f.out_scales = at<uint8_t>(workspace, p.inter_scales);

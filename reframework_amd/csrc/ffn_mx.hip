@@ -5,10 +5,13 @@
 // rows) of one expert and a tile of up to 16 of its tokens; its four waves split the
 // columns, two steps of 4 KB each in flight, and add their sums in LDS in a fixed
 // order. Weights sit on the M side of the product, tokens on the N side, so a lane
-// ends with 4 consecutive features of one token per group.
-// Weights of 8 experts of H 4096, I 14336 stream at 6.7 and 6.0 TB/s (gate|up and down, 8
-// rows each: 75 and 42 us), of 64 experts of H 2048, I 1408 at 6.2 and 5.1, of two
-// experts of the former for one token at 5.6 and 5.2 (22 and 12 us).
+// ends with 4 consecutive features of one token per group. The products are exact
+// (mx_mma.h) whatever the result's type is: the weights' stream hides them but for some
+// 1.5 us a call (8 experts of H 4096, I 14336, one token 39.0 us with scaled products, 40.7
+// with these; 64 of H 2048, I 1408, 16 tokens of 6 slots 50.1 and 50.9).
+// Weights of 64 experts of H 2048, I 1408 (those of them that 16 tokens reach) stream at 6.0
+// and 4.9 TB/s (gate|up and down, 26 and 15 us), of two experts of H 4096, I 14336 for one
+// token at 5.3 and 5.3 (24 and 12 us).
 #include "dma_pipe.h"
 #include "mx.h"
 
@@ -19,7 +22,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 #include "mx_mma.h"
 
-template <bool kGateUp, bool kExact>
+template <bool kGateUp>
 __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
   constexpr int D = 2;  // steps in flight per wave (4 need more registers and gain nothing)
   __shared__ f32x4 red[kWaves][4][kWave];
@@ -44,7 +47,7 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
   // rows past the tile's last read its first; their results are not stored
   const int p = row < row_end ? row : row0;
   const size_t src = kGateUp ? a.row_src[p] : p;
-  const uint8_t* xp = a.x + src * a.Kp + s0 * kMxStep + (kExact ? 32 * q : 16 * q);
+  const uint8_t* xp = a.x + src * a.Kp + s0 * kMxStep + 32 * q;
   const uint8_t* xsp = a.x_scales + src * (a.Kp / kMxBlock) + s0 * (kMxStep / kMxBlock);
 
   u32x4 wr[D][4], xr[D][2];
@@ -57,7 +60,7 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
     wsr[slot] = ws[st * kWave];
     const u32x4* x = reinterpret_cast<const u32x4*>(xp + st * kMxStep);
     xr[slot][0] = x[0];
-    xr[slot][1] = x[kExact ? 1 : 4];
+    xr[slot][1] = x[1];
     xsr[slot] = *reinterpret_cast<const uint32_t*>(xsp + st * (kMxStep / kMxBlock));
   };
   f32x4 acc[4];
@@ -66,21 +69,14 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
   auto consume = [&](int slot) {
     const uint32_t s = wsr[slot], xs = xsr[slot] >> (8 * q);
     const u32x4* x = xr[slot];
-    if constexpr (kExact) {
-      const float xf = scale_of(xs & 0xffu);
+    const float xf = scale_of(xs & 0xffu);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bf16x8 t = tokens_bf16(x[j / 2][2 * (j % 2)], x[j / 2][2 * (j % 2) + 1], xf);
+    for (int j = 0; j < 4; ++j) {
+      const bf16x8 t = tokens_bf16(x[j / 2][2 * (j % 2)], x[j / 2][2 * (j % 2) + 1], xf);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              weights_bf16(wr[slot][g][j], scale_of((s >> (8 * g)) & 0xffu)), t, acc[g], 0, 0, 0);
-      }
-    } else {
-      acc[0] = mma_scaled<0>(wr[slot][0], s, x, xs, acc[0]);
-      acc[1] = mma_scaled<1>(wr[slot][1], s, x, xs, acc[1]);
-      acc[2] = mma_scaled<2>(wr[slot][2], s, x, xs, acc[2]);
-      acc[3] = mma_scaled<3>(wr[slot][3], s, x, xs, acc[3]);
+      for (int g = 0; g < 4; ++g)
+        acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            weights_bf16(wr[slot][g][j], scale_of((s >> (8 * g)) & 0xffu)), t, acc[g], 0, 0, 0);
     }
   };
 #pragma unroll
@@ -110,7 +106,7 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
     }
     by_activation(a.act, [&](auto act) {
       float h[8];
-      uint32_t amax = gated_block<act.value, kExact>(v, h);
+      uint32_t amax = gated_block<act.value, true>(v, h);
       if (amax == kInfBits) amax = finite_max(h);
       const int scale = mx8_scale(__uint_as_float(block_max(amax)));
       if (row >= row_end) return;
@@ -131,22 +127,18 @@ __global__ __launch_bounds__(kThreads) void mx_ffn_kernel(const MxFfnArgs a) {
   }
 }
 
-template <bool kGateUp, bool kExact>
+template <bool kGateUp>
 hipError_t launch_t(const MxFfnArgs& a, hipStream_t s) {
   if (a.max_tiles == 0) return hipSuccess;
   const dim3 grid(a.max_tiles, a.n_super, a.splits), block(kThreads);
-  mx_ffn_kernel<kGateUp, kExact><<<grid, block, 0, s>>>(a);
+  mx_ffn_kernel<kGateUp><<<grid, block, 0, s>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_mx_gate_up(const MxFfnArgs& a, hipStream_t s) {
-  return a.exact ? launch_t<true, true>(a, s) : launch_t<true, false>(a, s);
-}
+hipError_t launch_mx_gate_up(const MxFfnArgs& a, hipStream_t s) { return launch_t<true>(a, s); }
 
-hipError_t launch_mx_down(const MxFfnArgs& a, hipStream_t s) {
-  return a.exact ? launch_t<false, true>(a, s) : launch_t<false, false>(a, s);
-}
+hipError_t launch_mx_down(const MxFfnArgs& a, hipStream_t s) { return launch_t<false>(a, s); }
 
 }  // namespace moe355

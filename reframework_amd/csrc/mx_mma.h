@@ -7,9 +7,14 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // One 16-row tile times 16 tokens over 128 columns on the scaled MFMA: the
 // instruction applies the blocks' scales. It aligns a step's products to their
-// largest and keeps about 14 bits below it (measured: an error of 5e-6 of the
-// result's typical size for normal data, far below the rounding of a bf16 result);
-// sums over the steps are in fp32.
+// largest and keeps about 14 bits below it (measured: an error of 5e-6 of a sum's
+// typical size for normal data); sums over the steps are in fp32. In gate|up this moves
+// one intermediate in some thousands across a border of its 8-bit code. A bf16 result,
+// whose rounding is off by 1.66e-3 of its size, is off by 1.73e-3 to 1.78e-3 with that (333
+// tokens of 12 experts of H 1248, I 3296; 1024 of 64 of H 2048, I 1408). The tiled kernels of
+// bf16 results take it because exact products cost them 13 to 50 % (us, scaled / exact, 64-row
+// tiles: 8 experts of H 4096, I 14336 at 49 rows 169 / 200; 64 of H 2048, I 1408 at 94 rows
+// 116 / 171; 32 of H 1280, I 3328 at 150 rows 116 / 172).
 template <int g>
 __device__ __forceinline__ f32x4 mma_scaled(u32x4 w, uint32_t ws, const u32x4* x, uint32_t xs, f32x4 c) {
   const i32x8 a = {static_cast<int>(w[0]), static_cast<int>(w[1]), static_cast<int>(w[2]),
@@ -23,7 +28,8 @@ __device__ __forceinline__ f32x4 mma_scaled(u32x4 w, uint32_t ws, const u32x4* x
 }
 
 // The same product in bf16, which holds every code times its scale exactly (4
-// significant bits at most), summed in fp32: for results of more bits than bf16.
+// significant bits at most), summed in fp32: for results of more bits than bf16, and
+// where the weights' stream hides it.
 // Lane (r, q) multiplies columns 32 q + 8 j .. + 7 in the j-th of four MFMAs (the
 // order of columns is free as long as both operands share it).
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));

@@ -509,3 +509,20 @@ def test_many_slots_per_token(T, K, dev):
     fused_experts_mxfp4(*args, out=acc, accumulate_f32=True)
     assert _rel(acc, want + 1) <= REL[torch.bfloat16]
     assert torch.equal(fused_experts_mxfp4(*args), got)
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("T,H,E,K,I", [(1, 4096, 8, 2, 2048), (5, 160, 4, 3, 96), (16, 2048, 64, 6, 1408),
+                                       (40, 1248, 12, 3, 416)])
+def test_few_tokens_per_expert_are_exact_in_bf16_too(T, H, E, K, I, activation, dev):
+    """Calls that stream the weights multiply exactly whatever the result's type is: a
+    bf16 result is the fp32 one rounded once."""
+    banner(f"fused_experts_mxfp4 exact in bf16 T={T} H={H} E={E} K={K} I={I} {activation}")
+    rng = np.random.default_rng(T + H)
+    w1, w2 = _random_codes(E, 2 * I, H, rng), _random_codes(E, H, I, rng)
+    x = quantize_mxfp8(torch.from_numpy(rng.normal(size=(T, H))).bfloat16().to(dev))
+    tw, ids = _routing(T, K, E, rng)
+    args = x, _experts(w1, w2, dev), torch.from_numpy(tw).to(dev), torch.from_numpy(ids).to(dev)
+    full = fused_experts_mxfp4(*args, activation=activation, out_dtype=torch.float32)
+    got = fused_experts_mxfp4(*args, activation=activation, out_dtype=torch.bfloat16)
+    assert torch.equal(got, full.bfloat16())
