@@ -793,44 +793,66 @@ class FusedMoE(BaseOP):
     def _bias_key(prefix: str) -> str:
         return f"{prefix}.gate.e_score_correction_bias" if prefix else "gate.e_score_correction_bias"
 
-    def _load_mxfp4(self, state_dict: Dict[str, torch.Tensor], prefix: str) -> None:
-        """4-bit experts of a quantised layer's state dict, which a layer that is not
-        quantised yet takes over as they are; a quantised layer takes no expert weights."""
+    @staticmethod
+    def _mxfp4_keys(prefix: str, name: str) -> List[str]:
+        head = f"{prefix}.{name}." if prefix else f"{name}."
+        return [head + k for k in ("w1", "w1_scales", "w2", "w2_scales")]
+
+    def _mxfp4_banks(self, state_dict: Dict[str, torch.Tensor],
+                     prefix: str) -> List[Tuple[str, Mxfp4Experts, List[str]]]:
+        """(attribute, bank to fill, its keys) of the 4-bit experts in a state dict, which a
+        layer that is not quantised yet takes over as they are; a quantised layer takes no
+        expert weights. Nothing is changed here: what does not fit is refused before the
+        first copy."""
         head = f"{prefix}." if prefix else ""
         if self.experts_mxfp4 is not None and any(
                 k.startswith((head + "experts.", head + "shared_experts.")) for k in state_dict):
             raise RuntimeError("the experts are in 4 bits already: load weights before "
                                "quantize_experts()")
-        folded, found = self._n_folded, []
-        for name, count, width in (("experts_mxfp4", self.num_experts + folded,
-                                    self.intermediate_size),
-                                   ("shared_mxfp4", 1, self._shared_piece)):
-            keys = [f"{head}{name}.{k}" for k in ("w1", "w1_scales", "w2", "w2_scales")]
-            if not all(k in state_dict for k in keys):
-                continue
+        unfolded = self._shared_piece > 0 and self._shared_piece != self.intermediate_size
+        own = {"experts_mxfp4": (self.num_experts + self._n_folded, self.intermediate_size)}
+        if unfolded:
+            own["shared_mxfp4"] = (1, self._shared_piece)
+        held = {}
+        for name in ("experts_mxfp4", "shared_mxfp4"):
+            keys = self._mxfp4_keys(prefix, name)
+            here = [k for k in keys if k in state_dict]
+            if here and name not in own:
+                raise ValueError(f"{here[0]}: this layer has no such experts")
+            if here and len(here) < len(keys):
+                raise ValueError(f"the state dict holds {', '.join(here)} without "
+                                 f"{', '.join(k for k in keys if k not in here)}")
+            if here:
+                held[name] = keys
+        if not held:
+            return []
+        if len(held) != len(own):
+            raise ValueError("the state dict holds 4-bit experts of only a part of this layer")
+        banks = []
+        for name, keys in held.items():
             mx = getattr(self, name)
             if mx is None:
                 if self.uses_offload or not len(self.experts_w1):
                     raise RuntimeError("4-bit experts load into a resident layer")
+                count, width = own[name]
                 mx = Mxfp4Experts(count, self.hidden_size, width, device=self.gate.device)
             for key, buf in zip(keys, (mx.w1, mx.w1_scales, mx.w2, mx.w2_scales)):
                 if state_dict[key].shape != buf.shape or state_dict[key].dtype != buf.dtype:
                     raise ValueError(f"{key}: {state_dict[key].dtype} {tuple(state_dict[key].shape)} "
                                      f"does not match {buf.dtype} {tuple(buf.shape)}")
+            banks.append((name, mx, keys))
+        return banks
+
+    def _take_mxfp4(self, state_dict: Dict[str, torch.Tensor],
+                    banks: List[Tuple[str, Mxfp4Experts, List[str]]]) -> None:
+        for name, mx, keys in banks:
             for key, buf in zip(keys, (mx.w1, mx.w1_scales, mx.w2, mx.w2_scales)):
                 buf.copy_(state_dict[key])
-            found.append((name, mx))
-        if not found:
-            return
-        unfolded = self._shared_piece > 0 and self._shared_piece != self.intermediate_size
-        names = [name for name, _ in found]
-        if self.experts_mxfp4 is None and names != ["experts_mxfp4"] + ["shared_mxfp4"] * unfolded:
-            raise ValueError("the state dict holds 4-bit experts of only a part of this layer")
-        for name, mx in found:
             setattr(self, name, mx)
-        for name in ("experts_w1", "experts_w2", "shared_w1", "shared_w2"):
-            setattr(self, name, torch.nn.ParameterList())
-        self._checked_tables.clear()
+        if banks:
+            for name in ("experts_w1", "experts_w2", "shared_w1", "shared_w2"):
+                setattr(self, name, torch.nn.ParameterList())
+            self._checked_tables.clear()
 
     def state_dict(self, *, prefix: str = "", result: Optional[dict] = None,
                    destination=None, keep_vars: bool = False) -> Dict[str, torch.Tensor]:
@@ -860,13 +882,14 @@ class FusedMoE(BaseOP):
 
     def load_state_dict(self, state_dict: Dict[str, torch.Tensor], *, prefix: str = "",
                         strict: bool = True, assign: bool = False) -> None:
+        banks = self._mxfp4_banks(state_dict, prefix)
         with torch.no_grad():
             g = f"{prefix}.gate.weight" if prefix else "gate.weight"
             if g in state_dict:
                 self.gate.copy_(state_dict[g].detach().to(dtype=self.dtype))
             if self.expert_bias is not None and self._bias_key(prefix) in state_dict:
                 self.expert_bias.copy_(state_dict[self._bias_key(prefix)].detach())
-            self._load_mxfp4(state_dict, prefix)
+            self._take_mxfp4(state_dict, banks)
             I = self.intermediate_size
             for e in range(len(self.experts_w1)):
                 p = f"{prefix}.experts.{e}" if prefix else f"experts.{e}"
