@@ -13,7 +13,7 @@ read lazily, tensor by tensor, from the ``*.safetensors`` files:
     Qwen2-MoE's per-token ``shared_expert_gate`` is refused: FusedMoE's shared
     experts are ungated, and loading it would silently drop the gate;
   * ``load_moe_layer`` copies one layer's router, experts and shared experts
-    into a FusedMoE's parameters;
+    into a FusedMoE's parameters, or its 4-bit experts;
   * ``load_moe_layer_offload`` copies the router (and shared experts) into the
     module but streams the routed experts straight into the pinned host pool
     of an ExpertOffloadCache, so a checkpoint larger than HBM never
@@ -117,15 +117,29 @@ def _reject_gated_shared_expert(index: SafetensorsIndex, prefix: str) -> None:
                          "load this layer")
 
 
+def _quantised_keys(index: SafetensorsIndex, prefix: str) -> List[str]:
+    """The tensors of a layer's 4-bit experts (mx.Mxfp4Experts), which load together."""
+    head = prefix + "." if prefix else ""
+    return [k for k in _layer_keys(index, prefix)
+            if k.startswith((head + "experts_mxfp4.", head + "shared_mxfp4."))]
+
+
 def load_moe_layer(index: SafetensorsIndex, moe, prefix: str) -> LayerLoadReport:
     """Copy router, routed experts and shared experts of the layer at
     ``prefix`` (e.g. ``model.layers.3.mlp``) into ``moe``'s parameters, one
-    tensor at a time."""
+    tensor at a time. A checkpoint of 4-bit experts (``experts_mxfp4.*``, and
+    ``shared_mxfp4.*`` where the shared experts are not folded) loads them
+    first, all at once; a layer that is not quantised yet then is."""
     _reject_gated_shared_expert(index, prefix)
     rep = LayerLoadReport(prefix)
+    quantised = _quantised_keys(index, prefix)
+    if quantised:
+        moe.load_state_dict({k: index.get(k) for k in quantised}, prefix=prefix)
     expected = list(moe.state_dict(prefix=prefix).keys())
     for key in expected:
-        if key in index:
+        if key in quantised:
+            rep.loaded.append(key)
+        elif key in index:
             moe.load_state_dict({key: index.get(key)}, prefix=prefix)
             rep.loaded.append(key)
         else:
@@ -139,8 +153,12 @@ def load_moe_layer_offload(index: SafetensorsIndex, moe, prefix: str, device,
                            lru_capacity: int) -> Tuple["object", LayerLoadReport]:
     """Router and shared experts into ``moe``; routed experts straight from the
     checkpoint into a new ExpertOffloadCache's host pool (``moe`` then runs
-    in offload mode). Returns (cache, report)."""
+    in offload mode). Returns (cache, report). 4-bit experts are not offloaded."""
     _reject_gated_shared_expert(index, prefix)
+    quantised = _quantised_keys(index, prefix)
+    if moe.experts_mxfp4 is not None or quantised:
+        raise ValueError(f"{prefix}: 4-bit experts are not offloaded"
+                         + (f" (the checkpoint holds {quantised[0]})" if quantised else ""))
     rep = LayerLoadReport(prefix)
     dense = [k for k in moe.state_dict(prefix=prefix).keys() if ".experts." not in k]
     for key in dense:

@@ -5,7 +5,9 @@ from __future__ import annotations
 
 import pytest
 import torch
+from safetensors.torch import save_file
 
+from reframework_amd.checkpoint import SafetensorsIndex, load_moe_layer, load_moe_layer_offload
 from reframework_amd.moe import FusedMoE, Mxfp4Experts
 
 E, K, H, I = 4, 2, 64, 64
@@ -110,3 +112,63 @@ def test_a_tensor_of_another_shape_is_refused_before_any_copy(quantised):
     with pytest.raises(ValueError, match="does not match"):
         moe.load_state_dict(sd)
     assert _holds(moe, before)
+
+
+def _checkpoint(tmp_path, sd):
+    save_file(sd, str(tmp_path / "layer.safetensors"))
+    return SafetensorsIndex(tmp_path)
+
+
+@pytest.mark.parametrize("kw", [{}, BIAS, {"n_shared_experts": 2}, APART],
+                         ids=["plain", "bias", "folded", "apart"])
+@pytest.mark.parametrize("quantised", [False, True])
+def test_checkpoint_of_a_quantised_layer(tmp_path, quantised, kw):
+    p = "model.layers.3.mlp"
+    sd = _bytes(11, p, shared=kw.get("n_shared_experts", 0), apart=kw is APART, bias=kw is BIAS)
+    index = _checkpoint(tmp_path, sd)
+    moe = _quantised(12, **kw) if quantised else _layer(12, **kw)
+    rep = load_moe_layer(index, moe, p)
+    assert sorted(rep.loaded) == sorted(sd) and not rep.missing and not rep.unexpected
+    assert _holds(moe, sd, p)
+
+
+def test_checkpoint_saved_from_a_layer_loads_into_another(tmp_path):
+    moe = _quantised(13, **BIAS)
+    index = _checkpoint(tmp_path, {k: v.detach().contiguous()
+                                   for k, v in moe.state_dict(prefix="m").items()})
+    other = _layer(14, **BIAS)
+    load_moe_layer(index, other, "m")
+    assert _holds(other, moe.state_dict())
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_checkpoint_without_a_tensor_of_a_bank(tmp_path, quantised):
+    sd = _bytes(15, "m")
+    del sd["m.experts_mxfp4.w1_scales"]
+    moe = _quantised(16) if quantised else _layer(16)
+    before = _snapshot(moe)
+    with pytest.raises(ValueError, match="without m.experts_mxfp4.w1_scales"):
+        load_moe_layer(_checkpoint(tmp_path, sd), moe, "m")
+    assert _holds(moe, before)
+
+
+def test_checkpoint_of_16_bit_experts_leaves_a_quantised_layers_experts_and_says_so(tmp_path):
+    plain = _layer(17)
+    index = _checkpoint(tmp_path, {k: v.detach().contiguous()
+                                   for k, v in plain.state_dict(prefix="m").items()})
+    moe = _quantised(18)
+    before = _snapshot(moe)
+    rep = load_moe_layer(index, moe, "m")
+    assert rep.loaded == ["m.gate.weight"] and len(rep.unexpected) == 3 * E
+    assert sorted(rep.missing) == sorted(f"m.experts_mxfp4.{k}" for k in BANK_KEYS)
+    before["gate.weight"] = plain.gate.detach()
+    assert _holds(moe, before)
+
+
+def test_offload_of_4_bit_experts_is_refused(tmp_path):
+    index = _checkpoint(tmp_path, _bytes(19, "m"))
+    for moe in (_layer(20), _quantised(20)):
+        before = _snapshot(moe)
+        with pytest.raises(ValueError, match="not offloaded"):
+            load_moe_layer_offload(index, moe, "m", torch.device("cpu"), 2)
+        assert _holds(moe, before)
