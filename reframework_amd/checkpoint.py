@@ -117,6 +117,15 @@ def _reject_gated_shared_expert(index: SafetensorsIndex, prefix: str) -> None:
                          "load this layer")
 
 
+def _reject_unused_choice_bias(index: SafetensorsIndex, moe, prefix: str) -> None:
+    """A bias for the choice of experts that the layer has no parameter for: it would
+    route without it and choose other experts."""
+    key = f"{prefix}.gate.e_score_correction_bias" if prefix else "gate.e_score_correction_bias"
+    if key in index and moe.expert_bias is None:
+        raise ValueError(f"{key} chooses the experts of this layer; build it with expert_bias=True "
+                         "(or from a config whose topk_method is \"noaux_tc\")")
+
+
 def _quantised_keys(index: SafetensorsIndex, prefix: str) -> List[str]:
     """The tensors of a layer's 4-bit experts (mx.Mxfp4Experts), which load together."""
     head = prefix + "." if prefix else ""
@@ -131,6 +140,7 @@ def load_moe_layer(index: SafetensorsIndex, moe, prefix: str) -> LayerLoadReport
     ``shared_mxfp4.*`` where the shared experts are not folded) loads them
     first, all at once; a layer that is not quantised yet then is."""
     _reject_gated_shared_expert(index, prefix)
+    _reject_unused_choice_bias(index, moe, prefix)
     rep = LayerLoadReport(prefix)
     quantised = _quantised_keys(index, prefix)
     if quantised:
@@ -140,7 +150,7 @@ def load_moe_layer(index: SafetensorsIndex, moe, prefix: str) -> LayerLoadReport
         if key in quantised:
             rep.loaded.append(key)
         elif key in index:
-            moe.load_state_dict({key: index.get(key)}, prefix=prefix)
+            moe.load_state_dict({key: index.get(key)}, prefix=prefix, strict=False)
             rep.loaded.append(key)
         else:
             rep.missing.append(key)
@@ -155,6 +165,7 @@ def load_moe_layer_offload(index: SafetensorsIndex, moe, prefix: str, device,
     checkpoint into a new ExpertOffloadCache's host pool (``moe`` then runs
     in offload mode). Returns (cache, report). 4-bit experts are not offloaded."""
     _reject_gated_shared_expert(index, prefix)
+    _reject_unused_choice_bias(index, moe, prefix)
     quantised = _quantised_keys(index, prefix)
     if moe.experts_mxfp4 is not None or quantised:
         raise ValueError(f"{prefix}: 4-bit experts are not offloaded"
@@ -163,7 +174,7 @@ def load_moe_layer_offload(index: SafetensorsIndex, moe, prefix: str, device,
     dense = [k for k in moe.state_dict(prefix=prefix).keys() if ".experts." not in k]
     for key in dense:
         if key in index:
-            moe.load_state_dict({key: index.get(key)}, prefix=prefix)
+            moe.load_state_dict({key: index.get(key)}, prefix=prefix, strict=False)
             rep.loaded.append(key)
         else:
             rep.missing.append(key)

@@ -68,6 +68,9 @@ from reframework_amd.mx import Mxfp4Experts, Mxfp8Rows
 
 logger = logging.getLogger(__name__)
 
+# Ways of choosing experts that configs name (topk_method).
+TOPK_METHODS = ("greedy", "group_limited_greedy", "noaux_tc")
+
 
 class CpuShuttle:
     """Byte-accounting stand-in for a device-to-device token shuttle.
@@ -202,10 +205,20 @@ class FusedMoE(BaseOP):
         moe_activation, moe_renormalize, dtype; optional entropy_adaptive_k,
         entropy_k_min), honouring RE_ENTROPY_K / RE_ENTROPY_K_MIN. Optional
         ``n_shared_experts`` / ``shared_intermediate_size`` add shared experts, and
-        optional ``scoring_func``, ``n_group``, ``topk_group``, ``routed_scaling_factor``,
-        ``moe_expert_bias`` and ``moe_group_score`` set the routing by groups (a group is
-        scored by its best two experts where there is a bias and nothing else is said)."""
-        expert_bias = bool(getattr(cfg, "moe_expert_bias", False))
+        optional ``scoring_func``, ``n_group``, ``topk_group`` and ``routed_scaling_factor``
+        set the routing by groups. ``topk_method`` says how experts are chosen:
+        ``"noaux_tc"`` with a bias and groups by their best two experts,
+        ``"group_limited_greedy"`` with groups by their best expert, ``"greedy"`` without
+        groups whatever ``n_group`` is; another one is refused, as its choice would be
+        another. ``moe_expert_bias`` and ``moe_group_score`` go before it (without any of
+        them there is no bias; a group is scored by its best two experts where there is a
+        bias)."""
+        method = getattr(cfg, "topk_method", None)
+        if method not in (None, *TOPK_METHODS):
+            raise ValueError(f"unknown topk_method {method!r}; known: {TOPK_METHODS}")
+        bias_field = getattr(cfg, "moe_expert_bias", None)
+        expert_bias = method == "noaux_tc" if bias_field is None else bool(bias_field)
+        grouped = method != "greedy"
         moe = cls(
             num_experts=cfg.num_experts,
             top_k=cfg.num_experts_per_tok,
@@ -217,9 +230,10 @@ class FusedMoE(BaseOP):
             n_shared_experts=int(getattr(cfg, "n_shared_experts", 0) or 0),
             shared_intermediate_size=getattr(cfg, "shared_intermediate_size", None),
             scoring=getattr(cfg, "scoring_func", None) or "softmax",
-            num_expert_groups=int(getattr(cfg, "n_group", None) or 1),
-            topk_groups=int(getattr(cfg, "topk_group", None) or 1),
-            group_score=getattr(cfg, "moe_group_score", None) or ("top2" if expert_bias else "max"),
+            num_expert_groups=int(grouped and getattr(cfg, "n_group", None) or 1),
+            topk_groups=int(grouped and getattr(cfg, "topk_group", None) or 1),
+            group_score=getattr(cfg, "moe_group_score", None) or
+            ("top2" if expert_bias and method != "group_limited_greedy" else "max"),
             expert_bias=expert_bias,
             routed_scale=float(getattr(cfg, "routed_scaling_factor", None) or 1.0),
         )
@@ -882,13 +896,22 @@ class FusedMoE(BaseOP):
 
     def load_state_dict(self, state_dict: Dict[str, torch.Tensor], *, prefix: str = "",
                         strict: bool = True, assign: bool = False) -> None:
+        """Takes the tensors that are there (parameters without one keep their values), but
+        not what would route or compute otherwise than the checkpoint means: a choice
+        bias for a layer without one, with ``strict`` a router without the bias that the
+        layer has, 4-bit experts that are not whole. A refused dict changes nothing."""
+        bias, gate = self._bias_key(prefix), f"{prefix}.gate.weight" if prefix else "gate.weight"
+        if self.expert_bias is None and bias in state_dict:
+            raise ValueError(f"{bias}: the layer was built without a bias for the choice of experts "
+                             "(expert_bias=True, or topk_method \"noaux_tc\" of a config)")
+        if strict and self.expert_bias is not None and gate in state_dict and bias not in state_dict:
+            raise ValueError(f"{gate} without {bias}, which this layer routes with")
         banks = self._mxfp4_banks(state_dict, prefix)
         with torch.no_grad():
-            g = f"{prefix}.gate.weight" if prefix else "gate.weight"
-            if g in state_dict:
-                self.gate.copy_(state_dict[g].detach().to(dtype=self.dtype))
-            if self.expert_bias is not None and self._bias_key(prefix) in state_dict:
-                self.expert_bias.copy_(state_dict[self._bias_key(prefix)].detach())
+            if gate in state_dict:
+                self.gate.copy_(state_dict[gate].detach().to(dtype=self.dtype))
+            if bias in state_dict:
+                self.expert_bias.copy_(state_dict[bias].detach())
             self._take_mxfp4(state_dict, banks)
             I = self.intermediate_size
             for e in range(len(self.experts_w1)):
