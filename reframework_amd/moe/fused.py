@@ -275,8 +275,7 @@ def fused_experts_mxfp4(
     if w1.device != dev or topk_weights.device != dev or topk_ids.device != dev:
         raise ValueError(f"experts on {w1.device}, weights on {topk_weights.device} and ids on "
                          f"{topk_ids.device} must be on the tokens' {dev}")
-    slots = topk_ids.numel()
-    if slots != topk_weights.numel() or (M and slots % M):
+    if topk_ids.dim() != 2 or topk_ids.shape[0] != M or topk_weights.shape != topk_ids.shape:
         raise ValueError(f"topk_ids {tuple(topk_ids.shape)} and topk_weights "
                          f"{tuple(topk_weights.shape)} are not [{M}, K]")
     out_type = torch.float32 if accumulate_f32 else dtype
@@ -291,7 +290,7 @@ def fused_experts_mxfp4(
         return out
     ids = topk_ids if topk_ids.dtype in (torch.int32, torch.int64) else topk_ids.long()
     w = topk_weights if topk_weights.dtype == torch.float32 else topk_weights.float()
-    E, I, K = experts.num_experts, experts.intermediate_size, slots // M
+    E, I, K = experts.num_experts, experts.intermediate_size, topk_ids.shape[1]
     # From the caching allocator on the current stream, not from a buffer that calls
     # share: captured graphs then have workspaces of their own.
     ws = torch.empty(_capi.mx_workspace_bytes(M, H, I, E, K, code, dev), dtype=torch.uint8,

@@ -235,3 +235,17 @@ def test_column_parts_are_never_empty():
         for c in (1, 2, 4):
             if c == 1 or steps >= 4 * c:
                 assert (c - 1) * -(-steps // c) < steps
+
+
+@pytest.mark.parametrize("w,ids", [
+    ((2, 6), (2, 6)),      # of the transposed routing of 6 tokens of 2 slots
+    ((6, 2), (2, 6)), ((2, 6), (6, 2)),
+    ((6, 2), (12,)), ((12,), (6, 2)), ((12,), (12,)),
+    ((3, 4), (3, 4)), ((6, 2), (3, 4)), ((6, 2), (6, 1, 2)), ((6, 2), (6, 3)),
+])
+def test_routing_of_another_shape_than_the_tokens(w, ids):
+    """As many numbers as [6, 2] has, or as their multiples, in other places."""
+    rows = Mxfp8Rows(torch.zeros(6, 128, dtype=torch.uint8).view(torch.float8_e4m3fn),
+                     torch.zeros(6, 4, dtype=torch.uint8).view(torch.float8_e8m0fnu), 64)
+    with pytest.raises(ValueError, match=r"are not \[6, K\]"):
+        fused_experts_mxfp4(rows, _cpu_experts(), torch.ones(w), torch.zeros(ids).long())
