@@ -39,7 +39,7 @@ struct Key;
 template <>
 struct Key<float> {
   typedef int type;
-  static constexpr int kDead = INT_MIN;
+  static constexpr int kDead = INT_MIN, kFirst = INT_MIN + 32;  // keys from kFirst on are of numbers
   __device__ __forceinline__ static int of(float v) {
     const int b = __float_as_int(v + 0.f);
     return v != v ? INT_MIN + 1 : b ^ ((b >> 31) & 0x7fffffff);
@@ -52,7 +52,7 @@ struct Key<float> {
 template <>
 struct Key<double> {
   typedef long long type;
-  static constexpr long long kDead = LLONG_MIN;
+  static constexpr long long kDead = LLONG_MIN, kFirst = LLONG_MIN + 2;
   __device__ __forceinline__ static long long of(double v) {
     const long long b = __double_as_longlong(v + 0.0);
     return v != v ? LLONG_MIN + 1 : b ^ ((b >> 63) & 0x7fffffffffffffffll);
@@ -148,6 +148,27 @@ __device__ __forceinline__ void top2_of_group(I& b1, I& b2, int width) {
   for (int o = 16; o < width; o <<= 1) merge(__shfl_xor(b1, o, kWave), __shfl_xor(b2, o, kWave));
 }
 
+// Whether the groups that are kept are left open: whether a kept one, less its error, does
+// not lie above each of the others, plus theirs. A group's error grows with the
+// choices that were added for it, not with what is left of them: two that
+// cancel leave a small score and the error of large ones. Infinite scores are
+// exact. max_of: the maximum over the token's lanes.
+template <typename KF, typename F, typename M>
+__device__ __forceinline__ bool group_open(typename KF::type score, F error, bool kept, bool group,
+                                           M max_of) {
+  typedef typename KF::type I;
+  const F v = KF::value(score);
+  error = fabs(v) < INFINITY ? error : F(0);
+  const bool real = score >= KF::kFirst;  // no NaN
+  const I low = real ? KF::of(v - error) : score, high = real ? KF::of(v + error) : score;
+  const I worst = ~max_of(kept ? ~low : KF::kDead), best = max_of(group && !kept ? high : KF::kDead);
+  return best >= KF::kFirst && !(KF::value(worst) > KF::value(best));
+}
+
+// The error of a group's score relative to the magnitudes of the choices in it: in each of
+// them 2^-24 from adding the bias, and as much from their sum and from `group_open`'s own.
+constexpr float kRounding = 2.5e-7f;
+
 // The choice of one token into chosen[0..K) (LDS). F float returns whether 32 bits
 // leave it open (`exact`: the choice is made on the logits themselves, which leave
 // nothing open); then nothing else is valid.
@@ -206,7 +227,7 @@ __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, c
   // Whether hi >= lo lie too near each other for 32 bits. The error of c, relative to
   // the largest score plus |c|, is below 4e-7 from the score (exp_of, where |v|
   // exp(-|v|) <= 0.37 bounds what its error grows by, the sum, a reciprocal) and 6e-8
-  // from the sum with the bias; twice that, and twice again for a sum of two.
+  // from the sum with the bias; twice that.
   auto near = [&](I hi, I lo, F eps) {
     const F x = KF::value(hi), y = KF::value(lo);
     return lo > KF::kDead + 1 && !(x - y > eps * (top + fabs(x)));  // infinite ones too
@@ -217,9 +238,8 @@ __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, c
     I b1 = key[0], b2 = NV > 1 ? key[NV > 1 ? 1 : 0] : KF::kDead;
     top2_of_group(b1, b2, p.width);
     // A group's score as a key; with a NaN, and of a single expert, its best.
-    I score = b1;
-    if (a.top2 && b1 > KF::kDead + 1 && b2 > KF::kDead + 1)
-      score = KF::of(KF::value(b1) + KF::value(b2));
+    const bool two = a.top2 && b1 > KF::kDead + 1 && b2 > KF::kDead + 1;
+    I score = two ? KF::of(KF::value(b1) + KF::value(b2)) : b1;
     if (p.group >= a.G) score = KF::kDead;
     int rank = 0;
     for (int g = 0; g < a.G; ++g) {
@@ -228,9 +248,9 @@ __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, c
     }
     const bool kept = p.group < a.G && rank < a.KG;
     if (kTest && !exact) {
-      const I worst = ~wave_max_key(kept ? ~score : KF::kDead);
-      const I best_out = wave_max_key(!kept && p.group < a.G ? score : KF::kDead);
-      open = near(worst, best_out, a.top2 ? F(2e-6) : F(1e-6));
+      const F size = fabs(KF::value(b1)) + (two ? fabs(KF::value(b2)) : F(0));
+      const F error = (two ? F(1e-6) : F(5e-7)) * top + F(kRounding) * size;
+      open = group_open<KF>(score, error, kept, p.group < a.G, [](I v) { return wave_max_key(v); });
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) key[i] = kept ? key[i] : KF::kDead;
@@ -361,6 +381,7 @@ __global__ __launch_bounds__(kThreads) void group_topk_kernel(const GroupTopkArg
 // values) lose nothing.
 constexpr int kRow = 16;
 constexpr int kRowTopk = 8;  // largest K
+constexpr float kRowRounding = kRounding + 0x1p-19f;  // with the cut of the keys
 
 __device__ __forceinline__ int row_max_key(int v) {
   v = max(v, dpp_key<0x121>(v));  // row_ror 1, 2, 4, 8
@@ -452,7 +473,7 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
   const bool lossless = exact && row_max_key(bits & 15) == 0;
   const auto near = [&](int hi, int lo, float eps) {
     const float x = cut(hi), y = cut(lo);
-    return lo >= INT_MIN + 32 && !(x - y > eps * (top + fabsf(x)));
+    return lo >= KF::kFirst && !(x - y > eps * (top + fabsf(x)));
   };
 
   // Largest first (odd-even merge sort of the NV keys).
@@ -478,27 +499,23 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
   if (a.KG < a.G) {
     int b1 = key[0], b2 = key[1];
     top2_of_group(b1, b2, wr);
-    int score = b1;
-    if (a.top2) score = b2 >= INT_MIN + 32 ? KF::of(cut(b1) + cut(b2)) : b1;
-    if (!a.top2) score = b1 & ~15;
+    const bool two = a.top2 && b2 >= KF::kFirst;
+    int score = two ? KF::of(cut(b1) + cut(b2)) : b1 & ~15;
     if (p.group >= a.G) score = KF::kDead;
-    int rank = 0, below = KF::kDead;  // groups above this one, the best score of the others
+    int rank = 0;  // groups above this one
     unroll<1, kRow>([&](auto d) {
       constexpr int D = decltype(d)::value;
       if (D % wr) return;
       const int other = row_ahead<D>(score);
       const bool first = sub + D >= kRow;  // `other` is of a lower group
-      const bool over = other > score || (other == score && first);
-      rank += over ? 1 : 0;
-      below = over ? below : max(below, other);
+      rank += other > score || (other == score && first) ? 1 : 0;
     });
     const bool kept = p.group < a.G && rank < a.KG;
-    // The last kept group and the first one left out lie next to each other.
-    const float eps = a.top2 ? 1.2e-5f : 6e-6f;
-    const int mine = score;
-    if (!lossless || a.top2)
-      open = (kept && rank == a.KG - 1 && below >= INT_MIN + 32 &&
-              !(KF::value(mine) - KF::value(below) > eps * (top + fabsf(KF::value(mine)))));
+    if (!lossless) {
+      const float size = fabsf(cut(b1)) + (two ? fabsf(cut(b2)) : 0.f);
+      const float error = (two ? 2.4e-6f : 1.2e-6f) * top + kRowRounding * size;
+      open = group_open<KF>(score, error, kept, p.group < a.G, [](int v) { return row_max_key(v); });
+    }
 #pragma unroll
     for (int i = 0; i < kList; ++i) key[i] = kept ? key[i] : KF::kDead;
   }

@@ -185,3 +185,20 @@ def test_starts_off_16_bytes_and_two_streams(T, dev):
         for (w, ids), (rw, rids) in zip(got, want):
             assert np.array_equal(ids.cpu().numpy(), rids)
             assert np.all(np.abs(ref.to64(w) - rw) <= TOL * np.abs(rw) + 1e-30)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("b", [100.0, 1.0e4, 1.0e6])
+@pytest.mark.parametrize("T", [6000, 9000])
+def test_groups_whose_best_two_cancel(T, b, scoring, dev):
+    """One expert of each group at +b, the others at -b: the sum of a group's best two
+    keeps nothing of b, but its 32-bit terms are rounded to the bits of b."""
+    banner(f"grouped_topk cancelling biases T={T} b={b} {scoring}")
+    rng = np.random.default_rng(17)
+    E, G = 64, 8
+    bias = np.full(E, -b, np.float32)
+    bias[np.arange(G) * (E // G) + rng.integers(0, E // G, G)] = b
+    for _ in range(4):
+        logits = (rng.normal(size=(T, E)) * 1.5).astype(np.float32)
+        _check(logits, 6, dev, bias=bias, scoring=scoring, num_groups=G, topk_groups=4,
+               group_score="top2")
