@@ -467,9 +467,11 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
     for (int i = 0; i < NV; ++i)
       key[i] = i < p.n ? max(KF::of(c[i]), INT_MIN + 16) & ~15 | (15 - i) : KF::kDead;
   }
-  // The value of a key and whether two lie too near each other: 2^-19 of each from
-  // its cut, and what `select` allows.
-  const auto cut = [](int k) { return KF::value(k & ~15); };
+  // A key without its place, cut towards zero (the bits of a negative value are
+  // inverted in its key, and those of -infinity have to stay), its value, and whether two
+  // lie too near each other: 2^-19 of each from the cut, and what `select` allows.
+  const auto placeless = [](int k) { return (k & ~15) | ((k >> 31) & 15); };
+  const auto cut = [&](int k) { return KF::value(placeless(k)); };
   const bool lossless = exact && row_max_key(bits & 15) == 0;
   const auto near = [&](int hi, int lo, float eps) {
     const float x = cut(hi), y = cut(lo);
@@ -500,7 +502,7 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
     int b1 = key[0], b2 = key[1];
     top2_of_group(b1, b2, wr);
     const bool two = a.top2 && b2 >= KF::kFirst;
-    int score = two ? KF::of(cut(b1) + cut(b2)) : b1 & ~15;
+    int score = two ? KF::of(cut(b1) + cut(b2)) : placeless(b1);
     if (p.group >= a.G) score = KF::kDead;
     int rank = 0;  // groups above this one
     unroll<1, kRow>([&](auto d) {

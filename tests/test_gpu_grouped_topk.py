@@ -202,3 +202,43 @@ def test_groups_whose_best_two_cancel(T, b, scoring, dev):
         logits = (rng.normal(size=(T, E)) * 1.5).astype(np.float32)
         _check(logits, 6, dev, bias=bias, scoring=scoring, num_groups=G, topk_groups=4,
                group_score="top2")
+
+
+@pytest.mark.parametrize("T", [500, 9000])
+def test_a_group_of_nans_is_below_one_that_is_shut_out(T, dev):
+    """A group of NaN, one of a single expert beside some with a bias of -inf (its best two
+    make -inf), two of many: with one group left out it is the NaN one, and the single
+    expert is the first choice."""
+    banner(f"grouped_topk NaN and -inf groups T={T}")
+    rng = np.random.default_rng(29)
+    logits = rng.normal(size=(T, 64)).astype(np.float32)
+    logits[:, :16] = np.nan
+    bias = np.zeros(64, np.float32)
+    bias[16:32] = -np.inf
+    bias[21] = 2.0
+    for score in ("max", "top2"):
+        for K in (4, 8):
+            _check(logits, K, dev, bias=bias, scoring="sigmoid", num_groups=4, topk_groups=3,
+                   group_score=score)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("value", [-np.inf, np.finfo(np.float32).min])
+@pytest.mark.parametrize("score", ["max", "top2"])
+@pytest.mark.parametrize("T", [500, 9000])
+def test_biases_that_shut_experts_out(T, score, value, scoring, dev):
+    """Most experts shut out by the bias, so that groups keep one expert or none; a NaN
+    logit ranks below them still."""
+    banner(f"grouped_topk shut out T={T} {value} {score} {scoring}")
+    rng = np.random.default_rng(23)
+    E, G = 64, 8
+    logits = (rng.normal(size=(T, E)) * 1.5).astype(np.float32)
+    if scoring == "sigmoid":  # a softmax with a NaN is NaN throughout
+        logits[::3, 8:16] = np.nan
+        logits[1::3, 32:40:2] = np.nan
+    bias = (rng.normal(size=E) * 0.1).astype(np.float32)
+    bias[rng.random(E) < 0.7] = value
+    bias[:8] = bias[24:32] = value
+    for KG in (2, 5, 7):
+        _check(logits, 6, dev, bias=bias, scoring=scoring, num_groups=G, topk_groups=KG,
+               group_score=score)
