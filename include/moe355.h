@@ -374,8 +374,9 @@ int moe355_add_rmsnorm_mxfp8(const void* x, const void* residual, void* residual
  *   group_score of c, the topk_groups best are kept, and of their experts the K of
  *   largest c are chosen, descending;
  *   w = s of the chosen, divided by their sum + 1e-20 when renormalize, times scale.
- * The ids are those of exact arithmetic on the given logits; ties go to the lower
- * group and expert, a NaN choice ranks last. topk_w [T,out_ld] fp32, topk_ids
+ * The ids are those of 64-bit arithmetic on the given logits and bias, and where nothing but
+ * their order counts (no bias, groups by their best) of the logits themselves. Ties go to
+ * the lower group and expert, a NaN choice ranks last. topk_w [T,out_ld] fp32, topk_ids
  * [T,out_ld] int32 or int64; columns K.. are left as they are.
  */
 int moe355_grouped_topk(const float* logits, const float* bias, int T, int E, int K, int scoring,

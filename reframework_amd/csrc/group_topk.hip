@@ -7,12 +7,28 @@
 //   w = s of the chosen, over their sum (+ 1e-20) if renormalize, times scale
 // Ties go to the lower group and the lower expert; a NaN choice ranks last.
 //
-// The chosen ids are those of exact arithmetic. Without a bias (and with groups
+// The chosen ids are those of 64-bit arithmetic. Without a bias (and with groups
 // by their best expert) the choice is made on the logits, in whose order the
 // scores are. Otherwise c is computed in 32 bits first, and where two values that
 // the result depends on lie within the error of that, the token's choice is made
 // again in 64 bits: seldom (a distance of some 1e-6 among values that lie 1e-2
-// apart) but for equal logits with equal biases, so it need not be fast.
+// apart) but for equal logits with equal biases, so it need not be fast. What 64
+// bits do not tell apart is a tie (sigmoid scores of logits over 37 are all 1).
+//
+// The error of 32 bits, which kScoreError, kRounding and their like cover (u = 2^-24):
+//   e = exp(v), v = l - max <= 0: the difference, log2(e) and the product are off by
+//     2.3 u |v| in all, the unit by 2 u, so e by (2.3 |v| + 2) u: at most 2.9 u of the largest
+//     e, as |v| exp(v) <= 0.37
+//   the sum of the e: 2 u and 2.3 u times the mean of |v| by e, which is at most 3.4 for 256
+//     experts, so 9.9 u; and u for each of its additions, 7 in a lane and 6 over the lanes
+//     (rows of 16 lanes: 15 and 4); its reciprocal u
+//   the difference of two scores: (9.9 + 13 + 1) u from the sum, common to both; 2.9 u and
+//     u from their products each: 31.7 u = 1.9e-6 of the largest score (rows: 37.7 u =
+//     2.25e-6); of two sums of two scores twice that
+//   sigmoid scores: 2 u from the reciprocal, u from 1 + e, less than that from e: below
+//     5 u each
+//   adding the bias: u |c|; the sum of two choices: u of it; the test's own difference: u
+// A distance is tested against the sum of both sides' errors, so each side's is half.
 //
 // One wave per token. A lane holds up to NV consecutive experts of one group (64
 // lanes over the groups, rounded up to a power of two), so lane order is expert
@@ -165,9 +181,9 @@ __device__ __forceinline__ bool group_open(typename KF::type score, F error, boo
   return best >= KF::kFirst && !(KF::value(worst) > KF::value(best));
 }
 
-// The error of a group's score relative to the magnitudes of the choices in it: in each of
-// them 2^-24 from adding the bias, and as much from their sum and from `group_open`'s own.
-constexpr float kRounding = 2.5e-7f;
+// The error of a score relative to the token's largest, of a choice relative to its own
+// magnitude (a group's: to those of the choices in it).
+constexpr float kScoreError = 1e-6f, kRounding = 2.5e-7f;
 
 // The choice of one token into chosen[0..K) (LDS). F float returns whether 32 bits
 // leave it open (`exact`: the choice is made on the logits themselves, which leave
@@ -224,13 +240,12 @@ __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, c
 #pragma unroll
   for (int i = NV - 1; i >= 0; --i) list = (list << 4) | static_cast<unsigned>(idx[i]);
 
-  // Whether hi >= lo lie too near each other for 32 bits. The error of c, relative to
-  // the largest score plus |c|, is below 4e-7 from the score (exp_of, where |v|
-  // exp(-|v|) <= 0.37 bounds what its error grows by, the sum, a reciprocal) and 6e-8
-  // from the sum with the bias; twice that.
-  auto near = [&](I hi, I lo, F eps) {
+  // Whether hi >= lo lie too near each other for 32 bits (of a lo twice as far from 0
+  // as hi the rounding is below the distance).
+  auto near = [&](I hi, I lo) {
     const F x = KF::value(hi), y = KF::value(lo);
-    return lo > KF::kDead + 1 && !(x - y > eps * (top + fabs(x)));  // infinite ones too
+    return lo >= KF::kFirst &&
+           !(x - y > F(2 * kScoreError) * top + F(2 * kRounding) * fabs(x));  // infinite ones too
   };
   constexpr bool kTest = sizeof(F) == sizeof(float);
   bool open = false;
@@ -249,7 +264,7 @@ __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, c
     const bool kept = p.group < a.G && rank < a.KG;
     if (kTest && !exact) {
       const F size = fabs(KF::value(b1)) + (two ? fabs(KF::value(b2)) : F(0));
-      const F error = (two ? F(1e-6) : F(5e-7)) * top + F(kRounding) * size;
+      const F error = F(two ? 2 * kScoreError : kScoreError) * top + F(kRounding) * size;
       open = group_open<KF>(score, error, kept, p.group < a.G, [](I v) { return wave_max_key(v); });
     }
 #pragma unroll
@@ -272,7 +287,7 @@ __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, c
   if (kTest && !exact) {
     const I down = __shfl_down(mine, 1, kWave);
     const I next = lane == a.K - 1 ? best : down;
-    open = open || __ballot(lane < a.K && near(mine, next, F(1e-6))) != 0;
+    open = open || __ballot(lane < a.K && near(mine, next)) != 0;
   }
   return open;
 }
@@ -381,6 +396,7 @@ __global__ __launch_bounds__(kThreads) void group_topk_kernel(const GroupTopkArg
 // values) lose nothing.
 constexpr int kRow = 16;
 constexpr int kRowTopk = 8;  // largest K
+constexpr float kRowScoreError = 1.2e-6f;             // its lanes' sums are longer
 constexpr float kRowRounding = kRounding + 0x1p-19f;  // with the cut of the keys
 
 __device__ __forceinline__ int row_max_key(int v) {
@@ -473,9 +489,9 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
   const auto placeless = [](int k) { return (k & ~15) | ((k >> 31) & 15); };
   const auto cut = [&](int k) { return KF::value(placeless(k)); };
   const bool lossless = exact && row_max_key(bits & 15) == 0;
-  const auto near = [&](int hi, int lo, float eps) {
+  const auto near = [&](int hi, int lo) {
     const float x = cut(hi), y = cut(lo);
-    return lo >= KF::kFirst && !(x - y > eps * (top + fabsf(x)));
+    return lo >= KF::kFirst && !(x - y > 2 * kRowScoreError * top + 3 * kRowRounding * fabsf(x));
   };
 
   // Largest first (odd-even merge sort of the NV keys).
@@ -515,7 +531,7 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
     const bool kept = p.group < a.G && rank < a.KG;
     if (!lossless) {
       const float size = fabsf(cut(b1)) + (two ? fabsf(cut(b2)) : 0.f);
-      const float error = (two ? 2.4e-6f : 1.2e-6f) * top + kRowRounding * size;
+      const float error = (two ? 2 : 1) * kRowScoreError * top + kRowRounding * size;
       open = group_open<KF>(score, error, kept, p.group < a.G, [](int v) { return row_max_key(v); });
     }
 #pragma unroll
@@ -562,8 +578,8 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
     const float after = __int_as_float(row_ahead<1>(__float_as_int(c)));
     const int e_after = row_ahead<1>(e);
     const bool ordered = exact ? c > after || (c == after && e < e_after)
-                               : c - after > 1e-6f * (top + fabsf(c));
-    open = open || (sub < a.K && near(mine, next, 6e-6f) && (sub == a.K - 1 || !ordered));
+                               : c - after > 2 * kRowScoreError * top + 2 * kRounding * fabsf(c);
+    open = open || (sub < a.K && near(mine, next) && (sub == a.K - 1 || !ordered));
   }
 
   // Tokens left open, one after the other by the whole wave: on the logits where those

@@ -112,9 +112,10 @@ def grouped_topk(
     ``c`` (``"max"``) or the sum of their best two (``"top2"``); the ``topk_groups`` best
     groups stay, and of their experts the ``topk`` of largest ``c`` are chosen, in
     descending order. The weights are their ``s``, over their sum if ``renormalize``,
-    times ``scale``. The ids are those of exact arithmetic on the fp32 logits and bias;
-    ties go to the lower group and the lower expert, a NaN ranks last. At most 64
-    groups and a topk of 64."""
+    times ``scale``. The ids are those of 64-bit arithmetic on the fp32 logits and bias, or
+    of the logits themselves where only their order counts (no bias, groups by their best).
+    Ties, also of scores that 64 bits do not tell apart, go to the lower group and the
+    lower expert; a NaN ranks last. At most 64 groups and a topk of 64."""
     require_gpu(gating_output, "gating_output")
     shape = gating_output.shape
     logits = gating_output
