@@ -404,8 +404,11 @@ int moe355_mx_matrix_bytes(int rows, int cols, int gate_up, size_t* codes, size_
 int moe355_mx_pack(const void* src, const void* src_scales, int rows, int cols, int gate_up,
                    int dtype, void* codes, void* scales, void* stream);
 
-/* Workspace of a moe355_mx_fused_experts call. */
+/* Workspace of any moe355_mx_fused_experts call of these sizes, and of one that is known to
+ * add to fp32 or not to (a bf16 one that does not needs up to half as much). */
 int moe355_mx_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes);
+int moe355_mx_call_workspace_bytes(int T, int H, int I, int E, int K, int dtype, int accumulate_f32,
+                                   size_t* bytes);
 
 /*
  * moe355_fused_experts on 4-bit weights and 8-bit rows (the products of
@@ -417,8 +420,8 @@ int moe355_mx_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size
  * other. H and I multiples of 32. Products are exact and summed in fp32 for f16, fp32 and
  * for up to 12 rows per expert (T * K / min(T * K, E), rounded down); for dtype bf16 and more
  * rows they are those of the scaled MFMA, which keeps about 14 bits of a product below the
- * largest one it adds in a step of 128 columns, and y may be kept to 11 bits (of values
- * down to 2^-28 of the largest in 64 columns), else in fp32. Slots whose id lies outside [0,E) or whose weight is 0 add nothing. out as in
+ * largest one it adds in a step of 128 columns, and without accumulate_f32 y may be kept to
+ * 11 bits (of values down to 2^-28 of the largest in 64 columns), else in fp32. Slots whose id lies outside [0,E) or whose weight is 0 add nothing. out as in
  * moe355_combine; it may be x. The workspace belongs to the call until its kernels end.
  */
 int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,

@@ -110,6 +110,7 @@ _SIGNATURES: Dict[str, Tuple[object, List[object]]] = {
     "moe355_mx_matrix_bytes": (_I, [_I, _I, _I, ctypes.POINTER(_Z), ctypes.POINTER(_Z)]),
     "moe355_mx_pack": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
     "moe355_mx_workspace_bytes": (_I, [_I, _I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
+    "moe355_mx_call_workspace_bytes": (_I, [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
     "moe355_mx_fused_experts": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                      _I, _P, _I, _P, _Z, _P]),
 }
@@ -513,14 +514,15 @@ _MX_WORKSPACES: "OrderedDict[Tuple[int, ...], int]" = OrderedDict()
 
 
 def mx_workspace_bytes(T: int, H: int, I: int, E: int, K: int, dtype: int,
-                       device: torch.device) -> int:
+                       device: torch.device, accumulate_f32: bool = False) -> int:
     """Workspace of an mx_fused_experts call. It depends on the sizes and the device's
     CU count, so it is cached."""
-    key = (T, H, I, E, K, dtype, device.index)
+    key = (T, H, I, E, K, dtype, device.index, accumulate_f32)
     n = _MX_WORKSPACES.get(key)
     if n is None:
         v = ctypes.c_size_t()
-        _call(device, "moe355_mx_workspace_bytes", _rows(T), H, I, E, K, dtype, ctypes.byref(v))
+        _call(device, "moe355_mx_call_workspace_bytes", _rows(T), H, I, E, K, dtype,
+              int(accumulate_f32), ctypes.byref(v))
         n = int(v.value)
         with _lock:
             _MX_WORKSPACES[key] = n

@@ -42,7 +42,7 @@ struct MxPlan {
       inter_scales, y, y_scales, bytes;
 };
 
-int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
+int mx_plan(int T, int H, int I, int E, int K, int dtype, bool accumulate, MxPlan* p) {
   if (T < 0) return fail(MOE355_EINVAL, "bad T=%d", T);
   if (H <= 0 || I <= 0) return fail(MOE355_EINVAL, "bad sizes H=%d I=%d", H, I);
   if (bad_blocks(H) || bad_blocks(I))
@@ -71,9 +71,10 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, MxPlan* p) {
   p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
   // A bf16 call of several slots per token keeps their results in 16 bits until they are
   // weighed and added: half the bytes (4096 tokens of 6 slots, H 2048: 259 us instead of
-  // 286). They are f16 with a scale per 64 columns, whose 11 bits leave the error of the
-  // bf16 sum as it is (0.0017 of the results' size; kept in bf16 it was 0.0024).
-  const bool narrow = p->tiled && !exact && K > 1;
+  // 286). They are f16 with a scale per 64 columns, whose 11 bits take the error of the
+  // bf16 sum from 0.0017 of the results' size to 0.0018 (kept in bf16 it was 0.0024). Sums
+  // that go on in fp32 keep fp32 slots: there the 11 bits would be most of the error.
+  const bool narrow = p->tiled && !exact && K > 1 && !accumulate;
   const int steps = p->Ip / kMxStep;
   int s = 1;
   if (p->tiled) {
@@ -133,15 +134,15 @@ int max_tokens(int H) { return INT_MAX / mx_pad(H); }
 
 // Bytes that a call of T tokens needs: those of its full parts or of its last one, whose
 // plan may cut the columns into more parts.
-int mx_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes) {
+int mx_bytes(int T, int H, int I, int E, int K, int dtype, bool accumulate, size_t* bytes) {
   MxPlan p;
-  if (int rc = mx_plan(T, H, I, E, K, dtype, &p)) return rc;
+  if (int rc = mx_plan(T, H, I, E, K, dtype, accumulate, &p)) return rc;
   if (T > max_tokens(H)) {
     const int rest = T % max_tokens(H);
-    if (int rc = mx_plan(max_tokens(H), H, I, E, K, dtype, &p)) return rc;
+    if (int rc = mx_plan(max_tokens(H), H, I, E, K, dtype, accumulate, &p)) return rc;
     *bytes = p.bytes;
     if (rest == 0) return MOE355_OK;
-    if (int rc = mx_plan(rest, H, I, E, K, dtype, &p)) return rc;
+    if (int rc = mx_plan(rest, H, I, E, K, dtype, accumulate, &p)) return rc;
     *bytes = std::max(*bytes, p.bytes);
     return MOE355_OK;
   }
@@ -366,7 +367,17 @@ int moe355_mx_pack(const void* src, const void* src_scales, int rows, int cols, 
 
 int moe355_mx_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes) {
   if (!bytes) return fail(MOE355_EINVAL, "NULL result");
-  return mx_bytes(T, H, I, E, K, dtype, bytes);
+  size_t stored, added;
+  if (int rc = mx_bytes(T, H, I, E, K, dtype, false, &stored)) return rc;
+  if (int rc = mx_bytes(T, H, I, E, K, dtype, true, &added)) return rc;
+  *bytes = std::max(stored, added);
+  return MOE355_OK;
+}
+
+int moe355_mx_call_workspace_bytes(int T, int H, int I, int E, int K, int dtype, int accumulate_f32,
+                                   size_t* bytes) {
+  if (!bytes) return fail(MOE355_EINVAL, "NULL result");
+  return mx_bytes(T, H, I, E, K, dtype, accumulate_f32 != 0, bytes);
 }
 
 int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
@@ -375,7 +386,7 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
                             int I, int E, int K, int dtype, int act, void* out, int accumulate_f32,
                             void* workspace, size_t workspace_bytes, void* stream) {
   size_t bytes;
-  if (int rc = mx_bytes(T, H, I, E, K, dtype, &bytes)) return rc;
+  if (int rc = mx_bytes(T, H, I, E, K, dtype, accumulate_f32 != 0, &bytes)) return rc;
   if (act < MOE355_ACT_SILU || act > MOE355_ACT_GELU_TANH)
     return fail(MOE355_EINVAL, "unknown activation %d", act);
   if (T == 0) return MOE355_OK;
@@ -394,7 +405,7 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
   for (int t = 0; t < T; t += max_tokens(H)) {
     const int n = std::min(T - t, max_tokens(H));
     MxPlan p;
-    if (int rc = mx_plan(n, H, I, E, K, dtype, &p)) return rc;
+    if (int rc = mx_plan(n, H, I, E, K, dtype, accumulate_f32 != 0, &p)) return rc;
     MxCall c{};
     c.x = static_cast<const char*>(x) + t * x_row;
     c.x_scales = x_scales ? static_cast<const uint8_t*>(x_scales) + t * static_cast<size_t>(p.Hp / kMxBlock) : nullptr;

@@ -526,3 +526,26 @@ def test_few_tokens_per_expert_are_exact_in_bf16_too(T, H, E, K, I, activation, 
     full = fused_experts_mxfp4(*args, activation=activation, out_dtype=torch.float32)
     got = fused_experts_mxfp4(*args, activation=activation, out_dtype=torch.bfloat16)
     assert torch.equal(got, full.bfloat16())
+
+
+@pytest.mark.parametrize("T,E,K", [(700, 3, 2), (250, 5, 3)])
+def test_bf16_slots_added_to_fp32_stay_in_fp32(T, E, K, dev):
+    """All slots in one call or one after the other: the same products, each of which is
+    weighed and added in 32 bits, so per slot two roundings of 2^-24 of it and of the sum
+    so far; slots kept to 11 bits would be off by some 2^-13."""
+    banner(f"fused_experts_mxfp4 fp32 slots T={T} E={E} K={K}")
+    rng = np.random.default_rng(T)
+    H, I = 288, 384
+    ex = _experts(_random_codes(E, 2 * I, H, rng), _random_codes(E, H, I, rng), dev)
+    x = torch.from_numpy(rng.normal(size=(T, H))).bfloat16().to(dev)
+    tw, ids = (torch.from_numpy(t).to(dev) for t in _routing(T, K, E, rng))
+    whole = torch.zeros((T, H), device=dev)
+    fused_experts_mxfp4(x, ex, tw, ids, out=whole, accumulate_f32=True)
+    apart, size = torch.zeros((T, H), device=dev), torch.zeros((T, H), device=dev)
+    for k in range(K):
+        one = torch.zeros((T, H), device=dev)
+        args = x, ex, tw[:, k:k + 1], ids[:, k:k + 1]
+        fused_experts_mxfp4(*args, out=one, accumulate_f32=True)
+        fused_experts_mxfp4(*args, out=apart, accumulate_f32=True)
+        size += one.abs()
+    assert bool(((whole - apart).abs() <= 2 * K * 2.0 ** -24 * 2 * size).all())

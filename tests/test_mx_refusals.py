@@ -249,3 +249,17 @@ def test_routing_of_another_shape_than_the_tokens(w, ids):
                      torch.zeros(6, 4, dtype=torch.uint8).view(torch.float8_e8m0fnu), 64)
     with pytest.raises(ValueError, match=r"are not \[6, K\]"):
         fused_experts_mxfp4(rows, _cpu_experts(), torch.ones(w), torch.zeros(ids).long())
+
+
+@pytest.mark.parametrize("T,H,I,E,K", [(0, 64, 64, 1, 1), (1, 4096, 14336, 8, 2), (4096, 2048, 1408, 64, 6),
+                                       (40000, 1 << 17, 256, 16, 2)])
+def test_workspace_of_any_call_and_of_a_known_one(T, H, I, E, K):
+    for dtype in (0, 1, 2):
+        known = [_capi.mx_workspace_bytes(T, H, I, E, K, dtype, torch.device("cpu"), acc)
+                 for acc in (False, True)]
+        both = ctypes.c_size_t()
+        assert _rc("moe355_mx_workspace_bytes", T, H, I, E, K, dtype, ctypes.byref(both))[0] == 0
+        assert both.value == max(known)
+        if dtype != 1:  # only bf16 results have slots of 16 bits
+            assert known[0] == known[1]
+    assert _rc("moe355_mx_call_workspace_bytes", T, H, I, E, K, 1, 0, None)[0] == -1
