@@ -14,8 +14,8 @@ namespace {
 bool bad_blocks(int n) { return n <= 0 || n % kMxBlock; }
 
 // Average rows per active expert up to which the weights are streamed past 16-row
-// tiles (ffn_mx.hip), and up to which the tiled kernels (ffn_mx_tiled.hip) take tiles
-// of 64 rows; above, 256 (exact products: 128). Whole calls of random routing, us.
+// tiles (ffn_mx.hip), and below which the tiled kernels (ffn_mx_tiled.hip) take tiles
+// of 64 rows; from there on, 256 (exact products: 128). Whole calls of random routing, us.
 // Streaming (exact) / 64 rows (scaled): 8 experts of H 4096, I 14336 at 8 rows 138 / 149, 10 rows
 // 133 / 148, 12 rows 159 / 150, 14 rows 172 / 152, 20 rows 251 / 155; 64 of H 2048, I 1408 (6 slots)
 // at 12 rows 70 / 75, 14 rows 78 / 76; 8 of H 2048, I 8192 at 10 rows 51 / 56, 12 rows 56 / 56; 32
@@ -65,7 +65,7 @@ int mx_plan(int T, int H, int I, int E, int K, int dtype, bool accumulate, MxPla
   p->tiled = avg > kMxStreamRows;
   const bool exact = dtype != MOE355_BF16;
   p->tile_rows = !p->tiled                                      ? kMxStreamTile
-                 : avg <= tile64_rows(p->Hp / kMxStep, exact) ? 64
+                 : avg < tile64_rows(p->Hp / kMxStep, exact) ? 64
                  : exact                                      ? 128
                                                               : 256;
   p->max_tiles = static_cast<int>((R + static_cast<long long>(active) * (p->tile_rows - 1)) / p->tile_rows);
