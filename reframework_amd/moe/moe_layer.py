@@ -399,7 +399,10 @@ class FusedMoE(BaseOP):
             # in a buffer of this call's own: captured graphs do not share it
             logits = torch.empty((T, self.num_experts), dtype=torch.float32, device=xd.device)
             _capi.router_logits(xd, gate, True, logits)
-            run_grouped_topk(logits, self.expert_bias, self.renormalize, self.scoring,
+            bias = self.expert_bias
+            if bias is not None and bias.device != xd.device:  # as the gate above
+                bias = bias.detach().to(xd.device)
+            run_grouped_topk(logits, bias, self.renormalize, self.scoring,
                              self.num_expert_groups, self.topk_groups, self.group_score,
                              self.routed_scale, self.top_k, w, ids)
             return w, ids
