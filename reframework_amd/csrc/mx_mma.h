@@ -29,7 +29,9 @@ __device__ __forceinline__ f32x4 mma_scaled(u32x4 w, uint32_t ws, const u32x4* x
 
 // The same product in bf16, which holds every code times its scale exactly (4
 // significant bits at most), summed in fp32: for results of more bits than bf16, and
-// where the weights' stream hides it.
+// where the weights' stream hides it. That holds for scale bytes 3 to 246 of tokens and up
+// to 252 of weights: over them the largest codes are past bf16's range (of tokens in
+// 16 or 32 bits none is), under 3 the smallest are rounded to multiples of 2^-133.
 // Lane (r, q) multiplies columns 32 q + 8 j .. + 7 in the j-th of four MFMAs (the
 // order of columns is free as long as both operands share it).
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));

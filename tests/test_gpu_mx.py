@@ -549,3 +549,49 @@ def test_bf16_slots_added_to_fp32_stay_in_fp32(T, E, K, dev):
         fused_experts_mxfp4(*args, out=apart, accumulate_f32=True)
         size += one.abs()
     assert bool(((whole - apart).abs() <= 2 * K * 2.0 ** -24 * 2 * size).all())
+
+
+@pytest.mark.parametrize("T,dt", [(1, torch.bfloat16), (1, torch.float32), (30, torch.float32),
+                                  (300, torch.float32), (300, torch.bfloat16)])
+def test_scales_at_the_ends_of_their_range(T, dt, dev):
+    """One product, of a token's block with scale byte b and a weights' block with the byte
+    that brings it back, through up, beside a gate of 384. Exact products are those of the
+    operands as bf16 numbers: bytes 3 to 246 of tokens and 1 to 252 of weights hold every
+    code; beyond, the largest codes are infinite (the result is NaN) and the smallest
+    multiples of 2^-133. The scaled MFMA (a bf16 result of many tokens) takes all as they
+    are. A byte of 255 is NaN."""
+    banner(f"fused_experts_mxfp4 scale bytes T={T} {dt}")
+    scaled = dt == torch.bfloat16 and T > 12
+    H, I = 128, 32
+    cases = [(bx, min(max(254 - bx, 0), 254), c8, 2)
+             for bx in (*range(0, 6), 100, 127, *range(244, 256)) for c8 in (1, 3, 9, 15, 56, 119, 126)]
+    cases += [(min(max(254 - bw, 0), 246), bw, 56, c4)
+              for bw in (0, 1, 2, 127, *range(250, 256)) for c4 in range(1, 8)]
+    bx, bw, c8, c4 = (np.array(v) for v in zip(*cases))
+    n = len(cases)  # one expert per case: its T rows are the same token
+    x, xs = np.zeros((n, T, H), np.uint8), np.full((n, T, H // 32), 127, np.uint8)
+    x[:, :, 0], x[:, :, 32], xs[:, :, 1] = 56, c8[:, None], bx[:, None]
+    w1, s1 = np.zeros((n, 2 * I, H // 2), np.uint8), np.full((n, 2 * I, H // 32), 127, np.uint8)
+    w1[:, :I, 0], s1[:, :I, 0] = 7, 127 + 6
+    w1[:, I:, 16], s1[:, I:, 1] = c4[:, None], bw[:, None]
+    w2, s2 = np.zeros((n, H, I // 2), np.uint8), np.full((n, H, 1), 127, np.uint8)
+    w2[:, :, 0] = 2
+    u8, u4 = ref.E4M3[c8] * ref.pow2(bx), ref.FP4[c4] * ref.pow2(bw)
+    if not scaled:
+        u8, u4 = (torch.from_numpy(v).float().bfloat16().double().numpy() for v in (u8, u4))
+    with np.errstate(invalid="ignore"):
+        h = np.repeat((384.0 * u8 * u4)[:, None], 32, 1)
+    want = np.where(np.isfinite(h), ref.mxfp8(h)[2], np.nan)[:, 0]
+    got = []
+    for k in range(0, n, 200):  # experts of one call
+        part = slice(k, k + 200)
+        m = len(bx[part])
+        q = Mxfp8Rows(torch.from_numpy(x[part].reshape(m * T, H)).to(dev).view(torch.float8_e4m3fn),
+                      torch.from_numpy(xs[part].reshape(m * T, -1)).to(dev).view(torch.float8_e8m0fnu), H)
+        ids = torch.arange(m, device=dev).repeat_interleave(T)[:, None]
+        got.append(fused_experts_mxfp4(q, _experts((w1[part], s1[part]), (w2[part], s2[part]), dev),
+                                       torch.ones((m * T, 1), device=dev), ids, out_dtype=dt))
+    got = ref.to64(torch.cat(got)).reshape(n, T, H)
+    assert np.isnan(want).any() and np.isfinite(want).sum() > 100
+    want = torch.from_numpy(want).to(dt).double().numpy()
+    assert np.array_equal(got, np.broadcast_to(want[:, None, None], got.shape), equal_nan=True)
