@@ -120,6 +120,14 @@ __device__ __forceinline__ float exp_of(float v) {
   return __builtin_amdgcn_exp2f(v * 1.4426950408889634f);
 }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
+// e * top + bias in two roundings: as one (where the compiler saw fit, which was not the
+// same for all places of a lane's list) equal choices differed in their last bit.
+template <typename F>
+__device__ __forceinline__ F choice_of(F e, F top, F bias) {
+#pragma clang fp contract(off)
+  const F score = e * top;
+  return score + bias;
+}
 __device__ __forceinline__ float inverse_of(float v) { return __builtin_amdgcn_rcpf(v); }
 __device__ __forceinline__ double inverse_of(double v) { return 1.0 / v; }
 
@@ -214,7 +222,7 @@ __device__ __forceinline__ bool select(const GroupTopkArgs& a, const Place& p, c
       }
       top = F(1) / wave_sum_of(sum);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) c[i] = c[i] * top + static_cast<F>(bias[i]);
+      for (int i = 0; i < NV; ++i) c[i] = choice_of<F>(c[i], top, static_cast<F>(bias[i]));
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -476,7 +484,7 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
       sum = row_sum(sum);
       top = 1.f / sum;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) c[i] = exact ? l[i] : c[i] * top + bias[i];
+      for (int i = 0; i < NV; ++i) c[i] = exact ? l[i] : choice_of(c[i], top, bias[i]);
     }
     if (exact) top = 0.f;
 #pragma unroll
@@ -572,8 +580,8 @@ __global__ __launch_bounds__(kThreads) void group_topk_rows_kernel(const GroupTo
     // chosen, where the cut values are near, by the whole ones.
     float c = x;
     if (!exact) {
-      c = a.sigmoid ? inverse_of(1.f + exp_of(-x)) : exp_of(x - m) * top;
-      if (a.bias) c += a.bias[e];
+      const float b = a.bias ? a.bias[e] : 0.f;
+      c = a.sigmoid ? inverse_of(1.f + exp_of(-x)) + b : choice_of(exp_of(x - m), top, b);
     }
     const float after = __int_as_float(row_ahead<1>(__float_as_int(c)));
     const int e_after = row_ahead<1>(e);

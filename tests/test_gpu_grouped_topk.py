@@ -242,3 +242,17 @@ def test_biases_that_shut_experts_out(T, score, value, scoring, dev):
     for KG in (2, 5, 7):
         _check(logits, 6, dev, bias=bias, scoring=scoring, num_groups=G, topk_groups=KG,
                group_score=score)
+
+
+@pytest.mark.parametrize("E,G,KG", [(100, 1, 1), (111, 1, 1), (128, 8, 3), (200, 5, 2), (256, 1, 1),
+                                    (255, 17, 9)])
+@pytest.mark.parametrize("T", [500, 7000])
+def test_equal_choices_of_many_experts(T, E, G, KG, dev):
+    """Experts of equal logits and equal biases tie wherever in a lane's list they are."""
+    banner(f"grouped_topk equal choices T={T} E={E} G={G}")
+    rng = np.random.default_rng(E)
+    logits = (np.round(rng.normal(size=(T, E)) * 6) / 4).astype(np.float32)
+    few = np.array([-0.3, 0.1, 0.25], np.float32)[rng.integers(0, 3, E)]
+    for bias in (np.full(E, 0.25, np.float32), np.full(E, -0.3, np.float32), few):
+        for scoring in ("softmax", "sigmoid"):
+            _check(logits, 6, dev, bias=bias, scoring=scoring, num_groups=G, topk_groups=KG)
