@@ -595,3 +595,23 @@ def test_scales_at_the_ends_of_their_range(T, dt, dev):
     assert np.isnan(want).any() and np.isfinite(want).sum() > 100
     want = torch.from_numpy(want).to(dt).double().numpy()
     assert np.array_equal(got, np.broadcast_to(want[:, None, None], got.shape), equal_nan=True)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,E,K,hot", [(60, 64, 4, 1), (60, 64, 4, 4), (130, 256, 6, 1), (40, 256, 8, 0)])
+def test_popular_experts_of_a_call_that_streams(T, E, K, hot, dt, dev):
+    """Few rows per expert on average, but the first `hot` experts are every token's: many
+    16-row tiles of one expert beside experts of one row or none."""
+    banner(f"fused_experts_mxfp4 popular experts T={T} E={E} K={K} hot={hot} {dt}")
+    rng = np.random.default_rng(T + E)
+    H, I = 288, 160
+    w1, w2 = _random_codes(E, 2 * I, H, rng), _random_codes(E, H, I, rng)
+    x = torch.from_numpy(rng.normal(size=(T, H))).to(dt)
+    tw, ids = _routing(T, K, E, rng)
+    for t in range(T):
+        ids[t] = [*range(hot), *(e for e in ids[t] if e >= hot), *range(hot, K)][:K]
+    assert T * K // min(T * K, E) <= 12 and all(len(set(r)) == K for r in ids.tolist())
+    want = ref.experts(ref.to64(x), ref.dequant4(*w1), ref.dequant4(*w2), tw, ids)
+    got = fused_experts_mxfp4(x.to(dev), _experts(w1, w2, dev), torch.from_numpy(tw).to(dev),
+                              torch.from_numpy(ids).to(dev))
+    assert _rel(got, want) <= REL[dt]
