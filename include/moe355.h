@@ -417,13 +417,15 @@ int moe355_mx_call_workspace_bytes(int T, int H, int I, int E, int K, int dtype,
  *   else x holds codes [T,Hp]), g, u = x . w1[e]^T, h = act(g) * u in 8 bits,
  *   y = h . w2[e]^T, out[t] = sum_k topk_w[t,k] * y.
  * w1, w1_scales, w2, w2_scales: the laid-out matrices of the E experts one after the
- * other. H and I multiples of 32. Products are exact and summed in fp32 for f16, fp32 and
- * for up to 12 rows per expert (T * K / min(T * K, E), rounded down), of operands that bf16
- * holds: those of scale bytes 3 to 246 (rows) and 0 to 252 (weights); beyond, the largest codes
- * are infinite, the smallest multiples of 2^-133. For dtype bf16 and more
- * rows they are those of the scaled MFMA, which keeps about 14 bits of a product below the
- * largest one it adds in a step of 128 columns, and without accumulate_f32 y may be kept to
- * 11 bits (of values down to 2^-28 of the largest in 64 columns), else in fp32. Slots whose id lies outside [0,E) or whose weight is 0 add nothing. out as in
+ * other. H and I multiples of 32.
+ * Products are exact and summed in fp32 for f16, fp32 and for up to 12 rows per expert
+ * (T * K / min(T * K, E), rounded down), of operands that bf16 holds: those of scale bytes
+ * 3 to 246 (rows) and 0 to 252 (weights); beyond, the largest codes are infinite, the
+ * smallest multiples of 2^-133. For dtype bf16 and more rows they are those of the scaled
+ * MFMA, which keeps about 14 bits of a product below the largest one it adds in a step of
+ * 128 columns, and without accumulate_f32 y may be kept to 11 bits (of values down to 2^-28
+ * of the largest in 64 columns); else y is fp32.
+ * Slots whose id lies outside [0,E) or whose weight is 0 add nothing. out as in
  * moe355_combine; it may be x. The workspace belongs to the call until its kernels end.
  */
 int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,

@@ -6,12 +6,13 @@
 // columns, two steps of 4 KB each in flight, and add their sums in LDS in a fixed
 // order. Weights sit on the M side of the product, tokens on the N side, so a lane
 // ends with 4 consecutive features of one token per group. The products are exact
-// (mx_mma.h) whatever the result's type is: the weights' stream hides them but for some
-// 1.5 us a call (8 experts of H 4096, I 14336, one token 39.0 us with scaled products, 40.7
-// with these; 64 of H 2048, I 1408, 16 tokens of 6 slots 50.1 and 50.9).
-// Weights of 64 experts of H 2048, I 1408 (those of them that 16 tokens reach) stream at 6.0
-// and 4.9 TB/s (gate|up and down, 26 and 15 us), of two experts of H 4096, I 14336 for one
-// token at 5.3 and 5.3 (24 and 12 us).
+// (mx_mma.h) whatever the result's type is: the weights' stream hides them but for 2 to
+// 5 % (us with scaled products / with these: 8 experts of H 4096, I 14336, one token 39.0 /
+// 40.7, 8 rows each 79 + 53 / 82 + 56; 64 of H 2048, I 1408, 16 tokens of 6 slots 50.1 / 50.9).
+// Weights of 8 experts of H 4096, I 14336 stream at 6.1 and 4.5 TB/s (gate|up and down, 8 rows
+// each: 82 and 56 us), of the 51 of 64 experts of H 2048, I 1408 that 16 tokens reach at 5.3
+// and 4.8 (29 and 16 us), of two experts of the former for one token at 5.0 and 4.9 (25 and
+// 13 us).
 #include "dma_pipe.h"
 #include "mx.h"
 

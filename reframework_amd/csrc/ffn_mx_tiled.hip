@@ -13,12 +13,13 @@
 // which two workgroups share a CU, do without turns: all waves read and multiply a step
 // between two barriers, and the other workgroup fills the gaps.
 //
-// Rates (random codes): 8 experts of 1024 rows, 4096 x 14336, 256-row tiles, gate|up 805 us
-// (2.39 PFLOP/s), down 345 (2.79), matrix cores 73 % busy at 1.73 to 1.88 GHz, so bound by
-// power; 64 experts of 384 rows, 2048 x 1408: 147 and 87 us, bound by the epilogues and
-// load latency of items of 16 and 11 steps; 8 of 49 rows, exact, 64-row tiles: 126 and 68 us,
-// 3.8 TB/s of weights. One barrier a step instead of two, with the groups half a step
-// apart, takes 865 and 387 us in the first of these.
+// Rates (random codes): 8 experts of 1024 rows, 4096 x 14336, 256-row tiles, gate|up 740 us
+// (2.60 PFLOP/s), down 342 (2.81), matrix cores 73 to 76 % busy at 1.73 to 1.98 GHz, so bound
+// by power (a long run of one launch after the other falls to 805 and 350); 64 experts of
+// 384 rows, 2048 x 1408: 152 and 85 us, bound by the epilogues and load latency of items of
+// 16 and 11 steps; 8 of 49 rows, exact, 64-row tiles: 123 and 68 us, 4.0 TB/s of weights. One
+// barrier a step instead of two, with the groups half a step apart, takes 865 and 387 us in
+// a long run of the first of these.
 //
 // A workgroup runs several items, whose steps follow each other in one stream of
 // loads: the first steps of an item are on their way while the item before it is

@@ -362,7 +362,9 @@ hipError_t launch_router_t(const RouterArgs& a, hipStream_t s) {
 }
 
 // The logits alone, by the kernels above: few tokens over (token, 8 experts)
-// workgroups, more on MFMA where the types and H allow it, else on the VALU.
+// workgroups, more on MFMA where the types and H allow it, else on the VALU. bf16: 8 tokens of
+// 64 experts, H 2048, 2.8 us, 4096 6.9 (2.6 TB/s); 256 of 256 experts, H 7168, 13.9, 4096 58 (the
+// tokens are read once per 64 experts). fp32, 4096 of 64, H 2048: 49.
 template <typename T>
 hipError_t launch_logits_t(const RouterArgs& a, hipStream_t s) {
   const dim3 block(kThreads);
