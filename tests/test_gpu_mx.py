@@ -615,3 +615,23 @@ def test_popular_experts_of_a_call_that_streams(T, E, K, hot, dt, dev):
     got = fused_experts_mxfp4(x.to(dev), _experts(w1, w2, dev), torch.from_numpy(tw).to(dev),
                               torch.from_numpy(ids).to(dev))
     assert _rel(got, want) <= REL[dt]
+
+
+@pytest.mark.parametrize("T", [0, 1, 90, 700])
+def test_result_of_another_type_than_the_tokens(T, dev):
+    banner(f"fused_experts_mxfp4 out_dtype T={T}")
+    rng = np.random.default_rng(T)
+    H, E, K, I = 288, 3, 2, 160
+    ex = _experts(_random_codes(E, 2 * I, H, rng), _random_codes(E, H, I, rng), dev)
+    x = torch.from_numpy(rng.normal(size=(T, H))).bfloat16().to(dev)
+    tw = torch.rand((T, K), device=dev) + 0.1
+    ids = torch.randint(0, E, (T, K), device=dev)
+    for dt in (torch.float32, torch.float16):
+        got = fused_experts_mxfp4(x, ex, tw, ids, out_dtype=dt)
+        assert got.dtype == dt and got.shape == (T, H)
+        assert torch.equal(got, fused_experts_mxfp4(quantize_mxfp8(x), ex, tw, ids, out_dtype=dt))
+    acc = torch.zeros((T, H), device=dev)
+    fused_experts_mxfp4(x, ex, tw, ids, out=acc, accumulate_f32=True, out_dtype=torch.float32)
+    assert torch.equal(acc, fused_experts_mxfp4(x, ex, tw, ids, out_dtype=torch.float32))
+    with pytest.raises((TypeError, ValueError)):
+        fused_experts_mxfp4(x, ex, tw, ids, out_dtype=torch.float64)
