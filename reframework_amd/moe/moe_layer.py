@@ -902,7 +902,8 @@ class FusedMoE(BaseOP):
         """Takes the tensors that are there (parameters without one keep their values), but
         not what would route or compute otherwise than the checkpoint means: a choice
         bias for a layer without one, with ``strict`` a router without the bias that the
-        layer has, 4-bit experts that are not whole. A refused dict changes nothing."""
+        layer has, 4-bit experts that are not whole: those are refused before anything is
+        copied."""
         bias, gate = self._bias_key(prefix), f"{prefix}.gate.weight" if prefix else "gate.weight"
         if self.expert_bias is None and bias in state_dict:
             raise ValueError(f"{bias}: the layer was built without a bias for the choice of experts "
