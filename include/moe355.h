@@ -434,6 +434,108 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
                             int I, int E, int K, int dtype, int act, void* out, int accumulate_f32,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * residual_out = x + residual (rounded to `dtype`; residual_out may alias x or residual),
+ * then out = (r - mean(r)) / sqrt(var(r) + eps) * weight (+ bias) of r = residual_out, in
+ * fp32, rounded once; var is the mean of the squares around the mean. With residual == NULL
+ * r = x, residual_out is unused and x may alias out. mean and rstd ([T] fp32, both or none)
+ * keep mean(r) and 1 / sqrt(var(r) + eps) for the backward pass. Any H up to 16384 (fp32:
+ * 8192), tensors aligned to their elements. The reference has no LayerNorm; this stands where
+ * RMSNorm.forward_add_residual does (reframework/layers/norm.py:27-53).
+ */
+int moe355_layer_norm(const void* x, const void* residual, void* residual_out, const void* weight,
+                      const void* bias, int weight_dtype, float eps, int T, int H, int dtype,
+                      void* out, float* mean, float* rstd, void* stream);
+
+/*
+ * Its gradient, from dy (of out), dres (of r as it went on, may be NULL) and what the
+ * forward pass kept:
+ *   dx = rstd * (g - mean(g) - xhat * mean(g * xhat)) + dres,  g = dy * weight,
+ *   dw = sum of dy * xhat over the rows, db = sum of dy,  xhat = (r - mean) * rstd
+ * in fp32, in a fixed order, dw and db rounded once to weight_dtype. Each of dx, dw and db may be
+ * NULL; dx may alias dy, dres or r. T >= 1. The workspace is needed for dw and db.
+ */
+int moe355_layer_norm_bwd_workspace_bytes(int T, int H, int dtype, size_t* bytes);
+int moe355_layer_norm_bwd(const void* dy, const void* dres, const void* r, const void* weight,
+                          int weight_dtype, const float* mean, const float* rstd, int T, int H,
+                          int dtype, void* dx, void* dw, void* db, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
+ * The order of the T * K routed slots by expert (the grouping of fused_experts,
+ * reframework/moe/fused.py:70-80), T >= 1: experts ascending, slots ascending within one.
+ * offsets [E+1]: rows of expert e are [offsets[e], offsets[e+1]); slot_to_row [T,K]: row of a
+ * slot, -1 for ids outside [0,E); row_src [T*K]: token of each row below offsets[E], the
+ * others are left as they are.
+ */
+int moe355_token_order_workspace_bytes(int T, int K, int E, size_t* bytes);
+int moe355_token_order(const void* topk_ids, int ids_int64, int T, int K, int E, int32_t* offsets,
+                       int32_t* slot_to_row, int32_t* row_src, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
+ * Token rows in that order and back (the gather and the weighted index_add_ of
+ * reframework/moe/fused.py:78-86 as operators of their own), tensors aligned to their
+ * elements:
+ *   permute_rows   rows[slot_to_row[t,k]] = x[t]; rows from offsets[E] on are zeros
+ *   combine_rows   out[t] = sum_k topk_w[t,k] * rows[slot_to_row[t,k]] in fp32, k ascending,
+ *                  without weights where topk_w is NULL: the gradient of permute_rows
+ *   combine_rows_bwd   drows[slot_to_row[t,k]] = topk_w[t,k] * dout[t], zeros from
+ *                  offsets[E] on; dw[t,k] = dot(dout[t], rows[slot_to_row[t,k]]) in
+ *                  fp32, 0 for a slot without a row; either may be NULL
+ */
+int moe355_permute_rows(const void* x, const int32_t* offsets, const int32_t* slot_to_row, int T,
+                        int H, int K, int E, int dtype, void* rows, void* stream);
+int moe355_combine_rows(const void* rows, const float* topk_w, const int32_t* slot_to_row, int T,
+                        int H, int K, int dtype, void* out, void* stream);
+int moe355_combine_rows_bwd(const void* dout, const void* rows, const float* topk_w,
+                            const int32_t* offsets, const int32_t* slot_to_row, int T, int H, int K,
+                            int E, int dtype, void* drows, float* dw, void* stream);
+
+/*
+ * Values in 8 bits with an fp32 scale per block of 128: rows are e4m3 codes [M, Kp] (Kp = K
+ * rounded up to 128, codes 0 from K on) with scales [M, ceil(K/128)], a scale per 128 consecutive
+ * values; weights are codes [N, Kp] with scales [ceil(N/128), ceil(K/128)], one per 128 x
+ * 128 block. With m a block's largest finite magnitude, at least 448 * 2^-126, the scale is
+ * m / 448 and a code v * 448 / m rounded to nearest even; infinities and NaN become NaN. The
+ * reference has no such format (its quantised experts are int8 on the host,
+ * reframework/moe/fused.py:140-197).
+ */
+int moe355_fp8_quantize(const void* x, int M, int K, int dtype, void* codes, float* scales,
+                        void* stream);
+int moe355_fp8_quantize_weight(const void* w, int N, int K, int dtype, void* codes, float* scales,
+                               void* stream);
+
+/*
+ * out [M,N] = rows [offsets[e], offsets[e+1]) of x [M,K] times matrix e of w [E,N,K],
+ * transposed (`x @ w[e].t()` of reframework/moe/fused.py:80-83); offsets [E+1] ascending
+ * within [0,M] on the device, rows of no matrix become zeros; NULL with E = 1: all rows. A step of
+ * 128 columns is summed by the matrix core, which keeps about 13 bits below its largest
+ * product; the steps are scaled and added in fp32, and rounded once to dtype. Any N and K up to
+ * 2^20 with N * Kp < 2^31.
+ */
+int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const float* w_scales,
+                      const int32_t* offsets, int M, int N, int K, int E, int dtype, void* out,
+                      void* stream);
+
+/*
+ * moe355_fused_experts on 8-bit weights and rows (the products of fused_experts,
+ * reframework/moe/fused.py:49-87): x in 8 bits (quantised here when x_scales is NULL: x is
+ * then [T,H] of dtype; else codes [T,Hp]), g, u = x . w1[e]^T, h = act(g) * u in 8 bits with
+ * a scale per 128 features, y = h . w2[e]^T, out[t] = sum_k topk_w[t,k] * y, all sums in fp32,
+ * rounded once. w1: codes [E,2I,Hp], gate rows first, scales [E, 2 ceil(I/128), ceil(H/128)],
+ * gate blocks first (the up half's blocks start at its first row); w2: codes [E,H,Ip], scales
+ * [E, ceil(H/128), ceil(I/128)]. H and I multiples of 16. Slots whose id lies outside [0,E) or
+ * whose weight is 0 add nothing. out may be x. The workspace belongs to the call until its
+ * kernels end.
+ */
+int moe355_fp8_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes);
+int moe355_fp8_fused_experts(const void* x, const float* x_scales, const void* w1,
+                             const float* w1_scales, const void* w2, const float* w2_scales,
+                             const float* topk_w, const void* topk_ids, int ids_int64, int T, int H,
+                             int I, int E, int K, int dtype, int act, void* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

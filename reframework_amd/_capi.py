@@ -113,6 +113,22 @@ _SIGNATURES: Dict[str, Tuple[object, List[object]]] = {
     "moe355_mx_call_workspace_bytes": (_I, [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
     "moe355_mx_fused_experts": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
                                      _I, _P, _I, _P, _Z, _P]),
+    "moe355_layer_norm": (_I, [_P, _P, _P, _P, _P, _I, ctypes.c_float, _I, _I, _I, _P, _P, _P,
+                               _P]),
+    "moe355_layer_norm_bwd_workspace_bytes": (_I, [_I, _I, _I, ctypes.POINTER(_Z)]),
+    "moe355_layer_norm_bwd": (_I, [_P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _Z,
+                                   _P]),
+    "moe355_token_order_workspace_bytes": (_I, [_I, _I, _I, ctypes.POINTER(_Z)]),
+    "moe355_token_order": (_I, [_P, _I, _I, _I, _I, _P, _P, _P, _P, _Z, _P]),
+    "moe355_permute_rows": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P]),
+    "moe355_combine_rows": (_I, [_P, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "moe355_combine_rows_bwd": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P]),
+    "moe355_fp8_quantize": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "moe355_fp8_quantize_weight": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "moe355_fp8_matmul": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P]),
+    "moe355_fp8_workspace_bytes": (_I, [_I, _I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
+    "moe355_fp8_fused_experts": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
+                                      _I, _P, _P, _Z, _P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -543,6 +559,145 @@ def mx_fused_experts(x: torch.Tensor, x_scales: Optional[torch.Tensor], T: int, 
           int(topk_ids.dtype == torch.int64), T, H, I, E, K, dtype, act, out.data_ptr(),
           int(accumulate_f32), workspace.data_ptr(), workspace.numel(),
           stream if stream is not None else stream_handle(device))
+
+
+_SIZES: "OrderedDict[Tuple, int]" = OrderedDict()
+
+
+def _size(device: torch.device, name: str, *args: int) -> int:
+    """What the size function ``name`` answers; it goes by its arguments and the device's CU
+    count, so it is cached."""
+    key = (name, device.index) + args
+    n = _SIZES.get(key)
+    if n is None:
+        v = ctypes.c_size_t()
+        _call(device, name, *args, ctypes.byref(v))
+        n = int(v.value)
+        with _lock:
+            _SIZES[key] = n
+            if len(_SIZES) > 1024:
+                _SIZES.popitem(last=False)
+    return n
+
+
+def layer_norm(T: int, H: int, x: torch.Tensor, residual: Optional[torch.Tensor],
+               residual_out: Optional[torch.Tensor], weight: torch.Tensor,
+               bias: Optional[torch.Tensor], eps: float, out: torch.Tensor,
+               stats: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
+    """x and its companions hold T rows of H, in any shape; ``stats`` [2, T] fp32 gets the
+    rows' means and reciprocal deviations."""
+    device = x.device
+    mean = rstd = None
+    if stats is not None:
+        mean = stats.data_ptr()
+        rstd = mean + 4 * T
+    _call(device, "moe355_layer_norm", x.data_ptr(),
+          None if residual is None else residual.data_ptr(),
+          None if residual_out is None else residual_out.data_ptr(), weight.data_ptr(),
+          None if bias is None else bias.data_ptr(), dtype_code(weight.dtype), eps, _rows(T), H,
+          dtype_code(x.dtype), out.data_ptr(), mean, rstd,
+          stream if stream is not None else stream_handle(device))
+
+
+def layer_norm_bwd(T: int, H: int, dy: torch.Tensor, dres: Optional[torch.Tensor], r: torch.Tensor,
+                   weight: torch.Tensor, stats: torch.Tensor, dx: Optional[torch.Tensor],
+                   dw: Optional[torch.Tensor], db: Optional[torch.Tensor],
+                   stream: Optional[int] = None) -> None:
+    device = r.device
+    code = dtype_code(r.dtype)
+    ws, nbytes = None, 0
+    if dw is not None or db is not None:
+        nbytes = _size(device, "moe355_layer_norm_bwd_workspace_bytes", _rows(T), H, code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    mean = stats.data_ptr()
+    _call(device, "moe355_layer_norm_bwd", dy.data_ptr(), _ptr(dres), r.data_ptr(),
+          weight.data_ptr(), dtype_code(weight.dtype), mean, mean + 4 * T, T, H, code, _ptr(dx),
+          _ptr(dw), _ptr(db), _ptr(ws), nbytes,
+          stream if stream is not None else stream_handle(device))
+
+
+def token_order(topk_ids: torch.Tensor, T: int, K: int, E: int, offsets: torch.Tensor,
+                slot_to_row: torch.Tensor, row_src: torch.Tensor,
+                stream: Optional[int] = None) -> None:
+    device = topk_ids.device
+    nbytes = _size(device, "moe355_token_order_workspace_bytes", _rows(T), K, E)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _call(device, "moe355_token_order", topk_ids.data_ptr(), int(topk_ids.dtype == torch.int64), T,
+          K, E, offsets.data_ptr(), slot_to_row.data_ptr(), row_src.data_ptr(), ws.data_ptr(),
+          nbytes, stream if stream is not None else stream_handle(device))
+
+
+def permute_rows(x: torch.Tensor, offsets: torch.Tensor, slot_to_row: torch.Tensor, E: int,
+                 rows: torch.Tensor, stream: Optional[int] = None) -> None:
+    device = x.device
+    T, K = slot_to_row.shape
+    _call(device, "moe355_permute_rows", x.data_ptr(), offsets.data_ptr(), slot_to_row.data_ptr(),
+          _rows(T), x.shape[1], K, E, dtype_code(x.dtype), rows.data_ptr(),
+          stream if stream is not None else stream_handle(device))
+
+
+def combine_rows(rows: torch.Tensor, topk_w: Optional[torch.Tensor], slot_to_row: torch.Tensor,
+                 out: torch.Tensor, stream: Optional[int] = None) -> None:
+    device = rows.device
+    T, K = slot_to_row.shape
+    _call(device, "moe355_combine_rows", rows.data_ptr(), _ptr(topk_w), slot_to_row.data_ptr(),
+          _rows(T), rows.shape[1], K, dtype_code(rows.dtype), out.data_ptr(),
+          stream if stream is not None else stream_handle(device))
+
+
+def combine_rows_bwd(dout: torch.Tensor, rows: Optional[torch.Tensor], topk_w: torch.Tensor,
+                     offsets: torch.Tensor, slot_to_row: torch.Tensor, E: int,
+                     drows: Optional[torch.Tensor], dw: Optional[torch.Tensor],
+                     stream: Optional[int] = None) -> None:
+    device = dout.device
+    T, K = slot_to_row.shape
+    _call(device, "moe355_combine_rows_bwd", dout.data_ptr(), _ptr(rows), topk_w.data_ptr(),
+          offsets.data_ptr(), slot_to_row.data_ptr(), _rows(T), dout.shape[1], K, E,
+          dtype_code(dout.dtype), _ptr(drows), _ptr(dw),
+          stream if stream is not None else stream_handle(device))
+
+
+def fp8_quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                 stream: Optional[int] = None) -> None:
+    M, K = x.shape
+    device = x.device
+    _call(device, "moe355_fp8_quantize", x.data_ptr(), _rows(M), K, dtype_code(x.dtype),
+          codes.data_ptr(), scales.data_ptr(),
+          stream if stream is not None else stream_handle(device))
+
+
+def fp8_quantize_weight(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                        stream: Optional[int] = None) -> None:
+    N, K = w.shape
+    device = w.device
+    _call(device, "moe355_fp8_quantize_weight", w.data_ptr(), _rows(N), K, dtype_code(w.dtype),
+          codes.data_ptr(), scales.data_ptr(),
+          stream if stream is not None else stream_handle(device))
+
+
+def fp8_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+               offsets: Optional[torch.Tensor], K: int, out: torch.Tensor,
+               stream: Optional[int] = None) -> None:
+    device = x.device
+    M, N = out.shape
+    _call(device, "moe355_fp8_matmul", x.data_ptr(), x_scales.data_ptr(), w.data_ptr(),
+          w_scales.data_ptr(), _ptr(offsets), _rows(M), N, K, w.shape[0], dtype_code(out.dtype),
+          out.data_ptr(), stream if stream is not None else stream_handle(device))
+
+
+def fp8_fused_experts(x: torch.Tensor, x_scales: Optional[torch.Tensor], T: int, H: int, I: int,
+                      E: int, K: int, w1: torch.Tensor, w1_scales: torch.Tensor, w2: torch.Tensor,
+                      w2_scales: torch.Tensor, topk_w: torch.Tensor, topk_ids: torch.Tensor,
+                      act: int, out: torch.Tensor, stream: Optional[int] = None) -> None:
+    device = x.device
+    code = dtype_code(out.dtype)
+    nbytes = _size(device, "moe355_fp8_workspace_bytes", _rows(T), H, I, E, K, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _call(device, "moe355_fp8_fused_experts", x.data_ptr(),
+          None if x_scales is None else x_scales.data_ptr(), w1.data_ptr(), w1_scales.data_ptr(),
+          w2.data_ptr(), w2_scales.data_ptr(), topk_w.data_ptr(), topk_ids.data_ptr(),
+          int(topk_ids.dtype == torch.int64), T, H, I, E, K, code, act, out.data_ptr(),
+          ws.data_ptr(), nbytes, stream if stream is not None else stream_handle(device))
 
 
 def cast_f32(src: torch.Tensor, dst: torch.Tensor, stream: Optional[int] = None) -> None:

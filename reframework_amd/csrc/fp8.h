@@ -1,0 +1,83 @@
+// Values in 8 bits (e4m3 codes, largest magnitude 448) with fp32 scales: rows have a scale
+// per 128 consecutive values, weights one per 128 x 128 block, blocks starting at multiples of
+// 128. With m the block's largest finite magnitude, at least 448 * 2^-126, its scale is m / 448
+// and a value's code is v * 448 / m rounded to nearest even. The quotient is formed from m, not
+// from the rounded scale: 16-bit values over 16-bit maxima are often ties, and
+// those would fall to the side the scale was rounded to. Infinities and NaN become NaN.
+//
+// Rows, of tokens and of weights, are padded to whole 128-value steps with codes of 0, so that
+// the matrix kernels never see a partial step.
+#pragma once
+
+#include "common.h"
+
+namespace moe355 {
+
+constexpr int kF8Block = 128;
+constexpr int kF8StreamTile = 16;  // token rows of a tile of the weight-streaming kernel
+
+__host__ __device__ constexpr int f8_blocks(int n) { return (n + kF8Block - 1) / kF8Block; }
+__host__ __device__ constexpr int f8_pad(int n) { return f8_blocks(n) * kF8Block; }
+
+// What a value times 448 is divided by, of a block's largest finite magnitude. Where the
+// product could overflow (of fp32 values) both are brought down by 2^-64.
+struct F8Div {
+  float mul, by, scale;
+};
+
+__device__ __forceinline__ F8Div f8_div(float amax) {
+  const float m = fmaxf(amax, 448.0f * 0x1p-126f);
+  const bool large = m > 0x1p100f;
+  return F8Div{large ? 448.0f * 0x1p-64f : 448.0f, large ? m * 0x1p-64f : m, m / 448.0f};
+}
+
+__device__ __forceinline__ float f8_finite_abs(float v) {
+  const float a = fabsf(v);
+  return a < INFINITY ? a : 0.f;
+}
+
+// v over its block's scale, or NaN. The product with 448 of a 24-bit value is rounded, so that
+// of the largest may come out over 448.
+__device__ __forceinline__ float f8_quotient(float v, const F8Div& d) {
+  const float q = __builtin_amdgcn_fmed3f(v * d.mul / d.by, -448.0f, 448.0f);
+  return fabsf(v) < INFINITY ? q : NAN;
+}
+
+// Codes of four values, the first in the low byte.
+__device__ __forceinline__ uint32_t f8_codes4(const float* v, const F8Div& d) {
+  int c = 0;
+  c = __builtin_amdgcn_cvt_pk_fp8_f32(f8_quotient(v[0], d), f8_quotient(v[1], d), c, false);
+  c = __builtin_amdgcn_cvt_pk_fp8_f32(f8_quotient(v[2], d), f8_quotient(v[3], d), c, true);
+  return static_cast<uint32_t>(c);
+}
+
+struct F8QuantArgs {
+  const void* x;    // [M, K]
+  uint8_t* codes;   // [M, Kp]
+  float* scales;    // rows: [M, blocks]; weights: [row blocks, blocks]
+  int M, K;
+};
+
+// One product, grouped: rows [offsets[e], offsets[e + 1]) of x times matrix e, transposed.
+struct F8MatmulArgs {
+  const uint8_t* x;        // [*, Kp]
+  const float* x_scales;   // [*, blocks of K]
+  const int32_t* row_src;  // x row of each row, or nullptr: the row itself
+  const int32_t* offsets;  // [E + 1], or nullptr: one matrix, all rows
+  const uint8_t* w;        // [E, N, Kp]
+  const float* w_scales;   // [E, blocks of N, blocks of K]; gate_up: of I twice
+  void* out;               // [M, N] (out_dtype)
+  uint8_t* out_codes;      // gate_up: [M, Ip]
+  float* out_scales;       // gate_up: [M, blocks of I]
+  int M, N, Kp, E;         // gate_up: N = 2 I
+  int out_dtype, act;
+  int zero_rest;           // rows of no matrix become zeros in out
+};
+
+hipError_t launch_f8_quantize(const F8QuantArgs& a, int dtype, hipStream_t s);
+hipError_t launch_f8_quantize_weight(const F8QuantArgs& a, int dtype, hipStream_t s);
+// gate_up: out_codes, out_scales = act(gate) * up in 8 bits, of gate rows 0 .. I - 1 and up
+// rows I .. 2 I - 1; else out.
+hipError_t launch_f8_stream(const F8MatmulArgs& a, bool gate_up, hipStream_t s);
+
+}  // namespace moe355

@@ -1,0 +1,96 @@
+// The product of 8-bit tiles and what the matrix kernels share (fp8_stream.hip,
+// fp8_tiled.hip). Included inside their anonymous namespaces.
+#pragma once
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// 16 weight rows x 16 token rows over one step of 128 columns, from zero: lane 16 q + r has
+// columns 16 q .. + 15 and 64 + 16 q .. + 15 of row r of both (the order of columns is free as
+// long as they share it) and gets weight rows 4 q .. 4 q + 3 of token r. A step is
+// one block of the scales, so its sum is scaled and added in fp32. The instruction aligns the
+// products of a step to their largest and keeps about 13 bits below it: of 128 products a sum is
+// off by 2^-16 of its typical size for normal data, 2^-14.5 where the values' sizes spread over
+// e^2, and at most by 2^-11 of its largest product (measured). That is a 16th of a bf16
+// rounding and half of an f16 one. The instruction of 32 columns keeps no more, at 2.26 instead of
+// 3.5 PFLOP/s (all products from registers, this one with the scaled sums).
+__device__ __forceinline__ f32x4 mma_f8(const u32x4* w, const u32x4* x) {
+  const i32x8 a = {static_cast<int>(w[0][0]), static_cast<int>(w[0][1]), static_cast<int>(w[0][2]),
+                   static_cast<int>(w[0][3]), static_cast<int>(w[1][0]), static_cast<int>(w[1][1]),
+                   static_cast<int>(w[1][2]), static_cast<int>(w[1][3])};
+  const i32x8 b = {static_cast<int>(x[0][0]), static_cast<int>(x[0][1]), static_cast<int>(x[0][2]),
+                   static_cast<int>(x[0][3]), static_cast<int>(x[1][0]), static_cast<int>(x[1][1]),
+                   static_cast<int>(x[1][2]), static_cast<int>(x[1][3])};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0,
+                                                          0, 0, 0);
+}
+
+// offsets[i] of the groups, kept within the rows whatever is given.
+__device__ __forceinline__ int group_start(const F8MatmulArgs& a, int i) {
+  if (!a.offsets) return i == 0 ? 0 : a.M;
+  return min(max(a.offsets[i], 0), a.M);
+}
+
+// Rows of a matrix that are multiplied together.
+struct RowTile {
+  int e, row0, row_end;  // e -1: none
+};
+
+// Tile `index` of all matrices' tiles of `rows` rows, matrices ascending. All lanes
+// of a wave call it; the answer is the same in all.
+__device__ __forceinline__ RowTile find_tile(const F8MatmulArgs& a, int rows, int index) {
+  constexpr int kPer = kMaxExperts / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int per = (a.E + kWave - 1) / kWave;
+  int at[kPer + 1], tiles[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i <= kPer; ++i) at[i] = i <= per ? group_start(a, min(lane * per + i, a.E)) : 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    tiles[i] = i < per ? (max(at[i + 1] - at[i], 0) + rows - 1) / rows : 0;
+    sum += tiles[i];
+  }
+  int end = sum;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int up = __shfl_up(end, o, kWave);
+    if (lane >= o) end += up;
+  }
+  int left = index - (end - sum);  // tiles of this lane before it
+  const unsigned long long has = __ballot(left >= 0 && left < sum);
+  if (!has) return RowTile{-1, 0, 0};
+  RowTile t{-1, 0, 0};
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (t.e < 0 && left < tiles[i]) t = RowTile{lane * per + i, at[i] + left * rows, at[i + 1]};
+    left -= tiles[i];
+  }
+  const int src = __ffsll(has) - 1;
+  t.e = __builtin_amdgcn_readlane(t.e, src);
+  t.row0 = __builtin_amdgcn_readlane(t.row0, src);
+  t.row_end = min(__builtin_amdgcn_readlane(t.row_end, src), t.row0 + rows);
+  return t;
+}
+
+// Four consecutive results of a row, the first at column n.
+template <typename OutT>
+__device__ __forceinline__ void store_results(const F8MatmulArgs& a, int row, int n, f32x4 v) {
+  OutT* p = static_cast<OutT*>(a.out) + static_cast<size_t>(row) * a.N + n;
+  if (a.N % 4 == 0) {
+    if (n < a.N) store4<OutT>(p, v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) p[i] = from_f32<OutT>(v[i]);
+  }
+}
+
+// Zeros in the rows of no matrix: before the first and behind the last one.
+template <typename OutT, int kThreads>
+__device__ __forceinline__ void zero_rest(const F8MatmulArgs& a) {
+  if (!a.zero_rest || !a.offsets) return;
+  const int first = group_start(a, 0), last = max(group_start(a, a.E), first);
+  for (int r = blockIdx.x; r < a.M - (last - first); r += gridDim.x) {
+    const size_t row = r < first ? r : r + (last - first);
+    for (int n = threadIdx.x; n < a.N; n += kThreads) static_cast<OutT*>(a.out)[row * a.N + n] = from_f32<OutT>(0.f);
+  }
+}

@@ -1,4 +1,4 @@
-"""RMSNorm on libmoe355 (one HIP kernel per call, GPU tensors only).
+"""RMSNorm and LayerNorm on libmoe355 (one HIP kernel per call, GPU tensors only).
 
 Same class surface as the reference's RMSNorm (reframework/layers/norm.py:17-53):
 ``RMSNorm(size, eps, bias=False)`` with ``weight`` (and ``bias``) parameters,
@@ -9,6 +9,9 @@ once to the input dtype; ``forward_add_residual`` first forms
 ``(rmsnorm(residual), residual)``. Parameters may be stored in fp32 or the
 activation dtype. ``forward_mxfp8`` and ``forward_add_residual_mxfp8`` also leave
 the normed rows in 8 bits (mx.Mxfp8Rows), for expert products that take them.
+
+``LayerNorm`` has the same surface (the reference has none) and gradients: with respect to
+its inputs and parameters wherever autograd records.
 """
 
 from __future__ import annotations
@@ -115,4 +118,119 @@ class RMSNorm(BaseOP):
         return out, q, new_res
 
 
-__all__ = ["RMSNorm"]
+class _LayerNormFn(torch.autograd.Function):
+    """(normed, x + residual), or (normed,) without a residual."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps):
+        ctx.set_materialize_grads(False)
+        H = x.shape[-1]
+        T = x.numel() // H
+        stats = torch.empty(2, T, dtype=torch.float32, device=x.device)
+        out = torch.empty_like(x)
+        r = x if residual is None else torch.empty_like(x)
+        _capi.layer_norm(T, H, x, residual, None if residual is None else r, weight, bias, eps, out,
+                         stats)
+        ctx.save_for_backward(r, weight, stats)
+        ctx.has_bias = bias is not None
+        return out if residual is None else (out, r)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dres=None):
+        r, weight, stats = ctx.saved_tensors
+        H = r.shape[-1]
+        T = r.numel() // H
+        need_x, need_res, need_w, need_b = ctx.needs_input_grad[:4]
+        if dy is None:  # only the sum went on
+            return (dres if need_x else None, dres if need_res else None,
+                    torch.zeros_like(weight) if need_w else None,
+                    torch.zeros_like(weight) if need_b else None, None)
+        dx = torch.empty_like(r) if need_x or need_res else None
+        dw = torch.empty_like(weight) if need_w else None
+        db = torch.empty_like(weight) if need_b else None
+        if T == 0:
+            return (dx if need_x else None, dx if need_res else None, None if dw is None else
+                    dw.zero_(), None if db is None else db.zero_(), None)
+        _capi.layer_norm_bwd(T, H, dy.contiguous(), None if dres is None else dres.contiguous(), r,
+                             weight, stats, dx, dw, db)
+        return (dx if need_x else None, dx if need_res else None, dw, db, None)
+
+
+class LayerNorm(BaseOP):
+    """``(r - mean(r)) / sqrt(var(r) + eps) * weight (+ bias)`` over the last dimension of
+    ``size``, in fp32 and rounded once to the input's type (float32, bfloat16, float16; up
+    to 16384 wide, 8192 in float32). Parameters may be of another of these types than the
+    inputs; their gradients are summed in fp32 over all rows, in a fixed order, and rounded
+    once."""
+
+    def __init__(self, size: int, eps: float, bias: bool = True) -> None:
+        super().__init__()
+        self.eps = eps
+        self.size = size
+        self.weight = nn.Parameter(torch.ones(size))
+        self.bias = nn.Parameter(torch.zeros(size)) if bias else None
+
+    def _check(self, x: torch.Tensor) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        w, b = self.weight, self.bias
+        dev = x.get_device()
+        if not x.is_cuda:
+            raise RuntimeError(f"reframework_amd LayerNorm runs on a ROCm GPU; input is on {x.device}")
+        if x.shape[-1] != self.size:
+            raise ValueError(f"input rows of {x.shape[-1]} do not match the norm's size {self.size}")
+        if w.get_device() != dev or (b is not None and b.get_device() != dev):
+            raise RuntimeError("LayerNorm parameters must be on the input's device")
+        if not w.is_contiguous():
+            w = w.contiguous()
+        if b is not None:
+            if b.dtype != w.dtype:
+                b = b.to(w.dtype)
+            if not b.is_contiguous():
+                b = b.contiguous()
+        return w, b
+
+    def _records(self, *inputs: torch.Tensor) -> bool:
+        return torch.is_grad_enabled() and (
+            self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad) or
+            any(t.requires_grad for t in inputs))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        w, b = self._check(x)
+        x = x.contiguous()
+        if self._records(x):
+            return _LayerNormFn.apply(x, None, w, b, self.eps)
+        out = torch.empty_like(x)
+        _capi.layer_norm(x.numel() // self.size, self.size, x, None, None, w, b, self.eps, out)
+        return out
+
+    def forward_inplace(self, x: torch.Tensor) -> None:
+        """``x`` is overwritten by its norm; no gradients are recorded through this one."""
+        w, b = self._check(x)
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("forward_inplace overwrites what a gradient needs; use forward")
+        if not x.is_contiguous():
+            with torch.no_grad():
+                x.copy_(self.forward(x))
+            return
+        _capi.layer_norm(x.numel() // self.size, self.size, x, None, None, w, b, self.eps, x)
+
+    def forward_add_residual(self, x: torch.Tensor,
+                             residual: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``residual = x + residual; x = layernorm(residual)`` in one launch; returns
+        (normed, new_residual). The inputs are not modified."""
+        w, b = self._check(x)
+        if residual.shape != x.shape or residual.get_device() != x.get_device():
+            raise ValueError(f"residual {tuple(residual.shape)} on {residual.device} does not match "
+                             f"x {tuple(x.shape)} on {x.device}")
+        x = x.contiguous()
+        if residual.dtype != x.dtype:
+            residual = residual.to(x.dtype)
+        residual = residual.contiguous()
+        if self._records(x, residual):
+            return _LayerNormFn.apply(x, residual, w, b, self.eps)
+        out, r = torch.empty_like(x), torch.empty_like(x)
+        _capi.layer_norm(x.numel() // self.size, self.size, x, residual, r, w, b, self.eps, out)
+        return out, r
+
+
+__all__ = ["RMSNorm", "LayerNorm"]

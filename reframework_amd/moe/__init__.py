@@ -1,8 +1,10 @@
 """MoE: routing, grouped expert compute and the host-offload expert cache.
 
 Import surface of the reference's ``reframework.moe`` (reframework/moe/
-__init__.py:8-18), and what it lacks: routing by groups (grouped_topk) and experts on
-4-bit weights (Mxfp4Experts, fused_experts_mxfp4).
+__init__.py:8-18), and what it lacks: routing by groups (grouped_topk), experts on 4-bit
+weights (Mxfp4Experts, fused_experts_mxfp4) and on 8-bit weights (Fp8Experts,
+fused_experts_fp8), the products with such weights (Fp8Weight, matmul_fp8) and the way of
+tokens to their experts and back with gradients (permute_tokens, combine_tokens).
 """
 
 import importlib
@@ -11,12 +13,15 @@ import sys
 import torch
 
 from reframework_amd import _capi
+from reframework_amd.fp8 import Fp8Experts, Fp8Rows, Fp8Weight, matmul_fp8, quantize_fp8
 from reframework_amd.moe import fused as _fused
-from reframework_amd.moe.fused import (fused_experts, fused_experts_mxfp4, grouped_topk,
-                                       torch_fused_topk)
+from reframework_amd.moe.fused import (fused_experts, fused_experts_fp8, fused_experts_mxfp4,
+                                       grouped_topk, torch_fused_topk)
 from reframework_amd.moe.moe_layer import CpuShuttle, FusedMoE
 from reframework_amd.moe.offload_cache import (ExpertOffloadCache, ExpertPool, OffloadStats,
                                                Prediction)
+from reframework_amd.moe.tokens import (TokenOrder, combine_tokens, permute_tokens,
+                                        token_order)
 from reframework_amd.mx import Mxfp4Experts, Mxfp8Rows, quantize_mxfp8
 
 
@@ -88,6 +93,16 @@ __all__ = [
     "Mxfp4Experts",
     "Mxfp8Rows",
     "quantize_mxfp8",
+    "fused_experts_fp8",
+    "Fp8Experts",
+    "Fp8Rows",
+    "Fp8Weight",
+    "quantize_fp8",
+    "matmul_fp8",
+    "TokenOrder",
+    "token_order",
+    "permute_tokens",
+    "combine_tokens",
     "FusedMoE",
     "CpuShuttle",
     "ExpertOffloadCache",
