@@ -29,8 +29,13 @@ int check_weights(int N, int K, int E) {
   return MOE355_OK;
 }
 
+// Average rows per matrix that has any.
+int average_rows(const F8MatmulArgs& a) { return a.M / std::max(1, std::min(a.M, a.E)); }
+
 hipError_t launch_matmul(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
-  return launch_f8_stream(a, gate_up, s);
+  const int rows = average_rows(a);
+  if (rows <= 16) return launch_f8_stream(a, gate_up, s);
+  return launch_f8_tiled(a, gate_up, rows < 100 ? 64 : 256, s);
 }
 
 // Where the data of an expert call lies in the workspace.

@@ -79,5 +79,7 @@ hipError_t launch_f8_quantize_weight(const F8QuantArgs& a, int dtype, hipStream_
 // gate_up: out_codes, out_scales = act(gate) * up in 8 bits, of gate rows 0 .. I - 1 and up
 // rows I .. 2 I - 1; else out.
 hipError_t launch_f8_stream(const F8MatmulArgs& a, bool gate_up, hipStream_t s);
+// tile_rows: 64 or 256
+hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, hipStream_t s);
 
 }  // namespace moe355

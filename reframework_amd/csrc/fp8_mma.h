@@ -13,6 +13,13 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 // e^2, and at most by 2^-11 of its largest product (measured). That is a 16th of a bf16
 // rounding and half of an f16 one. The instruction of 32 columns keeps no more, at 2.26 instead of
 // 3.5 PFLOP/s (all products from registers, this one with the scaled sums).
+//
+// The vector unit may read the result 12 wait states after the instruction, which the compiler
+// sees to within a block of instructions; across a branch (ROCm 7.2) it has been seen to leave
+// too few, and the sum then came out without its last product. So no branch may come between
+// this and the use of its result: a step's products and sums are straight-line code, counts of
+// tiles and steps are compile-time constants there (tests/test_mma_hazards.py looks at the
+// code that is built).
 __device__ __forceinline__ f32x4 mma_f8(const u32x4* w, const u32x4* x) {
   const i32x8 a = {static_cast<int>(w[0][0]), static_cast<int>(w[0][1]), static_cast<int>(w[0][2]),
                    static_cast<int>(w[0][3]), static_cast<int>(w[1][0]), static_cast<int>(w[1][1]),

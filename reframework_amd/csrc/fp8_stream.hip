@@ -51,13 +51,14 @@ __global__ __launch_bounds__(kPairs* kSplit* kWave) void stream_kernel(const F8M
   const float* xs = a.x_scales + src * steps;
 
   f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-  for (int k0 = split; k0 < steps; k0 += kSplit * kUnroll) {
-    u32x4 w[kUnroll][2][2], x[kUnroll][2];
-    float sx[kUnroll], sw[kUnroll][2];
+  // kCount steps from k0 on, straight-line (mma_f8), all their operands loaded at once.
+  auto run = [&](int k0, auto count) {
+    constexpr int kCount = decltype(count)::value;
+    u32x4 w[kCount][2][2], x[kCount][2];
+    float sx[kCount], sw[kCount][2];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < kCount; ++u) {
       const int k = k0 + u * kSplit;
-      if (k >= steps) continue;
       const size_t at = static_cast<size_t>(k) * kF8Block;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -70,8 +71,7 @@ __global__ __launch_bounds__(kPairs* kSplit* kWave) void stream_kernel(const F8M
       sx[u] = xs[k];
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (k0 + u * kSplit >= steps) continue;
+    for (int u = 0; u < kCount; ++u)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const f32x4 p = mma_f8(w[u][j], x[u]);
@@ -79,8 +79,14 @@ __global__ __launch_bounds__(kPairs* kSplit* kWave) void stream_kernel(const F8M
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(p[i], s, acc[j][i]);
       }
-    }
-  }
+  };
+  int k0 = split, left = (steps - split + kSplit - 1) / kSplit;  // this wave's steps
+  for (; left >= kUnroll; left -= kUnroll, k0 += kUnroll * kSplit)
+    run(k0, std::integral_constant<int, kUnroll>());
+  static_assert(kUnroll == 4, "what may be left");
+  if (left == 3) run(k0, std::integral_constant<int, 3>());
+  if (left == 2) run(k0, std::integral_constant<int, 2>());
+  if (left == 1) run(k0, std::integral_constant<int, 1>());
   if constexpr (kSplit > 1) {
     if (split > 0) {
 #pragma unroll
