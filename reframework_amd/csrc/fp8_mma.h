@@ -31,6 +31,27 @@ __device__ __forceinline__ f32x4 mma_f8(const u32x4* w, const u32x4* x) {
                                                           0, 0, 0);
 }
 
+// The largest of the four lanes of a token (rows of 16 lanes are exchanged without the LDS); v
+// is not negative.
+__device__ __forceinline__ float row_max(float v) {
+  uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(max(b[0], b[1]));
+}
+
+// f(activation as a compile-time constant).
+template <typename F>
+__device__ __forceinline__ void by_activation(int act, F f) {
+  if (act == MOE355_ACT_SILU)
+    f(std::integral_constant<int, MOE355_ACT_SILU>());
+  else if (act == MOE355_ACT_GELU)
+    f(std::integral_constant<int, MOE355_ACT_GELU>());
+  else
+    f(std::integral_constant<int, MOE355_ACT_GELU_TANH>());
+}
+
 // offsets[i] of the groups, kept within the rows whatever is given.
 __device__ __forceinline__ int group_start(const F8MatmulArgs& a, int i) {
   if (!a.offsets) return i == 0 ? 0 : a.M;

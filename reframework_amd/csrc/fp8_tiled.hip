@@ -53,44 +53,31 @@ struct Item {
   int e, row0, row_end, wt;
 };
 
-template <bool kGateUp, int BM, int WM>
-__global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a) {
-  typedef Shape<BM, WM> S;
-  constexpr int kMT = S::kMT, kNT = S::kNT;
-  __shared__ __attribute__((aligned(1024))) uint8_t stage[S::kStages][S::kStage];
-  __shared__ Item items[kMaxItems];
-  __shared__ int first_row[kMaxExperts + 1], first_tile[kMaxExperts + 1];
-  __shared__ float most[S::kWN][BM];
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int q = lane >> 4, r = lane & 15;
-  const int I = a.N / 2;
+__device__ __forceinline__ Item uniform(const Item* p) {
+  return Item{__builtin_amdgcn_readfirstlane(p->e), __builtin_amdgcn_readfirstlane(p->row0),
+              __builtin_amdgcn_readfirstlane(p->row_end), __builtin_amdgcn_readfirstlane(p->wt)};
+}
 
-  if constexpr (!kGateUp) {
-    if (a.out_dtype == MOE355_F32)
-      zero_rest<float, kThreads>(a);
-    else
-      zero_rest<f16, kThreads>(a);  // zeros of both 16-bit types
-  }
+// Writes this workgroup's items and returns how many there are: one of every gridDim.x, the
+// workgroups of an XCD taking neighbouring ones, each time some further, so that a matrix of
+// one full and one partial tile does not give one workgroup all full ones. The token
+// tiles of a matrix vary fastest, so that neighbours share its weights.
+template <int BM, int WM>
+__device__ __forceinline__ int list_items(const F8MatmulArgs& a, int nw, Item* items) {
+  constexpr int kShift = 15;
+  __shared__ int first_row[kMaxExperts + 1], first_tile[kMaxExperts + 1];
+  const int lane = threadIdx.x & (kWave - 1);
   for (int e = threadIdx.x; e <= a.E; e += kThreads) first_row[e] = group_start(a, e);
   __syncthreads();
-  if (wave == 0)
+  if (threadIdx.x < kWave)
     wave_scan(a.E, lane, [&](int e) { return (max(first_row[e + 1] - first_row[e], 0) + BM - 1) / BM; },
               first_tile);
   __syncthreads();
-
-  // This workgroup's items: one of every gridDim.x, the workgroups of an XCD taking
-  // neighbouring ones, each time some further, so that a matrix of one full and one partial
-  // tile does not give one workgroup all full ones. The token tiles of a matrix vary
-  // fastest, so that neighbours share its weights.
-  constexpr int kShift = 15;
-  const int nw = kGateUp ? f8_blocks(I) : (a.N + kBN - 1) / kBN;
   const int total = first_tile[a.E] * nw;
   const int G = gridDim.x, pid = blockIdx.x;
   const int rounds = min(total / G, kMaxItems - 1), tail = min(total - rounds * G, G);
   const int n_items = rounds + (pid < tail ? 1 : 0);
-  if (n_items == 0) return;
-  if (wave == 0 && lane < n_items) {
+  if (static_cast<int>(threadIdx.x) < n_items) {
     const int n = lane < rounds ? G : tail;
     const int L = lane * G + (xcd_remap(pid, n) + kShift * lane) % n;
     int lo = 0, hi = a.E - 1;  // the last matrix whose items start at or before L
@@ -107,32 +94,47 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
     items[lane] = Item{lo, row0, min(row0 + height, begin + rows), wt};
   }
   __syncthreads();
-  auto item_at = [&](int j) {
-    const Item* p = &items[j];
-    return Item{__builtin_amdgcn_readfirstlane(p->e), __builtin_amdgcn_readfirstlane(p->row0),
-                __builtin_amdgcn_readfirstlane(p->row_end), __builtin_amdgcn_readfirstlane(p->wt)};
-  };
-  const int steps = a.Kp / kF8Block;
+  return n_items;
+}
 
-  // Token rows whose codes (kTokLoads of them) and scales this lane loads, as rows of x; -1
-  // past the tile's last row.
-  const int tok64 = wave % (BM / 64);  // 64 tokens whose scales this wave loads
+// What a wave loads of the stream of its workgroup's steps.
+template <bool kGateUp, int BM, int WM>
+struct Loader {
+  typedef Shape<BM, WM> S;
+  const F8MatmulArgs& a;
+  const Item* items;
+  const int n_items, steps, wave;
+  // The item whose steps are being loaded: sources, and this lane's offsets.
+  __amdgpu_buffer_rsrc_t xsrc, xssrc, wsrc;
+  uint32_t xoff[S::kTokLoads], woff[S::kWgtLoads], soff;
+  // Token rows of the next item whose codes and scales this lane loads, as rows of x; -1 past
+  // the tile's last row.
   int src[S::kTokLoads + 1];
-  auto load_rows = [&](const Item& it) {
+  int item = 0, step = 0, loaded = 0;  // loaded: steps of all items
+
+  __device__ __forceinline__ Loader(const F8MatmulArgs& args, const Item* list, int n, int w)
+      : a(args), items(list), n_items(n), steps(args.Kp / kF8Block), wave(w) {
+    load_rows(uniform(items));
+    begin(uniform(items));
+  }
+  // 64 tokens whose scales this wave loads
+  __device__ __forceinline__ int tok64() const { return wave % (BM / 64); }
+  // The lane, opaque: what follows from it is computed where an item begins, not kept.
+  static __device__ __forceinline__ int lane_id() { return pipe::opaque(threadIdx.x & (kWave - 1)); }
+  __device__ __forceinline__ void load_rows(const Item& it) {
+    const int lane = lane_id();
 #pragma unroll
     for (int i = 0; i <= S::kTokLoads; ++i) {
-      const int row = i < S::kTokLoads ? 8 * (wave * S::kTokLoads + i) + (lane >> 3) : 64 * tok64 + lane;
+      const int row = i < S::kTokLoads ? 8 * (wave * S::kTokLoads + i) + (lane >> 3) : 64 * tok64() + lane;
       const int p = it.row0 + row;
       src[i] = p >= it.row_end ? -1 : a.row_src ? a.row_src[p] : row;
     }
-  };
-
-  // The item whose steps are being loaded: sources, and this lane's offsets. Where rows are not
-  // gathered they are counted from the tile's first, so that offsets stay small.
-  __amdgpu_buffer_rsrc_t xsrc, xssrc, wsrc;
-  uint32_t xoff[S::kTokLoads], woff[S::kWgtLoads], soff;
-  int load_item = 0, load_step = 0, loaded = 0;  // loaded: steps of all items
-  auto begin_loads = [&](const Item& it) {
+  }
+  // Chunk of a row (modulo 8) that a lane loads.
+  static __device__ __forceinline__ int chunk(int lane, int row) { return ((lane & 7) ^ ((row >> 1) & 7)) << 4; }
+  __device__ __forceinline__ void begin(const Item& it) {
+    const int lane = lane_id();
+    // Rows that are not gathered are counted from the tile's first, so that offsets stay small.
     const size_t first = a.row_src ? 0 : it.row0;
     xsrc = pipe::lds_rsrc(a.x + first * a.Kp);
     xssrc = pipe::lds_rsrc(a.x_scales + first * steps);
@@ -141,75 +143,263 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
     for (int i = 0; i < S::kTokLoads; ++i) {
       const int row = 8 * (wave * S::kTokLoads + i) + (lane >> 3);
       xoff[i] = src[i] < 0 ? pipe::kPadOffset  // out of range: zeros
-                           : static_cast<uint32_t>(src[i]) * a.Kp + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+                           : static_cast<uint32_t>(src[i]) * a.Kp + chunk(lane, row);
     }
 #pragma unroll
     for (int i = 0; i < S::kWgtLoads; ++i) {
-      const int row = 8 * (wave * S::kWgtLoads + i) + (lane >> 3);  // of the tile
-      int n;
-      bool in;
-      if constexpr (kGateUp) {
-        const int wn = row / (16 * kNT), g = row / 16 % kNT;
-        const int f = it.wt * kF8Block + wn * 8 * kNT + g % (kNT / 2) * 16 + row % 16;
-        in = f < I;
-        n = f + (g < kNT / 2 ? 0 : I);
-      } else {
-        n = it.wt * kBN + row;
-        in = n < a.N;
+      const int row = weight_row(i) + (lane >> 3);
+      const int wn = row / (16 * S::kNT), g = row / 16 % S::kNT;
+      int n = it.wt * kBN + row, end = a.N;
+      if constexpr (kGateUp) {  // gate and up of the same features, half of a wave's tiles each
+        end = a.N / 2;
+        n = it.wt * kF8Block + wn * 8 * S::kNT + g % (S::kNT / 2) * 16 + row % 16;
       }
-      woff[i] = in ? static_cast<uint32_t>(n) * a.Kp + (((lane & 7) ^ ((row >> 1) & 7)) << 4)
-                   : pipe::kPadOffset;
+      const int up = kGateUp && g >= S::kNT / 2 ? a.N / 2 : 0;
+      woff[i] = n < end ? static_cast<uint32_t>(n + up) * a.Kp + chunk(lane, row) : pipe::kPadOffset;
     }
     soff = src[S::kTokLoads] < 0 ? pipe::kPadOffset : static_cast<uint32_t>(src[S::kTokLoads]) * steps * 4;
-    load_step = 0;
-    if (load_item + 1 < n_items) load_rows(item_at(load_item + 1));
-  };
-  // Loads the next step of the stream, if there is one.
-  auto load = [&]() {
-    if (load_item >= n_items) return;
-    uint8_t* s = stage[loaded % S::kStages];
-    const int k = load_step;
+    step = 0;
+    if (item + 1 < n_items) load_rows(uniform(items + item + 1));
+  }
+  // First of the 8 rows of the weight tile (as it lies in LDS) that load i brings: the loads of
+  // the first half bring the first half of every wave's tiles.
+  __device__ __forceinline__ int weight_row(int i) const {
+    constexpr int kHalf = S::kWgtLoads / 2;
+    const int piece = wave * kHalf + i % kHalf + i / kHalf * (kHalf * kWaves);  // of 8 rows
+    const int half = piece / (kHalf * kWaves), p = piece % (kHalf * kWaves);
+    const int per = S::kNT;  // pieces of 8 rows in half of a wave's tiles
+    return (p / per) * 16 * S::kNT + half * 8 * S::kNT + p % per * 8;
+  }
+  __device__ __forceinline__ bool more() const { return item < n_items; }
+  __device__ __forceinline__ void load_tokens(uint8_t* s) const {
 #pragma unroll
     for (int i = 0; i < S::kTokLoads; ++i)
-      pipe::dma16_rsrc(xsrc, xoff[i], k * kF8Block, s + (wave * S::kTokLoads + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < S::kWgtLoads; ++i)
-      pipe::dma16_rsrc(wsrc, woff[i], k * kF8Block, s + S::kTokBytes + (wave * S::kWgtLoads + i) * 1024);
+      pipe::dma16_rsrc(xsrc, xoff[i], step * kF8Block, s + (wave * S::kTokLoads + i) * 1024);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        xssrc, (pipe::lds_void*)(s + S::kTokBytes + S::kWgtBytes + tok64 * 256), 4, soff, k * 4, 0, 0);
+        xssrc, (pipe::lds_void*)(s + S::kTokBytes + S::kWgtBytes + tok64() * 256), 4, soff, step * 4, 0, 0);
+  }
+  template <int kHalf>
+  __device__ __forceinline__ void load_weights(uint8_t* s) const {
+#pragma unroll
+    for (int i = kHalf * (S::kWgtLoads / 2); i < (kHalf + 1) * (S::kWgtLoads / 2); ++i)
+      pipe::dma16_rsrc(wsrc, woff[i], step * kF8Block,
+                       s + S::kTokBytes + weight_row(i) * kF8Block);
+  }
+  __device__ __forceinline__ void next() {
     ++loaded;
-    if (++load_step == steps && ++load_item < n_items) begin_loads(item_at(load_item));
+    if (++step == steps && ++item < n_items) begin(uniform(items + item));
+  }
+};
+
+// All waves; nothing moves across it.
+__device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Order of `n` products and the scaled sums of their results: each result is added while the
+// three products after it are on their way, which takes no more registers than those.
+template <int n>
+__device__ __forceinline__ void interleave() {
+  constexpr int kMfma = 0x8, kValu = 0x2, kAhead = n < 3 ? n : 3;
+  if constexpr (n > 0) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
+#pragma unroll
+    for (int i = kAhead; i < n; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kValu, 4, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kValu, 4 * kAhead, 0);
+  }
+}
+
+// f(mt as a compile-time constant), mt in [0, kMost].
+template <int kMost, typename F>
+__device__ __forceinline__ void by_count(int mt, F f) {
+  switch (mt) {
+    case 0: f(std::integral_constant<int, 0>()); break;
+    case 1: f(std::integral_constant<int, 1>()); break;
+    case 2: f(std::integral_constant<int, (kMost < 2 ? kMost : 2)>()); break;
+    case 3: f(std::integral_constant<int, (kMost < 3 ? kMost : 3)>()); break;
+    default: f(std::integral_constant<int, kMost>()); break;
+  }
+}
+
+// Scales of the weight rows of a wave in an item, by step: of gate (all of a product), of up.
+template <bool kGateUp, typename S>
+__device__ __forceinline__ void weight_scales(const F8MatmulArgs& a, const Item& it, int wn,
+                                              const const_f32** gate, const const_f32** up) {
+  const int I = a.N / 2, steps = a.Kp / kF8Block;
+  const int n_blocks = kGateUp ? 2 * f8_blocks(I) : f8_blocks(a.N);
+  const int block = kGateUp ? it.wt : min((it.wt * kBN + wn * 16 * S::kNT) / kF8Block, n_blocks - 1);
+  *gate = (const const_f32*)(a.w_scales + (static_cast<size_t>(it.e) * n_blocks + block) * steps);
+  *up = *gate + (kGateUp ? static_cast<size_t>(f8_blocks(I)) * steps : 0);
+}
+
+// gate_up's epilogue, first part: gate's place takes act(gate) * up; the largest of each token's
+// features in this wave goes to `most` [waves over weights][BM].
+template <typename S, int BM, int WM>
+__device__ __forceinline__ void activate(const F8MatmulArgs& a, const Item& it, f32x4 (&acc)[S::kMT][S::kNT],
+                                         int wm, int wn, float (*most)[BM]) {
+  constexpr int kHalf = S::kNT / 2;
+  const int lane = pipe::opaque(threadIdx.x & (kWave - 1)), q = lane >> 4, r = lane & 15;
+  const int f0 = it.wt * kF8Block + wn * 16 * kHalf + 4 * q, I = a.N / 2;
+  by_activation(a.act, [&](auto act) {
+#pragma unroll
+    for (int m = 0; m < S::kMT; ++m) {
+      float amax = 0.f;
+#pragma unroll
+      for (int g = 0; g < kHalf; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float h =
+              f0 + 16 * g + i < I ? gate_act_fast(act.value, acc[m][g][i]) * acc[m][g + kHalf][i] : 0.f;
+          acc[m][g][i] = h;
+          amax = fmaxf(amax, f8_finite_abs(h));
+        }
+      amax = row_max(amax);
+      if (q == 0) most[wn][16 * (wm + WM * m) + r] = amax;
+    }
+  });
+}
+
+// The second part, behind a barrier: the codes and scales.
+template <typename S, int BM, int WM>
+__device__ __forceinline__ void store_codes(const F8MatmulArgs& a, const Item& it,
+                                            const f32x4 (&acc)[S::kMT][S::kNT], int wm, int wn,
+                                            const float (*most)[BM]) {
+  constexpr int kHalf = S::kNT / 2;
+  const int lane = pipe::opaque(threadIdx.x & (kWave - 1)), q = lane >> 4, r = lane & 15;
+  const int f0 = it.wt * kF8Block + wn * 16 * kHalf + 4 * q;
+  const size_t Ip = f8_pad(a.N / 2);
+#pragma unroll
+  for (int m = 0; m < S::kMT; ++m) {
+    const int row = 16 * (wm + WM * m) + r;
+    if (row >= it.row_end - it.row0) continue;
+    float amax = most[0][row];
+#pragma unroll
+    for (int w = 1; w < S::kWN; ++w) amax = fmaxf(amax, most[w][row]);
+    const F8Div d = f8_div(amax);
+    uint8_t* out = a.out_codes + static_cast<size_t>(it.row0 + row) * Ip + f0;
+#pragma unroll
+    for (int g = 0; g < kHalf; ++g) {
+      const float h[4] = {acc[m][g][0], acc[m][g][1], acc[m][g][2], acc[m][g][3]};
+      *reinterpret_cast<uint32_t*>(out + 16 * g) = f8_codes4(h, d);
+    }
+    if (wn == 0 && q == 0)
+      a.out_scales[static_cast<size_t>(it.row0 + row) * (Ip / kF8Block) + it.wt] = d.scale;
+  }
+}
+
+typedef unsigned short u16;
+
+// Four results rounded to a 16-bit type.
+template <typename T>
+__device__ __forceinline__ u32x2 pack4(f32x4 v) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, T4{from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])});
+}
+
+// A product's epilogue. Stored relative to the tile's first row; an offset out of range stores
+// nothing, so that there are no branches per element.
+template <typename S, int WM, typename OutT>
+__device__ __forceinline__ void store_rows(const F8MatmulArgs& a, const Item& it,
+                                           const f32x4 (&acc)[S::kMT][S::kNT], int wm, int wn) {
+  const int lane = pipe::opaque(threadIdx.x & (kWave - 1)), q = lane >> 4, r = lane & 15;
+  constexpr int kSize = sizeof(OutT);
+  const auto out = pipe::lds_rsrc(static_cast<OutT*>(a.out) + static_cast<size_t>(it.row0) * a.N);
+  const int n_rows = it.row_end - it.row0;
+  const int n0 = it.wt * kBN + wn * S::kNT * 16;  // this wave's first column
+  if (a.N % 8 == 0) {
+#pragma unroll
+    for (int m = 0; m < S::kMT; ++m) {
+      const int row = 16 * (wm + WM * m) + r;
+      const uint32_t at = row < n_rows ? row * a.N * kSize : pipe::kPadOffset;
+#pragma unroll
+      for (int g = 0; g < S::kNT; g += kSize == 4 ? 1 : 2) {
+        if constexpr (kSize == 4) {
+          const int n = n0 + 16 * g + 4 * q;
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[m][g]), out,
+                                                 n < a.N ? at + n * kSize : pipe::kPadOffset, 0, 0);
+        } else {
+          // Two tiles' columns are exchanged between the lanes of a row, so that each stores 16
+          // bytes and a row gets 64 consecutive ones.
+          const u32x2 u = pack4<OutT>(acc[m][g]), w = pack4<OutT>(acc[m][g + 1]);
+          const auto lo = __builtin_amdgcn_permlane16_swap(u[0], w[0], false, false);
+          const auto hi = __builtin_amdgcn_permlane16_swap(u[1], w[1], false, false);
+          const int n = n0 + 16 * (g + (q & 1)) + 8 * (q >> 1);
+          __builtin_amdgcn_raw_buffer_store_b128(u32x4{lo[0], hi[0], lo[1], hi[1]}, out,
+                                                 n < a.N ? at + n * kSize : pipe::kPadOffset, 0, 0);
+        }
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int m = 0; m < S::kMT; ++m) {
+    const int row = 16 * (wm + WM * m) + r;
+    const uint32_t at = row < n_rows ? row * a.N * kSize : pipe::kPadOffset;
+#pragma unroll
+    for (int g = 0; g < S::kNT; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = n0 + 16 * g + 4 * q + i;
+        const uint32_t off = n < a.N ? at + n * kSize : pipe::kPadOffset;
+        const OutT v = from_f32<OutT>(acc[m][g][i]);
+        if constexpr (kSize == 4)
+          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), out, off, 0, 0);
+        else
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(u16, v), out, off, 0, 0);
+      }
+  }
+}
+
+// All waves read and multiply a step between two barriers.
+template <bool kGateUp, int BM, int WM, typename OutT>
+__global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a) {
+  typedef Shape<BM, WM> S;
+  constexpr int kMT = S::kMT, kNT = S::kNT;
+  __shared__ __attribute__((aligned(1024))) uint8_t stage[S::kStages][S::kStage];
+  __shared__ Item items[kMaxItems];
+  __shared__ float most[S::kWN][BM];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int q = lane >> 4, r = lane & 15, sw = (r >> 1) & 7;
+
+  if constexpr (!kGateUp) zero_rest<OutT, kThreads>(a);
+  const int nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
+  const int n_items = list_items<BM, WM>(a, nw, items);
+  if (n_items == 0) return;
+  const int steps = a.Kp / kF8Block;
+  Loader<kGateUp, BM, WM> ld(a, items, n_items, wave);
+  auto load = [&]() {
+    if (!ld.more()) return;
+    uint8_t* s = stage[ld.loaded % S::kStages];
+    ld.load_tokens(s);
+    ld.template load_weights<0>(s);
+    ld.template load_weights<1>(s);
+    ld.next();
   };
   // Waits until this wave's loads of step `step` of the stream have landed; of the steps after
   // it kStages - 2 may be in flight (fewer at the end of the stream, where it waits for
   // all).
   auto landed = [&](int step) {
-    if (loaded >= step + S::kStages - 1)
+    if (ld.loaded >= step + S::kStages - 1)
       pipe::wait_vmcnt<(S::kStages - 2) * S::kLoads>();
     else
       pipe::wait_vmcnt<0>();
   };
-  auto barrier = [&]() {
-    __builtin_amdgcn_sched_barrier(0);
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_barrier();
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-
-  load_rows(item_at(0));
-  begin_loads(item_at(0));
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) load();
   int done = 0;  // steps of the stream
   const int wm = wave % WM, wn = wave / WM;  // this wave's tokens and weight rows
   for (int j = 0; j < n_items; ++j) {
-    const Item it = item_at(j);
-    // scales of this wave's weight rows: of gate (all of a product) and of up
-    const int n_blocks = kGateUp ? 2 * f8_blocks(I) : f8_blocks(a.N);
-    const int block = kGateUp ? it.wt : min((it.wt * kBN + wn * 16 * kNT) / kF8Block, n_blocks - 1);
-    const const_f32* ws0 = (const const_f32*)(a.w_scales + (static_cast<size_t>(it.e) * n_blocks + block) * steps);
-    const const_f32* ws1 = ws0 + (kGateUp ? static_cast<size_t>(f8_blocks(I)) * steps : 0);
+    const Item it = uniform(items + j);
+    const const_f32 *ws0, *ws1;
+    weight_scales<kGateUp, S>(a, it, wn, &ws0, &ws1);
     f32x4 acc[kMT][kNT];
 #pragma unroll
     for (int m = 0; m < kMT; ++m)
@@ -218,8 +408,7 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
     // A wave has every WM-th 16 rows of the tile, so that the waves share the rows of one that
     // is not full; mt of its kMT hold any.
     const int mt = min((it.row_end - it.row0 + 16 * (WM - 1 - wm) + 15) / (16 * WM), kMT);
-    // One instance per count: mma_f8 needs straight-line code.
-    auto run_steps = [&](auto count) {
+    by_count<kMT>(mt, [&](auto count) {  // one instance per count: mma_f8 needs straight-line code
       constexpr int kM = decltype(count)::value;
       for (int st = 0; st < steps; ++st, ++done) {
         // Every wave has read step `done` - 1, whose buffer is filled again, and has seen its
@@ -232,7 +421,6 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
         const uint8_t* s = stage[done % S::kStages];
         const uint8_t* wtile = s + S::kTokBytes + (wn * kNT * 16 + r) * kF8Block;
         const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
-        const int sw = (r >> 1) & 7;  // rows of a tile start at multiples of 16
         u32x4 x[kM + 1][2];
         float sg[kM + 1], su[kM + 1];
 #pragma unroll
@@ -259,77 +447,173 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
           }
         }
       }
-    };
-    switch (mt) {
-      case 0: run_steps(std::integral_constant<int, 0>()); break;
-      case 1: run_steps(std::integral_constant<int, 1>()); break;
-      case 2: run_steps(std::integral_constant<int, (kMT < 2 ? kMT : 2)>()); break;
-      case 3: run_steps(std::integral_constant<int, (kMT < 3 ? kMT : 3)>()); break;
-      default: run_steps(std::integral_constant<int, kMT>()); break;
-    }
-
-    const int n_rows = it.row_end - it.row0, row1 = 16 * wm + r;
+    });
     if constexpr (kGateUp) {
-      constexpr int kHalf = kNT / 2;
-      const int f0 = it.wt * kF8Block + wn * 16 * kHalf + 4 * q;  // this lane's first feature
-      const size_t Ip = f8_pad(I);
-      // gate's place takes the activation
-      float amax[kMT];
-#pragma unroll
-      for (int m = 0; m < kMT; ++m) {
-        amax[m] = 0.f;
-#pragma unroll
-        for (int g = 0; g < kHalf; ++g)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float h =
-                f0 + 16 * g + i < I ? gate_act_fast(a.act, acc[m][g][i]) * acc[m][g + kHalf][i] : 0.f;
-            acc[m][g][i] = h;
-            amax[m] = fmaxf(amax[m], f8_finite_abs(h));
-          }
-        amax[m] = fmaxf(amax[m], __shfl_xor(amax[m], 16, kWave));
-        amax[m] = fmaxf(amax[m], __shfl_xor(amax[m], 32, kWave));
-        if (q == 0) most[wn][row1 + 16 * WM * m] = amax[m];
-      }
+      activate<S, BM, WM>(a, it, acc, wm, wn, most);
       pipe::wait_lgkm0();
       barrier();
-#pragma unroll
-      for (int m = 0; m < kMT; ++m) {
-        const int row = row1 + 16 * WM * m;
-        if (row >= n_rows) continue;
-#pragma unroll
-        for (int w = 0; w < S::kWN; ++w) amax[m] = fmaxf(amax[m], most[w][row]);
-        const F8Div d = f8_div(amax[m]);
-        uint8_t* out = a.out_codes + static_cast<size_t>(it.row0 + row) * Ip + f0;
-#pragma unroll
-        for (int g = 0; g < kHalf; ++g) {
-          const float h[4] = {acc[m][g][0], acc[m][g][1], acc[m][g][2], acc[m][g][3]};
-          *reinterpret_cast<uint32_t*>(out + 16 * g) = f8_codes4(h, d);
-        }
-        if (wn == 0 && q == 0)
-          a.out_scales[static_cast<size_t>(it.row0 + row) * (Ip / kF8Block) + it.wt] = d.scale;
-      }
       // `most` is written again by the next item's epilogue, behind a barrier of its steps
+      store_codes<S, BM, WM>(a, it, acc, wm, wn, most);
     } else {
-      auto store = [&](auto type) {
-#pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          const int row = row1 + 16 * WM * m;
-          if (row >= n_rows) continue;
-#pragma unroll
-          for (int g = 0; g < kNT; ++g)
-            store_results<decltype(type)>(a, it.row0 + row, it.wt * kBN + (wn * kNT + g) * 16 + 4 * q,
-                                          acc[m][g]);
-        }
-      };
-      if (a.out_dtype == MOE355_F32) store(float());
-      else if (a.out_dtype == MOE355_BF16) store(bf16());
-      else store(f16());
+      store_rows<S, WM, OutT>(a, it, acc, wm, wn);
     }
   }
 }
 
-template <bool kGateUp, int BM, int WM>
+// 256 token rows. Two waves share a SIMD and work in turns, half a step each: while the first
+// four waves multiply four of their eight tile columns, the others read the operands of
+// theirs from LDS, and a barrier swaps them, so that the matrix cores always have a wave with
+// its operands in registers. Reading and multiplying a step between two barriers, all waves read at once
+// while the matrix cores wait: 730 us instead of 515 for 8192 rows of 8 matrices of 14336 x
+// 4096.
+//
+// There is room for two steps in LDS. A step's tokens and the first half of its weight tiles
+// are read in the first of a step's two reading phases only, so their place is loaded again half a
+// step before that of the other half: each load has one and a half steps until it is
+// read.
+//   phase        4s          4s + 1      4s + 2      4s + 3
+//   waves 0-3    read s, 1   mul s, 1    read s, 2   mul s, 2
+//   waves 4-7    (mul s-1,2) read s, 1   mul s, 1    read s, 2
+// A wave asks for the second half of step s + 1 when it reads the first half of s, and for the
+// tokens and first half of s + 2 when it reads the second half of s: both places were read for the
+// last time in the phase before. Before a phase that reads a part, every wave has seen its
+// own loads of it land: those of at most the two parts asked for after it are in flight.
+template <bool kGateUp, typename OutT>
+__global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a) {
+  constexpr int BM = 256, WM = 4;
+  typedef Shape<BM, WM> S;
+  constexpr int kMT = S::kMT, kNT = S::kNT, kHalf = kNT / 2;
+  static_assert(S::kStages == 2, "room for two steps");
+  __shared__ __attribute__((aligned(1024))) uint8_t stage[S::kStages][S::kStage];
+  __shared__ Item items[kMaxItems];
+  __shared__ float most[S::kWN][BM];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int q = lane >> 4, r = lane & 15, sw = (r >> 1) & 7;
+
+  if constexpr (!kGateUp) zero_rest<OutT, kThreads>(a);
+  const int nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
+  const int n_items = list_items<BM, WM>(a, nw, items);
+  if (n_items == 0) return;
+  const int steps = a.Kp / kF8Block;
+  Loader<kGateUp, BM, WM> ld(a, items, n_items, wave);
+  auto load_first = [&]() {
+    if (!ld.more()) return;
+    uint8_t* s = stage[ld.loaded & 1];
+    ld.load_tokens(s);
+    ld.template load_weights<0>(s);
+  };
+  auto load_second = [&]() {
+    if (!ld.more()) return;
+    ld.template load_weights<1>(stage[ld.loaded & 1]);
+    ld.next();
+  };
+  // Waits for this wave's loads of a part of step `step`; `after`: steps whose loads have been
+  // asked for in full and lie behind it in the pipeline when that is full.
+  auto landed = [&](int full) {
+    if (ld.loaded >= full && ld.more())
+      pipe::wait_vmcnt<S::kLoads>();
+    else
+      pipe::wait_vmcnt<0>();
+  };
+  load_first();
+  load_second();
+  load_first();
+  const bool second = wave >= 4;
+  landed(1);
+  barrier();
+  if (second) barrier();
+
+  int done = 0;  // steps of the stream
+  // The four waves of a turn hold both halves of the weight rows of their tokens.
+  const int wm = wave >> 1, wn = wave & 1;
+  for (int j = 0; j < n_items; ++j) {
+    const Item it = uniform(items + j);
+    const const_f32 *ws0, *ws1;
+    weight_scales<kGateUp, S>(a, it, wn, &ws0, &ws1);
+    f32x4 acc[kMT][kNT];
+#pragma unroll
+    for (int m = 0; m < kMT; ++m)
+#pragma unroll
+      for (int g = 0; g < kNT; ++g) acc[m][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int mt = min((it.row_end - it.row0 + 16 * (WM - 1 - wm) + 15) / (16 * WM), kMT);
+    by_count<kMT>(mt, [&](auto count) {
+      constexpr int kM = decltype(count)::value;
+      for (int st = 0; st < steps; ++st, ++done) {
+        const uint8_t* s = stage[done & 1];
+        const uint8_t* wtile = s + S::kTokBytes + (wn * kNT * 16 + r) * kF8Block;
+        const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
+        const float s0 = ws0[st], s1 = kGateUp ? ws1[st] : 0.f;
+        u32x4 x[kM + 1][2], w[kHalf][2];
+        float sg[kM + 1], su[kM + 1];
+        auto read_weights = [&](int half) {
+#pragma unroll
+          for (int g = 0; g < (kM ? kHalf : 0); ++g) {
+            const uint8_t* p = wtile + (half * kHalf + g) * 16 * kF8Block;
+            w[g][0] = *reinterpret_cast<const u32x4*>(p + ((q ^ sw) << 4));
+            w[g][1] = *reinterpret_cast<const u32x4*>(p + (((4 + q) ^ sw) << 4));
+          }
+        };
+        auto multiply = [&](int half) {
+#pragma unroll
+          for (int g = 0; g < (kM ? kHalf : 0); ++g)
+#pragma unroll
+            for (int m = 0; m < kM; ++m) {
+              const f32x4 v = mma_f8(w[g], x[m]);
+              const float f = kGateUp && half ? su[m] : sg[m];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                acc[m][half * kHalf + g][i] = fmaf(v[i], f, acc[m][half * kHalf + g][i]);
+            }
+          interleave<kM ? kM * kHalf : 0>();
+          // here, not where the sums are used next: their addends would stay in registers
+#pragma unroll
+          for (int g = 0; g < (kM ? kHalf : 0); ++g)
+#pragma unroll
+            for (int m = 0; m < kM; ++m) asm volatile("" : "+v"(acc[m][half * kHalf + g]));
+        };
+        // read the first half
+        load_second();  // of step done + 1
+        read_weights(0);
+#pragma unroll
+        for (int m = 0; m < kM; ++m) {
+          const uint8_t* p = s + (16 * (wm + WM * m) + r) * kF8Block;
+          x[m][0] = *reinterpret_cast<const u32x4*>(p + ((q ^ sw) << 4));
+          x[m][1] = *reinterpret_cast<const u32x4*>(p + (((4 + q) ^ sw) << 4));
+          const float xs = *reinterpret_cast<const float*>(ts + 64 * WM * m);
+          sg[m] = xs * s0;
+          su[m] = xs * s1;
+        }
+        if (second) landed(done + 2);  // the second half of step done
+        pipe::wait_lgkm0();
+        barrier();
+        multiply(0);
+        if (!second) landed(done + 2);
+        barrier();
+        // read the second half
+        load_first();  // of step done + 2
+        read_weights(1);
+        if (second) landed(done + 2);  // the first half of step done + 1
+        pipe::wait_lgkm0();
+        barrier();
+        multiply(1);
+        if (!second) landed(done + 2);
+        barrier();
+      }
+    });
+    if constexpr (kGateUp) {
+      activate<S, BM, WM>(a, it, acc, wm, wn, most);
+      pipe::wait_lgkm0();
+      barrier();  // one turn more, for both groups of waves
+      store_codes<S, BM, WM>(a, it, acc, wm, wn, most);
+    } else {
+      store_rows<S, WM, OutT>(a, it, acc, wm, wn);
+    }
+  }
+  if (!second) barrier();
+}
+
+template <bool kGateUp, int BM, int WM, typename OutT>
 hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
   const long long nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
   // at most: every matrix that has rows has a tile that is not full
@@ -340,16 +624,27 @@ hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
   // the items of a workgroup have kMaxItems - 1 full rounds at most
   const long long most = grid * (kMaxItems - 1);
   grid = total < grid ? total : grid * ((total + most - 1) / most);
-  tiled_kernel<kGateUp, BM, WM><<<dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s>>>(a);
+  const dim3 groups(static_cast<unsigned>(grid));
+  if constexpr (BM == 256)
+    turns_kernel<kGateUp, OutT><<<groups, dim3(kThreads), 0, s>>>(a);
+  else
+    tiled_kernel<kGateUp, BM, WM, OutT><<<groups, dim3(kThreads), 0, s>>>(a);
   return hipGetLastError();
+}
+
+template <int BM, int WM>
+hipError_t launch_bm(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
+  if (gate_up) return launch<true, BM, WM, float>(a, s);
+  if (a.out_dtype == MOE355_F32) return launch<false, BM, WM, float>(a, s);
+  if (a.out_dtype == MOE355_BF16) return launch<false, BM, WM, bf16>(a, s);
+  return launch<false, BM, WM, f16>(a, s);
 }
 
 }  // namespace
 
 hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, hipStream_t s) {
   if (a.M == 0) return hipSuccess;
-  if (tile_rows == 256) return gate_up ? launch<true, 256, 4>(a, s) : launch<false, 256, 4>(a, s);
-  return gate_up ? launch<true, 64, 2>(a, s) : launch<false, 64, 2>(a, s);
+  return tile_rows == 256 ? launch_bm<256, 4>(a, gate_up, s) : launch_bm<64, 2>(a, gate_up, s);
 }
 
 }  // namespace moe355
