@@ -29,20 +29,34 @@ int check_weights(int N, int K, int E) {
   return MOE355_OK;
 }
 
-// Average rows per matrix that has any.
-int average_rows(const F8MatmulArgs& a) { return a.M / std::max(1, std::min(a.M, a.E)); }
+// Which kernels run a product of M rows of E matrices over Kp columns: tile_rows 0 streams
+// the weights; max_parts: parts of items that the tiled kernels may leave in memory.
+struct F8Path {
+  int tile_rows, max_parts;
+  size_t part_bytes;
+};
 
-hipError_t launch_matmul(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
-  const int rows = average_rows(a);
-  if (rows <= 16) return launch_f8_stream(a, gate_up, s);
-  return launch_f8_tiled(a, gate_up, rows < 100 ? 64 : 256, s);
+F8Path f8_path(int M, int E, int Kp) {
+  F8Path p{};
+  const int rows = M / std::max(1, std::min(M, E));  // per matrix that has any, on average
+  if (rows <= 16) return p;
+  p.tile_rows = rows < 100 ? 64 : 256;
+  // cutting items of few steps saves less than the second launch takes
+  if (Kp / kF8Block >= (p.tile_rows == 256 ? 16 : 24)) p.max_parts = device_cu_count();
+  p.part_bytes = static_cast<size_t>(p.max_parts) * f8_part_floats(p.tile_rows) * 4;
+  return p;
+}
+
+hipError_t launch_matmul(const F8Path& p, const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
+  return p.tile_rows ? launch_f8_tiled(a, gate_up, p.tile_rows, s) : launch_f8_stream(a, gate_up, s);
 }
 
 // Where the data of an expert call lies in the workspace.
 struct F8Plan {
   int rows, n_blocks, max_tiles;
+  F8Path up, down;
   size_t block_counts, offsets, slot_to_row, row_src, tile_map, xq, xq_scales, inter, inter_scales,
-      y, bytes;
+      y, parts, bytes;
 };
 
 int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
@@ -60,6 +74,8 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->rows = static_cast<int>(R);
   p->n_blocks = R <= kPermuteSingleMax ? 1 : static_cast<int>((R + kPermuteChunk - 1) / kPermuteChunk);
   p->max_tiles = E + p->rows / (1 << 20);
+  p->up = f8_path(p->rows, E, f8_pad(H));
+  p->down = f8_path(p->rows, E, f8_pad(I));
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -76,6 +92,7 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->inter = take(static_cast<size_t>(R) * f8_pad(I));
   p->inter_scales = take(static_cast<size_t>(R) * f8_blocks(I) * 4);
   p->y = take(static_cast<size_t>(R) * H * 4);
+  p->parts = take(std::max(p->up.part_bytes, p->down.part_bytes));
   p->bytes = off;
   return MOE355_OK;
 }
@@ -112,9 +129,17 @@ int moe355_fp8_quantize_weight(const void* w, int N, int K, int dtype, void* cod
   return check_hip(launch_f8_quantize_weight(a, dtype, as_stream(stream)), "fp8_quantize_weight launch");
 }
 
+int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, size_t* bytes) {
+  if (!bytes) return fail(MOE355_EINVAL, "NULL result");
+  if (int rc = check_weights(N, K, E)) return rc;
+  if (M < 0) return fail(MOE355_EINVAL, "bad M=%d", M);
+  *bytes = M == 0 ? 0 : f8_path(M, E, f8_pad(K)).part_bytes;
+  return MOE355_OK;
+}
+
 int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const float* w_scales,
                       const int32_t* offsets, int M, int N, int K, int E, int dtype, void* out,
-                      void* stream) {
+                      void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_weights(N, K, E)) return rc;
   if (M < 0) return fail(MOE355_EINVAL, "bad M=%d", M);
   if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
@@ -122,13 +147,18 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
   if (M == 0) return MOE355_OK;
   if (!x || !x_scales || !w || !w_scales || !out) return fail(MOE355_EINVAL, "NULL tensor argument");
   if (!aligned16(x) || !aligned16(w) || !aligned4(x_scales) || !aligned4(w_scales) ||
-      !aligned4(offsets) || !aligned16(out))
-    return fail(MOE355_EINVAL, "x/w/scales/offsets/out not aligned");
+      !aligned4(offsets) || !aligned16(out) || !aligned16(workspace))
+    return fail(MOE355_EINVAL, "x/w/scales/offsets/out/workspace not aligned");
+  const F8Path p = f8_path(M, E, f8_pad(K));
+  if (p.part_bytes > 0 && (!workspace || workspace_bytes < p.part_bytes))
+    return fail(MOE355_EWORKSPACE, "workspace of %zu bytes, the call needs %zu", workspace_bytes,
+                p.part_bytes);
   F8MatmulArgs a{};
   a.x = static_cast<const uint8_t*>(x); a.x_scales = x_scales; a.offsets = offsets;
   a.w = static_cast<const uint8_t*>(w); a.w_scales = w_scales; a.out = out;
   a.M = M; a.N = N; a.Kp = f8_pad(K); a.E = E; a.out_dtype = dtype; a.zero_rest = 1;
-  return check_hip(launch_matmul(a, false, as_stream(stream)), "fp8_matmul launch");
+  a.parts = static_cast<float*>(workspace); a.max_parts = p.max_parts;
+  return check_hip(launch_matmul(p, a, false, as_stream(stream)), "fp8_matmul launch");
 }
 
 int moe355_fp8_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes) {
@@ -198,14 +228,16 @@ int moe355_fp8_fused_experts(const void* x, const float* x_scales, const void* w
     a.out_codes = at<uint8_t>(workspace, p.inter);
     a.out_scales = at<float>(workspace, p.inter_scales);
     a.M = p.rows; a.N = 2 * I; a.Kp = Hp; a.E = E; a.act = act;
-    if (int rc = check_hip(launch_matmul(a, true, s), "fp8 gate_up launch")) return rc;
+    a.parts = at<float>(workspace, p.parts); a.max_parts = p.up.max_parts;
+    if (int rc = check_hip(launch_matmul(p.up, a, true, s), "fp8 gate_up launch")) return rc;
 
     F8MatmulArgs d{};
     d.x = a.out_codes; d.x_scales = a.out_scales; d.offsets = pa.offsets;
     d.w = static_cast<const uint8_t*>(w2); d.w_scales = w2_scales;
     d.out = at<void>(workspace, p.y);
     d.M = p.rows; d.N = H; d.Kp = f8_pad(I); d.E = E; d.out_dtype = MOE355_F32;
-    if (int rc = check_hip(launch_matmul(d, false, s), "fp8 down launch")) return rc;
+    d.parts = a.parts; d.max_parts = p.down.max_parts;
+    if (int rc = check_hip(launch_matmul(p.down, d, false, s), "fp8 down launch")) return rc;
 
     CombineArgs c{};
     c.y = d.out; c.topk_w = weights; c.slot_to_row = pa.slot_to_row;

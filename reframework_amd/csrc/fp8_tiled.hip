@@ -37,7 +37,8 @@ struct Shape {
   static constexpr int kTokBytes = BM * kF8Block;
   static constexpr int kWgtBytes = kBN * kF8Block;
   static constexpr int kStage = kTokBytes + kWgtBytes + BM * 4;
-  static constexpr int kSpare = kMaxItems * 16 + (kMaxExperts + 1) * 8 + kWN * BM * 4 + 64;
+  static constexpr int kPartTile = kMT * kNT * kThreads * 4;  // floats of a part's sums
+  static constexpr int kSpare = kMaxItems * 32 + (kMaxExperts + 1) * 8 + kWN * BM * 4 + 64;
   static constexpr int kStages = (160 * 1024 - kSpare) / kStage;
   // direct-to-LDS loads of a wave per step: 1 KB of codes each, and 256 bytes of scales
   // (some waves' a second time)
@@ -48,24 +49,48 @@ struct Shape {
   static_assert(kStages >= 2 && (kStages - 1) * kLoads < 64, "pipeline");
 };
 
-// Weight tile `wt` of the token rows [row0, row_end) of matrix e.
+// Weight tile `wt` of the token rows [row0, row_end) of matrix e, steps [k0, k1). part: where its
+// sums go where they are only some of the steps, else -1.
 struct Item {
-  int e, row0, row_end, wt;
+  int e, row0, row_end, wt, k0, k1, part;
 };
 
 __device__ __forceinline__ Item uniform(const Item* p) {
-  return Item{__builtin_amdgcn_readfirstlane(p->e), __builtin_amdgcn_readfirstlane(p->row0),
-              __builtin_amdgcn_readfirstlane(p->row_end), __builtin_amdgcn_readfirstlane(p->wt)};
+  return Item{__builtin_amdgcn_readfirstlane(p->e),  __builtin_amdgcn_readfirstlane(p->row0),
+              __builtin_amdgcn_readfirstlane(p->row_end), __builtin_amdgcn_readfirstlane(p->wt),
+              __builtin_amdgcn_readfirstlane(p->k0), __builtin_amdgcn_readfirstlane(p->k1),
+              __builtin_amdgcn_readfirstlane(p->part)};
 }
 
-// Writes this workgroup's items and returns how many there are: one of every gridDim.x, the
-// workgroups of an XCD taking neighbouring ones, each time some further, so that a matrix of
-// one full and one partial tile does not give one workgroup all full ones. The token
-// tiles of a matrix vary fastest, so that neighbours share its weights.
-template <int BM, int WM>
-__device__ __forceinline__ int list_items(const F8MatmulArgs& a, int nw, Item* items) {
-  constexpr int kShift = 15;
-  __shared__ int first_row[kMaxExperts + 1], first_tile[kMaxExperts + 1];
+// The items of a launch of G workgroups: `rounds` of one per workgroup, and `tail` more. Run as
+// they are those would take a whole item's time on some of the CUs; cut into `split` parts of
+// the steps each they take a part of it on all, and a second launch adds the parts and stores.
+struct Rounds {
+  int rounds, tail, split;
+};
+
+// What a cut saves and costs, in steps of an item: a part's sums go to memory and back, all
+// workgroups' at once (256 rows: 0.5 MB per unit at 5 TB/s, against 2 us a step), and the
+// second launch takes 4 us.
+template <int BM>
+__device__ __forceinline__ Rounds plan_rounds(int total, int G, int steps, int max_parts) {
+  Rounds p{min(total / G, kMaxItems - 1), 0, 1};
+  p.tail = min(total - p.rounds * G, G);
+  const int cap = min(max_parts, G);
+  int best = 40 * steps;
+  for (int s = 2; s <= 16 && s * p.tail <= cap && steps >= 4 * s; s *= 2) {
+    const int cost = (40 * steps + s - 1) / s + 80 + 2 * s * p.tail;
+    if (cost < best) {
+      best = cost;
+      p.split = s;
+    }
+  }
+  return p;
+}
+
+// The matrices' first rows and tiles (the last entries: the ends).
+template <int BM>
+__device__ __forceinline__ void list_tiles(const F8MatmulArgs& a, int* first_row, int* first_tile) {
   const int lane = threadIdx.x & (kWave - 1);
   for (int e = threadIdx.x; e <= a.E; e += kThreads) first_row[e] = group_start(a, e);
   __syncthreads();
@@ -73,25 +98,51 @@ __device__ __forceinline__ int list_items(const F8MatmulArgs& a, int nw, Item* i
     wave_scan(a.E, lane, [&](int e) { return (max(first_row[e + 1] - first_row[e], 0) + BM - 1) / BM; },
               first_tile);
   __syncthreads();
-  const int total = first_tile[a.E] * nw;
-  const int G = gridDim.x, pid = blockIdx.x;
-  const int rounds = min(total / G, kMaxItems - 1), tail = min(total - rounds * G, G);
-  const int n_items = rounds + (pid < tail ? 1 : 0);
-  if (static_cast<int>(threadIdx.x) < n_items) {
-    const int n = lane < rounds ? G : tail;
-    const int L = lane * G + (xcd_remap(pid, n) + kShift * lane) % n;
-    int lo = 0, hi = a.E - 1;  // the last matrix whose items start at or before L
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first_tile[mid] * nw <= L) lo = mid; else hi = mid - 1;
+}
+
+// Item L of all. The token tiles of a matrix vary fastest, so that neighbours share its
+// weights.
+template <int BM, int WM>
+__device__ __forceinline__ Item decode_item(const F8MatmulArgs& a, int nw, const int* first_row,
+                                            const int* first_tile, int L) {
+  int lo = 0, hi = a.E - 1;  // the last matrix whose items start at or before L
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first_tile[mid] * nw <= L) lo = mid; else hi = mid - 1;
+  }
+  const int begin = first_row[lo], rows = first_row[lo + 1] - begin;
+  const int tiles = first_tile[lo + 1] - first_tile[lo];
+  // the matrix's rows are shared evenly by its tiles, in whole 16 rows of all waves
+  const int height = ((rows + tiles - 1) / tiles + 16 * WM - 1) / (16 * WM) * (16 * WM);
+  const int at = L - first_tile[lo] * nw, wt = at / tiles;
+  const int row0 = begin + (at - wt * tiles) * height;
+  return Item{lo, row0, min(row0 + height, begin + rows), wt, 0, a.Kp / kF8Block, -1};
+}
+
+// Writes this workgroup's items and returns how many there are: one of every gridDim.x, the
+// workgroups of an XCD taking neighbouring ones, each time some further, so that a matrix of
+// one full and one partial tile does not give one workgroup all full ones.
+template <int BM, int WM>
+__device__ __forceinline__ int list_items(const F8MatmulArgs& a, int nw, Item* items) {
+  constexpr int kShift = 15;
+  __shared__ int first_row[kMaxExperts + 1], first_tile[kMaxExperts + 1];
+  list_tiles<BM>(a, first_row, first_tile);
+  const int G = gridDim.x, pid = blockIdx.x, lane = threadIdx.x, steps = a.Kp / kF8Block;
+  const Rounds p = plan_rounds<BM>(first_tile[a.E] * nw, G, steps, a.max_parts);
+  const int units = p.tail * p.split;
+  const int n_items = p.rounds + (pid < units ? 1 : 0);
+  if (lane < n_items) {
+    const bool full = lane < p.rounds;
+    const int n = full ? G : units;
+    const int u = (xcd_remap(pid, n) + kShift * lane) % n;
+    Item it = decode_item<BM, WM>(a, nw, first_row, first_tile, lane * G + (full ? u : u / p.split));
+    if (!full && p.split > 1) {
+      const int part = u % p.split;
+      it.k0 = part * steps / p.split;
+      it.k1 = (part + 1) * steps / p.split;
+      it.part = u;
     }
-    const int begin = first_row[lo], rows = first_row[lo + 1] - begin;
-    const int tiles = first_tile[lo + 1] - first_tile[lo];
-    // the matrix's rows are shared evenly by its tiles
-    const int height = ((rows + tiles - 1) / tiles + 16 * WM - 1) / (16 * WM) * (16 * WM);
-    const int at = L - first_tile[lo] * nw, wt = at / tiles;
-    const int row0 = begin + (at - wt * tiles) * height;
-    items[lane] = Item{lo, row0, min(row0 + height, begin + rows), wt};
+    items[lane] = it;
   }
   __syncthreads();
   return n_items;
@@ -110,7 +161,7 @@ struct Loader {
   // Token rows of the next item whose codes and scales this lane loads, as rows of x; -1 past
   // the tile's last row.
   int src[S::kTokLoads + 1];
-  int item = 0, step = 0, loaded = 0;  // loaded: steps of all items
+  int item = 0, step = 0, end = 0, loaded = 0;  // loaded: steps of all items
 
   __device__ __forceinline__ Loader(const F8MatmulArgs& args, const Item* list, int n, int w)
       : a(args), items(list), n_items(n), steps(args.Kp / kF8Block), wave(w) {
@@ -158,7 +209,8 @@ struct Loader {
       woff[i] = n < end ? static_cast<uint32_t>(n + up) * a.Kp + chunk(lane, row) : pipe::kPadOffset;
     }
     soff = src[S::kTokLoads] < 0 ? pipe::kPadOffset : static_cast<uint32_t>(src[S::kTokLoads]) * steps * 4;
-    step = 0;
+    step = it.k0;
+    end = it.k1;
     if (item + 1 < n_items) load_rows(uniform(items + item + 1));
   }
   // First of the 8 rows of the weight tile (as it lies in LDS) that load i brings: the loads of
@@ -187,7 +239,7 @@ struct Loader {
   }
   __device__ __forceinline__ void next() {
     ++loaded;
-    if (++step == steps && ++item < n_items) begin(uniform(items + item));
+    if (++step == end && ++item < n_items) begin(uniform(items + item));
   }
 };
 
@@ -200,19 +252,19 @@ __device__ __forceinline__ void barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Order of `n` products and the scaled sums of their results: each result is added while the
-// three products after it are on their way, which takes no more registers than those.
-template <int n>
-__device__ __forceinline__ void interleave() {
-  constexpr int kMfma = 0x8, kValu = 0x2, kAhead = n < 3 ? n : 3;
-  if constexpr (n > 0) {
-    __builtin_amdgcn_sched_group_barrier(kMfma, kAhead, 0);
+// n products and the scaled sums of their results, product(i) and add(i, its result), each result
+// added behind the third product after it: it is there by then (12 wait states), without
+// waits between the products. Left to itself the compiler waits for every result: 10 % slower.
+template <int n, typename P, typename A>
+__device__ __forceinline__ void interleaved(P product, A add) {
+  constexpr int kAhead = n < 3 ? n : 3;
+  f32x4 v[kAhead + 1];
 #pragma unroll
-    for (int i = kAhead; i < n; ++i) {
-      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(kValu, 4, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(kValu, 4 * kAhead, 0);
+  for (int i = 0; i < n + kAhead; ++i) {
+    if (i < n) v[i % (kAhead + 1)] = product(i);
+    __builtin_amdgcn_sched_barrier(0);
+    if (i >= kAhead) add(i - kAhead, v[(i - kAhead) % (kAhead + 1)]);
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -239,17 +291,18 @@ __device__ __forceinline__ void weight_scales(const F8MatmulArgs& a, const Item&
   *up = *gate + (kGateUp ? static_cast<size_t>(f8_blocks(I)) * steps : 0);
 }
 
-// gate_up's epilogue, first part: gate's place takes act(gate) * up; the largest of each token's
+// The epilogues take kM of a wave's kMT tile rows, from m0 on.
+// gate_up's, first part: gate's place takes act(gate) * up; the largest of each token's
 // features in this wave goes to `most` [waves over weights][BM].
-template <typename S, int BM, int WM>
-__device__ __forceinline__ void activate(const F8MatmulArgs& a, const Item& it, f32x4 (&acc)[S::kMT][S::kNT],
-                                         int wm, int wn, float (*most)[BM]) {
+template <typename S, int BM, int WM, int kM>
+__device__ __forceinline__ void activate(const F8MatmulArgs& a, const Item& it, f32x4 (&acc)[kM][S::kNT],
+                                         int wm, int wn, int m0, float (*most)[BM]) {
   constexpr int kHalf = S::kNT / 2;
   const int lane = pipe::opaque(threadIdx.x & (kWave - 1)), q = lane >> 4, r = lane & 15;
   const int f0 = it.wt * kF8Block + wn * 16 * kHalf + 4 * q, I = a.N / 2;
   by_activation(a.act, [&](auto act) {
 #pragma unroll
-    for (int m = 0; m < S::kMT; ++m) {
+    for (int m = 0; m < kM; ++m) {
       float amax = 0.f;
 #pragma unroll
       for (int g = 0; g < kHalf; ++g)
@@ -261,23 +314,23 @@ __device__ __forceinline__ void activate(const F8MatmulArgs& a, const Item& it, 
           amax = fmaxf(amax, f8_finite_abs(h));
         }
       amax = row_max(amax);
-      if (q == 0) most[wn][16 * (wm + WM * m) + r] = amax;
+      if (q == 0) most[wn][16 * (wm + WM * (m0 + m)) + r] = amax;
     }
   });
 }
 
 // The second part, behind a barrier: the codes and scales.
-template <typename S, int BM, int WM>
+template <typename S, int BM, int WM, int kM>
 __device__ __forceinline__ void store_codes(const F8MatmulArgs& a, const Item& it,
-                                            const f32x4 (&acc)[S::kMT][S::kNT], int wm, int wn,
+                                            const f32x4 (&acc)[kM][S::kNT], int wm, int wn, int m0,
                                             const float (*most)[BM]) {
   constexpr int kHalf = S::kNT / 2;
   const int lane = pipe::opaque(threadIdx.x & (kWave - 1)), q = lane >> 4, r = lane & 15;
   const int f0 = it.wt * kF8Block + wn * 16 * kHalf + 4 * q;
   const size_t Ip = f8_pad(a.N / 2);
 #pragma unroll
-  for (int m = 0; m < S::kMT; ++m) {
-    const int row = 16 * (wm + WM * m) + r;
+  for (int m = 0; m < kM; ++m) {
+    const int row = 16 * (wm + WM * (m0 + m)) + r;
     if (row >= it.row_end - it.row0) continue;
     float amax = most[0][row];
 #pragma unroll
@@ -305,9 +358,9 @@ __device__ __forceinline__ u32x2 pack4(f32x4 v) {
 
 // A product's epilogue. Stored relative to the tile's first row; an offset out of range stores
 // nothing, so that there are no branches per element.
-template <typename S, int WM, typename OutT>
+template <typename S, int WM, typename OutT, int kM>
 __device__ __forceinline__ void store_rows(const F8MatmulArgs& a, const Item& it,
-                                           const f32x4 (&acc)[S::kMT][S::kNT], int wm, int wn) {
+                                           const f32x4 (&acc)[kM][S::kNT], int wm, int wn, int m0) {
   const int lane = pipe::opaque(threadIdx.x & (kWave - 1)), q = lane >> 4, r = lane & 15;
   constexpr int kSize = sizeof(OutT);
   const auto out = pipe::lds_rsrc(static_cast<OutT*>(a.out) + static_cast<size_t>(it.row0) * a.N);
@@ -315,8 +368,8 @@ __device__ __forceinline__ void store_rows(const F8MatmulArgs& a, const Item& it
   const int n0 = it.wt * kBN + wn * S::kNT * 16;  // this wave's first column
   if (a.N % 8 == 0) {
 #pragma unroll
-    for (int m = 0; m < S::kMT; ++m) {
-      const int row = 16 * (wm + WM * m) + r;
+    for (int m = 0; m < kM; ++m) {
+      const int row = 16 * (wm + WM * (m0 + m)) + r;
       const uint32_t at = row < n_rows ? row * a.N * kSize : pipe::kPadOffset;
 #pragma unroll
       for (int g = 0; g < S::kNT; g += kSize == 4 ? 1 : 2) {
@@ -339,8 +392,8 @@ __device__ __forceinline__ void store_rows(const F8MatmulArgs& a, const Item& it
     return;
   }
 #pragma unroll
-  for (int m = 0; m < S::kMT; ++m) {
-    const int row = 16 * (wm + WM * m) + r;
+  for (int m = 0; m < kM; ++m) {
+    const int row = 16 * (wm + WM * (m0 + m)) + r;
     const uint32_t at = row < n_rows ? row * a.N * kSize : pipe::kPadOffset;
 #pragma unroll
     for (int g = 0; g < S::kNT; ++g)
@@ -354,6 +407,54 @@ __device__ __forceinline__ void store_rows(const F8MatmulArgs& a, const Item& it
         else
           __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(u16, v), out, off, 0, 0);
       }
+  }
+}
+
+// Sums of some of an item's steps, as they lie in the lanes.
+template <typename S>
+__device__ __forceinline__ f32x4* part_at(const F8MatmulArgs& a, int part, int m) {
+  return reinterpret_cast<f32x4*>(a.parts + static_cast<size_t>(part) * S::kPartTile) +
+         m * S::kNT * kThreads + threadIdx.x;
+}
+
+template <typename S>
+__device__ __forceinline__ void store_part(const F8MatmulArgs& a, const Item& it,
+                                           const f32x4 (&acc)[S::kMT][S::kNT]) {
+#pragma unroll
+  for (int m = 0; m < S::kMT; ++m)
+#pragma unroll
+    for (int g = 0; g < S::kNT; ++g) part_at<S>(a, it.part, m)[g * kThreads] = acc[m][g];
+}
+
+// Adds the parts of the items of the last round, in their order, and stores: a workgroup takes
+// one tile row of every wave.
+template <bool kGateUp, int BM, int WM, typename OutT>
+__global__ __launch_bounds__(kThreads) void parts_kernel(const F8MatmulArgs a, int G) {
+  typedef Shape<BM, WM> S;
+  __shared__ int first_row[kMaxExperts + 1], first_tile[kMaxExperts + 1];
+  __shared__ float most[S::kWN][BM];
+  list_tiles<BM>(a, first_row, first_tile);
+  const int nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
+  const Rounds p = plan_rounds<BM>(first_tile[a.E] * nw, G, a.Kp / kF8Block, a.max_parts);
+  const int i = blockIdx.x / S::kMT, m = blockIdx.x % S::kMT;
+  if (p.split == 1 || i >= p.tail) return;
+  const Item it = decode_item<BM, WM>(a, nw, first_row, first_tile, p.rounds * G + i);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wm = wave / S::kWN, wn = wave % S::kWN;
+  f32x4 acc[1][S::kNT];
+#pragma unroll
+  for (int g = 0; g < S::kNT; ++g) acc[0][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.split; ++s) {
+    const f32x4* part = part_at<S>(a, i * p.split + s, m);
+#pragma unroll
+    for (int g = 0; g < S::kNT; ++g) acc[0][g] += part[g * kThreads];
+  }
+  if constexpr (kGateUp) {
+    activate<S, BM, WM>(a, it, acc, wm, wn, m, most);
+    __syncthreads();
+    store_codes<S, BM, WM>(a, it, acc, wm, wn, m, most);
+  } else {
+    store_rows<S, WM, OutT>(a, it, acc, wm, wn, m);
   }
 }
 
@@ -373,7 +474,6 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
   const int nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
   const int n_items = list_items<BM, WM>(a, nw, items);
   if (n_items == 0) return;
-  const int steps = a.Kp / kF8Block;
   Loader<kGateUp, BM, WM> ld(a, items, n_items, wave);
   auto load = [&]() {
     if (!ld.more()) return;
@@ -395,7 +495,7 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) load();
   int done = 0;  // steps of the stream
-  const int wm = wave % WM, wn = wave / WM;  // this wave's tokens and weight rows
+  const int wm = wave / S::kWN, wn = wave % S::kWN;  // this wave's tokens and weight rows
   for (int j = 0; j < n_items; ++j) {
     const Item it = uniform(items + j);
     const const_f32 *ws0, *ws1;
@@ -410,7 +510,7 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
     const int mt = min((it.row_end - it.row0 + 16 * (WM - 1 - wm) + 15) / (16 * WM), kMT);
     by_count<kMT>(mt, [&](auto count) {  // one instance per count: mma_f8 needs straight-line code
       constexpr int kM = decltype(count)::value;
-      for (int st = 0; st < steps; ++st, ++done) {
+      for (int st = it.k0; st < it.k1; ++st, ++done) {
         // Every wave has read step `done` - 1, whose buffer is filled again, and has seen its
         // loads of step `done` land.
         landed(done);
@@ -448,14 +548,16 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
         }
       }
     });
-    if constexpr (kGateUp) {
-      activate<S, BM, WM>(a, it, acc, wm, wn, most);
+    if (it.part >= 0) {
+      store_part<S>(a, it, acc);
+    } else if constexpr (kGateUp) {
+      activate<S, BM, WM>(a, it, acc, wm, wn, 0, most);
       pipe::wait_lgkm0();
       barrier();
       // `most` is written again by the next item's epilogue, behind a barrier of its steps
-      store_codes<S, BM, WM>(a, it, acc, wm, wn, most);
+      store_codes<S, BM, WM>(a, it, acc, wm, wn, 0, most);
     } else {
-      store_rows<S, WM, OutT>(a, it, acc, wm, wn);
+      store_rows<S, WM, OutT>(a, it, acc, wm, wn, 0);
     }
   }
 }
@@ -495,7 +597,6 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
   const int nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
   const int n_items = list_items<BM, WM>(a, nw, items);
   if (n_items == 0) return;
-  const int steps = a.Kp / kF8Block;
   Loader<kGateUp, BM, WM> ld(a, items, n_items, wave);
   auto load_first = [&]() {
     if (!ld.more()) return;
@@ -526,7 +627,7 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
 
   int done = 0;  // steps of the stream
   // The four waves of a turn hold both halves of the weight rows of their tokens.
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / S::kWN, wn = wave % S::kWN;
   for (int j = 0; j < n_items; ++j) {
     const Item it = uniform(items + j);
     const const_f32 *ws0, *ws1;
@@ -539,7 +640,7 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
     const int mt = min((it.row_end - it.row0 + 16 * (WM - 1 - wm) + 15) / (16 * WM), kMT);
     by_count<kMT>(mt, [&](auto count) {
       constexpr int kM = decltype(count)::value;
-      for (int st = 0; st < steps; ++st, ++done) {
+      for (int st = it.k0; st < it.k1; ++st, ++done) {
         const uint8_t* s = stage[done & 1];
         const uint8_t* wtile = s + S::kTokBytes + (wn * kNT * 16 + r) * kF8Block;
         const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
@@ -555,22 +656,19 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
           }
         };
         auto multiply = [&](int half) {
+          if constexpr (kM > 0) {
+            interleaved<kM * kHalf>(
+                [&](int i) { return mma_f8(w[i / kM], x[i % kM]); },
+                [&](int i, f32x4 v) {
+                  const int m = i % kM;
+                  const float f = kGateUp && half ? su[m] : sg[m];
+                  f32x4& sum = acc[m][half * kHalf + i / kM];
 #pragma unroll
-          for (int g = 0; g < (kM ? kHalf : 0); ++g)
-#pragma unroll
-            for (int m = 0; m < kM; ++m) {
-              const f32x4 v = mma_f8(w[g], x[m]);
-              const float f = kGateUp && half ? su[m] : sg[m];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                acc[m][half * kHalf + g][i] = fmaf(v[i], f, acc[m][half * kHalf + g][i]);
-            }
-          interleave<kM ? kM * kHalf : 0>();
-          // here, not where the sums are used next: their addends would stay in registers
-#pragma unroll
-          for (int g = 0; g < (kM ? kHalf : 0); ++g)
-#pragma unroll
-            for (int m = 0; m < kM; ++m) asm volatile("" : "+v"(acc[m][half * kHalf + g]));
+                  for (int j = 0; j < 4; ++j) sum[j] = fmaf(v[j], f, sum[j]);
+                  // added here, not where the sum is used next
+                  asm volatile("" : "+v"(sum));
+                });
+          }
         };
         // read the first half
         load_second();  // of step done + 1
@@ -601,13 +699,15 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
         barrier();
       }
     });
-    if constexpr (kGateUp) {
-      activate<S, BM, WM>(a, it, acc, wm, wn, most);
+    if (it.part >= 0) {
+      store_part<S>(a, it, acc);
+    } else if constexpr (kGateUp) {
+      activate<S, BM, WM>(a, it, acc, wm, wn, 0, most);
       pipe::wait_lgkm0();
       barrier();  // one turn more, for both groups of waves
-      store_codes<S, BM, WM>(a, it, acc, wm, wn, most);
+      store_codes<S, BM, WM>(a, it, acc, wm, wn, 0, most);
     } else {
-      store_rows<S, WM, OutT>(a, it, acc, wm, wn);
+      store_rows<S, WM, OutT>(a, it, acc, wm, wn, 0);
     }
   }
   if (!second) barrier();
@@ -629,6 +729,11 @@ hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
     turns_kernel<kGateUp, OutT><<<groups, dim3(kThreads), 0, s>>>(a);
   else
     tiled_kernel<kGateUp, BM, WM, OutT><<<groups, dim3(kThreads), 0, s>>>(a);
+  if (a.max_parts > 0 && hipPeekAtLastError() == hipSuccess) {
+    // at least two parts an item
+    const unsigned tails = static_cast<unsigned>((total < a.max_parts / 2 ? total : a.max_parts / 2) * Shape<BM, WM>::kMT);
+    parts_kernel<kGateUp, BM, WM, OutT><<<dim3(tails), dim3(kThreads), 0, s>>>(a, static_cast<int>(grid));
+  }
   return hipGetLastError();
 }
 
@@ -641,6 +746,10 @@ hipError_t launch_bm(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
 }
 
 }  // namespace
+
+size_t f8_part_floats(int tile_rows) {
+  return tile_rows == 256 ? Shape<256, 4>::kPartTile : Shape<64, 2>::kPartTile;
+}
 
 hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, hipStream_t s) {
   if (a.M == 0) return hipSuccess;

@@ -131,7 +131,9 @@ def spread(M, E, seed):
 
 SHAPES = [(1, 1, 1, 1), (1, 16, 128, 1), (1, 4096, 512, 3), (5, 130, 200, 4), (16, 64, 2048, 2), (17, 33, 384, 1),
           (64, 300, 1000, 7), (65, 256, 128, 1), (130, 515, 260, 5), (257, 1024, 640, 1), (300, 1000, 1248, 12),
-          (1000, 272, 144, 64), (2000, 768, 256, 3), (777, 2049, 136, 2), (3000, 512, 896, 8), (40, 64, 64, 256)]
+          (1000, 272, 144, 64), (2000, 768, 256, 3), (777, 2049, 136, 2), (3000, 512, 896, 8), (40, 64, 64, 256),
+          # items of the last round cut along the columns, on both tile heights
+          (1500, 1040, 2100, 3), (700, 514, 4096, 2), (130, 1000, 3300, 5), (33, 2100, 4000, 1), (4000, 4200, 2048, 9)]
 
 
 @pytest.mark.parametrize("M,N,K,E", SHAPES)
