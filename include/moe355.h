@@ -510,12 +510,13 @@ int moe355_fp8_quantize_weight(const void* w, int N, int K, int dtype, void* cod
  * out [M,N] = rows [offsets[e], offsets[e+1]) of x [M,K] times matrix e of w [E,N,K],
  * transposed (`x @ w[e].t()` of reframework/moe/fused.py:80-83); offsets [E+1] ascending
  * within [0,M] on the device, rows of no matrix become zeros; NULL with E = 1: all rows. A step of
- * 128 columns is summed by the matrix core, which keeps about 13 bits below its largest
- * product; the steps are scaled and added in fp32, and rounded once to dtype. Any N and K up to
+ * 128 columns is summed by the matrix core, which for 16-bit results keeps about 13 bits below
+ * its largest product (fp32 results have exact products, summed in fp32); the steps are scaled
+ * and added in fp32, and rounded once to dtype. Any N and K up to
  * 2^20 with N * Kp < 2^31. The workspace (0 bytes: none) belongs to the call until its kernels
  * end.
  */
-int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, size_t* bytes);
+int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, int dtype, size_t* bytes);
 int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const float* w_scales,
                       const int32_t* offsets, int M, int N, int K, int E, int dtype, void* out,
                       void* workspace, size_t workspace_bytes, void* stream);
@@ -524,8 +525,8 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
  * moe355_fused_experts on 8-bit weights and rows (the products of fused_experts,
  * reframework/moe/fused.py:49-87): x in 8 bits (quantised here when x_scales is NULL: x is
  * then [T,H] of dtype; else codes [T,Hp]), g, u = x . w1[e]^T, h = act(g) * u in 8 bits with
- * a scale per 128 features, y = h . w2[e]^T, out[t] = sum_k topk_w[t,k] * y, all sums in fp32,
- * rounded once. w1: codes [E,2I,Hp], gate rows first, scales [E, 2 ceil(I/128), ceil(H/128)],
+ * a scale per 128 features, y = h . w2[e]^T, out[t] = sum_k topk_w[t,k] * y, sums as in
+ * moe355_fp8_matmul, of g and u with exact products for f16 too, rounded once. w1: codes [E,2I,Hp], gate rows first, scales [E, 2 ceil(I/128), ceil(H/128)],
  * gate blocks first (the up half's blocks start at its first row); w2: codes [E,H,Ip], scales
  * [E, ceil(H/128), ceil(I/128)]. H and I multiples of 16. Slots whose id lies outside [0,E) or
  * whose weight is 0 add nothing. out may be x. The workspace belongs to the call until its

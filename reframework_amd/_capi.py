@@ -125,7 +125,7 @@ _SIGNATURES: Dict[str, Tuple[object, List[object]]] = {
     "moe355_combine_rows_bwd": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P]),
     "moe355_fp8_quantize": (_I, [_P, _I, _I, _I, _P, _P, _P]),
     "moe355_fp8_quantize_weight": (_I, [_P, _I, _I, _I, _P, _P, _P]),
-    "moe355_fp8_matmul_workspace_bytes": (_I, [_I, _I, _I, _I, ctypes.POINTER(_Z)]),
+    "moe355_fp8_matmul_workspace_bytes": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
     "moe355_fp8_matmul": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _Z, _P]),
     "moe355_fp8_workspace_bytes": (_I, [_I, _I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
     "moe355_fp8_fused_experts": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I,
@@ -682,10 +682,11 @@ def fp8_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     device = x.device
     M, N = out.shape
     E = w.shape[0]
-    nbytes = _size(device, "moe355_fp8_matmul_workspace_bytes", _rows(M), N, K, E)
+    code = dtype_code(out.dtype)
+    nbytes = _size(device, "moe355_fp8_matmul_workspace_bytes", _rows(M), N, K, E, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _call(device, "moe355_fp8_matmul", x.data_ptr(), x_scales.data_ptr(), w.data_ptr(),
-          w_scales.data_ptr(), _ptr(offsets), M, N, K, E, dtype_code(out.dtype),
+          w_scales.data_ptr(), _ptr(offsets), M, N, K, E, code,
           out.data_ptr(), _ptr(ws), nbytes, stream if stream is not None else stream_handle(device))
 
 

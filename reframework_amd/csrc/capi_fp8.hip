@@ -36,13 +36,13 @@ struct F8Path {
   size_t part_bytes;
 };
 
-F8Path f8_path(int M, int E, int Kp) {
+F8Path f8_path(int M, int E, int Kp, bool exact) {
   F8Path p{};
   const int rows = M / std::max(1, std::min(M, E));  // per matrix that has any, on average
   if (rows <= 16) return p;
-  p.tile_rows = rows < 100 ? 64 : 256;
+  p.tile_rows = rows < 100 ? 64 : exact ? 128 : 256;
   // cutting items of few steps saves less than the second launch takes
-  if (Kp / kF8Block >= (p.tile_rows == 256 ? 16 : 24)) p.max_parts = device_cu_count();
+  if (Kp / kF8Block >= (p.tile_rows > 64 ? 16 : 24)) p.max_parts = device_cu_count();
   p.part_bytes = static_cast<size_t>(p.max_parts) * f8_part_floats(p.tile_rows) * 4;
   return p;
 }
@@ -55,6 +55,7 @@ hipError_t launch_matmul(const F8Path& p, const F8MatmulArgs& a, bool gate_up, h
 struct F8Plan {
   int rows, n_blocks, max_tiles;
   F8Path up, down;
+  bool exact_up, exact_down;
   size_t block_counts, offsets, slot_to_row, row_src, tile_map, xq, xq_scales, inter, inter_scales,
       y, parts, bytes;
 };
@@ -74,8 +75,10 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->rows = static_cast<int>(R);
   p->n_blocks = R <= kPermuteSingleMax ? 1 : static_cast<int>((R + kPermuteChunk - 1) / kPermuteChunk);
   p->max_tiles = E + p->rows / (1 << 20);
-  p->up = f8_path(p->rows, E, f8_pad(H));
-  p->down = f8_path(p->rows, E, f8_pad(I));
+  p->exact_up = dtype != MOE355_BF16;
+  p->exact_down = dtype == MOE355_F32;
+  p->up = f8_path(p->rows, E, f8_pad(H), p->exact_up);
+  p->down = f8_path(p->rows, E, f8_pad(I), p->exact_down);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -129,11 +132,12 @@ int moe355_fp8_quantize_weight(const void* w, int N, int K, int dtype, void* cod
   return check_hip(launch_f8_quantize_weight(a, dtype, as_stream(stream)), "fp8_quantize_weight launch");
 }
 
-int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, size_t* bytes) {
+int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, int dtype, size_t* bytes) {
   if (!bytes) return fail(MOE355_EINVAL, "NULL result");
   if (int rc = check_weights(N, K, E)) return rc;
   if (M < 0) return fail(MOE355_EINVAL, "bad M=%d", M);
-  *bytes = M == 0 ? 0 : f8_path(M, E, f8_pad(K)).part_bytes;
+  if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  *bytes = M == 0 ? 0 : f8_path(M, E, f8_pad(K), dtype == MOE355_F32).part_bytes;
   return MOE355_OK;
 }
 
@@ -149,7 +153,7 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
   if (!aligned16(x) || !aligned16(w) || !aligned4(x_scales) || !aligned4(w_scales) ||
       !aligned4(offsets) || !aligned16(out) || !aligned16(workspace))
     return fail(MOE355_EINVAL, "x/w/scales/offsets/out/workspace not aligned");
-  const F8Path p = f8_path(M, E, f8_pad(K));
+  const F8Path p = f8_path(M, E, f8_pad(K), dtype == MOE355_F32);
   if (p.part_bytes > 0 && (!workspace || workspace_bytes < p.part_bytes))
     return fail(MOE355_EWORKSPACE, "workspace of %zu bytes, the call needs %zu", workspace_bytes,
                 p.part_bytes);
@@ -157,6 +161,7 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
   a.x = static_cast<const uint8_t*>(x); a.x_scales = x_scales; a.offsets = offsets;
   a.w = static_cast<const uint8_t*>(w); a.w_scales = w_scales; a.out = out;
   a.M = M; a.N = N; a.Kp = f8_pad(K); a.E = E; a.out_dtype = dtype; a.zero_rest = 1;
+  a.exact = dtype == MOE355_F32;
   a.parts = static_cast<float*>(workspace); a.max_parts = p.max_parts;
   return check_hip(launch_matmul(p, a, false, as_stream(stream)), "fp8_matmul launch");
 }
@@ -228,7 +233,7 @@ int moe355_fp8_fused_experts(const void* x, const float* x_scales, const void* w
     a.out_codes = at<uint8_t>(workspace, p.inter);
     a.out_scales = at<float>(workspace, p.inter_scales);
     a.M = p.rows; a.N = 2 * I; a.Kp = Hp; a.E = E; a.act = act;
-    a.parts = at<float>(workspace, p.parts); a.max_parts = p.up.max_parts;
+    a.parts = at<float>(workspace, p.parts); a.max_parts = p.up.max_parts; a.exact = p.exact_up;
     if (int rc = check_hip(launch_matmul(p.up, a, true, s), "fp8 gate_up launch")) return rc;
 
     F8MatmulArgs d{};
@@ -236,7 +241,7 @@ int moe355_fp8_fused_experts(const void* x, const float* x_scales, const void* w
     d.w = static_cast<const uint8_t*>(w2); d.w_scales = w2_scales;
     d.out = at<void>(workspace, p.y);
     d.M = p.rows; d.N = H; d.Kp = f8_pad(I); d.E = E; d.out_dtype = MOE355_F32;
-    d.parts = a.parts; d.max_parts = p.down.max_parts;
+    d.parts = a.parts; d.max_parts = p.down.max_parts; d.exact = p.exact_down;
     if (int rc = check_hip(launch_matmul(p.down, d, false, s), "fp8 down launch")) return rc;
 
     CombineArgs c{};

@@ -71,6 +71,7 @@ struct F8MatmulArgs {
   float* out_scales;       // gate_up: [M, blocks of I]
   int M, N, Kp, E;         // gate_up: N = 2 I
   int out_dtype, act;
+  int exact;               // products in bf16 (fp8_mma.h); out_dtype is fp32 then
   int zero_rest;           // rows of no matrix become zeros in out
   float* parts;            // tiled: sums of parts of the last round's items
   int max_parts;           // room there, 0: items are not cut
@@ -81,7 +82,7 @@ hipError_t launch_f8_quantize_weight(const F8QuantArgs& a, int dtype, hipStream_
 // gate_up: out_codes, out_scales = act(gate) * up in 8 bits, of gate rows 0 .. I - 1 and up
 // rows I .. 2 I - 1; else out.
 hipError_t launch_f8_stream(const F8MatmulArgs& a, bool gate_up, hipStream_t s);
-// tile_rows: 64 or 256. Room of one part of an item, in floats.
+// tile_rows: 64, or 256 (exact: 128). Room of one part of an item, in floats.
 size_t f8_part_floats(int tile_rows);
 hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, hipStream_t s);
 

@@ -12,7 +12,7 @@ namespace {
 
 #include "fp8_mma.h"
 
-template <bool kGateUp, int kPairs, int kSplit, typename OutT>
+template <bool kGateUp, int kPairs, int kSplit, bool kExact, typename OutT>
 __global__ __launch_bounds__(kPairs* kSplit* kWave) void stream_kernel(const F8MatmulArgs a) {
   constexpr int kThreads = kPairs * kSplit * kWave;
   constexpr int kUnroll = 4;  // steps whose operands are loaded at once
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(kPairs* kSplit* kWave) void stream_kernel(const F8M
     for (int u = 0; u < kCount; ++u)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const f32x4 p = mma_f8(w[u][j], x[u]);
+        const f32x4 p = kExact ? mma_f8_exact(to_bf16(w[u][j]), to_bf16(x[u])) : mma_f8(w[u][j], x[u]);
         const float s = sx[u] * sw[u][j];
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(p[i], s, acc[j][i]);
@@ -130,14 +130,14 @@ __global__ __launch_bounds__(kPairs* kSplit* kWave) void stream_kernel(const F8M
   }
 }
 
-template <bool kGateUp, int kPairs, int kSplit, typename OutT>
+template <bool kGateUp, int kPairs, int kSplit, bool kExact, typename OutT>
 hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
   const long long groups = kGateUp ? f8_blocks(a.N / 2) : (a.N + 32 * kPairs - 1) / (32 * kPairs);
   // at most: every matrix that has rows has a tile that is not full
   const long long tiles = a.offsets ? a.M / kF8StreamTile + (a.E < a.M ? a.E : a.M)
                                     : (a.M + kF8StreamTile - 1) / kF8StreamTile;
   if (groups * tiles > 0x7fffffffll) return hipErrorInvalidValue;
-  stream_kernel<kGateUp, kPairs, kSplit, OutT>
+  stream_kernel<kGateUp, kPairs, kSplit, kExact, OutT>
       <<<dim3(static_cast<unsigned>(groups * tiles)), dim3(kPairs * kSplit * kWave), 0, s>>>(a);
   return hipGetLastError();
 }
@@ -146,10 +146,11 @@ hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
 
 hipError_t launch_f8_stream(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
   if (a.M == 0) return hipSuccess;
-  if (gate_up) return launch<true, 8, 2, float>(a, s);
-  if (a.out_dtype == MOE355_F32) return launch<false, 1, 4, float>(a, s);
-  if (a.out_dtype == MOE355_BF16) return launch<false, 1, 4, bf16>(a, s);
-  return launch<false, 1, 4, f16>(a, s);
+  if (gate_up) return a.exact ? launch<true, 8, 2, true, float>(a, s) : launch<true, 8, 2, false, float>(a, s);
+  if (a.exact) return launch<false, 1, 4, true, float>(a, s);
+  if (a.out_dtype == MOE355_F32) return launch<false, 1, 4, false, float>(a, s);
+  if (a.out_dtype == MOE355_BF16) return launch<false, 1, 4, false, bf16>(a, s);
+  return launch<false, 1, 4, false, f16>(a, s);
 }
 
 }  // namespace moe355

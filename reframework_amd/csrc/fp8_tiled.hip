@@ -253,11 +253,11 @@ __device__ __forceinline__ void barrier() {
 }
 
 // n products and the scaled sums of their results, product(i) and add(i, its result), each result
-// added behind the third product after it: it is there by then (12 wait states), without
-// waits between the products. Left to itself the compiler waits for every result: 10 % slower.
-template <int n, typename P, typename A>
+// added behind the third product after it (kMostAhead): it is there by then (12 wait states),
+// without waits between the products. Left to itself the compiler waits for every result: 10 % slower.
+template <int n, int kMostAhead, typename P, typename A>
 __device__ __forceinline__ void interleaved(P product, A add) {
-  constexpr int kAhead = n < 3 ? n : 3;
+  constexpr int kAhead = n < kMostAhead ? n : kMostAhead;
   f32x4 v[kAhead + 1];
 #pragma unroll
   for (int i = 0; i < n + kAhead; ++i) {
@@ -458,8 +458,23 @@ __global__ __launch_bounds__(kThreads) void parts_kernel(const F8MatmulArgs a, i
   }
 }
 
+// A row's operand as it lies in LDS, or in bf16.
+struct Codes {
+  u32x4 v[2];
+};
+template <typename Row>
+__device__ __forceinline__ Row row_of(const uint8_t* lo, const uint8_t* hi) {
+  const u32x4 c[2] = {*reinterpret_cast<const u32x4*>(lo), *reinterpret_cast<const u32x4*>(hi)};
+  if constexpr (std::is_same<Row, Codes>::value)
+    return Codes{{c[0], c[1]}};
+  else
+    return to_bf16(c);
+}
+__device__ __forceinline__ f32x4 product(const Codes& w, const Codes& x) { return mma_f8(w.v, x.v); }
+__device__ __forceinline__ f32x4 product(const Bf16Row& w, const Bf16Row& x) { return mma_f8_exact(w, x); }
+
 // All waves read and multiply a step between two barriers.
-template <bool kGateUp, int BM, int WM, typename OutT>
+template <bool kGateUp, int BM, int WM, bool kExact, typename OutT>
 __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a) {
   typedef Shape<BM, WM> S;
   constexpr int kMT = S::kMT, kNT = S::kNT;
@@ -521,26 +536,24 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
         const uint8_t* s = stage[done % S::kStages];
         const uint8_t* wtile = s + S::kTokBytes + (wn * kNT * 16 + r) * kF8Block;
         const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
-        u32x4 x[kM + 1][2];
+        typedef typename std::conditional<kExact, Bf16Row, Codes>::type Row;
+        Row x[kM + 1];
         float sg[kM + 1], su[kM + 1];
 #pragma unroll
         for (int m = 0; m < kM; ++m) {
           const uint8_t* p = s + (16 * (wm + WM * m) + r) * kF8Block;
-          x[m][0] = *reinterpret_cast<const u32x4*>(p + ((q ^ sw) << 4));
-          x[m][1] = *reinterpret_cast<const u32x4*>(p + (((4 + q) ^ sw) << 4));
+          x[m] = row_of<Row>(p + ((q ^ sw) << 4), p + (((4 + q) ^ sw) << 4));
           const float xs = *reinterpret_cast<const float*>(ts + 64 * WM * m);
           sg[m] = xs * s0;
           su[m] = xs * s1;
         }
 #pragma unroll
         for (int g = 0; g < (kM ? kNT : 0); ++g) {
-          u32x4 w[2];
           const uint8_t* p = wtile + g * 16 * kF8Block;
-          w[0] = *reinterpret_cast<const u32x4*>(p + ((q ^ sw) << 4));
-          w[1] = *reinterpret_cast<const u32x4*>(p + (((4 + q) ^ sw) << 4));
+          const Row w = row_of<Row>(p + ((q ^ sw) << 4), p + (((4 + q) ^ sw) << 4));
 #pragma unroll
           for (int m = 0; m < kM; ++m) {
-            const f32x4 v = mma_f8(w, x[m]);
+            const f32x4 v = product(w, x[m]);
             const float f = kGateUp && g >= kNT / 2 ? su[m] : sg[m];
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[m][g][i] = fmaf(v[i], f, acc[m][g][i]);
@@ -657,7 +670,8 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
         };
         auto multiply = [&](int half) {
           if constexpr (kM > 0) {
-            interleaved<kM * kHalf>(
+            // gate_up's second scales leave registers for two results on their way
+            interleaved<kM * kHalf, kGateUp ? 2 : 3>(
                 [&](int i) { return mma_f8(w[i / kM], x[i % kM]); },
                 [&](int i, f32x4 v) {
                   const int m = i % kM;
@@ -713,7 +727,7 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
   if (!second) barrier();
 }
 
-template <bool kGateUp, int BM, int WM, typename OutT>
+template <bool kGateUp, int BM, int WM, bool kExact, typename OutT>
 hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
   const long long nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
   // at most: every matrix that has rows has a tile that is not full
@@ -728,7 +742,7 @@ hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
   if constexpr (BM == 256)
     turns_kernel<kGateUp, OutT><<<groups, dim3(kThreads), 0, s>>>(a);
   else
-    tiled_kernel<kGateUp, BM, WM, OutT><<<groups, dim3(kThreads), 0, s>>>(a);
+    tiled_kernel<kGateUp, BM, WM, kExact, OutT><<<groups, dim3(kThreads), 0, s>>>(a);
   if (a.max_parts > 0 && hipPeekAtLastError() == hipSuccess) {
     // at least two parts an item
     const unsigned tails = static_cast<unsigned>((total < a.max_parts / 2 ? total : a.max_parts / 2) * Shape<BM, WM>::kMT);
@@ -738,22 +752,34 @@ hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
 }
 
 template <int BM, int WM>
-hipError_t launch_bm(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
-  if (gate_up) return launch<true, BM, WM, float>(a, s);
-  if (a.out_dtype == MOE355_F32) return launch<false, BM, WM, float>(a, s);
-  if (a.out_dtype == MOE355_BF16) return launch<false, BM, WM, bf16>(a, s);
-  return launch<false, BM, WM, f16>(a, s);
+hipError_t launch_scaled(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
+  if (gate_up) return launch<true, BM, WM, false, float>(a, s);
+  if (a.out_dtype == MOE355_F32) return launch<false, BM, WM, false, float>(a, s);
+  if (a.out_dtype == MOE355_BF16) return launch<false, BM, WM, false, bf16>(a, s);
+  return launch<false, BM, WM, false, f16>(a, s);
+}
+
+template <int BM, int WM>
+hipError_t launch_exact(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
+  return gate_up ? launch<true, BM, WM, true, float>(a, s) : launch<false, BM, WM, true, float>(a, s);
 }
 
 }  // namespace
 
 size_t f8_part_floats(int tile_rows) {
-  return tile_rows == 256 ? Shape<256, 4>::kPartTile : Shape<64, 2>::kPartTile;
+  static_assert(Shape<256, 4>::kPartTile == 256 * kBN && Shape<64, 2>::kPartTile == 64 * kBN, "a part");
+  return static_cast<size_t>(tile_rows) * kBN;
 }
 
 hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, hipStream_t s) {
   if (a.M == 0) return hipSuccess;
-  return tile_rows == 256 ? launch_bm<256, 4>(a, gate_up, s) : launch_bm<64, 2>(a, gate_up, s);
+  // Exact products leave no registers for a 256-row tile.
+  if (a.exact) {
+    if (tile_rows == 128) return launch_exact<128, 2>(a, gate_up, s);
+    return tile_rows == 64 ? launch_exact<64, 2>(a, gate_up, s) : hipErrorInvalidValue;
+  }
+  if (tile_rows == 256) return launch_scaled<256, 4>(a, gate_up, s);
+  return tile_rows == 64 ? launch_scaled<64, 2>(a, gate_up, s) : hipErrorInvalidValue;
 }
 
 }  // namespace moe355

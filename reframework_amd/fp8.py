@@ -312,8 +312,9 @@ def matmul_fp8(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight,
     only one.
 
     ``x`` is brought to 8 bits first unless it is Fp8Rows. Steps of 128 columns are summed by
-    the matrix cores, which keep about 13 bits below a step's largest product, then scaled
-    and added in fp32. Where ``x`` records gradients, its gradient is the same product of
+    the matrix cores, which for 16-bit results keep about 13 bits below a step's largest
+    product (float32 results have exact products, summed in fp32), then scaled and added in
+    fp32. Where ``x`` records gradients, its gradient is the same product of
     the result's, brought to 8 bits, with the transposed matrices, which ``weight`` has to
     hold; the rounding to 8 bits counts as the identity."""
     if isinstance(x, Fp8Rows):

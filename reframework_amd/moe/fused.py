@@ -321,9 +321,8 @@ def fused_experts_fp8(
 
     Tokens go through gate|up in 8 bits (``hidden_states`` quantised first unless they are
     Fp8Rows) and the gated activation, not rounded in between, through down in 8 bits. The result
-    is of ``out_dtype``: the tokens' type, bfloat16 for Fp8Rows. Steps of 128 columns are
-    summed by the matrix cores (about 13 bits below a step's largest product), all else in
-    fp32, rounded once. Slots whose id lies outside the experts or whose weight is 0 add
+    is of ``out_dtype``: the tokens' type, bfloat16 for Fp8Rows. Sums are those of
+    matmul_fp8, with exact products in gate|up for float16 results too, rounded once. Slots whose id lies outside the experts or whose weight is 0 add
     nothing. No gradients are recorded."""
     act = activation_code(activation)
     if isinstance(hidden_states, Fp8Rows):

@@ -274,8 +274,9 @@ def make_experts(E, H, I, dev, seed):
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 def test_experts(T, H, I, E, K, act, dt, dev):
     """Off by half a step of the type; and an intermediate whose quotient lies as near to a
-    border as the matrix core's sums are exact (2^-14) becomes the other neighbour, 2^-3 away at
-    most: a share of 2^-14 / 2^-4 of them, so 2^-3 * 2^-5 = 2^-8 in the norm."""
+    border as the sums are exact becomes the other neighbour, 2^-3 away at most. In bf16 the
+    matrix core's sums are (2^-14): a share of 2^-14 / 2^-4 of them, so 2^-3 * 2^-5 = 2^-8 in the
+    norm. Sums of exact products in fp32 are to 2^-18: 2^-3 * 2^-7 = 2^-10."""
     banner(f"fp8 experts T={T} H={H} I={I} E={E} K={K} {act} {dt}")
     dt = DT[dt]
     ex = make_experts(E, H, I, dev, seed=T)
@@ -290,11 +291,12 @@ def test_experts(T, H, I, E, K, act, dt, dev):
     want = ref.experts(ref.f64(x), ref.f64(ex.dequantize("w1")), ref.f64(ex.dequantize("w2")),
                        ref.f64(tw), ids.cpu().numpy(), act)
     rel = np.linalg.norm(ref.f64(got) - want) / max(np.linalg.norm(want), 1e-30)
-    assert got.dtype == dt and rel <= REL[dt] + 2.0 ** -8
+    assert got.dtype == dt and rel <= REL[dt] + 2.0 ** (-8 if dt == torch.bfloat16 else -10)
     rows = quantize_fp8(x)
     assert torch.equal(fused_experts_fp8(rows, ex, tw, ids.int(), activation=act, out_dtype=dt), got)
     other = fused_experts_fp8(x, ex, tw, ids, activation=act, out_dtype=torch.float32)
-    assert torch.equal(other.to(dt), got)
+    rel = np.linalg.norm(ref.f64(other) - want) / max(np.linalg.norm(want), 1e-30)
+    assert other.dtype == torch.float32 and rel <= 2.0 ** -10
 
 
 def test_operators_together(dev):
@@ -321,7 +323,7 @@ def test_operators_together(dev):
     out = combine_tokens(y, order, tw) + new_res
     whole_call = fused_experts_fp8(normed, ex, tw, ids) + new_res
     # the same sums, but for tipped codes of the intermediate
-    assert float((out - whole_call).norm() / (whole_call - new_res).norm()) <= 2.0 ** -8
+    assert float(((out - whole_call).norm() / (whole_call - new_res).norm()).detach()) <= 2.0 ** -8
     dout = torch.randn(T, H, generator=g, device=dev)
     got = torch.autograd.grad(out, [x, tw, norm.weight, norm.bias], dout)
 

@@ -2,7 +2,7 @@
 use of its result (CPU: compiles to assembly, runs nothing).
 
 The vector unit may read the result of v_mfma_f32_16x16x128_f8f6f4 12 wait states after it was
-issued (16x16x32 in 16 bits: 8 at most). The compiler fills up with s_nop inside a block of
+issued (16x16x32 in bf16: 8). The compiler fills up with s_nop inside a block of
 instructions; across a branch it was seen to leave too few. So every block has to keep the
 distance by itself: each read of a result by another than a matrix instruction, and the end
 of the block, come late enough after it."""
@@ -17,7 +17,7 @@ import pytest
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "reframework_amd",
                     "csrc")
-WAIT = 12
+WAIT = {"v_mfma_f32_16x16x128_f8f6f4": 12, "v_mfma_f32_16x16x32_bf16": 8}
 
 
 def assembly(source, tmp_path):
@@ -33,38 +33,34 @@ def assembly(source, tmp_path):
 
 def registers(text):
     found = set()
-    for a, b in re.findall(r"\bv\[(\d+):(\d+)\]", text):
-        found.update(range(int(a), int(b) + 1))
-    found.update(int(r) for r in re.findall(r"\bv(\d+)\b", text))
+    for k, a, b in re.findall(r"\b([va])\[(\d+):(\d+)\]", text):
+        found.update((k, r) for r in range(int(a), int(b) + 1))
+    found.update((k, int(r)) for k, r in re.findall(r"\b([va])(\d+)\b", text))
     return found
 
 
 def broken(text):
     """Lines that come too early after a matrix instruction."""
-    bad, pending, mmas = [], {}, 0  # register -> wait states since its instruction
+    bad, pending, mmas = [], {}, 0  # register -> wait states that are still missing
     for line in text.splitlines():
         code = line.split(";")[0].strip()
         if not code or (code.startswith(".") and not code.endswith(":")):
             continue
         if code.endswith(":") or code.startswith(("s_cbranch", "s_branch", "s_endpgm", "s_setpc")):
             # the branch itself is one wait state
-            if any(n < WAIT - 1 for n in pending.values()):
+            if any(n > 1 for n in pending.values()):
                 bad.append(line)
             pending = {}
             continue
         name, _, rest = code.partition(" ")
         mma = name.startswith("v_mfma")
-        if not mma:
-            hit = [r for r in registers(rest) if pending.get(r, WAIT) < WAIT]
-            if hit:
-                bad.append(line)
-        step = 1
-        if name == "s_nop":
-            step = int(rest, 0) + 1
-        pending = {r: n + step for r, n in pending.items() if n + step < WAIT}
+        if not mma and any(r in pending for r in registers(rest)):
+            bad.append(line)
+        step = int(rest, 0) + 1 if name == "s_nop" else 1
+        pending = {r: n - step for r, n in pending.items() if n > step}
         if mma:
             mmas += 1
-            pending.update({r: 0 for r in registers(rest.split(",")[0])})
+            pending.update({r: WAIT[name] for r in registers(rest.split(",")[0])})
     return bad, mmas
 
 
