@@ -74,10 +74,11 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   *p = F8Plan{};
   p->rows = static_cast<int>(R);
   p->n_blocks = R <= kPermuteSingleMax ? 1 : static_cast<int>((R + kPermuteChunk - 1) / kPermuteChunk);
-  p->max_tiles = E + p->rows / (1 << 20);
-  p->exact_up = dtype != MOE355_BF16;
+  p->max_tiles = E + p->rows / kF8StreamTile;
   p->exact_down = dtype == MOE355_F32;
-  p->up = f8_path(p->rows, E, f8_pad(H), p->exact_up);
+  p->up = f8_path(p->rows, E, f8_pad(H), dtype != MOE355_BF16);
+  // where the weights stream, exact products hide behind them (16 tokens: @)
+  p->exact_up = dtype != MOE355_BF16 || p->up.tile_rows == 0;
   p->down = f8_path(p->rows, E, f8_pad(I), p->exact_down);
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -205,13 +206,13 @@ int moe355_fp8_fused_experts(const void* x, const float* x_scales, const void* w
     const float* weights = topk_w + first * K;
 
     F8MatmulArgs a{};
+    F8QuantArgs qa{};
     if (x_scales) {
       a.x = static_cast<const uint8_t*>(x) + first * Hp;
       a.x_scales = x_scales + first * (Hp / kF8Block);
     } else {
-      F8QuantArgs qa{static_cast<const char*>(x) + first * H * esz, at<uint8_t>(workspace, p.xq),
-                     at<float>(workspace, p.xq_scales), n, H};
-      if (int rc = check_hip(launch_f8_quantize(qa, dtype, s), "fp8 quantize launch")) return rc;
+      qa = F8QuantArgs{static_cast<const char*>(x) + first * H * esz, at<uint8_t>(workspace, p.xq),
+                       at<float>(workspace, p.xq_scales), n, H};
       a.x = qa.codes;
       a.x_scales = qa.scales;
     }
@@ -223,10 +224,10 @@ int moe355_fp8_fused_experts(const void* x, const float* x_scales, const void* w
     pa.row_src = at<int32_t>(workspace, p.row_src);
     pa.tile_map = at<int32_t>(workspace, p.tile_map);
     pa.R = p.rows; pa.K = K; pa.E = E; pa.n_blocks = p.n_blocks;
-    pa.tile_rows = 1 << 20; pa.max_tiles = p.max_tiles;
+    pa.tile_rows = kF8StreamTile; pa.max_tiles = p.max_tiles;
     pa.ids_int64 = ids_int64 != 0;
     pa.weights = weights;
-    if (int rc = check_hip(launch_permute(pa, s), "fp8 permute launch")) return rc;
+    if (int rc = check_hip(launch_f8_prepare(pa, qa, dtype, s), "fp8 prepare launch")) return rc;
 
     a.row_src = pa.row_src; a.offsets = pa.offsets;
     a.w = static_cast<const uint8_t*>(w1); a.w_scales = w1_scales;

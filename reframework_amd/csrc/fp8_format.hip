@@ -1,4 +1,6 @@
 // Values to 8 bits with a scale per block of 128 (formats: fp8.h).
+#include <climits>
+
 #include "fp8.h"
 
 namespace moe355 {
@@ -7,10 +9,13 @@ namespace {
 #include "chunk.h"
 
 constexpr int kThreads = 256;
+constexpr int kRows = kF8StreamTile;
+#include "group_slots.h"
+#include "permute_body.h"
+
 constexpr int kWaves = kThreads / kWave;
 constexpr int kPer = 8;                    // values of a lane
 constexpr int kLanes = kF8Block / kPer;    // lanes of a block
-constexpr int kWaveBlocks = kWave / kLanes;
 
 // kPer values from p on, of which n (may be under 1) exist; zeros for the others.
 template <typename T>
@@ -27,31 +32,74 @@ __device__ __forceinline__ void load_values(const T* p, int n, float* v) {
   }
 }
 
-__device__ __forceinline__ float block_max16(float v) {
+// The largest of 16 neighbouring lanes (a row of the wave's lanes, exchanged without the LDS).
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, kWave));
+  for (int o = 8; o > 0; o >>= 1) {
+    const int u = o == 8   ? __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false)
+                  : o == 4 ? __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, false)
+                  : o == 2 ? __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, false)
+                           : __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, false);
+    v = fmaxf(v, __int_as_float(u));
+  }
   return v;
 }
 
-// A wave takes 4 blocks of a row at a time, 16 lanes each. Bound by memory: a row is read once,
-// its codes and scales written once.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void quantize_kernel(const F8QuantArgs a) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const size_t row = static_cast<size_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;
-  if (row >= static_cast<size_t>(a.M)) return;
-  const int blocks = f8_blocks(a.K);
-  const T* x = static_cast<const T*>(a.x) + row * a.K;
-  uint8_t* codes = a.codes + row * blocks * kF8Block;
-  for (int b = blockIdx.y * kWaveBlocks + lane / kLanes; b < blocks; b += gridDim.y * kWaveBlocks) {
-    const int e = b * kF8Block + (lane % kLanes) * kPer;
-    float v[kPer], amax = 0.f;
-    load_values<T>(x + e, a.K - e, v);
+// The largest finite magnitude of a lane's values; infinities cost a branch that is seldom
+// taken.
+__device__ __forceinline__ float finite_max(const float* v) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) amax = fmaxf(amax, fabsf(v[i]));  // ignores NaN
+  if (amax == INFINITY) {
+    amax = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) amax = fmaxf(amax, f8_finite_abs(v[i]));
-    const F8Div d = f8_div(block_max16(amax));
-    *reinterpret_cast<u32x2*>(codes + e) = u32x2{f8_codes4(v, d), f8_codes4(v + 4, d)};
-    if (lane % kLanes == 0) a.scales[row * blocks + b] = d.scale;
+  }
+  return amax;
+}
+
+// Workgroup g of a launch of `threads` quantises that many times 8 values, 16 lanes to a block.
+// Bound by memory: a row is read once, its codes and scales written once.
+template <typename T>
+__device__ __forceinline__ void quantize_group(const F8QuantArgs& a, size_t g, int threads) {
+  const int blocks = f8_blocks(a.K), per = threads / kLanes;
+  const size_t first = g * per, row0 = first / blocks;  // the same for the workgroup
+  const int at = static_cast<int>(first - row0 * blocks) + threadIdx.x / kLanes;
+  const size_t row = row0 + at / blocks;
+  if (row >= static_cast<size_t>(a.M)) return;
+  const int b = at % blocks, lane = threadIdx.x % kLanes, e = b * kF8Block + lane * kPer;
+  float v[kPer];
+  load_values<T>(static_cast<const T*>(a.x) + row * a.K + e, a.K - e, v);
+  const F8Div d = f8_div(lanes_max(finite_max(v)));
+  *reinterpret_cast<u32x2*>(a.codes + row * blocks * kF8Block + e) = u32x2{f8_codes4(v, d), f8_codes4(v + 4, d)};
+  if (lane == 0) a.scales[row * blocks + b] = d.scale;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void quantize_kernel(const F8QuantArgs a) {
+  quantize_group<T>(a, blockIdx.x, kThreads);
+}
+
+// The first launch of an expert call. Its first workgroups group the slots: one wave up to 64
+// slots, one workgroup of a thread per slot up to kPermuteSingleMax, above it the permute's
+// counts; the others quantise x. In two launches a call of 16 tokens takes @ us longer.
+enum class Group { kWave, kOne, kCount };
+
+template <typename T, Group kGroup>
+__global__ __launch_bounds__(kGroup == Group::kOne ? kOneThreads : kThreads) void prepare_kernel(
+    const PermuteArgs p, const F8QuantArgs x) {
+  const int n_group = kGroup == Group::kCount ? p.n_blocks : 1, b = blockIdx.x;
+  if (b >= n_group) {
+    quantize_group<T>(x, b - n_group, kGroup == Group::kOne ? kOneThreads : kThreads);
+  } else if constexpr (kGroup == Group::kCount) {
+    permute_count(p, b);
+  } else if constexpr (kGroup == Group::kOne) {
+    permute_one(p);
+  } else if (threadIdx.x < kWave) {
+    __shared__ int meta[4], rowsrc[kWave], estart[kGroupExpertsPerLane * kWave];
+    __shared__ unsigned long long emask[kGroupExpertsPerLane * kWave];
+    group_slots(p, 0, true, meta, rowsrc, emask, estart);
   }
 }
 
@@ -68,8 +116,7 @@ __global__ __launch_bounds__(kThreads) void quantize_weight_kernel(const F8Quant
     const int row = blockIdx.y * kF8Block + i * kRowsAtOnce + tid / kLanes;
     load_values<T>(static_cast<const T*>(a.x) + static_cast<size_t>(row) * a.K + e,
                    row < a.M ? a.K - e : 0, v[i]);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) amax = fmaxf(amax, f8_finite_abs(v[i][j]));
+    amax = fmaxf(amax, finite_max(v[i]));
   }
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o, kWave));
@@ -88,6 +135,12 @@ __global__ __launch_bounds__(kThreads) void quantize_weight_kernel(const F8Quant
   if (tid == 0) a.scales[static_cast<size_t>(blockIdx.y) * blocks + blockIdx.x] = d.scale;
 }
 
+// Workgroups of `threads` that quantise a.
+size_t groups_of(const F8QuantArgs& a, int threads) {
+  const size_t per = threads / kLanes;
+  return a.x ? (static_cast<size_t>(a.M) * f8_blocks(a.K) + per - 1) / per : 0;
+}
+
 template <typename F>
 hipError_t by_type(int dtype, F f) {
   if (dtype == MOE355_F32) return f(float());
@@ -99,15 +152,28 @@ hipError_t by_type(int dtype, F f) {
 
 hipError_t launch_f8_quantize(const F8QuantArgs& a, int dtype, hipStream_t s) {
   if (a.M == 0) return hipSuccess;
-  // a wave walks along its row, unless the rows are too few to fill the card
-  const int parts = (f8_blocks(a.K) + kWaveBlocks - 1) / kWaveBlocks;
-  const int rows = (a.M + kWaves - 1) / kWaves;
-  const int want = (8 * device_cu_count() + rows - 1) / rows;
-  const dim3 grid(rows, parts < want ? parts : want);
+  const size_t groups = groups_of(a, kThreads);
+  if (groups > INT_MAX) return hipErrorInvalidValue;
   return by_type(dtype, [&](auto t) {
-    quantize_kernel<decltype(t)><<<grid, dim3(kThreads), 0, s>>>(a);
+    quantize_kernel<decltype(t)><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, s>>>(a);
     return hipGetLastError();
   });
+}
+
+hipError_t launch_f8_prepare(const PermuteArgs& p, const F8QuantArgs& x, int dtype, hipStream_t s) {
+  if (groups_of(x, kThreads) + p.n_blocks > INT_MAX) return hipErrorInvalidValue;
+  const hipError_t err = by_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    auto grid = [&](int first, int threads) { return dim3(static_cast<unsigned>(first + groups_of(x, threads))); };
+    if (p.R <= kWave)
+      prepare_kernel<T, Group::kWave><<<grid(1, kThreads), dim3(kThreads), 0, s>>>(p, x);
+    else if (p.n_blocks == 1)
+      prepare_kernel<T, Group::kOne><<<grid(1, kOneThreads), dim3(kOneThreads), 0, s>>>(p, x);
+    else
+      prepare_kernel<T, Group::kCount><<<grid(p.n_blocks, kThreads), dim3(kThreads), 0, s>>>(p, x);
+    return hipGetLastError();
+  });
+  return err != hipSuccess || p.n_blocks == 1 ? err : launch_permute_scatter(p, s);
 }
 
 hipError_t launch_f8_quantize_weight(const F8QuantArgs& a, int dtype, hipStream_t s) {

@@ -13,9 +13,9 @@ namespace {
 #include "fp8_mma.h"
 
 template <bool kGateUp, int kPairs, int kSplit, bool kExact, typename OutT>
-__global__ __launch_bounds__(kPairs* kSplit* kWave) void stream_kernel(const F8MatmulArgs a) {
+__global__ __launch_bounds__(kPairs* kSplit* kWave, 4) void stream_kernel(const F8MatmulArgs a) {
   constexpr int kThreads = kPairs * kSplit * kWave;
-  constexpr int kUnroll = 4;  // steps whose operands are loaded at once
+  constexpr int kUnroll = kGateUp ? 3 : 4;  // steps whose operands are loaded at once
   __shared__ f32x4 part[kSplit > 1 ? kSplit - 1 : 1][kPairs][2][kWave];
   __shared__ float most[kPairs][16];
   const int lane = threadIdx.x & (kWave - 1), q = lane >> 4, r = lane & 15;
@@ -83,8 +83,8 @@ __global__ __launch_bounds__(kPairs* kSplit* kWave) void stream_kernel(const F8M
   int k0 = split, left = (steps - split + kSplit - 1) / kSplit;  // this wave's steps
   for (; left >= kUnroll; left -= kUnroll, k0 += kUnroll * kSplit)
     run(k0, std::integral_constant<int, kUnroll>());
-  static_assert(kUnroll == 4, "what may be left");
-  if (left == 3) run(k0, std::integral_constant<int, 3>());
+  static_assert(kUnroll <= 4, "what may be left");
+  if (kUnroll > 3 && left == 3) run(k0, std::integral_constant<int, 3>());
   if (left == 2) run(k0, std::integral_constant<int, 2>());
   if (left == 1) run(k0, std::integral_constant<int, 1>());
   if constexpr (kSplit > 1) {
@@ -130,27 +130,48 @@ __global__ __launch_bounds__(kPairs* kSplit* kWave) void stream_kernel(const F8M
   }
 }
 
+// Workgroups at most: every matrix that has rows has a tile that is not full.
+long long stream_groups(const F8MatmulArgs& a, bool gate_up) {
+  const long long groups = gate_up ? f8_blocks(a.N / 2) : (a.N + 31) / 32;
+  return groups * (a.offsets ? a.M / kF8StreamTile + (a.E < a.M ? a.E : a.M)
+                             : (a.M + kF8StreamTile - 1) / kF8StreamTile);
+}
+
 template <bool kGateUp, int kPairs, int kSplit, bool kExact, typename OutT>
 hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
-  const long long groups = kGateUp ? f8_blocks(a.N / 2) : (a.N + 32 * kPairs - 1) / (32 * kPairs);
-  // at most: every matrix that has rows has a tile that is not full
-  const long long tiles = a.offsets ? a.M / kF8StreamTile + (a.E < a.M ? a.E : a.M)
-                                    : (a.M + kF8StreamTile - 1) / kF8StreamTile;
-  if (groups * tiles > 0x7fffffffll) return hipErrorInvalidValue;
+  const long long groups = stream_groups(a, kGateUp);
+  if (groups > 0x7fffffffll) return hipErrorInvalidValue;
   stream_kernel<kGateUp, kPairs, kSplit, kExact, OutT>
-      <<<dim3(static_cast<unsigned>(groups * tiles)), dim3(kPairs * kSplit * kWave), 0, s>>>(a);
+      <<<dim3(static_cast<unsigned>(groups)), dim3(kPairs * kSplit * kWave), 0, s>>>(a);
   return hipGetLastError();
+}
+
+// More waves share a tile's columns where there are few tiles. us with 4 / 8 waves: 256 workgroups
+// (2 rows of 2 matrices, 4096 x 14336) 26.6 / 23.6, 128 (1 row, 4096 x 4096) 8.0 / 7.3, 896
+// (2 rows of 2, 14336 x 4096) 23.1 / 25.3, 5632 (96 rows of 64, 2816 x 2048) 62 / 73.
+template <bool kExact, typename OutT>
+hipError_t launch_product(const F8MatmulArgs& a, hipStream_t s) {
+  return stream_groups(a, false) <= 2ll * device_cu_count() ? launch<false, 1, 8, kExact, OutT>(a, s)
+                                                            : launch<false, 1, 4, kExact, OutT>(a, s);
+}
+
+// Likewise. Whole calls, us with 1 / 2 waves: 224 workgroups (1 token, 8 experts of H 4096, I 14336)
+// @ / @, 561 (16 tokens, 64 of H 2048, I 1408) @ / @.
+template <bool kExact>
+hipError_t launch_gate_up(const F8MatmulArgs& a, hipStream_t s) {
+  return stream_groups(a, true) <= device_cu_count() ? launch<true, 8, 2, kExact, float>(a, s)
+                                                     : launch<true, 8, 1, kExact, float>(a, s);
 }
 
 }  // namespace
 
 hipError_t launch_f8_stream(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
   if (a.M == 0) return hipSuccess;
-  if (gate_up) return a.exact ? launch<true, 8, 2, true, float>(a, s) : launch<true, 8, 2, false, float>(a, s);
-  if (a.exact) return launch<false, 1, 4, true, float>(a, s);
-  if (a.out_dtype == MOE355_F32) return launch<false, 1, 4, false, float>(a, s);
-  if (a.out_dtype == MOE355_BF16) return launch<false, 1, 4, false, bf16>(a, s);
-  return launch<false, 1, 4, false, f16>(a, s);
+  if (gate_up) return a.exact ? launch_gate_up<true>(a, s) : hipErrorInvalidValue;
+  if (a.exact) return launch_product<true, float>(a, s);
+  if (a.out_dtype == MOE355_F32) return launch_product<false, float>(a, s);
+  if (a.out_dtype == MOE355_BF16) return launch_product<false, bf16>(a, s);
+  return launch_product<false, f16>(a, s);
 }
 
 }  // namespace moe355
