@@ -495,16 +495,19 @@ int moe355_combine_rows_bwd(const void* dout, const void* rows, const float* top
 /*
  * Values in 8 bits with an fp32 scale per block of 128: rows are e4m3 codes [M, Kp] (Kp = K
  * rounded up to 128, codes 0 from K on) with scales [M, ceil(K/128)], a scale per 128 consecutive
- * values; weights are codes [N, Kp] with scales [ceil(N/128), ceil(K/128)], one per 128 x
- * 128 block. With m a block's largest finite magnitude, at least 448 * 2^-126, the scale is
- * m / 448 and a code v * 448 / m rounded to nearest even; infinities and NaN become NaN. The
- * reference has no such format (its quantised experts are int8 on the host,
- * reframework/moe/fused.py:140-197).
+ * values; weights [N, K] are cells of 128 x 128 codes, [ceil(N/128), ceil(K/128), 16384] bytes
+ * with codes 0 past N and K, and scales [ceil(N/128), ceil(K/128)], one per cell. Within a cell
+ * row n and column k lie at byte n/16 * 2048 + k%128/64 * 1024 + (k/16%4 * 16 + n%16) * 16 + k%16.
+ * With m a block's largest finite magnitude, at least 448 * 2^-126, the scale is m / 448 and
+ * a code v * 448 / m rounded to nearest even; infinities and NaN become NaN. The reference has
+ * no such format (its quantised experts are int8 on the host, reframework/moe/fused.py:140-197).
+ * fp8_pack lays codes [N, K] out as cells.
  */
 int moe355_fp8_quantize(const void* x, int M, int K, int dtype, void* codes, float* scales,
                         void* stream);
-int moe355_fp8_quantize_weight(const void* w, int N, int K, int dtype, void* codes, float* scales,
+int moe355_fp8_quantize_weight(const void* w, int N, int K, int dtype, void* cells, float* scales,
                                void* stream);
+int moe355_fp8_pack(const void* codes, int N, int K, void* cells, void* stream);
 
 /*
  * out [M,N] = rows [offsets[e], offsets[e+1]) of x [M,K] times matrix e of w [E,N,K],
@@ -513,7 +516,7 @@ int moe355_fp8_quantize_weight(const void* w, int N, int K, int dtype, void* cod
  * 128 columns is summed by the matrix core, which for 16-bit results keeps about 13 bits below
  * its largest product (fp32 results have exact products, summed in fp32); the steps are scaled
  * and added in fp32, and rounded once to dtype. Any N and K up to
- * 2^20 with N * Kp < 2^31. The workspace (0 bytes: none) belongs to the call until its kernels
+ * 2^20 whose cells are under 2 GB. The workspace (0 bytes: none) belongs to the call until its kernels
  * end.
  */
 int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, int dtype, size_t* bytes);
@@ -526,9 +529,9 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
  * reframework/moe/fused.py:49-87): x in 8 bits (quantised here when x_scales is NULL: x is
  * then [T,H] of dtype; else codes [T,Hp]), g, u = x . w1[e]^T, h = act(g) * u in 8 bits with
  * a scale per 128 features, y = h . w2[e]^T, out[t] = sum_k topk_w[t,k] * y, sums as in
- * moe355_fp8_matmul, of g and u with exact products for f16 too, rounded once. w1: codes [E,2I,Hp], gate rows first, scales [E, 2 ceil(I/128), ceil(H/128)],
- * gate blocks first (the up half's blocks start at its first row); w2: codes [E,H,Ip], scales
- * [E, ceil(H/128), ceil(I/128)]. H and I multiples of 16. Slots whose id lies outside [0,E) or
+ * moe355_fp8_matmul, of g and u with exact products for f16 too, rounded once. w1: cells
+ * [E, 2 ceil(I/128), ceil(H/128), 16384], gate's rows of cells first, then up's (which start
+ * at its first row), and their scales; w2: cells [E, ceil(H/128), ceil(I/128), 16384]. H and I multiples of 16. Slots whose id lies outside [0,E) or
  * whose weight is 0 add nothing. out may be x. The workspace belongs to the call until its
  * kernels end.
  */

@@ -125,6 +125,7 @@ _SIGNATURES: Dict[str, Tuple[object, List[object]]] = {
     "moe355_combine_rows_bwd": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P]),
     "moe355_fp8_quantize": (_I, [_P, _I, _I, _I, _P, _P, _P]),
     "moe355_fp8_quantize_weight": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "moe355_fp8_pack": (_I, [_P, _I, _I, _P, _P]),
     "moe355_fp8_matmul_workspace_bytes": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
     "moe355_fp8_matmul": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _Z, _P]),
     "moe355_fp8_workspace_bytes": (_I, [_I, _I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
@@ -667,6 +668,13 @@ def fp8_quantize(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
           stream if stream is not None else stream_handle(device))
 
 
+def fp8_pack(codes: torch.Tensor, cells: torch.Tensor, stream: Optional[int] = None) -> None:
+    N, K = codes.shape
+    device = codes.device
+    _call(device, "moe355_fp8_pack", codes.data_ptr(), _rows(N), K, cells.data_ptr(),
+          stream if stream is not None else stream_handle(device))
+
+
 def fp8_quantize_weight(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                         stream: Optional[int] = None) -> None:
     N, K = w.shape
@@ -677,11 +685,10 @@ def fp8_quantize_weight(w: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
 
 
 def fp8_matmul(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
-               offsets: Optional[torch.Tensor], K: int, out: torch.Tensor,
+               offsets: Optional[torch.Tensor], E: int, K: int, out: torch.Tensor,
                stream: Optional[int] = None) -> None:
     device = x.device
     M, N = out.shape
-    E = w.shape[0]
     code = dtype_code(out.dtype)
     nbytes = _size(device, "moe355_fp8_matmul_workspace_bytes", _rows(M), N, K, E, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None

@@ -24,13 +24,21 @@ int check_weights(int N, int K, int E) {
   if (E < 1 || E > MOE355_MAX_EXPERTS)
     return fail(MOE355_EUNSUPPORTED, "E=%d outside [1, %d]", E, MOE355_MAX_EXPERTS);
   // the kernels address a matrix by 31-bit offsets
-  if (static_cast<long long>(N) * f8_pad(K) > INT_MAX)
+  if (static_cast<long long>(f8_pad(N)) * f8_pad(K) > INT_MAX)
     return fail(MOE355_EUNSUPPORTED, "a matrix of %d x %d is over 2 GB", N, K);
   return MOE355_OK;
 }
 
 // Which kernels run a product of M rows of E matrices over Kp columns: tile_rows 0 streams
 // the weights; max_parts: parts of items that the tiled kernels may leave in memory.
+// Up to kF8StreamRows rows per matrix the weights stream past 16-row tiles (fp8_stream.hip);
+// random routing leaves some matrices with more than a tile, which reads their weights again.
+// Whole expert calls, us streaming / on 64-row tiles: 8 experts of H 4096, I 14336 at 1 row 82 /
+// 148, 2 rows 289 / 299, 5 rows 312 / 328, 8 rows 325 / 324, 12 rows 350 / 328; 64 of H 2048,
+// I 1408 at 1 row 110 / 105, 6 rows 131 / 114, 12 rows 161 / 126; 32 of H 1280, I 3328 at 1 row 54 /
+// 60, 4 rows 106 / 101, 8 rows 112 / 102. One row of one 4096 x 4096 matrix 7.4 / 22.8.
+constexpr int kF8StreamRows = 5;
+
 struct F8Path {
   int tile_rows, max_parts;
   size_t part_bytes;
@@ -39,7 +47,7 @@ struct F8Path {
 F8Path f8_path(int M, int E, int Kp, bool exact) {
   F8Path p{};
   const int rows = M / std::max(1, std::min(M, E));  // per matrix that has any, on average
-  if (rows <= 16) return p;
+  if (rows <= kF8StreamRows) return p;
   p.tile_rows = rows < 100 ? 64 : exact ? 128 : 256;
   // cutting items of few steps saves less than the second launch takes
   if (Kp / kF8Block >= (p.tile_rows > 64 ? 16 : 24)) p.max_parts = device_cu_count();
@@ -65,7 +73,7 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   if (H <= 0 || I <= 0) return fail(MOE355_EINVAL, "bad sizes H=%d I=%d", H, I);
   if (H % 16 || I % 16) return fail(MOE355_EUNSUPPORTED, "H=%d and I=%d must be multiples of 16", H, I);
   if (H > (1 << 20) || I > (1 << 19)) return fail(MOE355_EUNSUPPORTED, "H=%d or I=%d over 2^20 / 2^19", H, I);
-  if (int rc = check_weights(2 * I, H, E)) return rc;
+  if (int rc = check_weights(2 * f8_pad(I), H, E)) return rc;
   if (int rc = check_weights(H, I, E)) return rc;
   if (K < 1 || K > E) return fail(MOE355_EINVAL, "top-k K=%d outside [1, E=%d]", K, E);
   if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
@@ -77,8 +85,11 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->max_tiles = E + p->rows / kF8StreamTile;
   p->exact_down = dtype == MOE355_F32;
   p->up = f8_path(p->rows, E, f8_pad(H), dtype != MOE355_BF16);
-  // where the weights stream, exact products hide behind them (16 tokens: @)
-  p->exact_up = dtype != MOE355_BF16 || p->up.tile_rows == 0;
+  // Up to 64-row tiles the weights' stream hides most of what exact products take (us, scaled /
+  // exact: 197 tokens of 2 of 16, H 4096, I 6400 301 / 306; 128 of 6 of 64, H 2048, I 1408 126 /
+  // 133; above, 4096 of 2 of 8, H 4096, I 14336 1620 / @). A bf16 result of few tokens is
+  // off by up to 0.0025 of its size with the scaled ones, by 0.0017 with these.
+  p->exact_up = dtype != MOE355_BF16 || p->up.tile_rows <= 64;
   p->down = f8_path(p->rows, E, f8_pad(I), p->exact_down);
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -121,16 +132,24 @@ int moe355_fp8_quantize(const void* x, int M, int K, int dtype, void* codes, flo
   return check_hip(launch_f8_quantize(a, dtype, as_stream(stream)), "fp8_quantize launch");
 }
 
-int moe355_fp8_quantize_weight(const void* w, int N, int K, int dtype, void* codes, float* scales,
+int moe355_fp8_quantize_weight(const void* w, int N, int K, int dtype, void* cells, float* scales,
                                void* stream) {
   if (int rc = check_weights(N, K, 1)) return rc;
   if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
   if (f8_blocks(N) > 65535) return fail(MOE355_EUNSUPPORTED, "N=%d too large", N);
-  if (!w || !codes || !scales) return fail(MOE355_EINVAL, "NULL tensor argument");
-  if (reinterpret_cast<uintptr_t>(w) % elem_size(dtype) || !aligned16(codes) || !aligned4(scales))
-    return fail(MOE355_EINVAL, "w/codes/scales not aligned");
-  F8QuantArgs a{w, static_cast<uint8_t*>(codes), scales, N, K};
+  if (!w || !cells || !scales) return fail(MOE355_EINVAL, "NULL tensor argument");
+  if (reinterpret_cast<uintptr_t>(w) % elem_size(dtype) || !aligned16(cells) || !aligned4(scales))
+    return fail(MOE355_EINVAL, "w/cells/scales not aligned");
+  F8QuantArgs a{w, static_cast<uint8_t*>(cells), scales, N, K};
   return check_hip(launch_f8_quantize_weight(a, dtype, as_stream(stream)), "fp8_quantize_weight launch");
+}
+
+int moe355_fp8_pack(const void* codes, int N, int K, void* cells, void* stream) {
+  if (int rc = check_weights(N, K, 1)) return rc;
+  if (!codes || !cells) return fail(MOE355_EINVAL, "NULL tensor argument");
+  if (!aligned16(cells)) return fail(MOE355_EINVAL, "cells not 16-byte aligned");
+  F8PackArgs a{static_cast<const uint8_t*>(codes), static_cast<uint8_t*>(cells), N, K};
+  return check_hip(launch_f8_pack(a, as_stream(stream)), "fp8_pack launch");
 }
 
 int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, int dtype, size_t* bytes) {

@@ -5,8 +5,13 @@
 // from the rounded scale: 16-bit values over 16-bit maxima are often ties, and
 // those would fall to the side the scale was rounded to. Infinities and NaN become NaN.
 //
-// Rows, of tokens and of weights, are padded to whole 128-value steps with codes of 0, so that
-// the matrix kernels never see a partial step.
+// Rows of tokens are padded to whole 128-value steps with codes of 0, so that the matrix kernels
+// never see a partial step. Matrices are laid out once, as cells of 128 x 128 codes (16 KB, one
+// scale) in rows of cells, padded with codes of 0. A cell holds 8 tiles of 16 rows (2 KB), each as
+// the matrix instruction takes it: lane 16 q + r has row r, columns 16 q .. + 15 in the
+// first KB and 64 + 16 q .. + 15 in the second. So every load of a wave is 1 KB in a row, and a
+// workgroup's step 16 or 32. Row by row, a step's 256 rows are as many pieces of 128 bytes: loaded
+// to LDS by one workgroup a CU that way 3.8 TB/s, as cells 4.9, by two 4.2 and 6.1.
 #pragma once
 
 #include "common.h"
@@ -55,12 +60,33 @@ __device__ __forceinline__ uint32_t f8_codes4(const float* v, const F8Div& d) {
   return static_cast<uint32_t>(c);
 }
 
+constexpr int kF8Cell = kF8Block * kF8Block;  // bytes
+constexpr int kF8Tile = 16 * kF8Block;
+
+// Place in its matrix of the 16 codes of row n from column k on (a multiple of 16).
+__host__ __device__ __forceinline__ size_t f8_place(int n, int k, int k_blocks) {
+  const size_t cell = static_cast<size_t>(n / kF8Block) * k_blocks + k / kF8Block;
+  const int q = k / 16 % 4, half = k / 64 % 2;
+  return cell * kF8Cell + n % kF8Block / 16 * kF8Tile + half * (kF8Tile / 2) + (16 * q + n % 16) * 16;
+}
+
 struct F8QuantArgs {
   const void* x;    // [M, K]
-  uint8_t* codes;   // [M, Kp]
+  uint8_t* codes;   // rows: [M, Kp]; weights: cells
   float* scales;    // rows: [M, blocks]; weights: [row blocks, blocks]
   int M, K;
 };
+
+struct F8PackArgs {
+  const uint8_t* src;  // codes [N, K]
+  uint8_t* cells;
+  int N, K;
+};
+
+// Rows of cells of a matrix of n rows; gate_up: of gate's and up's together.
+__host__ __device__ constexpr int f8_cell_rows(int n, bool gate_up) {
+  return gate_up ? 2 * f8_blocks(n / 2) : f8_blocks(n);
+}
 
 // One product, grouped: rows [offsets[e], offsets[e + 1]) of x times matrix e, transposed.
 struct F8MatmulArgs {
@@ -68,7 +94,7 @@ struct F8MatmulArgs {
   const float* x_scales;   // [*, blocks of K]
   const int32_t* row_src;  // x row of each row, or nullptr: the row itself
   const int32_t* offsets;  // [E + 1], or nullptr: one matrix, all rows
-  const uint8_t* w;        // [E, N, Kp]
+  const uint8_t* w;        // [E] matrices of cells (gate_up: gate's, then up's)
   const float* w_scales;   // [E, blocks of N, blocks of K]; gate_up: of I twice
   void* out;               // [M, N] (out_dtype)
   uint8_t* out_codes;      // gate_up: [M, Ip]
@@ -86,6 +112,7 @@ hipError_t launch_f8_quantize(const F8QuantArgs& a, int dtype, hipStream_t s);
 // (x.x NULL: it is in 8 bits already).
 hipError_t launch_f8_prepare(const PermuteArgs& p, const F8QuantArgs& x, int dtype, hipStream_t s);
 hipError_t launch_f8_quantize_weight(const F8QuantArgs& a, int dtype, hipStream_t s);
+hipError_t launch_f8_pack(const F8PackArgs& a, hipStream_t s);
 // gate_up: out_codes, out_scales = act(gate) * up in 8 bits, of gate rows 0 .. I - 1 and up
 // rows I .. 2 I - 1; else out.
 hipError_t launch_f8_stream(const F8MatmulArgs& a, bool gate_up, hipStream_t s);

@@ -125,14 +125,32 @@ __global__ __launch_bounds__(kThreads) void quantize_weight_kernel(const F8Quant
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) amax = fmaxf(amax, most[w]);
   const F8Div d = f8_div(amax);
+  uint8_t* cell = a.codes + (static_cast<size_t>(blockIdx.y) * blocks + blockIdx.x) * kF8Cell;
+  const int col = tid % kLanes * kPer;
 #pragma unroll
-  for (int i = 0; i < kRounds; ++i) {
-    const int row = blockIdx.y * kF8Block + i * kRowsAtOnce + tid / kLanes;
-    if (row < a.M)
-      *reinterpret_cast<u32x2*>(a.codes + static_cast<size_t>(row) * blocks * kF8Block + e) =
-          u32x2{f8_codes4(v[i], d), f8_codes4(v[i] + 4, d)};
-  }
+  for (int i = 0; i < kRounds; ++i)
+    *reinterpret_cast<u32x2*>(cell + f8_place(i * kRowsAtOnce + tid / kLanes, col & ~15, 1) + (col & 8)) =
+        u32x2{f8_codes4(v[i], d), f8_codes4(v[i] + 4, d)};
   if (tid == 0) a.scales[static_cast<size_t>(blockIdx.y) * blocks + blockIdx.x] = d.scale;
+}
+
+// A checkpoint's codes as cells: a thread per 16 codes of the result. Runs once per matrix.
+__global__ __launch_bounds__(kThreads) void pack_kernel(const F8PackArgs a) {
+  const int blocks = f8_blocks(a.K), rows = f8_pad(a.N), per_row = blocks * (kF8Block / 16);
+  const size_t i = static_cast<size_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (i >= static_cast<size_t>(rows) * per_row) return;
+  const int n = static_cast<int>(i / per_row), k = static_cast<int>(i % per_row) * 16;
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (n < a.N && k < a.K) {
+    const uint8_t* p = a.src + static_cast<size_t>(n) * a.K + k;
+    typedef u32x4 u32x4_byte __attribute__((aligned(1)));
+    if (k + 16 <= a.K) {
+      v = *reinterpret_cast<const u32x4_byte*>(p);
+    } else {
+      for (int j = 0; j < a.K - k; ++j) v[j / 4] |= static_cast<uint32_t>(p[j]) << (8 * (j % 4));
+    }
+  }
+  *reinterpret_cast<u32x4*>(a.cells + f8_place(n, k, blocks)) = v;
 }
 
 // Workgroups of `threads` that quantise a.
@@ -182,6 +200,14 @@ hipError_t launch_f8_quantize_weight(const F8QuantArgs& a, int dtype, hipStream_
     quantize_weight_kernel<decltype(t)><<<grid, dim3(kThreads), 0, s>>>(a);
     return hipGetLastError();
   });
+}
+
+hipError_t launch_f8_pack(const F8PackArgs& a, hipStream_t s) {
+  const size_t threads = static_cast<size_t>(f8_pad(a.N)) * f8_blocks(a.K) * (kF8Block / 16);
+  const size_t groups = (threads + kThreads - 1) / kThreads;
+  if (groups > INT_MAX) return hipErrorInvalidValue;
+  pack_kernel<<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, s>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace moe355

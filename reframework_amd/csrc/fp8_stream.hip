@@ -32,18 +32,18 @@ __global__ __launch_bounds__(kPairs* kSplit* kWave, 4) void stream_kernel(const 
   const int steps = a.Kp / kF8Block;
   // this wave's two tiles: their first rows and, of the scales, their blocks of rows
   const int first = (group * kPairs + pair) * (kGateUp ? 16 : 32);
-  const int n_blocks = kGateUp ? 2 * f8_blocks(I) : f8_blocks(a.N);
+  const int cell_rows = f8_cell_rows(a.N, kGateUp);
   const uint8_t* wp[2];
   const float* ws[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
+    // Rows past the matrix's last: cells are padded; tiles past the last cell read it again. Those
+    // results are not stored.
     const int n = first + (kGateUp ? 0 : 16 * j);
-    const int most_n = (kGateUp ? I : a.N) - 1;
-    // rows past the last read it again; those results are not stored
-    const size_t row = static_cast<size_t>(t.e) * a.N + (kGateUp && j ? I : 0) + min(n + r, most_n);
-    wp[j] = a.w + row * a.Kp + q * 16;
-    const int block = min(n, most_n) / kF8Block + (kGateUp && j ? f8_blocks(I) : 0);
-    ws[j] = a.w_scales + (static_cast<size_t>(t.e) * n_blocks + block) * steps;
+    const int block = min(n / kF8Block + (kGateUp && j ? cell_rows / 2 : 0), cell_rows - 1);
+    const size_t cells = (static_cast<size_t>(t.e) * cell_rows + block) * steps;
+    wp[j] = a.w + cells * kF8Cell + n % kF8Block / 16 * kF8Tile + lane * 16;
+    ws[j] = a.w_scales + cells;
   }
   const int row = min(t.row0 + r, t.row_end - 1);  // tokens past the last: it again
   const size_t src = a.row_src ? a.row_src[row] : row;
@@ -62,8 +62,8 @@ __global__ __launch_bounds__(kPairs* kSplit* kWave, 4) void stream_kernel(const 
       const size_t at = static_cast<size_t>(k) * kF8Block;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        w[u][j][0] = *reinterpret_cast<const u32x4*>(wp[j] + at);
-        w[u][j][1] = *reinterpret_cast<const u32x4*>(wp[j] + at + 64);
+        w[u][j][0] = *reinterpret_cast<const u32x4*>(wp[j] + at * kF8Block);
+        w[u][j][1] = *reinterpret_cast<const u32x4*>(wp[j] + at * kF8Block + kF8Tile / 2);
         sw[u][j] = ws[j][k];
       }
       x[u][0] = *reinterpret_cast<const u32x4*>(xp + at);

@@ -2,9 +2,9 @@
 // an item multiplies BM token rows by 256 weight rows (gate_up: gate and up of 128
 // features, a block of the result's scales), a step of 128 columns at a time.
 //
-// Rows of both operands go straight to LDS, 128 bytes a row and step, with their 16-byte chunks
-// XORed by half the row number, which leaves the fragment reads without bank
-// conflicts. A step is one block of both operands' scales, so the matrix core sums it from
+// Both operands go straight to LDS: weight tiles as they are laid out, token rows by 128 bytes a
+// step, with their 16-byte chunks XORed by half the row number, which leaves the fragment
+// reads without bank conflicts. A step is one block of both operands' scales, so the matrix core sums it from
 // zero and the sum is scaled and added in fp32 by the vector unit, whose instructions run beside
 // the next products. Token scales go to LDS with the rows; the weights' one (gate_up: two) of a
 // wave and step is a scalar load.
@@ -36,13 +36,14 @@ struct Shape {
   static constexpr int kMT = BM / WM / 16, kNT = kBN / kWN / 16;  // 16 x 16 tiles of a wave
   static constexpr int kTokBytes = BM * kF8Block;
   static constexpr int kWgtBytes = kBN * kF8Block;
-  static constexpr int kStage = kTokBytes + kWgtBytes + BM * 4;
+  static constexpr int kStage = kTokBytes + kWgtBytes + (BM < 64 ? 64 : BM) * 4;
   static constexpr int kPartTile = kMT * kNT * kThreads * 4;  // floats of a part's sums
   static constexpr int kSpare = kMaxItems * 32 + (kMaxExperts + 1) * 8 + kWN * BM * 4 + 64;
   static constexpr int kStages = (160 * 1024 - kSpare) / kStage;
   // direct-to-LDS loads of a wave per step: 1 KB of codes each, and 256 bytes of scales
   // (some waves' a second time)
-  static constexpr int kTokLoads = kTokBytes / 1024 / kWaves;
+  static constexpr int kTokPieces = BM / 8;  // of 8 rows, 1 KB
+  static constexpr int kTokLoads = (kTokPieces + kWaves - 1) / kWaves;
   static constexpr int kWgtLoads = kWgtBytes / 1024 / kWaves;
   static constexpr int kLoads = kTokLoads + kWgtLoads + 1;
   static_assert(kMT >= 1 && kNT >= 2 && kTokLoads >= 1, "tiles of a wave");
@@ -157,7 +158,7 @@ struct Loader {
   const int n_items, steps, wave;
   // The item whose steps are being loaded: sources, and this lane's offsets.
   __amdgpu_buffer_rsrc_t xsrc, xssrc, wsrc;
-  uint32_t xoff[S::kTokLoads], woff[S::kWgtLoads], soff;
+  uint32_t xoff[S::kTokLoads], cell[2], soff;
   // Token rows of the next item whose codes and scales this lane loads, as rows of x; -1 past
   // the tile's last row.
   int src[S::kTokLoads + 1];
@@ -169,14 +170,17 @@ struct Loader {
     begin(uniform(items));
   }
   // 64 tokens whose scales this wave loads
-  __device__ __forceinline__ int tok64() const { return wave % (BM / 64); }
+  __device__ __forceinline__ int tok64() const { return BM <= 64 ? 0 : wave % (BM / 64); }
+  // Piece of the tokens that load i brings (some waves' a second time where there are few).
+  __device__ __forceinline__ int piece(int i) const { return (wave * S::kTokLoads + i) % S::kTokPieces; }
   // The lane, opaque: what follows from it is computed where an item begins, not kept.
   static __device__ __forceinline__ int lane_id() { return pipe::opaque(threadIdx.x & (kWave - 1)); }
+  static __device__ __forceinline__ uint32_t lane16() { return (threadIdx.x & (kWave - 1)) * 16; }
   __device__ __forceinline__ void load_rows(const Item& it) {
     const int lane = lane_id();
 #pragma unroll
     for (int i = 0; i <= S::kTokLoads; ++i) {
-      const int row = i < S::kTokLoads ? 8 * (wave * S::kTokLoads + i) + (lane >> 3) : 64 * tok64() + lane;
+      const int row = i < S::kTokLoads ? 8 * piece(i) + (lane >> 3) : 64 * tok64() + lane;
       const int p = it.row0 + row;
       src[i] = p >= it.row_end ? -1 : a.row_src ? a.row_src[p] : row;
     }
@@ -189,53 +193,55 @@ struct Loader {
     const size_t first = a.row_src ? 0 : it.row0;
     xsrc = pipe::lds_rsrc(a.x + first * a.Kp);
     xssrc = pipe::lds_rsrc(a.x_scales + first * steps);
-    wsrc = pipe::lds_rsrc(a.w + static_cast<size_t>(it.e) * a.N * a.Kp);
+    wsrc = pipe::lds_rsrc(a.w + static_cast<size_t>(it.e) * f8_cell_rows(a.N, kGateUp) * steps * kF8Cell);
 #pragma unroll
     for (int i = 0; i < S::kTokLoads; ++i) {
-      const int row = 8 * (wave * S::kTokLoads + i) + (lane >> 3);
+      const int row = 8 * piece(i) + (lane >> 3);
       xoff[i] = src[i] < 0 ? pipe::kPadOffset  // out of range: zeros
                            : static_cast<uint32_t>(src[i]) * a.Kp + chunk(lane, row);
     }
+    // Cells past the last of a matrix are out of range: zeros.
+    const int cell_rows = f8_cell_rows(a.N, kGateUp);
 #pragma unroll
-    for (int i = 0; i < S::kWgtLoads; ++i) {
-      const int row = weight_row(i) + (lane >> 3);
-      const int wn = row / (16 * S::kNT), g = row / 16 % S::kNT;
-      int n = it.wt * kBN + row, end = a.N;
-      if constexpr (kGateUp) {  // gate and up of the same features, half of a wave's tiles each
-        end = a.N / 2;
-        n = it.wt * kF8Block + wn * 8 * S::kNT + g % (S::kNT / 2) * 16 + row % 16;
-      }
-      const int up = kGateUp && g >= S::kNT / 2 ? a.N / 2 : 0;
-      woff[i] = n < end ? static_cast<uint32_t>(n + up) * a.Kp + chunk(lane, row) : pipe::kPadOffset;
+    for (int i = 0; i < 2; ++i) {
+      const int block = kGateUp ? it.wt + i * (cell_rows / 2) : it.wt * 2 + i;
+      cell[i] = block < cell_rows ? static_cast<uint32_t>(block) * steps * kF8Cell : pipe::kPadOffset;
     }
     soff = src[S::kTokLoads] < 0 ? pipe::kPadOffset : static_cast<uint32_t>(src[S::kTokLoads]) * steps * 4;
     step = it.k0;
     end = it.k1;
     if (item + 1 < n_items) load_rows(uniform(items + item + 1));
   }
-  // First of the 8 rows of the weight tile (as it lies in LDS) that load i brings: the loads of
-  // the first half bring the first half of every wave's tiles.
-  __device__ __forceinline__ int weight_row(int i) const {
-    constexpr int kHalf = S::kWgtLoads / 2;
-    const int piece = wave * kHalf + i % kHalf + i / kHalf * (kHalf * kWaves);  // of 8 rows
-    const int half = piece / (kHalf * kWaves), p = piece % (kHalf * kWaves);
-    const int per = S::kNT;  // pieces of 8 rows in half of a wave's tiles
-    return (p / per) * 16 * S::kNT + half * 8 * S::kNT + p % per * 8;
+  // The 2 KB tile of its cell that loads i, i ^ 1 bring, and its place in LDS, where a wave's
+  // tiles follow each other: loads of the first half bring the first half of every wave's
+  // (gate_up: gate's; up's are the second).
+  struct Piece {
+    int cell, tile, at;
+  };
+  __device__ __forceinline__ Piece piece_of(int i) const {
+    constexpr int kHalf = S::kWgtLoads / 4;  // tiles of this wave and half
+    const int half = i / (2 * kHalf), n = wave * kHalf + i / 2 % kHalf;  // of 8
+    const int wn = n / (S::kNT / 2), g = n % (S::kNT / 2);
+    const int at = wn * S::kNT + half * (S::kNT / 2) + g;
+    return kGateUp ? Piece{half, n, at} : Piece{at / 8, at % 8, at};
   }
   __device__ __forceinline__ bool more() const { return item < n_items; }
   __device__ __forceinline__ void load_tokens(uint8_t* s) const {
 #pragma unroll
     for (int i = 0; i < S::kTokLoads; ++i)
-      pipe::dma16_rsrc(xsrc, xoff[i], step * kF8Block, s + (wave * S::kTokLoads + i) * 1024);
+      pipe::dma16_rsrc(xsrc, xoff[i], step * kF8Block, s + piece(i) * 1024);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         xssrc, (pipe::lds_void*)(s + S::kTokBytes + S::kWgtBytes + tok64() * 256), 4, soff, step * 4, 0, 0);
   }
   template <int kHalf>
   __device__ __forceinline__ void load_weights(uint8_t* s) const {
 #pragma unroll
-    for (int i = kHalf * (S::kWgtLoads / 2); i < (kHalf + 1) * (S::kWgtLoads / 2); ++i)
-      pipe::dma16_rsrc(wsrc, woff[i], step * kF8Block,
-                       s + S::kTokBytes + weight_row(i) * kF8Block);
+    for (int i = kHalf * (S::kWgtLoads / 2); i < (kHalf + 1) * (S::kWgtLoads / 2); ++i) {
+      const Piece p = piece_of(i);
+      const int part = i % 2 * (kF8Tile / 2);
+      pipe::dma16_rsrc(wsrc, (p.cell ? cell[1] : cell[0]) + lane16(), step * kF8Cell + p.tile * kF8Tile + part,
+                       s + S::kTokBytes + p.at * kF8Tile + part);
+    }
   }
   __device__ __forceinline__ void next() {
     ++loaded;
@@ -534,7 +540,7 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
         load();
         const float s0 = ws0[st], s1 = kGateUp ? ws1[st] : 0.f;
         const uint8_t* s = stage[done % S::kStages];
-        const uint8_t* wtile = s + S::kTokBytes + (wn * kNT * 16 + r) * kF8Block;
+        const uint8_t* wtile = s + S::kTokBytes + wn * kNT * kF8Tile + lane * 16;
         const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
         typedef typename std::conditional<kExact, Bf16Row, Codes>::type Row;
         Row x[kM + 1];
@@ -549,8 +555,8 @@ __global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a
         }
 #pragma unroll
         for (int g = 0; g < (kM ? kNT : 0); ++g) {
-          const uint8_t* p = wtile + g * 16 * kF8Block;
-          const Row w = row_of<Row>(p + ((q ^ sw) << 4), p + (((4 + q) ^ sw) << 4));
+          const uint8_t* p = wtile + g * kF8Tile;
+          const Row w = row_of<Row>(p, p + kF8Tile / 2);
 #pragma unroll
           for (int m = 0; m < kM; ++m) {
             const f32x4 v = product(w, x[m]);
@@ -655,7 +661,7 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
       constexpr int kM = decltype(count)::value;
       for (int st = it.k0; st < it.k1; ++st, ++done) {
         const uint8_t* s = stage[done & 1];
-        const uint8_t* wtile = s + S::kTokBytes + (wn * kNT * 16 + r) * kF8Block;
+        const uint8_t* wtile = s + S::kTokBytes + wn * kNT * kF8Tile + lane * 16;
         const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
         const float s0 = ws0[st], s1 = kGateUp ? ws1[st] : 0.f;
         u32x4 x[kM + 1][2], w[kHalf][2];
@@ -663,9 +669,9 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
         auto read_weights = [&](int half) {
 #pragma unroll
           for (int g = 0; g < (kM ? kHalf : 0); ++g) {
-            const uint8_t* p = wtile + (half * kHalf + g) * 16 * kF8Block;
-            w[g][0] = *reinterpret_cast<const u32x4*>(p + ((q ^ sw) << 4));
-            w[g][1] = *reinterpret_cast<const u32x4*>(p + (((4 + q) ^ sw) << 4));
+            const uint8_t* p = wtile + (half * kHalf + g) * kF8Tile;
+            w[g][0] = *reinterpret_cast<const u32x4*>(p);
+            w[g][1] = *reinterpret_cast<const u32x4*>(p + kF8Tile / 2);
           }
         };
         auto multiply = [&](int half) {

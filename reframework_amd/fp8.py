@@ -5,7 +5,8 @@
 
 Blocks start at multiples of 128; the last of a row or matrix may be smaller. With m a
 block's largest finite magnitude, at least 448 * 2^-126, its scale is m / 448 and a value's
-code is value * 448 / m, rounded to nearest even; infinities and NaN become NaN.
+code is value * 448 / m, rounded to nearest even; infinities and NaN become NaN. Weights
+are laid out once, block by block in the order in which the kernels load them.
 
 The reference has neither; its quantised experts are int8 with one scale per tensor, on the
 host (reframework/moe/fused.py:140-197).
@@ -13,7 +14,7 @@ host (reframework/moe/fused.py:140-197).
 
 from __future__ import annotations
 
-from typing import Optional, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -84,11 +85,6 @@ class Fp8Rows:
         return v.reshape(len(self), -1)[:, :self.size].to(dtype)
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` where it starts on 16 bytes, else a copy that does."""
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
 def _quantize(x: torch.Tensor) -> Fp8Rows:
     q = Fp8Rows.empty(x.shape[0], x.shape[1], x.device)
     _capi.fp8_quantize(x, q.padded_codes, q.scales)
@@ -122,24 +118,41 @@ def _check_codes(codes: torch.Tensor, scales: torch.Tensor, name: str, scale_row
     _require_gpu(codes, name)
 
 
-def _padded_codes(codes: torch.Tensor) -> torch.Tensor:
-    """[E, rows, K] codes as bytes in rows of whole blocks, without a copy where they are that."""
-    codes = codes.detach().view(torch.uint8)
-    if codes.shape[2] % BLOCK == 0:
-        return _aligned(codes.contiguous())
-    return torch.nn.functional.pad(codes, (0, padded(codes.shape[2]) - codes.shape[2]))
+CELL = BLOCK * BLOCK
+
+
+def _cells(E: int, N: int, K: int, device: torch.device) -> torch.Tensor:
+    """Room for E matrices [N, K] as cells of 128 x 128 codes (include/moe355.h)."""
+    return torch.empty(E, blocks(N), blocks(K), CELL, dtype=torch.uint8, device=device)
+
+
+def _pack(codes: torch.Tensor) -> torch.Tensor:
+    """[E, N, K] codes as cells."""
+    codes = codes.detach().view(torch.uint8).contiguous()
+    cells = _cells(*codes.shape, codes.device)
+    for c, m in zip(codes, cells):
+        _capi.fp8_pack(c, m)
+    return cells
+
+
+def _unpack(cells: torch.Tensor, N: int, K: int) -> torch.Tensor:
+    """The bytes [E, N, K] of matrices of cells."""
+    E, n, k, _ = cells.shape
+    # a cell: tile of 16 rows, half of 64 columns, 16 columns, row, column
+    c = cells.reshape(E, n, k, 8, 2, 4, 16, 16).permute(0, 1, 3, 6, 2, 4, 5, 7)
+    return c.reshape(E, n * BLOCK, k * BLOCK)[:, :N, :K]
 
 
 class _Codes(torch.nn.Module):
     """Holds codes and scales as buffers that a change of the module's dtype leaves alone (the
     scales by their bits)."""
 
-    def _hold(self, name: str, codes: torch.Tensor, scales: torch.Tensor) -> None:
-        self.register_buffer(name, codes)
+    def _hold(self, name: str, cells: torch.Tensor, scales: torch.Tensor) -> None:
+        self.register_buffer(name, cells)
         self.register_buffer(name + "_scales", scales.detach().contiguous().view(torch.int32))
 
     def _held(self, name: str) -> Tuple[torch.Tensor, torch.Tensor]:
-        """(bytes, scales) as the kernels take them."""
+        """(cells, scales) as the kernels take them."""
         b = self._buffers
         return b[name], b[name + "_scales"]
 
@@ -148,21 +161,21 @@ class _Codes(torch.nn.Module):
         return sum(b.numel() * b.element_size() for b in self._buffers.values())
 
 
-def _dequantize(codes: torch.Tensor, scales: torch.Tensor, K: int) -> torch.Tensor:
-    E, N, Kp = codes.shape
-    s = scales.view(torch.float32).repeat_interleave(BLOCK, 1)[:, :N]
-    v = codes.view(E4M3).float().reshape(E, N, -1, BLOCK) * s[..., None]
-    return v.reshape(E, N, Kp)[..., :K]
+def _dequantize(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """fp32 [E, N, K] of codes and the scales of their blocks."""
+    E, N, K = codes.shape
+    s = scales.repeat_interleave(BLOCK, 1)[:, :N].repeat_interleave(BLOCK, 2)[..., :K]
+    return codes.float() * s
 
 
-def _quantize_matrices(w) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(bytes [E, N, Kp], scales) of a sequence of [N, K] matrices."""
+def _quantize_matrices(w: Sequence[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(cells, scales) of [N, K] matrices."""
     N, K = w[0].shape
-    codes = torch.empty(len(w), N, padded(K), dtype=torch.uint8, device=w[0].device)
+    cells = _cells(len(w), N, K, w[0].device)
     scales = torch.empty(len(w), blocks(N), blocks(K), dtype=torch.float32, device=w[0].device)
-    for m, c, s in zip(w, codes, scales):
+    for m, c, s in zip(w, cells, scales):
         _capi.fp8_quantize_weight(m.detach().contiguous(), c, s)
-    return codes, scales
+    return cells, scales
 
 
 class Fp8Weight(_Codes):
@@ -170,14 +183,14 @@ class Fp8Weight(_Codes):
     ``transposed``: it also holds the matrices transposed, which gradients of the rows are
     multiplied by. The weights themselves are constants."""
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int,
+    def __init__(self, cells: torch.Tensor, scales: torch.Tensor, rows: int, columns: int,
                  transposed: bool = False) -> None:
         super().__init__()
-        self.num_matrices, self.rows, self.columns = codes.shape[0], codes.shape[1], columns
-        self._hold("w", codes, scales)
+        self.num_matrices, self.rows, self.columns = cells.shape[0], rows, columns
+        self._hold("w", cells, scales)
         if transposed:
-            t = codes[..., :columns].transpose(1, 2)
-            self._hold("wt", _padded_codes(t), scales.transpose(1, 2))
+            self._hold("wt", _pack(_unpack(cells, rows, columns).transpose(1, 2)),
+                       scales.transpose(1, 2))
 
     @classmethod
     def quantize(cls, w: torch.Tensor, transposed: bool = False) -> "Fp8Weight":
@@ -189,18 +202,17 @@ class Fp8Weight(_Codes):
         m = list(w) if w.dim() == 3 else [w]
         if len(m) > _capi.MAX_EXPERTS:
             raise ValueError(f"{len(m)} matrices, at most {_capi.MAX_EXPERTS}")
-        return cls(*_quantize_matrices(m), w.shape[-1], transposed)
+        return cls(*_quantize_matrices(m), *w.shape[-2:], transposed)
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor,
                    transposed: bool = False) -> "Fp8Weight":
         """From a checkpoint's codes (float8_e4m3fn, or their bytes) [N, K] or [E, N, K] and
-        scales float32 [(E,) ceil(N/128), ceil(K/128)], on the GPU. Codes of whole blocks
-        are kept as they are, without a copy."""
+        scales float32 [(E,) ceil(N/128), ceil(K/128)], on the GPU."""
         if codes.dim() == 2 and scales.dim() == 2:
             codes, scales = codes[None], scales[None]
         _check_codes(codes, scales, "weights")
-        return cls(_padded_codes(codes), scales, codes.shape[2], transposed)
+        return cls(_pack(codes), scales, *codes.shape[1:], transposed)
 
     @property
     def device(self) -> torch.device:
@@ -210,9 +222,14 @@ class Fp8Weight(_Codes):
     def has_transposed(self) -> bool:
         return "wt" in self._buffers
 
+    def codes(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(codes [E, N, K], scales) as from_codes takes them."""
+        cells, scales = self._held("w")
+        return _unpack(cells, self.rows, self.columns).view(E4M3), scales.view(torch.float32)
+
     def dequantize(self) -> torch.Tensor:
         """[E, N, K] in fp32."""
-        return _dequantize(*self._held("w"), self.columns)
+        return _dequantize(*self.codes())
 
 
 class Fp8Experts(_Codes):
@@ -220,13 +237,13 @@ class Fp8Experts(_Codes):
     [E, H, I]. H and I are multiples of 16. The blocks of w1's gate and up halves start at the
     first row of each."""
 
-    def __init__(self, w1, w1_scales, w2, w2_scales, hidden_size: int,
-                 intermediate_size: int) -> None:
+    def __init__(self, w1: Tuple[torch.Tensor, torch.Tensor], w2: Tuple[torch.Tensor, torch.Tensor],
+                 hidden_size: int, intermediate_size: int) -> None:
         super().__init__()
-        self.num_experts = w1.shape[0]
+        self.num_experts = w2[0].shape[0]
         self.hidden_size, self.intermediate_size = hidden_size, intermediate_size
-        self._hold("w1", w1, w1_scales)
-        self._hold("w2", w2, w2_scales)
+        self._hold("w1", *(t.reshape(self.num_experts, -1, *t.shape[2:]) for t in w1))
+        self._hold("w2", *w2)
 
     @staticmethod
     def _check_sizes(w1: torch.Tensor, w2: torch.Tensor) -> Tuple[int, int, int]:
@@ -250,10 +267,9 @@ class Fp8Experts(_Codes):
                                  f"{tuple(w.shape)}")
             _require_gpu(w, name)
             _capi.dtype_code(w.dtype)
-        E, I, H = cls._check_sizes(w1, w2)
-        codes, scales = _quantize_matrices([h for m in w1 for h in (m[:I], m[I:])])
-        return cls(codes.reshape(E, 2 * I, -1), scales.reshape(E, 2 * blocks(I), -1),
-                   *_quantize_matrices(list(w2)), H, I)
+        _, I, H = cls._check_sizes(w1, w2)
+        return cls(_quantize_matrices([h for m in w1 for h in (m[:I], m[I:])]),
+                   _quantize_matrices(list(w2)), H, I)
 
     @classmethod
     def from_codes(cls, w1: torch.Tensor, w1_scales: torch.Tensor, w2: torch.Tensor,
@@ -266,40 +282,54 @@ class Fp8Experts(_Codes):
         E, I, H = cls._check_sizes(w1, w2)
         _check_codes(w1, w1_scales, "w1", 2 * blocks(I))
         _check_codes(w2, w2_scales, "w2")
-        return cls(_padded_codes(w1), w1_scales, _padded_codes(w2), w2_scales, H, I)
+        halves = w1.detach().contiguous().reshape(2 * E, I, H)
+        return cls((_pack(halves), w1_scales.reshape(2 * E, blocks(I), -1)), (_pack(w2), w2_scales),
+                   H, I)
 
     @property
     def device(self) -> torch.device:
         return self._buffers["w1"].device
 
+    def codes(self, name: str) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``"w1"`` or ``"w2"`` as from_codes takes it: (codes, scales)."""
+        cells, scales = self._held(name)
+        H, I = self.hidden_size, self.intermediate_size
+        if name == "w2":
+            return _unpack(cells, H, I).view(E4M3), scales.view(torch.float32)
+        halves = cells.reshape(2 * self.num_experts, blocks(I), *cells.shape[2:])
+        codes = _unpack(halves, I, H).reshape(self.num_experts, 2 * I, H)
+        return codes.view(E4M3), scales.view(torch.float32)
+
     def dequantize(self, name: str) -> torch.Tensor:
         """``"w1"`` [E, 2I, H] or ``"w2"`` [E, H, I] in fp32."""
-        codes, scales = self._held(name)
+        codes, scales = self.codes(name)
         if name == "w2":
-            return _dequantize(codes, scales, self.intermediate_size)
-        E, I = self.num_experts, self.intermediate_size
-        return _dequantize(codes.reshape(2 * E, I, -1), scales.reshape(2 * E, blocks(I), -1),
-                           self.hidden_size).reshape(E, 2 * I, -1)
+            return _dequantize(codes, scales)
+        I = self.intermediate_size
+        return _dequantize(codes.reshape(-1, I, codes.shape[2]), scales.reshape(-1, blocks(I), scales.shape[2])
+                           ).reshape(codes.shape)
 
 
-def _matmul(q: Fp8Rows, w: Tuple[torch.Tensor, torch.Tensor], offsets: Optional[torch.Tensor],
-            dtype: torch.dtype) -> torch.Tensor:
-    codes, scales = w
-    out = torch.empty(len(q), codes.shape[1], dtype=dtype, device=q.device)
-    _capi.fp8_matmul(q.padded_codes, q.scales, codes, scales, offsets, q.size, out)
+def _matmul(q: Fp8Rows, w: Tuple[torch.Tensor, torch.Tensor], N: int,
+            offsets: Optional[torch.Tensor], dtype: torch.dtype) -> torch.Tensor:
+    cells, scales = w
+    out = torch.empty(len(q), N, dtype=dtype, device=q.device)
+    _capi.fp8_matmul(q.padded_codes, q.scales, cells, scales, offsets, cells.shape[0], q.size, out)
     return out
 
 
 class _MatmulFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets, dtype):
-        ctx.wt, ctx.offsets, ctx.dtype = weight._held("wt"), offsets, x.dtype
-        return _matmul(_quantize(x), weight._held("w"), offsets, dtype)
+        ctx.wt, ctx.columns = weight._held("wt"), weight.columns
+        ctx.offsets, ctx.dtype = offsets, x.dtype
+        return _matmul(_quantize(x), weight._held("w"), weight.rows, offsets, dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        return _matmul(_quantize(dout.contiguous()), ctx.wt, ctx.offsets, ctx.dtype), None, None, None
+        dx = _matmul(_quantize(dout.contiguous()), ctx.wt, ctx.columns, ctx.offsets, ctx.dtype)
+        return dx, None, None, None
 
 
 def matmul_fp8(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight,
@@ -346,14 +376,14 @@ def matmul_fp8(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight,
             offsets = offsets.int()
         offsets = offsets.contiguous()
     if isinstance(x, Fp8Rows):
-        return _matmul(x, weight._held("w"), offsets, dtype)
+        return _matmul(x, weight._held("w"), weight.rows, offsets, dtype)
     x = x.contiguous()
     if torch.is_grad_enabled() and x.requires_grad:
         if not weight.has_transposed:
             raise RuntimeError("gradients need weights that hold the transposed matrices "
                                "(transposed=True)")
         return _MatmulFn.apply(x, weight, offsets, dtype)
-    return _matmul(_quantize(x), weight._held("w"), offsets, dtype)
+    return _matmul(_quantize(x), weight._held("w"), weight.rows, offsets, dtype)
 
 
 __all__ = ["Fp8Rows", "Fp8Weight", "Fp8Experts", "quantize_fp8", "matmul_fp8"]

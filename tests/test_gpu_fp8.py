@@ -95,8 +95,8 @@ def test_weights(N, K, dt, dev):
                 # the product of code and scale is rounded to fp32; an fp32 quotient may tip a tie
                 tie = 0 if dt == "bf16" else 2.0 ** -3
                 assert (d <= (2.0 ** -23 + tie) * np.abs(want) + 1e-30).all() and (d > 2.0 ** -23 * np.abs(want)).mean() < 1e-3
-    codes, scales = fw._held("w")
-    again = Fp8Weight.from_codes(codes[..., :K].view(E4M3), scales.view(torch.float32), transposed=True)
+    again = Fp8Weight.from_codes(*fw.codes(), transposed=True)
+    assert torch.equal(again.codes()[0].view(torch.uint8), fw.codes()[0].view(torch.uint8))
     for name in ("w", "wt"):
         assert all(torch.equal(a, b) for a, b in zip(fw._held(name), again._held(name)))
     assert fw.to(torch.bfloat16).dequantize().dtype == torch.float32
@@ -249,10 +249,10 @@ def test_no_rows_and_views(dev):
     strided = torch.tensor([0, 9, 33, 9], dtype=torch.int32, device=dev)[::2]
     assert torch.equal(matmul_fp8(v, weight, strided), matmul_fp8(v, weight))
     # codes that start off 16 bytes
-    codes, scales = weight._held("w")
-    raw = torch.empty(codes.numel() + 4, dtype=torch.uint8, device=dev)[4:].view_as(codes)
-    raw.copy_(codes)
-    odd = Fp8Weight.from_codes(raw.view(E4M3)[..., :96], scales.view(torch.float32))
+    codes, scales = weight.codes()
+    raw = torch.empty(codes.numel() + 3, dtype=torch.uint8, device=dev)[3:].view(codes.shape)
+    raw.copy_(codes.view(torch.uint8))
+    odd = Fp8Weight.from_codes(raw, scales)
     assert torch.equal(matmul_fp8(v, odd), matmul_fp8(v, weight))
 
 
@@ -308,8 +308,8 @@ def test_operators_together(dev):
     banner("operators together")
     T, H, I, E, K = 200, 256, 384, 6, 2
     ex = make_experts(E, H, I, dev, seed=8)
-    w1 = Fp8Weight.from_codes(*[t.view(v) for t, v in zip(ex._held("w1"), (E4M3, torch.float32))], transposed=True)
-    w2 = Fp8Weight.from_codes(*[t.view(v) for t, v in zip(ex._held("w2"), (E4M3, torch.float32))], transposed=True)
+    w1 = Fp8Weight.from_codes(*ex.codes("w1"), transposed=True)
+    w2 = Fp8Weight.from_codes(*ex.codes("w2"), transposed=True)
     norm = LayerNorm(H, 1e-5).to(dev)
     g = torch.Generator(device=dev).manual_seed(9)
     x = torch.randn(T, H, generator=g, device=dev, requires_grad=True)
