@@ -29,29 +29,41 @@ int check_weights(int N, int K, int E) {
   return MOE355_OK;
 }
 
-// Which kernels run a product of M rows of E matrices over Kp columns: tile_rows 0 streams
-// the weights; max_parts: parts of items that the tiled kernels may leave in memory.
-// Up to kF8StreamRows rows per matrix the weights stream past 16-row tiles (fp8_stream.hip);
-// random routing leaves some matrices with more than a tile, which reads their weights again.
-// Whole expert calls, us streaming / on 64-row tiles: 8 experts of H 4096, I 14336 at 1 row 82 /
-// 148, 2 rows 289 / 299, 5 rows 312 / 328, 8 rows 325 / 324, 12 rows 350 / 328; 64 of H 2048,
-// I 1408 at 1 row 110 / 105, 6 rows 131 / 114, 12 rows 161 / 126; 32 of H 1280, I 3328 at 1 row 54 /
-// 60, 4 rows 106 / 101, 8 rows 112 / 102. One row of one 4096 x 4096 matrix 7.4 / 22.8.
-constexpr int kF8StreamRows = 5;
-
+// Which kernels run a product of M rows of E matrices of N x Kp (gate_up: N of both): tile_rows
+// 0 streams the weights past 16-row tiles; max_parts: parts of items that the 256-row tiles may
+// leave in memory.
 struct F8Path {
   int tile_rows, max_parts;
   size_t part_bytes;
 };
 
-F8Path f8_path(int M, int E, int Kp, bool exact) {
+// By rows per matrix that has any, on average; random routing gives some matrices a tile more.
+// Whole expert calls in us, A: 8 experts of H 4096, I 14336 (2 slots), B: 64 of H 2048, I 1408
+// (6), C: 32 of H 1280, I 3328 (4), D: 16 of H 4096, I 6400 (2).
+// Streaming / 64-row tiles: A at 1 row 82 / 148, 2 rows 289 / 299, 8 rows 325 / 324, 12 rows 350 /
+// 328; B at 1 row 110 / 105, 6 rows 131 / 114, 12 rows 161 / 126; C at 4 rows 106 / 101, 8 rows
+// 112 / 102. One row of one 4096 x 4096 matrix 7.4 / 22.8. (Row by row matrices; later both gained.)
+// 32 / 64: A at 12 rows 267 / 273; B at 12 rows 123 / 116; D at 25 rows 254 / 276; A at 64 rows
+// 479 / 417.
+// 64 / 128: A at 32 rows 302 / 290, 64 rows 398 / 320; B at 36 rows 157 / 157, 65 rows 212 / 178;
+// C at 64 rows 167 / 135.
+// 128 / 256: A at 120 rows 390 / 523, 140 rows 492 / 461; B at 96 rows 195 / 219, 122 rows 221 /
+// 224; C at 106 rows 151 / 186, 128 rows 204 / 195, 150 rows 234 / 184; 4 experts of H 1024, I
+// 1024 at 1000 rows, 128 items, 59 / 77. Exact products of f16 (8 of H 2048, I 4096; 256: the
+// weights through LDS, a kernel since removed) at 512 rows 298 / 360, 1024 rows 560 / 561.
+constexpr int kF8StreamRows = 5;
+
+F8Path f8_path(int M, int N, int Kp, int E, bool exact) {
   F8Path p{};
-  const int rows = M / std::max(1, std::min(M, E));  // per matrix that has any, on average
+  const int active = std::max(1, std::min(M, E)), rows = M / active;
   if (rows <= kF8StreamRows) return p;
-  p.tile_rows = rows < 100 ? 64 : exact ? 128 : 256;
+  const long long items = (static_cast<long long>(M) / 256 + active / 2) * ((N + 255) / 256);
+  p.tile_rows = rows <= 26 ? (rows >= 16 ? 32 : 64)
+                : rows < 128 || exact || items < device_cu_count() ? 128
+                                                                   : 256;
   // cutting items of few steps saves less than the second launch takes
-  if (Kp / kF8Block >= (p.tile_rows > 64 ? 16 : 24)) p.max_parts = device_cu_count();
-  p.part_bytes = static_cast<size_t>(p.max_parts) * f8_part_floats(p.tile_rows) * 4;
+  if (p.tile_rows == 256 && Kp / kF8Block >= 16) p.max_parts = device_cu_count();
+  p.part_bytes = static_cast<size_t>(p.max_parts) * f8_part_floats() * 4;
   return p;
 }
 
@@ -83,14 +95,15 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->rows = static_cast<int>(R);
   p->n_blocks = R <= kPermuteSingleMax ? 1 : static_cast<int>((R + kPermuteChunk - 1) / kPermuteChunk);
   p->max_tiles = E + p->rows / kF8StreamTile;
+  // Where the weights' stream bounds the call exact products cost little (us, scaled / exact: A
+  // of f8_path at 32 rows 290 / 295, 64 rows 320 / 342, 100 rows 348 / 403; B at 36 rows 157 /
+  // 161, 96 rows 194 / 229). A bf16 result of few tokens is off by up to 0.0025 of its size
+  // with the scaled ones, by 0.0017 with these.
+  const int rows = static_cast<int>(R) / std::max(1, std::min(static_cast<int>(R), E));
+  p->exact_up = dtype != MOE355_BF16 || rows <= 40;
   p->exact_down = dtype == MOE355_F32;
-  p->up = f8_path(p->rows, E, f8_pad(H), dtype != MOE355_BF16);
-  // Up to 64-row tiles the weights' stream hides most of what exact products take (us, scaled /
-  // exact: 197 tokens of 2 of 16, H 4096, I 6400 301 / 306; 128 of 6 of 64, H 2048, I 1408 126 /
-  // 133; above, 4096 of 2 of 8, H 4096, I 14336 1620 / @). A bf16 result of few tokens is
-  // off by up to 0.0025 of its size with the scaled ones, by 0.0017 with these.
-  p->exact_up = dtype != MOE355_BF16 || p->up.tile_rows <= 64;
-  p->down = f8_path(p->rows, E, f8_pad(I), p->exact_down);
+  p->up = f8_path(p->rows, 2 * I, f8_pad(H), E, p->exact_up);
+  p->down = f8_path(p->rows, H, f8_pad(I), E, p->exact_down);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -157,7 +170,7 @@ int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, int dtype, siz
   if (int rc = check_weights(N, K, E)) return rc;
   if (M < 0) return fail(MOE355_EINVAL, "bad M=%d", M);
   if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
-  *bytes = M == 0 ? 0 : f8_path(M, E, f8_pad(K), dtype == MOE355_F32).part_bytes;
+  *bytes = M == 0 ? 0 : f8_path(M, N, f8_pad(K), E, dtype == MOE355_F32).part_bytes;
   return MOE355_OK;
 }
 
@@ -173,7 +186,7 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
   if (!aligned16(x) || !aligned16(w) || !aligned4(x_scales) || !aligned4(w_scales) ||
       !aligned4(offsets) || !aligned16(out) || !aligned16(workspace))
     return fail(MOE355_EINVAL, "x/w/scales/offsets/out/workspace not aligned");
-  const F8Path p = f8_path(M, E, f8_pad(K), dtype == MOE355_F32);
+  const F8Path p = f8_path(M, N, f8_pad(K), E, dtype == MOE355_F32);
   if (p.part_bytes > 0 && (!workspace || workspace_bytes < p.part_bytes))
     return fail(MOE355_EWORKSPACE, "workspace of %zu bytes, the call needs %zu", workspace_bytes,
                 p.part_bytes);

@@ -46,7 +46,7 @@ __device__ __forceinline__ float f8_finite_abs(float v) {
 // reciprocal by its remainder, which is exact: where the quotient has few bits, as a tie between
 // two codes has, it comes out as it is. The product with 448 of a 24-bit value is rounded, so
 // that the largest may come out a little over 448, which the conversion rounds to 448. (A
-// division by the compiler takes three times the instructions: 8192 x 4096 bf16 29 us, so @.)
+// division by the compiler takes three times the instructions: 8192 x 4096 bf16 29 us, so 27.)
 __device__ __forceinline__ float f8_quotient(float v, const F8Div& d) {
   const float n = v * d.mul, q = n * d.inv;
   return fmaf(fmaf(-q, d.by, n), d.inv, q);
@@ -116,8 +116,9 @@ hipError_t launch_f8_pack(const F8PackArgs& a, hipStream_t s);
 // gate_up: out_codes, out_scales = act(gate) * up in 8 bits, of gate rows 0 .. I - 1 and up
 // rows I .. 2 I - 1; else out.
 hipError_t launch_f8_stream(const F8MatmulArgs& a, bool gate_up, hipStream_t s);
-// tile_rows: 64, or 256 (exact: 128). Room of one part of an item, in floats.
-size_t f8_part_floats(int tile_rows);
+// tile_rows: 32, 64, 128 or 256 (not of exact products). Room of one part of an item of 256
+// rows, in floats.
+size_t f8_part_floats();
 hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, hipStream_t s);
 
 }  // namespace moe355

@@ -83,7 +83,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const F8QuantArgs a)
 
 // The first launch of an expert call. Its first workgroups group the slots: one wave up to 64
 // slots, one workgroup of a thread per slot up to kPermuteSingleMax, above it the permute's
-// counts; the others quantise x. In two launches a call of 16 tokens takes @ us longer.
+// counts; the others quantise x. In two launches a call of 16 tokens takes 5 us longer.
 enum class Group { kWave, kOne, kCount };
 
 template <typename T, Group kGroup>

@@ -2,15 +2,17 @@
 // an item multiplies BM token rows by 256 weight rows (gate_up: gate and up of 128
 // features, a block of the result's scales), a step of 128 columns at a time.
 //
-// Both operands go straight to LDS: weight tiles as they are laid out, token rows by 128 bytes a
-// step, with their 16-byte chunks XORed by half the row number, which leaves the fragment
-// reads without bank conflicts. A step is one block of both operands' scales, so the matrix core sums it from
+// Tokens go straight to LDS, rows by 128 bytes a step, with their 16-byte chunks XORed by half
+// the row number, which leaves the fragment reads without bank conflicts. Weight tiles go to LDS
+// as they are laid out where 256 rows share them (turns_kernel, bound by the matrix cores), and
+// to the registers of the one wave that needs them up to 128 rows (rows_kernel, bound by the
+// weights' stream). A step is one block of both operands' scales, so the matrix core sums it from
 // zero and the sum is scaled and added in fp32 by the vector unit, whose instructions run beside
 // the next products. Token scales go to LDS with the rows; the weights' one (gate_up: two) of a
 // wave and step is a scalar load.
 //
-// A workgroup runs several items, whose steps follow each other in one stream of loads:
-// the first steps of an item are on their way while the item before it is multiplied and
+// A workgroup of turns_kernel runs several items, whose steps follow each other in one stream of
+// loads: the first steps of an item are on their way while the item before it is multiplied and
 // stored.
 #include <climits>
 
@@ -172,7 +174,7 @@ struct Loader {
   // 64 tokens whose scales this wave loads
   __device__ __forceinline__ int tok64() const { return BM <= 64 ? 0 : wave % (BM / 64); }
   // Piece of the tokens that load i brings (some waves' a second time where there are few).
-  __device__ __forceinline__ int piece(int i) const { return (wave * S::kTokLoads + i) % S::kTokPieces; }
+  __device__ __forceinline__ int piece(int i) const { return wave * S::kTokLoads + i; }
   // The lane, opaque: what follows from it is computed where an item begins, not kept.
   static __device__ __forceinline__ int lane_id() { return pipe::opaque(threadIdx.x & (kWave - 1)); }
   static __device__ __forceinline__ uint32_t lane16() { return (threadIdx.x & (kWave - 1)) * 16; }
@@ -218,7 +220,7 @@ struct Loader {
   struct Piece {
     int cell, tile, at;
   };
-  __device__ __forceinline__ Piece piece_of(int i) const {
+  __device__ __forceinline__ Piece piece_of(int wave, int i) const {
     constexpr int kHalf = S::kWgtLoads / 4;  // tiles of this wave and half
     const int half = i / (2 * kHalf), n = wave * kHalf + i / 2 % kHalf;  // of 8
     const int wn = n / (S::kNT / 2), g = n % (S::kNT / 2);
@@ -226,18 +228,28 @@ struct Loader {
     return kGateUp ? Piece{half, n, at} : Piece{at / 8, at % 8, at};
   }
   __device__ __forceinline__ bool more() const { return item < n_items; }
+  // The wave's number, opaque like the lane: places in LDS are computed again rather than kept
+  // in scalar registers, which are few (kept, they were moved to vector lanes and back every
+  // step).
+  __device__ __forceinline__ int wave_id() const {
+    int w = wave;
+    asm volatile("" : "+s"(w));
+    return w;
+  }
   __device__ __forceinline__ void load_tokens(uint8_t* s) const {
+    uint8_t* to = s + wave_id() * S::kTokLoads * 1024;
 #pragma unroll
     for (int i = 0; i < S::kTokLoads; ++i)
-      pipe::dma16_rsrc(xsrc, xoff[i], step * kF8Block, s + piece(i) * 1024);
+      pipe::dma16_rsrc(xsrc, xoff[i], step * kF8Block, to + i * 1024);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         xssrc, (pipe::lds_void*)(s + S::kTokBytes + S::kWgtBytes + tok64() * 256), 4, soff, step * 4, 0, 0);
   }
   template <int kHalf>
   __device__ __forceinline__ void load_weights(uint8_t* s) const {
+    const int w = wave_id();
 #pragma unroll
     for (int i = kHalf * (S::kWgtLoads / 2); i < (kHalf + 1) * (S::kWgtLoads / 2); ++i) {
-      const Piece p = piece_of(i);
+      const Piece p = piece_of(w, i);
       const int part = i % 2 * (kF8Tile / 2);
       pipe::dma16_rsrc(wsrc, (p.cell ? cell[1] : cell[0]) + lane16(), step * kF8Cell + p.tile * kF8Tile + part,
                        s + S::kTokBytes + p.at * kF8Tile + part);
@@ -274,15 +286,22 @@ __device__ __forceinline__ void interleaved(P product, A add) {
   }
 }
 
-// f(mt as a compile-time constant), mt in [0, kMost].
+// f(mt as a compile-time constant, above 4 rounded up to even ones), mt in [0, kMost].
 template <int kMost, typename F>
 __device__ __forceinline__ void by_count(int mt, F f) {
-  switch (mt) {
-    case 0: f(std::integral_constant<int, 0>()); break;
-    case 1: f(std::integral_constant<int, 1>()); break;
-    case 2: f(std::integral_constant<int, (kMost < 2 ? kMost : 2)>()); break;
-    case 3: f(std::integral_constant<int, (kMost < 3 ? kMost : 3)>()); break;
-    default: f(std::integral_constant<int, kMost>()); break;
+  if constexpr (kMost > 4) {
+    if (mt > kMost - 2)
+      f(std::integral_constant<int, kMost>());
+    else
+      by_count<kMost - 2>(mt, f);
+  } else {
+    switch (mt) {
+      case 0: f(std::integral_constant<int, 0>()); break;
+      case 1: f(std::integral_constant<int, 1>()); break;
+      case 2: f(std::integral_constant<int, (kMost < 2 ? kMost : 2)>()); break;
+      case 3: f(std::integral_constant<int, (kMost < 3 ? kMost : 3)>()); break;
+      default: f(std::integral_constant<int, kMost>()); break;
+    }
   }
 }
 
@@ -469,115 +488,186 @@ struct Codes {
   u32x4 v[2];
 };
 template <typename Row>
-__device__ __forceinline__ Row row_of(const uint8_t* lo, const uint8_t* hi) {
-  const u32x4 c[2] = {*reinterpret_cast<const u32x4*>(lo), *reinterpret_cast<const u32x4*>(hi)};
+__device__ __forceinline__ Row row_of(const u32x4* c) {
   if constexpr (std::is_same<Row, Codes>::value)
     return Codes{{c[0], c[1]}};
   else
     return to_bf16(c);
 }
+template <typename Row>
+__device__ __forceinline__ Row row_of(const uint8_t* lo, const uint8_t* hi) {
+  const u32x4 c[2] = {*reinterpret_cast<const u32x4*>(lo), *reinterpret_cast<const u32x4*>(hi)};
+  return row_of<Row>(c);
+}
 __device__ __forceinline__ f32x4 product(const Codes& w, const Codes& x) { return mma_f8(w.v, x.v); }
 __device__ __forceinline__ f32x4 product(const Bf16Row& w, const Bf16Row& x) { return mma_f8_exact(w, x); }
 
-// All waves read and multiply a step between two barriers.
-template <bool kGateUp, int BM, int WM, bool kExact, typename OutT>
-__global__ __launch_bounds__(kThreads, 2) void tiled_kernel(const F8MatmulArgs a) {
+// Up to 128 token rows, where the weights' stream counts: a workgroup multiplies BM rows by 256
+// weight rows, a wave by 32 of them, whose tiles it alone needs: they go straight to its
+// registers, kAhead steps ahead, 1 KB a load. The tokens, which all waves need, go through LDS,
+// kAhead steps at a time, so that the waves meet once in as many steps. Two workgroups share a
+// CU where 128 registers do. (With the weights in LDS every step waits for all waves: 394 rows
+// of 16 matrices of 12800 x 4096 179 us, so 157, 5.35 TB/s of weights.)
+template <bool kGateUp, int BM, bool kExact, typename OutT>
+__global__ __launch_bounds__(kThreads, kExact || BM > 64 ? 2 : 4) void rows_kernel(const F8MatmulArgs a) {
+  constexpr int WM = 1, kAhead = kExact || BM > 64 ? 3 : 2;
   typedef Shape<BM, WM> S;
   constexpr int kMT = S::kMT, kNT = S::kNT;
-  __shared__ __attribute__((aligned(1024))) uint8_t stage[S::kStages][S::kStage];
-  __shared__ Item items[kMaxItems];
+  static_assert(kNT == 2, "a wave's tiles");
+  static_assert((BM + 63) / 64 * kAhead <= kWaves, "a wave a piece of the scales");
+  constexpr int kPieces = BM / 8;  // of a step's tokens, 8 rows each
+  constexpr int kTokLoads = (kPieces * kAhead + kWaves - 1) / kWaves;
+  constexpr int kWgtLoads = 2 * kNT;  // of a step
+  __shared__ __attribute__((aligned(1024))) uint8_t tokens[2][kAhead][BM * kF8Block];
+  constexpr int kScales = (BM + 63) / 64;  // pieces of 64
+  __shared__ float scales[2][kAhead][kScales * 64];
   __shared__ float most[S::kWN][BM];
-  const int lane = threadIdx.x & (kWave - 1);
+  const int lane = threadIdx.x & (kWave - 1), q = lane >> 4, r = lane & 15, sw = (r >> 1) & 7;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int q = lane >> 4, r = lane & 15, sw = (r >> 1) & 7;
-
   if constexpr (!kGateUp) zero_rest<OutT, kThreads>(a);
-  const int nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
-  const int n_items = list_items<BM, WM>(a, nw, items);
-  if (n_items == 0) return;
-  Loader<kGateUp, BM, WM> ld(a, items, n_items, wave);
-  auto load = [&]() {
-    if (!ld.more()) return;
-    uint8_t* s = stage[ld.loaded % S::kStages];
-    ld.load_tokens(s);
-    ld.template load_weights<0>(s);
-    ld.template load_weights<1>(s);
-    ld.next();
+
+  const int cell_rows = f8_cell_rows(a.N, kGateUp), steps = a.Kp / kF8Block;
+  const int nw = kGateUp ? cell_rows / 2 : (cell_rows + 1) / 2;
+  // The token tiles of a matrix vary fastest and neighbours run on one XCD: they share its weights.
+  const int id = xcd_remap(blockIdx.x, gridDim.x), tiles = gridDim.x / nw;
+  const RowTile t = find_tile(a, BM, id % tiles);
+  if (t.e < 0) return;
+  const Item it{t.e, t.row0, t.row_end, id / tiles, 0, steps, -1};
+  const int n_rows = it.row_end - it.row0;
+
+  // tokens: rows of a piece, offsets as in Loader
+  const size_t first = a.row_src ? 0 : it.row0;
+  const auto xsrc = pipe::lds_rsrc(a.x + first * a.Kp);
+  const auto xssrc = pipe::lds_rsrc(a.x_scales + first * steps);
+  auto source = [&](int row) {
+    return row >= n_rows ? -1 : a.row_src ? a.row_src[it.row0 + row] : row;
   };
-  // Waits until this wave's loads of step `step` of the stream have landed; of the steps after
-  // it kStages - 2 may be in flight (fewer at the end of the stream, where it waits for
-  // all).
-  auto landed = [&](int step) {
-    if (ld.loaded >= step + S::kStages - 1)
-      pipe::wait_vmcnt<(S::kStages - 2) * S::kLoads>();
-    else
-      pipe::wait_vmcnt<0>();
+  // this wave's pieces: of every step where there are as many as waves or more
+  constexpr int kRows8 = kPieces > kWaves ? kPieces / kWaves : 1;
+  uint32_t xoff[kRows8];
+#pragma unroll
+  for (int i = 0; i < kRows8; ++i) {
+    const int row = (wave + i * kWaves) % kPieces * 8 + (lane >> 3), src = source(row);
+    xoff[i] = src < 0 ? pipe::kPadOffset
+                      : static_cast<uint32_t>(src) * a.Kp + (((lane & 7) ^ ((row >> 1) & 7)) << 4);
+  }
+  const int s64 = wave % kScales, src64 = source(s64 * 64 + lane);
+  const uint32_t soff = src64 < 0 ? pipe::kPadOffset : static_cast<uint32_t>(src64) * steps * 4;
+  auto load_tokens = [&](int k0, int buffer) {
+#pragma unroll
+    for (int i = 0; i < kTokLoads; ++i) {
+      // some waves load a step's a second time
+      const int u = min((wave + i * kWaves) / kPieces, kAhead - 1), k = min(k0 + u, steps - 1);
+      const int piece = (wave + i * kWaves) % kPieces;
+      pipe::dma16_rsrc(xsrc, xoff[i % kRows8], k * kF8Block, &tokens[buffer][u][piece * 1024]);
+    }
+    const int u = wave / kScales % kAhead, k = min(k0 + u, steps - 1);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(xssrc, (pipe::lds_void*)(&scales[buffer][u][s64 * 64]), 4, soff, k * 4, 0, 0);
   };
+
+  // this wave's two tiles (gate_up: gate and up of the same features)
+  const uint8_t* wp[kNT];
+  const const_f32* ws[kNT];
 #pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) load();
-  int done = 0;  // steps of the stream
-  const int wm = wave / S::kWN, wn = wave % S::kWN;  // this wave's tokens and weight rows
-  for (int j = 0; j < n_items; ++j) {
-    const Item it = uniform(items + j);
-    const const_f32 *ws0, *ws1;
-    weight_scales<kGateUp, S>(a, it, wn, &ws0, &ws1);
-    f32x4 acc[kMT][kNT];
+  for (int g = 0; g < kNT; ++g) {
+    const int block = min(kGateUp ? it.wt + g * (cell_rows / 2) : it.wt * 2 + wave / 4, cell_rows - 1);
+    const int tile = kGateUp ? wave : wave % 4 * 2 + g;
+    const size_t cells = (static_cast<size_t>(it.e) * cell_rows + block) * steps;
+    wp[g] = a.w + cells * kF8Cell + tile * kF8Tile + lane * 16;
+    ws[g] = (const const_f32*)(a.w_scales + cells);
+  }
+  u32x4 w[kAhead][kNT][2];
+  // always as many loads, the last step again past it: the waits for the tokens count them
+  auto load_weights = [&](int k, u32x4 (*to)[2]) {
+    const size_t at = static_cast<size_t>(min(k, steps - 1)) * kF8Cell;
 #pragma unroll
-    for (int m = 0; m < kMT; ++m)
+    for (int g = 0; g < kNT; ++g) {
+      to[g][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp[g] + at));
+      to[g][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp[g] + at + kF8Tile / 2));
+    }
+  };
+
+  load_tokens(0, 0);
 #pragma unroll
-      for (int g = 0; g < kNT; ++g) acc[m][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // A wave has every WM-th 16 rows of the tile, so that the waves share the rows of one that
-    // is not full; mt of its kMT hold any.
-    const int mt = min((it.row_end - it.row0 + 16 * (WM - 1 - wm) + 15) / (16 * WM), kMT);
-    by_count<kMT>(mt, [&](auto count) {  // one instance per count: mma_f8 needs straight-line code
-      constexpr int kM = decltype(count)::value;
-      for (int st = it.k0; st < it.k1; ++st, ++done) {
-        // Every wave has read step `done` - 1, whose buffer is filled again, and has seen its
-        // loads of step `done` land.
-        landed(done);
-        pipe::wait_lgkm0();
-        barrier();
-        load();
-        const float s0 = ws0[st], s1 = kGateUp ? ws1[st] : 0.f;
-        const uint8_t* s = stage[done % S::kStages];
-        const uint8_t* wtile = s + S::kTokBytes + wn * kNT * kF8Tile + lane * 16;
-        const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
+  for (int u = 0; u < kAhead; ++u) load_weights(u, w[u]);
+  f32x4 acc[kMT][kNT];
+#pragma unroll
+  for (int m = 0; m < kMT; ++m)
+#pragma unroll
+    for (int g = 0; g < kNT; ++g) acc[m][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+  by_count<kMT>((n_rows + 15) / 16, [&](auto count) {
+    constexpr int kM = decltype(count)::value > 0 ? decltype(count)::value : 1;  // a tile has rows
+    // n steps from k0 on, straight-line (mma_f8)
+    auto run = [&](int k0, int buffer, auto n) {
+#pragma unroll
+      for (int u = 0; u < decltype(n)::value; ++u) {
+        const int k = k0 + u;
+        const float s0 = ws[0][k], s1 = ws[1][k];
         typedef typename std::conditional<kExact, Bf16Row, Codes>::type Row;
-        Row x[kM + 1];
-        float sg[kM + 1], su[kM + 1];
+        const Row w0 = row_of<Row>(w[u][0]), w1 = row_of<Row>(w[u][1]);
+        auto read = [&](int m) {
+          const uint8_t* p = tokens[buffer][u] + (16 * m + r) * kF8Block;
+          return row_of<Row>(p + ((q ^ sw) << 4), p + (((4 + q) ^ sw) << 4));
+        };
+        // A tile row at a time: its products, the sums of the one before, and the reads of the
+        // next.
+        f32x4 v[2][kNT];
+        Row x = read(0);
 #pragma unroll
-        for (int m = 0; m < kM; ++m) {
-          const uint8_t* p = s + (16 * (wm + WM * m) + r) * kF8Block;
-          x[m] = row_of<Row>(p + ((q ^ sw) << 4), p + (((4 + q) ^ sw) << 4));
-          const float xs = *reinterpret_cast<const float*>(ts + 64 * WM * m);
-          sg[m] = xs * s0;
-          su[m] = xs * s1;
-        }
-#pragma unroll
-        for (int g = 0; g < (kM ? kNT : 0); ++g) {
-          const uint8_t* p = wtile + g * kF8Tile;
-          const Row w = row_of<Row>(p, p + kF8Tile / 2);
-#pragma unroll
-          for (int m = 0; m < kM; ++m) {
-            const f32x4 v = product(w, x[m]);
-            const float f = kGateUp && g >= kNT / 2 ? su[m] : sg[m];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][g][i] = fmaf(v[i], f, acc[m][g][i]);
+        for (int m = 0; m <= kM; ++m) {
+          if (m < kM) {
+            v[m & 1][0] = product(w0, x);
+            v[m & 1][1] = product(w1, x);
+            if (m + 1 < kM)
+              x = read(m + 1);
+            else
+              load_weights(k + kAhead, w[u]);  // into the registers that are free now
           }
+          if (m > 0) {
+            const float xs = scales[buffer][u][16 * (m - 1) + r];
+#pragma unroll
+            for (int g = 0; g < kNT; ++g) {
+              const float f = xs * (g ? s1 : s0);
+              f32x4& sum = acc[m - 1][g];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum[i] = fmaf(v[(m - 1) & 1][g][i], f, sum[i]);
+              asm volatile("" : "+v"(sum));  // added here (mma_f8)
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
-    });
-    if (it.part >= 0) {
-      store_part<S>(a, it, acc);
-    } else if constexpr (kGateUp) {
-      activate<S, BM, WM>(a, it, acc, wm, wn, 0, most);
+    };
+    auto next_tokens = [&](int k0, int buffer) {
+      // Of this wave's loads of these tokens: behind them those of kAhead steps' weights
+      pipe::wait_vmcnt<kWgtLoads * kAhead>();
       pipe::wait_lgkm0();
-      barrier();
-      // `most` is written again by the next item's epilogue, behind a barrier of its steps
-      store_codes<S, BM, WM>(a, it, acc, wm, wn, 0, most);
-    } else {
-      store_rows<S, WM, OutT>(a, it, acc, wm, wn, 0);
+      barrier();  // all have read the tokens before
+      load_tokens(k0 + kAhead, buffer ^ 1);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    int buffer = 0, k0 = 0;
+    for (; k0 + kAhead <= steps; k0 += kAhead, buffer ^= 1) {
+      next_tokens(k0, buffer);
+      run(k0, buffer, std::integral_constant<int, kAhead>());
     }
+    if (k0 < steps) {
+      next_tokens(k0, buffer);
+      static_assert(kAhead <= 4, "what may be left");
+      if (kAhead > 3 && steps - k0 == 3)
+        run(k0, buffer, std::integral_constant<int, (kAhead > 3 ? 3 : 1)>());
+      else if (kAhead > 2 && steps - k0 == 2)
+        run(k0, buffer, std::integral_constant<int, 2>());
+      else
+        run(k0, buffer, std::integral_constant<int, 1>());
+    }
+  });
+  if constexpr (kGateUp) {
+    activate<S, BM, WM>(a, it, acc, 0, wave, 0, most);
+    __syncthreads();
+    store_codes<S, BM, WM>(a, it, acc, 0, wave, 0, most);
+  } else {
+    store_rows<S, WM, OutT>(a, it, acc, 0, wave, 0);
   }
 }
 
@@ -733,59 +823,67 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
   if (!second) barrier();
 }
 
-template <bool kGateUp, int BM, int WM, bool kExact, typename OutT>
-hipError_t launch(const F8MatmulArgs& a, hipStream_t s) {
-  const long long nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
-  // at most: every matrix that has rows has a tile that is not full
-  const long long tiles = a.offsets ? a.M / BM + (a.E < a.M ? a.E : a.M) : (a.M + BM - 1) / BM;
-  const long long total = tiles * nw;
+// Tiles of rows at most: every matrix that has rows has a tile that is not full.
+long long row_tiles(const F8MatmulArgs& a, int rows) {
+  return a.offsets ? a.M / rows + (a.E < a.M ? a.E : a.M) : (a.M + rows - 1) / rows;
+}
+
+template <bool kGateUp, typename OutT>
+hipError_t launch_turns(const F8MatmulArgs& a, hipStream_t s) {
+  constexpr int BM = 256, WM = 4;
+  const int cell_rows = f8_cell_rows(a.N, kGateUp);
+  const long long nw = kGateUp ? cell_rows / 2 : (cell_rows + 1) / 2;
+  const long long total = row_tiles(a, BM) * nw;
   if (total > INT_MAX) return hipErrorInvalidValue;
   long long grid = device_cu_count();
   // the items of a workgroup have kMaxItems - 1 full rounds at most
   const long long most = grid * (kMaxItems - 1);
   grid = total < grid ? total : grid * ((total + most - 1) / most);
-  const dim3 groups(static_cast<unsigned>(grid));
-  if constexpr (BM == 256)
-    turns_kernel<kGateUp, OutT><<<groups, dim3(kThreads), 0, s>>>(a);
-  else
-    tiled_kernel<kGateUp, BM, WM, kExact, OutT><<<groups, dim3(kThreads), 0, s>>>(a);
+  turns_kernel<kGateUp, OutT><<<dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s>>>(a);
   if (a.max_parts > 0 && hipPeekAtLastError() == hipSuccess) {
     // at least two parts an item
-    const unsigned tails = static_cast<unsigned>((total < a.max_parts / 2 ? total : a.max_parts / 2) * Shape<BM, WM>::kMT);
-    parts_kernel<kGateUp, BM, WM, OutT><<<dim3(tails), dim3(kThreads), 0, s>>>(a, static_cast<int>(grid));
+    const long long tails = total < a.max_parts / 2 ? total : a.max_parts / 2;
+    parts_kernel<kGateUp, BM, WM, OutT>
+        <<<dim3(static_cast<unsigned>(tails * Shape<BM, WM>::kMT)), dim3(kThreads), 0, s>>>(a, static_cast<int>(grid));
   }
   return hipGetLastError();
 }
 
-template <int BM, int WM>
-hipError_t launch_scaled(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
-  if (gate_up) return launch<true, BM, WM, false, float>(a, s);
-  if (a.out_dtype == MOE355_F32) return launch<false, BM, WM, false, float>(a, s);
-  if (a.out_dtype == MOE355_BF16) return launch<false, BM, WM, false, bf16>(a, s);
-  return launch<false, BM, WM, false, f16>(a, s);
+template <bool kGateUp, int BM, bool kExact, typename OutT>
+hipError_t launch_rows(const F8MatmulArgs& a, hipStream_t s) {
+  const int cell_rows = f8_cell_rows(a.N, kGateUp);
+  const long long nw = kGateUp ? cell_rows / 2 : (cell_rows + 1) / 2;
+  const long long groups = row_tiles(a, BM) * nw;
+  if (groups > INT_MAX) return hipErrorInvalidValue;
+  rows_kernel<kGateUp, BM, kExact, OutT><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, s>>>(a);
+  return hipGetLastError();
 }
 
-template <int BM, int WM>
-hipError_t launch_exact(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
-  return gate_up ? launch<true, BM, WM, true, float>(a, s) : launch<false, BM, WM, true, float>(a, s);
+template <int BM>
+hipError_t launch_rows_of(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
+  if (gate_up && a.exact) return launch_rows<true, BM, true, float>(a, s);
+  if (gate_up)  // not where exact products cost next to nothing (f8_plan)
+    return BM == 128 ? launch_rows<true, 128, false, float>(a, s) : hipErrorInvalidValue;
+  if (a.exact) return launch_rows<false, BM, true, float>(a, s);
+  if (a.out_dtype == MOE355_F32) return launch_rows<false, BM, false, float>(a, s);
+  if (a.out_dtype == MOE355_BF16) return launch_rows<false, BM, false, bf16>(a, s);
+  return launch_rows<false, BM, false, f16>(a, s);
 }
 
 }  // namespace
 
-size_t f8_part_floats(int tile_rows) {
-  static_assert(Shape<256, 4>::kPartTile == 256 * kBN && Shape<64, 2>::kPartTile == 64 * kBN, "a part");
-  return static_cast<size_t>(tile_rows) * kBN;
-}
+size_t f8_part_floats() { return 256 * kBN; }
 
 hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, hipStream_t s) {
   if (a.M == 0) return hipSuccess;
-  // Exact products leave no registers for a 256-row tile.
-  if (a.exact) {
-    if (tile_rows == 128) return launch_exact<128, 2>(a, gate_up, s);
-    return tile_rows == 64 ? launch_exact<64, 2>(a, gate_up, s) : hipErrorInvalidValue;
-  }
-  if (tile_rows == 256) return launch_scaled<256, 4>(a, gate_up, s);
-  return tile_rows == 64 ? launch_scaled<64, 2>(a, gate_up, s) : hipErrorInvalidValue;
+  if (tile_rows == 32) return launch_rows_of<32>(a, gate_up, s);
+  if (tile_rows == 64) return launch_rows_of<64>(a, gate_up, s);
+  if (tile_rows == 128) return launch_rows_of<128>(a, gate_up, s);
+  if (tile_rows != 256 || a.exact) return hipErrorInvalidValue;
+  if (gate_up) return launch_turns<true, float>(a, s);
+  if (a.out_dtype == MOE355_F32) return launch_turns<false, float>(a, s);
+  if (a.out_dtype == MOE355_BF16) return launch_turns<false, bf16>(a, s);
+  return launch_turns<false, f16>(a, s);
 }
 
 }  // namespace moe355
