@@ -155,19 +155,14 @@ hipError_t launch_product(const F8MatmulArgs& a, hipStream_t s) {
                                                             : launch<false, 1, 4, kExact, OutT>(a, s);
 }
 
-// Likewise. Whole calls, us with 1 / 2 waves: 224 workgroups (1 token, 8 experts of H 4096, I 14336)
-// @ / @, 561 (16 tokens, 64 of H 2048, I 1408) @ / @.
-template <bool kExact>
-hipError_t launch_gate_up(const F8MatmulArgs& a, hipStream_t s) {
-  return stream_groups(a, true) <= device_cu_count() ? launch<true, 8, 2, kExact, float>(a, s)
-                                                     : launch<true, 8, 1, kExact, float>(a, s);
-}
-
 }  // namespace
 
 hipError_t launch_f8_stream(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
   if (a.M == 0) return hipSuccess;
-  if (gate_up) return a.exact ? launch_gate_up<true>(a, s) : hipErrorInvalidValue;
+  // Two waves a pair of tiles, as above, gain nothing here: whole calls, us with 1 / 2, 1 token
+  // of 8 experts of H 4096, I 14336 88 / 87, of H 1024, I 1024 18.6 / 18.2; 16 tokens of 64 of H
+  // 2048, I 1408 100 / 103.
+  if (gate_up) return a.exact ? launch<true, 8, 1, true, float>(a, s) : hipErrorInvalidValue;
   if (a.exact) return launch_product<true, float>(a, s);
   if (a.out_dtype == MOE355_F32) return launch_product<false, float>(a, s);
   if (a.out_dtype == MOE355_BF16) return launch_product<false, bf16>(a, s);
