@@ -440,7 +440,7 @@ int moe355_mx_fused_experts(const void* x, const void* x_scales, const void* w1,
  * fp32, rounded once; var is the mean of the squares around the mean. With residual == NULL
  * r = x, residual_out is unused and x may alias out. mean and rstd ([T] fp32, both or none)
  * keep mean(r) and 1 / sqrt(var(r) + eps) for the backward pass. Any H up to 16384 (fp32:
- * 8192), tensors aligned to their elements. The reference has no LayerNorm; this stands where
+ * 8192), less than 2^24 rows, tensors aligned to their elements. The reference has no LayerNorm; this stands where
  * RMSNorm.forward_add_residual does (reframework/layers/norm.py:27-53).
  */
 int moe355_layer_norm(const void* x, const void* residual, void* residual_out, const void* weight,
@@ -483,6 +483,7 @@ int moe355_token_order(const void* topk_ids, int ids_int64, int T, int K, int E,
  *   combine_rows_bwd   drows[slot_to_row[t,k]] = topk_w[t,k] * dout[t], zeros from
  *                  offsets[E] on; dw[t,k] = dot(dout[t], rows[slot_to_row[t,k]]) in
  *                  fp32, 0 for a slot without a row; either may be NULL
+ * Slots whose row lies outside [0, T*K) have none. A call takes less than 2^26 tokens.
  */
 int moe355_permute_rows(const void* x, const int32_t* offsets, const int32_t* slot_to_row, int T,
                         int H, int K, int E, int dtype, void* rows, void* stream);

@@ -29,6 +29,13 @@ int check_weights(int N, int K, int E) {
   return MOE355_OK;
 }
 
+int check_rows(int M, int dtype) {
+  if (M < 0) return fail(MOE355_EINVAL, "bad M=%d", M);
+  if (M > INT_MAX / 2) return fail(MOE355_EUNSUPPORTED, "M=%d too large", M);
+  if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  return MOE355_OK;
+}
+
 // Which kernels run a product of M rows of E matrices of N x Kp (gate_up: N of both): tile_rows
 // 0 streams the weights past 16-row tiles; max_parts: parts of items that the 256-row tiles may
 // leave in memory.
@@ -137,6 +144,9 @@ int moe355_fp8_quantize(const void* x, int M, int K, int dtype, void* codes, flo
                         void* stream) {
   if (int rc = check_matrix(M, K)) return rc;
   if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  // a launch holds less than 2^32 threads, 16 a block
+  if (static_cast<long long>(M) * f8_blocks(K) >= 1 << 28)
+    return fail(MOE355_EUNSUPPORTED, "M=%d rows of K=%d: a call takes less than 2^28 blocks", M, K);
   if (M == 0) return MOE355_OK;
   if (!x || !codes || !scales) return fail(MOE355_EINVAL, "NULL tensor argument");
   if (reinterpret_cast<uintptr_t>(x) % elem_size(dtype) || !aligned16(codes) || !aligned4(scales))
@@ -168,8 +178,7 @@ int moe355_fp8_pack(const void* codes, int N, int K, void* cells, void* stream) 
 int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, int dtype, size_t* bytes) {
   if (!bytes) return fail(MOE355_EINVAL, "NULL result");
   if (int rc = check_weights(N, K, E)) return rc;
-  if (M < 0) return fail(MOE355_EINVAL, "bad M=%d", M);
-  if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  if (int rc = check_rows(M, dtype)) return rc;
   *bytes = M == 0 ? 0 : f8_path(M, N, f8_pad(K), E, dtype == MOE355_F32).part_bytes;
   return MOE355_OK;
 }
@@ -178,8 +187,7 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
                       const int32_t* offsets, int M, int N, int K, int E, int dtype, void* out,
                       void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_weights(N, K, E)) return rc;
-  if (M < 0) return fail(MOE355_EINVAL, "bad M=%d", M);
-  if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  if (int rc = check_rows(M, dtype)) return rc;
   if (!offsets && E != 1) return fail(MOE355_EINVAL, "%d matrices without offsets", E);
   if (M == 0) return MOE355_OK;
   if (!x || !x_scales || !w || !w_scales || !out) return fail(MOE355_EINVAL, "NULL tensor argument");

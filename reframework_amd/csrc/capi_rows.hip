@@ -19,6 +19,8 @@ int check_norm(int T, int H, int dtype, int weight_dtype) {
     return fail(MOE355_EINVAL, "unknown dtype %d / weight dtype %d", dtype, weight_dtype);
   if (H > norm_max_hidden(dtype))
     return fail(MOE355_EUNSUPPORTED, "LayerNorm needs H <= %d", norm_max_hidden(dtype));
+  // a launch holds less than 2^32 threads, 256 a row
+  if (T >= 1 << 24) return fail(MOE355_EUNSUPPORTED, "T=%d: a call takes less than 2^24 rows", T);
   return MOE355_OK;
 }
 
@@ -26,6 +28,8 @@ int check_slots(int T, int K, int E, int H, int dtype) {
   if (T < 0 || K < 1) return fail(MOE355_EINVAL, "bad sizes T=%d K=%d", T, K);
   if (E < 1 || E > MOE355_MAX_EXPERTS)
     return fail(MOE355_EUNSUPPORTED, "E=%d outside [1, %d]", E, MOE355_MAX_EXPERTS);
+  // a launch holds less than 2^32 threads, 64 a token
+  if (T >= 1 << 26) return fail(MOE355_EUNSUPPORTED, "T=%d: a call takes less than 2^26 tokens", T);
   if (static_cast<long long>(T) * K > INT_MAX / 2)
     return fail(MOE355_EUNSUPPORTED, "T*K=%lld too large", static_cast<long long>(T) * K);
   if (H <= 0) return fail(MOE355_EINVAL, "bad H=%d", H);

@@ -858,7 +858,7 @@ hipError_t launch_rows(const F8MatmulArgs& a, hipStream_t s) {
   const int cell_rows = f8_cell_rows(a.N, kGateUp);
   const long long nw = kGateUp ? cell_rows / 2 : (cell_rows + 1) / 2;
   const long long groups = row_tiles(a, BM) * nw;
-  if (groups > INT_MAX) return hipErrorInvalidValue;
+  if (groups * kThreads > UINT_MAX) return hipErrorInvalidValue;
   rows_kernel<kGateUp, BM, kExact, OutT><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, s>>>(a);
   return hipGetLastError();
 }

@@ -26,12 +26,17 @@ __device__ __forceinline__ int wave_of_block() {
   return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 }
 
+// Rows outside the R there are count as none.
+__device__ __forceinline__ bool has_row(int row, int R) {
+  return static_cast<unsigned>(row) < static_cast<unsigned>(R);
+}
+
 // Zeros in the rows from n on, this workgroup's share of them and of their chunks.
 template <typename T>
 __device__ __forceinline__ void zero_tail(T* rows, int n, int R, int H, int lane, int wave) {
   constexpr int N = Vec16<T>::N;
   const int parts = gridDim.x * kTokens;
-  for (int r = n + blockIdx.x * kTokens + wave; r < R; r += parts)
+  for (int r = max(n, 0) + blockIdx.x * kTokens + wave; r < R; r += parts)
     for (int e = (blockIdx.y * kWave + lane) * N; e < H; e += gridDim.y * kWave * N)
       store_chunk<T>(rows + static_cast<size_t>(r) * H + e, u32x4{0u, 0u, 0u, 0u}, H - e);
 }
@@ -53,7 +58,7 @@ __global__ __launch_bounds__(kThreads) void permute_rows_kernel(const TokenRowsA
     const int32_t* rows = a.slot_to_row + static_cast<size_t>(t) * a.K;
     for (int k = 0; k < a.K; ++k) {
       const int row = rows[k];
-      if (row < 0) continue;
+      if (!has_row(row, a.R)) continue;
 #pragma unroll
       for (int c = 0; c < kCpt; ++c) {
         const int e = ((blockIdx.y * kCpt + c) * kWave + lane) * N;
@@ -86,6 +91,7 @@ __global__ __launch_bounds__(kThreads) void combine_rows_kernel(const TokenRowsA
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       row[j] = k0 + j < a.K ? rows[k0 + j] : -1;
+      if (!has_row(row[j], a.R)) row[j] = -1;
       w[j] = kWeights && k0 + j < a.K ? weights[k0 + j] : 1.f;
     }
 #pragma unroll
@@ -141,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void combine_rows_bwd_kernel(const Combin
     for (int k = 0; k < a.K; ++k) {
       const size_t slot = static_cast<size_t>(t) * a.K + k;
       const int row = a.slot_to_row[slot];
-      if (row < 0) {
+      if (!has_row(row, a.R)) {
         if (a.dw && lane == 0) a.dw[slot] = 0.f;
         continue;
       }

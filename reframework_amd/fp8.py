@@ -321,14 +321,15 @@ def _matmul(q: Fp8Rows, w: Tuple[torch.Tensor, torch.Tensor], N: int,
 class _MatmulFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets, dtype):
-        ctx.wt, ctx.columns = weight._held("wt"), weight.columns
-        ctx.offsets, ctx.dtype = offsets, x.dtype
+        ctx.columns, ctx.dtype = weight.columns, x.dtype
+        ctx.save_for_backward(*weight._held("wt"), offsets)
         return _matmul(_quantize(x), weight._held("w"), weight.rows, offsets, dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        dx = _matmul(_quantize(dout.contiguous()), ctx.wt, ctx.columns, ctx.offsets, ctx.dtype)
+        cells, scales, offsets = ctx.saved_tensors
+        dx = _matmul(_quantize(dout.contiguous()), (cells, scales), ctx.columns, offsets, ctx.dtype)
         return dx, None, None, None
 
 

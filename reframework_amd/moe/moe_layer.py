@@ -60,7 +60,7 @@ import numpy as np
 import torch
 
 from reframework_amd import _capi, env
-from reframework_amd.layers import BaseOP, activation_code
+from reframework_amd.layers import BaseOP, LayerNorm, activation_code
 from reframework_amd.moe.fused import (fused_experts_mxfp4, require_gpu, run_experts,
                                        run_grouped_topk)
 from reframework_amd.moe.offload_cache import ExpertOffloadCache, Prediction
@@ -556,7 +556,12 @@ class FusedMoE(BaseOP):
         """``f, residual = norm.forward_add_residual(x, residual); f = self(f)``
         (reframework/models/base.py:135-136) with the residual add, the
         RMSNorm and the router in one library call; returns (output, new
-        residual). ``norm`` is an RMSNorm (its weight, optional bias and eps)."""
+        residual). ``norm`` is an RMSNorm (its weight, optional bias and eps), or a LayerNorm,
+        which is a call of its own before the layer's."""
+        if isinstance(norm, LayerNorm):
+            with torch.no_grad():
+                normed, new_res = norm.forward_add_residual(x.to(self.dtype), residual.to(self.dtype))
+                return self(normed).to(x.dtype), new_res.to(residual.dtype)
         shape = x.shape
         x2 = x.reshape(-1, self.hidden_size)
         require_gpu(x2)

@@ -76,16 +76,16 @@ def _permute(x: torch.Tensor, order: TokenOrder) -> torch.Tensor:
 class _PermuteFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, order):
-        ctx.order = order
+        ctx.save_for_backward(order.slot_to_row)
         return _permute(x, order)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, drows):
-        order = ctx.order
-        dx = torch.empty(order.slot_to_row.shape[0], drows.shape[1], dtype=drows.dtype,
+        slot_to_row, = ctx.saved_tensors
+        dx = torch.empty(slot_to_row.shape[0], drows.shape[1], dtype=drows.dtype,
                          device=drows.device)
-        _capi.combine_rows(drows.contiguous(), None, order.slot_to_row, dx)
+        _capi.combine_rows(drows.contiguous(), None, slot_to_row, dx)
         return dx, None
 
 
@@ -94,23 +94,24 @@ class _CombineFn(torch.autograd.Function):
     def forward(ctx, rows, weights, order):
         out = torch.empty(weights.shape[0], rows.shape[1], dtype=rows.dtype, device=rows.device)
         _capi.combine_rows(rows, weights, order.slot_to_row, out)
-        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights)
-        ctx.order = order
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights, order.offsets,
+                              order.slot_to_row)
+        ctx.num_experts = order.num_experts
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        rows, weights = ctx.saved_tensors
-        order, dout = ctx.order, dout.contiguous()
+        rows, weights, offsets, slot_to_row = ctx.saved_tensors
+        dout = dout.contiguous()
         drows = dw = None
         if ctx.needs_input_grad[0]:
-            drows = torch.empty(order.row_src.shape[0], dout.shape[1], dtype=dout.dtype,
+            drows = torch.empty(slot_to_row.numel(), dout.shape[1], dtype=dout.dtype,
                                 device=dout.device)
         if ctx.needs_input_grad[1]:
             dw = torch.empty_like(weights)
-        _capi.combine_rows_bwd(dout, rows, weights, order.offsets, order.slot_to_row,
-                               order.num_experts, drows, dw)
+        _capi.combine_rows_bwd(dout, rows, weights, offsets, slot_to_row, ctx.num_experts, drows,
+                               dw)
         return drows, dw, None
 
 

@@ -17,6 +17,7 @@ import torch
 
 from _helpers import DT, banner
 from reframework_amd.layers import LayerNorm
+from reframework_amd.moe import FusedMoE
 
 pytestmark = pytest.mark.gpu
 EPS = 1e-5
@@ -258,3 +259,25 @@ def test_streams_and_graphs(dev):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_before_an_expert_layer(dev):
+    """FusedMoE.forward_with_norm takes a LayerNorm: the norm's call, then the layer's."""
+    banner("layer_norm before FusedMoE")
+    torch.manual_seed(5)
+    E, K, H, I, T = 4, 2, 256, 128, 19
+    moe = FusedMoE(E, K, H, I, dtype=torch.bfloat16).to(dev)
+    with torch.no_grad():
+        for p in moe.parameters():
+            p.normal_(std=0.05)
+    norm = LayerNorm(H, 1e-5).to(dev)
+    with torch.no_grad():
+        norm.weight.uniform_(0.5, 1.5)
+        norm.bias.normal_()
+    x, res = (torch.randn(T, H, device=dev).to(torch.bfloat16) for _ in range(2))
+    out, new_res = moe.forward_with_norm(x, res, norm)
+    with torch.no_grad():
+        normed, want_res = norm.forward_add_residual(x, res)
+        want = moe(normed)
+    assert torch.equal(new_res, want_res) and torch.equal(out, want)
+    assert not out.requires_grad and not new_res.requires_grad

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from _helpers import DT, banner
-from reframework_amd.moe import combine_tokens, permute_tokens, token_order
+from reframework_amd.moe import TokenOrder, combine_tokens, permute_tokens, token_order
 
 pytestmark = pytest.mark.gpu
 
@@ -198,3 +198,32 @@ def test_streams_and_graphs(dev):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_slots_of_rows_that_are_not_there(dev):
+    """An order that names rows behind the last: they count as none."""
+    banner("tokens rows out of range")
+    T, H, E, K = 5, 40, 3, 2
+    ids, w = routing(T, K, E, seed=3)
+    x, y, _, dout = data(T, T * K, H, torch.float32, dev, seed=6)
+    order = token_order(torch.from_numpy(ids).to(dev), E)
+    bad = TokenOrder(order.offsets, order.slot_to_row.clone(), order.row_src, E)
+    bad.slot_to_row[1, 0], bad.slot_to_row[4, 1] = T * K, 2 ** 31 - 1
+    wt = torch.from_numpy(w).to(dev).requires_grad_()
+    y.requires_grad_()
+    out = combine_tokens(y, bad, wt)
+    cut = wt.detach().clone()
+    cut[1, 0] = cut[4, 1] = 0.0
+    assert torch.equal(out.detach(), combine_tokens(y.detach(), order, cut))
+    dw, = torch.autograd.grad(out, [wt], [dout])
+    assert dw[1, 0] == 0 and dw[4, 1] == 0 and bool((dw != 0).sum() == T * K - 2)
+
+
+def test_an_order_changed_before_the_backward_pass(dev):
+    banner("tokens order changed")
+    ids = torch.tensor([[0, 1], [1, 2]], device=dev)
+    x = torch.randn(2, 16, device=dev, requires_grad=True)
+    rows, order = permute_tokens(x, ids, 3)
+    order.slot_to_row.add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        rows.sum().backward()

@@ -39,7 +39,7 @@ NORM = dict(x=P, residual=P, residual_out=P, weight=P, bias=P, wdtype=0, eps=1e-
 
 @pytest.mark.parametrize("over,code,msg", [
     ({"T": -1}, -1, "T=-1"), ({"H": 0}, -1, "H=0"), ({"H": 16385}, -2, "H <= 16384"),
-    ({"H": 8193, "dtype": 0}, -2, "H <= 8192"), ({"dtype": 3}, -1, "dtype"), ({"wdtype": -1}, -1, "dtype"),
+    ({"H": 8193, "dtype": 0}, -2, "H <= 8192"), ({"T": 1 << 24}, -2, "2^24 rows"), ({"dtype": 3}, -1, "dtype"), ({"wdtype": -1}, -1, "dtype"),
     ({"eps": -1.0}, -1, "eps"), ({"eps": float("nan")}, -1, "eps"), ({"x": None}, -1, "NULL"),
     ({"weight": None}, -1, "NULL"), ({"out": None}, -1, "NULL"), ({"residual_out": None}, -1, "residual_out"),
     ({"mean": None}, -1, "mean and rstd"), ({"rstd": None}, -1, "mean and rstd"), ({"x": P + 1}, -1, "aligned"),
@@ -66,7 +66,8 @@ ORDER = dict(ids=P, i64=1, T=4, K=2, E=8, offsets=P, slots=P, src=P, ws=P, ws_by
 
 @pytest.mark.parametrize("over,code,msg", [
     ({"T": 0}, -1, "no slots"), ({"T": -1}, -1, "T=-1"), ({"K": 0}, -1, "K=0"), ({"E": 0}, -2, "E=0"),
-    ({"E": 257}, -2, "E=257"), ({"T": 1 << 30}, -2, "too large"), ({"ids": None}, -1, "NULL"),
+    ({"E": 257}, -2, "E=257"), ({"T": 1 << 25, "K": 64}, -2, "too large"),
+    ({"T": 1 << 26}, -2, "2^26 tokens"), ({"ids": None}, -1, "NULL"),
     ({"offsets": None}, -1, "NULL"), ({"ws": None}, -3, "workspace"), ({"ws_bytes": 8}, -3, "workspace"),
     ({"ws": P + 4}, -1, "aligned")])
 def test_token_order(over, code, msg):
@@ -102,6 +103,7 @@ def test_token_rows(name, defaults, cases):
 @pytest.mark.parametrize("name,defaults,cases", [
     ("moe355_fp8_quantize", dict(x=P, M=4, K=60, dtype=1, codes=P, scales=P), [
         ({"M": -1}, -1, "sizes"), ({"K": 0}, -1, "sizes"), ({"K": (1 << 20) + 1}, -2, "2^20"), ({"dtype": 5}, -1, "dtype"),
+        ({"M": 1 << 24, "K": 2000}, -2, "2^28 blocks"),
         ({"x": None}, -1, "NULL"), ({"scales": None}, -1, "NULL"), ({"codes": P + 8}, -1, "aligned"),
         ({"x": P + 1}, -1, "aligned"), ({"M": 0, "x": None}, 0, None)]),
     ("moe355_fp8_quantize_weight", dict(w=P, N=100, K=60, dtype=0, cells=P, scales=P), [
@@ -112,7 +114,7 @@ def test_token_rows(name, defaults, cases):
         ({"N": 1 << 20, "K": 1 << 20}, -2, "2 GB")]),
     ("moe355_fp8_matmul", dict(x=P, xs=P, w=P, ws=P, offsets=P, M=4, N=100, K=60, E=3, dtype=1, out=P, space=P,
                                bytes=1 << 40), [
-        ({"M": -1}, -1, "M=-1"), ({"E": 0}, -2, "E=0"), ({"E": 300}, -2, "E=300"), ({"N": 0}, -1, "N=0"),
+        ({"M": -1}, -1, "M=-1"), ({"M": 1 << 30}, -2, "too large"), ({"E": 0}, -2, "E=0"), ({"E": 300}, -2, "E=300"), ({"N": 0}, -1, "N=0"),
         ({"dtype": 8}, -1, "dtype"), ({"offsets": None}, -1, "without offsets"), ({"xs": None}, -1, "NULL"),
         ({"out": None}, -1, "NULL"), ({"x": P + 8}, -1, "aligned"), ({"offsets": P + 2}, -1, "aligned"),
         ({"out": P + 4}, -1, "aligned"), ({"space": P + 8}, -1, "aligned"), ({"M": 0, "x": None}, 0, None),
