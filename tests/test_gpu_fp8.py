@@ -133,7 +133,9 @@ SHAPES = [(1, 1, 1, 1), (1, 16, 128, 1), (1, 4096, 512, 3), (5, 130, 200, 4), (1
           (64, 300, 1000, 7), (65, 256, 128, 1), (130, 515, 260, 5), (257, 1024, 640, 1), (300, 1000, 1248, 12),
           (1000, 272, 144, 64), (2000, 768, 256, 3), (777, 2049, 136, 2), (3000, 512, 896, 8), (40, 64, 64, 256),
           # items of the last round cut along the columns, on both tile heights
-          (1500, 1040, 2100, 3), (700, 514, 4096, 2), (130, 1000, 3300, 5), (33, 2100, 4000, 1), (4000, 4200, 2048, 9)]
+          (1500, 1040, 2100, 3), (700, 514, 4096, 2), (130, 1000, 3300, 5), (33, 2100, 4000, 1), (4000, 4200, 2048, 9),
+          # tiles of 256 rows, whole and in parts, few columns and many
+          (2600, 8000, 1100, 5), (1700, 16390, 136, 1), (900, 33000, 260, 4)]
 
 
 @pytest.mark.parametrize("M,N,K,E", SHAPES)
@@ -270,7 +272,9 @@ def make_experts(E, H, I, dev, seed):
 @pytest.mark.parametrize("T,H,I,E,K,act", [
     (1, 256, 512, 4, 2, "silu"), (1, 64, 16, 1, 1, "gelu"), (7, 400, 336, 8, 3, "gelu_tanh"),
     (16, 512, 256, 64, 6, "silu"), (100, 256, 128, 2, 1, "silu"), (260, 384, 1040, 4, 2, "gelu"),
-    (1100, 256, 640, 6, 2, "silu"), (33, 16, 144, 256, 8, "silu")])
+    (1100, 256, 640, 6, 2, "silu"), (33, 16, 144, 256, 8, "silu"),
+    # gate|up on tiles of 256 rows, in parts too
+    (1200, 256, 9008, 4, 2, "gelu"), (1300, 2048, 6000, 2, 1, "silu")])
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 def test_experts(T, H, I, E, K, act, dt, dev):
     """Off by half a step of the type; and an intermediate whose quotient lies as near to a
