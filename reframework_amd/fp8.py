@@ -19,6 +19,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from reframework_amd import _capi
+from reframework_amd.grad import once_differentiable
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
@@ -326,7 +327,7 @@ class _MatmulFn(torch.autograd.Function):
         return _matmul(_quantize(x), weight._held("w"), weight.rows, offsets, dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dout):
         cells, scales, offsets = ctx.saved_tensors
         dx = _matmul(_quantize(dout.contiguous()), (cells, scales), ctx.columns, offsets, ctx.dtype)

@@ -22,6 +22,7 @@ import torch
 import torch.nn as nn
 
 from reframework_amd import _capi
+from reframework_amd.grad import once_differentiable
 from reframework_amd.layers.base import BaseOP
 from reframework_amd.mx import BLOCK, Mxfp8Rows
 
@@ -136,7 +137,7 @@ class _LayerNormFn(torch.autograd.Function):
         return out if residual is None else (out, r)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dy, dres=None):
         r, weight, stats = ctx.saved_tensors
         H = r.shape[-1]

@@ -22,6 +22,7 @@ from typing import Tuple
 import torch
 
 from reframework_amd import _capi
+from reframework_amd.grad import once_differentiable
 
 
 class TokenOrder:
@@ -80,7 +81,7 @@ class _PermuteFn(torch.autograd.Function):
         return _permute(x, order)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, drows):
         slot_to_row, = ctx.saved_tensors
         dx = torch.empty(slot_to_row.shape[0], drows.shape[1], dtype=drows.dtype,
@@ -100,7 +101,7 @@ class _CombineFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once_differentiable
     def backward(ctx, dout):
         rows, weights, offsets, slot_to_row = ctx.saved_tensors
         dout = dout.contiguous()

@@ -16,6 +16,7 @@ import torch
 import _fp8_ref as ref
 from _helpers import DT, banner
 from reframework_amd.fp8 import Fp8Rows, blocks, padded
+from reframework_amd.layers import LayerNorm
 from reframework_amd.moe import (Fp8Experts, Fp8Weight, combine_tokens, fused_experts,
                                  fused_experts_fp8, matmul_fp8, permute_tokens, quantize_fp8)
 
@@ -415,3 +416,27 @@ def test_against_16_bit_experts(dev):
     a = fused_experts(x, w1, w2, tw, ids).float()
     b = fused_experts_fp8(x, Fp8Experts.quantize(w1, w2), tw, ids).float()
     assert float((a - b).norm() / a.norm()) <= 0.08
+
+
+def test_no_second_derivatives(dev):
+    """First derivatives under create_graph are as without; a second one is refused."""
+    banner("no second derivatives")
+    norm = LayerNorm(256, 1e-5).to(dev)
+    x = torch.randn(9, 256, device=dev, requires_grad=True)
+    ids = torch.tensor([[0, 1]] * 9, device=dev)
+    w = torch.rand(9, 2, device=dev, requires_grad=True)
+    weight = Fp8Weight.quantize(torch.randn(2, 128, 256, device=dev), transposed=True)
+
+    def both(v):
+        rows, order = permute_tokens(v, ids, 2)
+        return combine_tokens(rows, order, w)
+
+    def product(v):
+        return matmul_fp8(v, weight, torch.tensor([0, 4, 9], dtype=torch.int32, device=dev))
+
+    for f in (norm, both, product):
+        first, = torch.autograd.grad(f(x).square().sum(), [x])
+        again, = torch.autograd.grad(f(x).square().sum(), [x], create_graph=True)
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            again.sum().backward()
