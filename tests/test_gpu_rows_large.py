@@ -17,6 +17,14 @@ BF16 = torch.bfloat16
 LAST = 40
 
 
+@pytest.fixture(autouse=True)
+def give_back():
+    """The memory of a test here goes back to the device, not to the tests behind it."""
+    yield
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+
+
 def random(shape, dev, seed, dtype=BF16):
     g = torch.Generator(device=dev).manual_seed(seed)
     return torch.empty(shape, dtype=dtype, device=dev).normal_(generator=g)
