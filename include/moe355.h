@@ -483,7 +483,8 @@ int moe355_token_order(const void* topk_ids, int ids_int64, int T, int K, int E,
  *   combine_rows_bwd   drows[slot_to_row[t,k]] = topk_w[t,k] * dout[t], zeros from
  *                  offsets[E] on; dw[t,k] = dot(dout[t], rows[slot_to_row[t,k]]) in
  *                  fp32, 0 for a slot without a row; either may be NULL
- * Slots whose row lies outside [0, T*K) have none. A call takes less than 2^26 tokens.
+ * Slots whose row lies outside [0, T*K) have none. A call takes less than 2^26 tokens of
+ * less than 2^24 values.
  */
 int moe355_permute_rows(const void* x, const int32_t* offsets, const int32_t* slot_to_row, int T,
                         int H, int K, int E, int dtype, void* rows, void* stream);

@@ -33,6 +33,7 @@ int check_slots(int T, int K, int E, int H, int dtype) {
   if (static_cast<long long>(T) * K > INT_MAX / 2)
     return fail(MOE355_EUNSUPPORTED, "T*K=%lld too large", static_cast<long long>(T) * K);
   if (H <= 0) return fail(MOE355_EINVAL, "bad H=%d", H);
+  if (H >= 1 << 24) return fail(MOE355_EUNSUPPORTED, "H=%d: rows are less than 2^24 wide", H);
   if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
   return MOE355_OK;
 }

@@ -37,8 +37,26 @@ class TokenOrder:
 
     def __init__(self, offsets: torch.Tensor, slot_to_row: torch.Tensor, row_src: torch.Tensor,
                  num_experts: int) -> None:
+        if slot_to_row.dim() != 2 or tuple(offsets.shape) != (num_experts + 1,) or \
+                tuple(row_src.shape) != (slot_to_row.numel(),):
+            raise ValueError(f"offsets {tuple(offsets.shape)}, slot_to_row {tuple(slot_to_row.shape)} and "
+                             f"row_src {tuple(row_src.shape)} are not [{num_experts + 1}], [M, K], [M*K]")
+        for t in (offsets, slot_to_row, row_src):
+            if t.dtype != torch.int32 or not t.is_contiguous() or t.device != slot_to_row.device:
+                raise ValueError("an order is contiguous int32, on one device")
         self.offsets, self.slot_to_row, self.row_src = offsets, slot_to_row, row_src
         self.num_experts = num_experts
+
+    @classmethod
+    def _empty(cls, M: int, K: int, num_experts: int, device: torch.device) -> "TokenOrder":
+        """For a kernel to fill; without slots (M 0) as it is."""
+        order = cls.__new__(cls)
+        new = torch.zeros if M == 0 else torch.empty
+        order.offsets = new(num_experts + 1, dtype=torch.int32, device=device)
+        order.slot_to_row = torch.empty(M, K, dtype=torch.int32, device=device)
+        order.row_src = torch.empty(M * K, dtype=torch.int32, device=device)
+        order.num_experts = num_experts
+        return order
 
     @property
     def device(self) -> torch.device:
@@ -57,11 +75,7 @@ def token_order(topk_ids: torch.Tensor, num_experts: int) -> TokenOrder:
         raise TypeError(f"topk_ids are whole numbers, not {topk_ids.dtype}")
     M, K = topk_ids.shape
     ids = topk_ids if topk_ids.dtype in (torch.int32, torch.int64) else topk_ids.long()
-    dev = topk_ids.device
-    new = torch.zeros if M == 0 else torch.empty
-    order = TokenOrder(new(num_experts + 1, dtype=torch.int32, device=dev),
-                       torch.empty(M, K, dtype=torch.int32, device=dev),
-                       torch.empty(M * K, dtype=torch.int32, device=dev), num_experts)
+    order = TokenOrder._empty(M, K, num_experts, topk_ids.device)
     if M:
         _capi.token_order(ids.contiguous(), M, K, num_experts, order.offsets, order.slot_to_row,
                           order.row_src)

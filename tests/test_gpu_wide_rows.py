@@ -96,3 +96,17 @@ def test_experts(dev):
     want = fused_experts_fp8(x[-LAST:], experts, w[-LAST:], ids[-LAST:])
     # the intermediate values may fall on neighbouring codes, 2^-3 of a value apart at most
     assert off(out[-LAST:], want) <= 2.0 ** -3
+
+
+def test_experts_in_parts(dev):
+    """Tokens of more than 2 GB in 8 bits: the call runs in two parts."""
+    T, H, I, E = 262_143 + LAST, 8192, 16, 2
+    banner("8-bit experts in parts")
+    x = random((T, H), dev, 8)
+    experts = Fp8Experts.quantize(random((E, 2 * I, H), dev, 9) / 90, random((E, H, I), dev, 10) / 4)
+    ids = torch.arange(T, device=dev)[:, None] % E
+    w = torch.rand(T, 1, device=dev)
+    out = fused_experts_fp8(x, experts, w, ids)
+    for part in (slice(0, LAST), slice(262_143 - LAST, 262_143), slice(262_143, T)):
+        want = fused_experts_fp8(x[part], experts, w[part], ids[part])
+        assert off(out[part], want) <= 2.0 ** -3  # as above

@@ -86,6 +86,7 @@ def test_token_order_workspace(T, K, E):
 @pytest.mark.parametrize("name,defaults,cases", [
     ("moe355_permute_rows", dict(x=P, offsets=P, slots=P, T=4, H=60, K=2, E=8, dtype=1, rows=P), [
         ({"T": -1}, -1, "T=-1"), ({"H": 0}, -1, "H=0"), ({"dtype": 4}, -1, "dtype"), ({"x": None}, -1, "NULL"),
+        ({"H": 1 << 24}, -2, "2^24 wide"),
         ({"rows": None}, -1, "NULL"), ({"x": P + 1}, -1, "aligned"), ({"T": 0, "x": None}, 0, None)]),
     ("moe355_combine_rows", dict(rows=P, w=None, slots=P, T=4, H=60, K=2, dtype=1, out=P), [
         ({"K": 0}, -1, "K=0"), ({"rows": None}, -1, "NULL"), ({"out": None}, -1, "NULL"),
@@ -222,6 +223,12 @@ def test_tokens_check_their_tensors():
     order = TokenOrder(torch.zeros(5).int(), torch.zeros(3, 2).int(), torch.zeros(6).int(), 4)
     with pytest.raises(RuntimeError, match="GPU"):
         combine_tokens(torch.zeros(6, 8), order, torch.zeros(3, 2))
+    o, s, r = torch.zeros(5).int(), torch.zeros(3, 2).int(), torch.zeros(6).int()
+    for args, msg in (((o, s, r, 5), "are not"), ((o, s.flatten(), r, 4), "are not"), ((o, s, r[:5], 4), "are not"),
+                      ((o.long(), s, r, 4), "int32"), ((o, s.long(), r, 4), "int32"),
+                      ((o, torch.zeros(2, 3).int().t(), r, 4), "contiguous")):
+        with pytest.raises(ValueError, match=msg):
+            TokenOrder(*args)
 
 
 def test_codes_leave_a_module_as_they_came():
