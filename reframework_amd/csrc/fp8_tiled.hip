@@ -759,7 +759,7 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
         const uint8_t* ts = s + S::kTokBytes + S::kWgtBytes + (16 * wm + r) * 4;
         const float s0 = ws0[st], s1 = kGateUp ? ws1[st] : 0.f;
         u32x4 x[kM + 1][2], w[kHalf][2];
-        float sg[kM + 1], su[kM + 1];
+        float sg[kM + 1], su[kM + 1], xs[kM + 1];
         auto read_weights = [&](int half) {
 #pragma unroll
           for (int g = 0; g < (kM ? kHalf : 0); ++g) {
@@ -785,16 +785,22 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
           }
         };
         // read the first half
-        load_second();  // of step done + 1
         read_weights(0);
 #pragma unroll
         for (int m = 0; m < kM; ++m) {
           const uint8_t* p = s + (16 * (wm + WM * m) + r) * kF8Block;
           x[m][0] = *reinterpret_cast<const u32x4*>(p + ((q ^ sw) << 4));
           x[m][1] = *reinterpret_cast<const u32x4*>(p + (((4 + q) ^ sw) << 4));
-          const float xs = *reinterpret_cast<const float*>(ts + 64 * WM * m);
-          sg[m] = xs * s0;
-          su[m] = xs * s1;
+          xs[m] = *reinterpret_cast<const float*>(ts + 64 * WM * m);
+        }
+        // Asked for behind the reads, while they are on their way (before them: 8192 rows of 8
+        // matrices of 14336 x 4096 522 us, so 497).
+        __builtin_amdgcn_sched_barrier(0);
+        load_second();  // of step done + 1
+#pragma unroll
+        for (int m = 0; m < kM; ++m) {
+          sg[m] = xs[m] * s0;
+          su[m] = xs[m] * s1;
         }
         if (second) landed(done + 2);  // the second half of step done
         pipe::wait_lgkm0();
