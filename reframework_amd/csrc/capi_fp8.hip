@@ -82,10 +82,12 @@ hipError_t launch_matmul(const F8Path& p, const F8MatmulArgs& a, bool gate_up, h
 struct F8Plan {
   int rows, n_blocks, max_tiles;
   F8Path up, down;
-  bool exact_up, exact_down;
+  bool exact_up, exact_down, narrow;
   size_t block_counts, offsets, slot_to_row, row_src, tile_map, xq, xq_scales, inter, inter_scales,
-      y, parts, bytes;
+      y, y_scales, parts, bytes;
 };
+
+int y_blocks(int H) { return (H + kScaled16Block - 1) / kScaled16Block; }
 
 int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   if (T < 0) return fail(MOE355_EINVAL, "bad T=%d", T);
@@ -111,6 +113,11 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->exact_down = dtype == MOE355_F32;
   p->up = f8_path(p->rows, 2 * I, f8_pad(H), E, p->exact_up);
   p->down = f8_path(p->rows, H, f8_pad(I), E, p->exact_down);
+  // Results of a bf16 call's slots wait in 16 bits until they are weighed and added: f16 with a
+  // power of two per 64 columns, whose 11 bits add little to the 8 of the result (4096 tokens of
+  // 2 of 8 experts, H 4096, I 14336 1554 us, so 1539; 2048 of 6 of 64, H 2048, I 1408 238, so 225).
+  // f16 results, whose own rounding is no finer, and a single slot keep fp32.
+  p->narrow = dtype == MOE355_BF16 && K > 1 && p->down.tile_rows == 256;
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -126,7 +133,8 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->xq_scales = take(static_cast<size_t>(T) * f8_blocks(H) * 4);
   p->inter = take(static_cast<size_t>(R) * f8_pad(I));
   p->inter_scales = take(static_cast<size_t>(R) * f8_blocks(I) * 4);
-  p->y = take(static_cast<size_t>(R) * H * 4);
+  p->y = take(static_cast<size_t>(R) * H * (p->narrow ? 2 : 4));
+  p->y_scales = take(p->narrow ? static_cast<size_t>(R) * y_blocks(H) : 0);
   p->parts = take(std::max(p->up.part_bytes, p->down.part_bytes));
   p->bytes = off;
   return MOE355_OK;
@@ -282,6 +290,7 @@ int moe355_fp8_fused_experts(const void* x, const float* x_scales, const void* w
     d.w = static_cast<const uint8_t*>(w2); d.w_scales = w2_scales;
     d.out = at<void>(workspace, p.y);
     d.M = p.rows; d.N = H; d.Kp = f8_pad(I); d.E = E; d.out_dtype = MOE355_F32;
+    if (p.narrow) d.slot_scales = at<uint8_t>(workspace, p.y_scales);
     d.parts = a.parts; d.max_parts = p.down.max_parts; d.exact = p.exact_down;
     if (int rc = check_hip(launch_matmul(p.down, d, false, s), "fp8 down launch")) return rc;
 
@@ -289,6 +298,7 @@ int moe355_fp8_fused_experts(const void* x, const float* x_scales, const void* w
     c.y = d.out; c.topk_w = weights; c.slot_to_row = pa.slot_to_row;
     c.out = static_cast<char*>(out) + first * H * esz;
     c.T = n; c.K = K; c.H = H; c.R = p.rows; c.splits = 1;
+    c.y16 = p.narrow; c.y_scales = d.slot_scales; c.y_blocks = y_blocks(H);
     if (int rc = check_hip(launch_combine(c, dtype, s), "combine launch")) return rc;
   }
   return MOE355_OK;

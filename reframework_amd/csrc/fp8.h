@@ -97,6 +97,7 @@ struct F8MatmulArgs {
   const uint8_t* w;        // [E] matrices of cells (gate_up: gate's, then up's)
   const float* w_scales;   // [E, blocks of N, blocks of K]; gate_up: of I twice
   void* out;               // [M, N] (out_dtype)
+  uint8_t* slot_scales;    // 256-row tiles, with it: out is Scaled16 with bytes [M, ceil(N/64)]
   uint8_t* out_codes;      // gate_up: [M, Ip]
   float* out_scales;       // gate_up: [M, blocks of I]
   int M, N, Kp, E;         // gate_up: N = 2 I

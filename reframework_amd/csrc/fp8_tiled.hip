@@ -383,6 +383,19 @@ __device__ __forceinline__ u32x2 pack4(f32x4 v) {
   return __builtin_bit_cast(u32x2, T4{from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])});
 }
 
+// Two tiles' values of 16 bits, from column n on. They are exchanged between the lanes of a row,
+// so that each stores 16 bytes and a row gets 64 consecutive ones.
+template <typename T>
+__device__ __forceinline__ void store16(__amdgpu_buffer_rsrc_t out, uint32_t at, int n, int N, int q, f32x4 v0,
+                                        f32x4 v1) {
+  const u32x2 u = pack4<T>(v0), w = pack4<T>(v1);
+  const auto lo = __builtin_amdgcn_permlane16_swap(u[0], w[0], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(u[1], w[1], false, false);
+  n += 16 * (q & 1) + 8 * (q >> 1);
+  __builtin_amdgcn_raw_buffer_store_b128(u32x4{lo[0], hi[0], lo[1], hi[1]}, out,
+                                         n < N ? at + n * 2 : pipe::kPadOffset, 0, 0);
+}
+
 // A product's epilogue. Stored relative to the tile's first row; an offset out of range stores
 // nothing, so that there are no branches per element.
 template <typename S, int WM, typename OutT, int kM>
@@ -393,7 +406,35 @@ __device__ __forceinline__ void store_rows(const F8MatmulArgs& a, const Item& it
   const auto out = pipe::lds_rsrc(static_cast<OutT*>(a.out) + static_cast<size_t>(it.row0) * a.N);
   const int n_rows = it.row_end - it.row0;
   const int n0 = it.wt * kBN + wn * S::kNT * 16;  // this wave's first column
-  if (a.N % 8 == 0) {
+  if constexpr (std::is_same<OutT, Scaled16>::value) {  // N is a multiple of 16
+    static_assert(S::kNT % 4 == 0 && kScaled16Block == 64, "four tiles a scale");
+    const int blocks = (a.N + kScaled16Block - 1) / kScaled16Block;
+    const auto scales = pipe::lds_rsrc(a.slot_scales + static_cast<size_t>(it.row0) * blocks);
+#pragma unroll
+    for (int m = 0; m < kM; ++m) {
+      const int row = 16 * (wm + WM * (m0 + m)) + r;
+      const uint32_t at = row < n_rows ? row * a.N * kSize : pipe::kPadOffset;
+#pragma unroll
+      for (int b = 0; b < S::kNT; b += 4) {
+        float amax = 0.f;
+#pragma unroll
+        for (int g = b; g < b + 4; ++g)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) amax = fmaxf(amax, f8_finite_abs(acc[m][g][i]));
+        amax = fmaxf(amax, __shfl_xor(amax, 16, kWave));
+        amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
+        const int byte = scaled16_byte(__float_as_uint(amax));
+        const float f = scaled16_factor(byte);
+#pragma unroll
+        for (int g = b; g < b + 4; g += 2) store16<f16>(out, at, n0 + 16 * g, a.N, q, acc[m][g] * f, acc[m][g + 1] * f);
+        const int n = n0 + 16 * b;
+        __builtin_amdgcn_raw_buffer_store_b8(
+            static_cast<uint8_t>(byte), scales,
+            q == 0 && row < n_rows && n < a.N ? row * blocks + n / kScaled16Block : pipe::kPadOffset, 0, 0);
+      }
+    }
+    return;
+  } else if (a.N % 8 == 0) {
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
       const int row = 16 * (wm + WM * (m0 + m)) + r;
@@ -405,35 +446,28 @@ __device__ __forceinline__ void store_rows(const F8MatmulArgs& a, const Item& it
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[m][g]), out,
                                                  n < a.N ? at + n * kSize : pipe::kPadOffset, 0, 0);
         } else {
-          // Two tiles' columns are exchanged between the lanes of a row, so that each stores 16
-          // bytes and a row gets 64 consecutive ones.
-          const u32x2 u = pack4<OutT>(acc[m][g]), w = pack4<OutT>(acc[m][g + 1]);
-          const auto lo = __builtin_amdgcn_permlane16_swap(u[0], w[0], false, false);
-          const auto hi = __builtin_amdgcn_permlane16_swap(u[1], w[1], false, false);
-          const int n = n0 + 16 * (g + (q & 1)) + 8 * (q >> 1);
-          __builtin_amdgcn_raw_buffer_store_b128(u32x4{lo[0], hi[0], lo[1], hi[1]}, out,
-                                                 n < a.N ? at + n * kSize : pipe::kPadOffset, 0, 0);
+          store16<OutT>(out, at, n0 + 16 * g, a.N, q, acc[m][g], acc[m][g + 1]);
         }
       }
     }
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int m = 0; m < kM; ++m) {
-    const int row = 16 * (wm + WM * (m0 + m)) + r;
-    const uint32_t at = row < n_rows ? row * a.N * kSize : pipe::kPadOffset;
+    for (int m = 0; m < kM; ++m) {
+      const int row = 16 * (wm + WM * (m0 + m)) + r;
+      const uint32_t at = row < n_rows ? row * a.N * kSize : pipe::kPadOffset;
 #pragma unroll
-    for (int g = 0; g < S::kNT; ++g)
+      for (int g = 0; g < S::kNT; ++g)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int n = n0 + 16 * g + 4 * q + i;
-        const uint32_t off = n < a.N ? at + n * kSize : pipe::kPadOffset;
-        const OutT v = from_f32<OutT>(acc[m][g][i]);
-        if constexpr (kSize == 4)
-          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), out, off, 0, 0);
-        else
-          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(u16, v), out, off, 0, 0);
-      }
+        for (int i = 0; i < 4; ++i) {
+          const int n = n0 + 16 * g + 4 * q + i;
+          const uint32_t off = n < a.N ? at + n * kSize : pipe::kPadOffset;
+          const OutT v = from_f32<OutT>(acc[m][g][i]);
+          if constexpr (kSize == 4)
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), out, off, 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(u16, v), out, off, 0, 0);
+        }
+    }
   }
 }
 
@@ -704,7 +738,7 @@ __global__ __launch_bounds__(kThreads, 2) void turns_kernel(const F8MatmulArgs a
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int q = lane >> 4, r = lane & 15, sw = (r >> 1) & 7;
 
-  if constexpr (!kGateUp) zero_rest<OutT, kThreads>(a);
+  if constexpr (!kGateUp && !std::is_same<OutT, Scaled16>::value) zero_rest<OutT, kThreads>(a);
   const int nw = kGateUp ? f8_blocks(a.N / 2) : (a.N + kBN - 1) / kBN;
   const int n_items = list_items<BM, WM>(a, nw, items);
   if (n_items == 0) return;
@@ -891,6 +925,7 @@ hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, h
   if (tile_rows == 128) return launch_rows_of<128>(a, gate_up, s);
   if (tile_rows != 256 || a.exact) return hipErrorInvalidValue;
   if (gate_up) return launch_turns<true, float>(a, s);
+  if (a.slot_scales) return a.zero_rest ? hipErrorInvalidValue : launch_turns<false, Scaled16>(a, s);
   if (a.out_dtype == MOE355_F32) return launch_turns<false, float>(a, s);
   if (a.out_dtype == MOE355_BF16) return launch_turns<false, bf16>(a, s);
   return launch_turns<false, f16>(a, s);

@@ -275,12 +275,14 @@ def make_experts(E, H, I, dev, seed):
     (16, 512, 256, 64, 6, "silu"), (100, 256, 128, 2, 1, "silu"), (260, 384, 1040, 4, 2, "gelu"),
     (1100, 256, 640, 6, 2, "silu"), (33, 16, 144, 256, 8, "silu"),
     # gate|up on tiles of 256 rows, in parts too
-    (1200, 256, 9008, 4, 2, "gelu"), (1300, 2048, 6000, 2, 1, "silu")])
+    (1200, 256, 9008, 4, 2, "gelu"), (1300, 2048, 6000, 2, 1, "silu"),
+    # down on tiles of 256 rows (bf16: to slots of 16 bits), in parts too
+    (1792, 4112, 144, 4, 2, "silu"), (1792, 4112, 2064, 4, 2, "gelu_tanh")])
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 def test_experts(T, H, I, E, K, act, dt, dev):
-    """Off by half a step of the type; and an intermediate whose quotient lies as near to a
-    border as the sums are exact becomes the other neighbour, 2^-3 away at most. In bf16 the
-    matrix core's sums are (2^-14): a share of 2^-14 / 2^-4 of them, so 2^-3 * 2^-5 = 2^-8 in the
+    """Off by half a step of the type (and 2^-12 where bf16 slots wait in f16); and an
+    intermediate whose quotient lies as near to a border as the sums are exact becomes the other
+    neighbour, 2^-3 away at most. In bf16 the matrix core's sums are (2^-14): a share of 2^-14 / 2^-4 of them, so 2^-3 * 2^-5 = 2^-8 in the
     norm. Sums of exact products in fp32 are to 2^-18: 2^-3 * 2^-7 = 2^-10."""
     banner(f"fp8 experts T={T} H={H} I={I} E={E} K={K} {act} {dt}")
     dt = DT[dt]

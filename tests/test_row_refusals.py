@@ -148,7 +148,8 @@ def test_fp8_workspace_covers_every_stage(T, H, I, E, K):
     R = part * K
     for dtype in (0, 1, 2):
         n = _capi._size(torch.device("cpu"), "moe355_fp8_workspace_bytes", T, H, I, E, K, dtype)
-        assert n >= part * (padded(H) + 4 * blocks(H)) + R * (padded(I) + 4 * blocks(I)) + R * H * 4 + R * 8
+        assert n >= part * (padded(H) + 4 * blocks(H)) + R * (padded(I) + 4 * blocks(I)) + \
+            R * H * (2 if dtype == 1 else 4) + R * 8
 
 
 def _weight(E=2, N=40, K=70):
