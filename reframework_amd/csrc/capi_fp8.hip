@@ -218,10 +218,15 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
 int moe355_fp8_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes) {
   if (!bytes) return fail(MOE355_EINVAL, "NULL result");
   F8Plan p;
-  if (int rc = f8_plan(H > 0 ? std::min(T, max_tokens(H)) : T, H, I, E, K, dtype, &p)) return rc;
+  const int most = H > 0 ? max_tokens(H) : T;
+  if (int rc = f8_plan(std::min(T, most), H, I, E, K, dtype, &p)) return rc;
   if (static_cast<long long>(T) * K > INT_MAX / 2)
     return fail(MOE355_EUNSUPPORTED, "T*K=%lld too large", static_cast<long long>(T) * K);
   *bytes = p.bytes;
+  if (T > most) {  // the last part has fewer rows, which may take other kernels and more memory
+    if (int rc = f8_plan(T % most, H, I, E, K, dtype, &p)) return rc;
+    *bytes = std::max(*bytes, p.bytes);
+  }
   return MOE355_OK;
 }
 

@@ -152,6 +152,20 @@ def test_fp8_workspace_covers_every_stage(T, H, I, E, K):
             R * H * (2 if dtype == 1 else 4) + R * 8
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("last", [1, 100, 4000, 8000, 10000, 16000])
+def test_fp8_workspace_of_a_call_in_parts(last, dtype):
+    """What the last part takes may be more than the first: fewer rows, but other kernels."""
+    H, I, E, K = 122880, 16, 256, 2
+    first = 0x7FFFFFFF // H
+
+    def size(T):
+        return _capi._size(torch.device("cpu"), "moe355_fp8_workspace_bytes", T, H, I, E, K, dtype)
+
+    assert size(first + last) >= max(size(first), size(last))
+    assert size(2 * first + last) == size(first + last)
+
+
 def _weight(E=2, N=40, K=70):
     cells = torch.zeros(E, blocks(N), blocks(K), 16384, dtype=torch.uint8)
     return Fp8Weight(cells, torch.zeros(E, blocks(N), blocks(K)), N, K)
