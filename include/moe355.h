@@ -531,10 +531,12 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
  * reframework/moe/fused.py:49-87): x in 8 bits (quantised here when x_scales is NULL: x is
  * then [T,H] of dtype; else codes [T,Hp]), g, u = x . w1[e]^T, h = act(g) * u in 8 bits with
  * a scale per 128 features, y = h . w2[e]^T, out[t] = sum_k topk_w[t,k] * y, sums as in
- * moe355_fp8_matmul, of g and u with exact products for f16 too, rounded once. w1: cells
- * [E, 2 ceil(I/128), ceil(H/128), 16384], gate's rows of cells first, then up's (which start
- * at its first row), and their scales; w2: cells [E, ceil(H/128), ceil(I/128), 16384]. H and I multiples of 16. Slots whose id lies outside [0,E) or
- * whose weight is 0 add nothing. out may be x. The workspace belongs to the call until its
+ * moe355_fp8_matmul, of g and u with exact products for f16 and in calls of few tokens too. y is
+ * fp32, in large bf16 calls of several slots a token f16 with a power of two per 64 columns;
+ * its sum is fp32, rounded once. w1: cells [E, 2 ceil(I/128), ceil(H/128), 16384], gate's rows of
+ * cells first, then up's (which start at its first row), and their scales; w2: cells
+ * [E, ceil(H/128), ceil(I/128), 16384]. H and I multiples of 16. Slots whose id lies outside
+ * [0,E) or whose weight is 0 add nothing. out may be x. The workspace belongs to the call until its
  * kernels end.
  */
 int moe355_fp8_workspace_bytes(int T, int H, int I, int E, int K, int dtype, size_t* bytes);

@@ -321,9 +321,11 @@ def fused_experts_fp8(
 
     Tokens go through gate|up in 8 bits (``hidden_states`` quantised first unless they are
     Fp8Rows) and the gated activation, not rounded in between, through down in 8 bits. The result
-    is of ``out_dtype``: the tokens' type, bfloat16 for Fp8Rows. Sums are those of
-    matmul_fp8, with exact products in gate|up for float16 results too, rounded once. Slots whose id lies outside the experts or whose weight is 0 add
-    nothing. No gradients are recorded."""
+    is of ``out_dtype``: the tokens' type, bfloat16 for Fp8Rows. Sums are those of matmul_fp8, with
+    exact products in gate|up for float16 results and calls of few tokens too; the slots' results
+    are added in fp32 and rounded once, but those of large bfloat16 calls wait for that in 16 bits
+    (f16 with a power of two per 64 columns). Slots whose id lies outside the experts or whose
+    weight is 0 add nothing. No gradients are recorded."""
     act = activation_code(activation)
     if isinstance(hidden_states, Fp8Rows):
         x, x_scales = hidden_states.padded_codes, hidden_states.scales
