@@ -47,9 +47,12 @@ struct F8Path {
 // By rows per matrix that has any, on average; random routing gives some matrices a tile more.
 // Whole expert calls in us, A: 8 experts of H 4096, I 14336 (2 slots), B: 64 of H 2048, I 1408
 // (6), C: 32 of H 1280, I 3328 (4), D: 16 of H 4096, I 6400 (2).
-// Streaming / 64-row tiles: A at 1 row 82 / 148, 2 rows 289 / 299, 8 rows 325 / 324, 12 rows 350 /
-// 328; B at 1 row 110 / 105, 6 rows 131 / 114, 12 rows 161 / 126; C at 4 rows 106 / 101, 8 rows
-// 112 / 102. One row of one 4096 x 4096 matrix 7.4 / 22.8. (Row by row matrices; later both gained.)
+// Streaming / 32-row tiles: A at 1 row 112 / 165, 3 rows 228 / 247; B at 1 row 80 / 91, 2 rows 103 /
+// 96, 6 rows 118 / 106; C at 4 rows 88 / 96, 12 rows 95 / 100; D at 4 rows 214 / 232. Where the tiles of
+// 256 weight rows are fewer than would keep the CUs busy, or have few steps, streaming pays longer;
+// products, streaming / 64 rows: one matrix of 28672 x 4096 at 8 rows 24 / 33, of 4096 x 4096
+// at 12 rows 7.5 / 26; 8 of 4096 x 14336 at 8 rows 83 / 106, 12 rows to fp32 89 / 102; 32 of 6656 x 1280 at
+// 8 rows 43 / 53; but 8 of 14336 x 4096 (448 such tiles) at 8 rows 83 / 75.
 // 32 / 64: A at 12 rows 267 / 273; B at 12 rows 123 / 116; D at 25 rows 254 / 276; A at 64 rows
 // 479 / 417.
 // 64 / 128: A at 32 rows 302 / 290, 64 rows 398 / 320; B at 36 rows 157 / 157, 65 rows 212 / 178;
@@ -58,12 +61,14 @@ struct F8Path {
 // 224; C at 106 rows 151 / 186, 128 rows 204 / 195, 150 rows 234 / 184; 4 experts of H 1024, I
 // 1024 at 1000 rows, 128 items, 59 / 77. Exact products of f16 (8 of H 2048, I 4096; 256: the
 // weights through LDS, a kernel since removed) at 512 rows 298 / 360, 1024 rows 560 / 561.
-constexpr int kF8StreamRows = 5;
+constexpr int kF8StreamRows = 5, kF8StreamRowsFew = 12;
 
 F8Path f8_path(int M, int N, int Kp, int E, bool exact) {
   F8Path p{};
   const int active = std::max(1, std::min(M, E)), rows = M / active;
-  if (rows <= kF8StreamRows) return p;
+  const long long wide = static_cast<long long>(active) * ((N + 255) / 256);
+  const bool few = 2 * wide < 3 * device_cu_count() || Kp / kF8Block < 16;
+  if (rows <= (few ? kF8StreamRowsFew : kF8StreamRows)) return p;
   const long long items = (static_cast<long long>(M) / 256 + active / 2) * ((N + 255) / 256);
   p.tile_rows = rows <= 26 ? (rows >= 16 ? 32 : 64)
                 : rows < 128 || exact || items < device_cu_count() ? 128
