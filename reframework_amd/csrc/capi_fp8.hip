@@ -69,6 +69,11 @@ F8Path f8_path(int M, int N, int Kp, int E, bool exact) {
   const long long wide = static_cast<long long>(active) * ((N + 255) / 256);
   const bool few = 2 * wide < 3 * device_cu_count() || Kp / kF8Block < 16;
   if (rows <= (few ? kF8StreamRowsFew : kF8StreamRows)) return p;
+  // Very few wide tiles leave most CUs idle. One matrix, streaming / tiled, of 4096 x 4096 at 16 rows
+  // 7.9 / 24, 100 rows 16 / 34, of 8192 x 8192 at 64 rows 41 / 56, of 28672 x 4096 at 16 rows 26 / 32; but of
+  // 16384 x 4096 at 64 rows 42 / 32, of 32768 x 4096 at 32 rows 41 / 33.
+  const int cus = device_cu_count();
+  if (rows < 128 && (8 * wide <= cus || (rows <= kF8StreamTile && 2 * wide <= cus))) return p;
   const long long items = (static_cast<long long>(M) / 256 + active / 2) * ((N + 255) / 256);
   p.tile_rows = rows <= 26 ? (rows >= 16 ? 32 : 64)
                 : rows < 128 || exact || items < device_cu_count() ? 128
@@ -117,6 +122,7 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->exact_up = dtype != MOE355_BF16 || rows <= 40;
   p->exact_down = dtype == MOE355_F32;
   p->up = f8_path(p->rows, 2 * I, f8_pad(H), E, p->exact_up);
+  if (p->up.tile_rows == 0) p->exact_up = true;  // the only gate_up that streams
   p->down = f8_path(p->rows, H, f8_pad(I), E, p->exact_down);
   // Results of a bf16 call's slots wait in 16 bits until they are weighed and added: f16 with a
   // power of two per 64 columns, whose 11 bits add little to the 8 of the result (4096 tokens of
