@@ -558,12 +558,14 @@ class FusedMoE(BaseOP):
         RMSNorm and the router in one library call; returns (output, new
         residual). ``norm`` is an RMSNorm (its weight, optional bias and eps), or a LayerNorm,
         which is a call of its own before the layer's."""
-        if isinstance(norm, LayerNorm):
-            with torch.no_grad():
-                normed, new_res = norm.forward_add_residual(x.to(self.dtype), residual.to(self.dtype))
-                return self(normed).to(x.dtype), new_res.to(residual.dtype)
         shape = x.shape
         x2 = x.reshape(-1, self.hidden_size)
+        if isinstance(norm, LayerNorm):
+            with torch.no_grad():
+                normed, new_res = norm.forward_add_residual(
+                    x2.to(self.dtype), residual.reshape(-1, self.hidden_size).to(self.dtype))
+                return (self(normed).to(x.dtype).reshape(shape),
+                        new_res.reshape(shape).to(residual.dtype))
         require_gpu(x2)
         xd = x2.to(self.dtype).contiguous()
         res = residual.reshape(-1, self.hidden_size).to(self.dtype).contiguous()

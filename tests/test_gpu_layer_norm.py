@@ -281,3 +281,27 @@ def test_before_an_expert_layer(dev):
         want = moe(normed)
     assert torch.equal(new_res, want_res) and torch.equal(out, want)
     assert not out.requires_grad and not new_res.requires_grad
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_before_an_expert_layer_in_any_shape(dt, dev):
+    """Results have the input's shape, as behind an RMSNorm, and are those of the rows."""
+    banner(f"layer_norm before FusedMoE, shapes, {dt}")
+    torch.manual_seed(6)
+    H = 256
+    moe = FusedMoE(4, 2, H, 128, dtype=torch.bfloat16).to(dev)
+    with torch.no_grad():
+        for p in moe.parameters():
+            p.normal_(std=0.05)
+    norm = LayerNorm(H, EPS).to(dev)
+    for shape in ((2, 5, H), (3, 1, H), (1, 1, H), (2, 2, 3, H), (H,), (0, H), (2, 0, H)):
+        x, res = (torch.randn(shape, device=dev).to(DT[dt]) for _ in range(2))
+        out, new_res = moe.forward_with_norm(x, res, norm)
+        assert out.shape == x.shape and new_res.shape == x.shape
+        assert out.dtype == x.dtype and new_res.dtype == res.dtype
+        if x.numel():
+            rows = moe.forward_with_norm(x.reshape(-1, H), res.reshape(-1, H), norm)
+            assert torch.equal(out.reshape(-1, H), rows[0]) and torch.equal(new_res.reshape(-1, H), rows[1])
+    x = torch.randn(2, 5, H, device=dev).to(DT[dt])
+    out, new_res = moe.forward_with_norm(x, x.reshape(10, H), norm)  # the residual in rows
+    assert out.shape == x.shape and new_res.shape == x.shape
