@@ -19,7 +19,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from reframework_amd import _capi
-from reframework_amd.grad import once_differentiable
+from reframework_amd.grad import once_differentiable, records
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
@@ -348,7 +348,7 @@ def matmul_fp8(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight,
     product (float32 results have exact products, summed in fp32), then scaled and added in
     fp32. Where ``x`` records gradients, its gradient is the same product of
     the result's, brought to 8 bits, with the transposed matrices, which ``weight`` has to
-    hold; the rounding to 8 bits counts as the identity."""
+    hold; the rounding to 8 bits counts as the identity. Tangents are refused."""
     if isinstance(x, Fp8Rows):
         M, K, dev = len(x), x.size, x.device
         dtype = out_dtype or torch.bfloat16
@@ -380,7 +380,7 @@ def matmul_fp8(x: Union[torch.Tensor, Fp8Rows], weight: Fp8Weight,
     if isinstance(x, Fp8Rows):
         return _matmul(x, weight._held("w"), weight.rows, offsets, dtype)
     x = x.contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
+    if records(x):
         if not weight.has_transposed:
             raise RuntimeError("gradients need weights that hold the transposed matrices "
                                "(transposed=True)")

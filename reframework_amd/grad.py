@@ -2,9 +2,27 @@
 
 from __future__ import annotations
 
-from typing import Callable
+from typing import Callable, Optional
 
 import torch
+from torch.autograd import forward_ad
+
+
+def records(*inputs: Optional[torch.Tensor]) -> bool:
+    """Whether autograd takes note of what is made of ``inputs``: for a gradient, or as one of
+    them carries a tangent, which these operators' Functions then refuse (a kernel called beside
+    autograd would drop it)."""
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t is not None and t.requires_grad:
+                return True
+    return has_tangent(*inputs)
+
+
+def has_tangent(*inputs: Optional[torch.Tensor]) -> bool:
+    # the level is that of the innermost forward_ad.dual_level(), -1 outside
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in inputs)
 
 
 def once_differentiable(backward: Callable) -> Callable:

@@ -11,7 +11,8 @@ activation dtype. ``forward_mxfp8`` and ``forward_add_residual_mxfp8`` also leav
 the normed rows in 8 bits (mx.Mxfp8Rows), for expert products that take them.
 
 ``LayerNorm`` has the same surface (the reference has none) and gradients: with respect to
-its inputs and parameters wherever autograd records.
+its inputs and parameters wherever autograd records. Tangents (forward-mode derivatives) are
+refused.
 """
 
 from __future__ import annotations
@@ -22,7 +23,7 @@ import torch
 import torch.nn as nn
 
 from reframework_amd import _capi
-from reframework_amd.grad import once_differentiable
+from reframework_amd.grad import has_tangent, once_differentiable, records
 from reframework_amd.layers.base import BaseOP
 from reframework_amd.mx import BLOCK, Mxfp8Rows
 
@@ -190,15 +191,10 @@ class LayerNorm(BaseOP):
                 b = b.contiguous()
         return w, b
 
-    def _records(self, *inputs: torch.Tensor) -> bool:
-        return torch.is_grad_enabled() and (
-            self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad) or
-            any(t.requires_grad for t in inputs))
-
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         w, b = self._check(x)
         x = x.contiguous()
-        if self._records(x):
+        if records(x, w, b):
             return _LayerNormFn.apply(x, None, w, b, self.eps)
         out = torch.empty_like(x)
         _capi.layer_norm(x.numel() // self.size, self.size, x, None, None, w, b, self.eps, out)
@@ -207,8 +203,8 @@ class LayerNorm(BaseOP):
     def forward_inplace(self, x: torch.Tensor) -> None:
         """``x`` is overwritten by its norm; no gradients are recorded through this one."""
         w, b = self._check(x)
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise RuntimeError("forward_inplace overwrites what a gradient needs; use forward")
+        if torch.is_grad_enabled() and x.requires_grad or has_tangent(x, w, b):
+            raise RuntimeError("forward_inplace overwrites what a derivative needs; use forward")
         if not x.is_contiguous():
             with torch.no_grad():
                 x.copy_(self.forward(x))
@@ -227,7 +223,7 @@ class LayerNorm(BaseOP):
         if residual.dtype != x.dtype:
             residual = residual.to(x.dtype)
         residual = residual.contiguous()
-        if self._records(x, residual):
+        if records(x, residual, w, b):
             return _LayerNormFn.apply(x, residual, w, b, self.eps)
         out, r = torch.empty_like(x), torch.empty_like(x)
         _capi.layer_norm(x.numel() // self.size, self.size, x, residual, r, w, b, self.eps, out)

@@ -12,7 +12,7 @@ the token rows move in one launch each way:
     token's rows, in fp32 and slot order.
 
 Both are differentiable where autograd records, the latter in the weights too; sums run in a
-fixed order, so equal calls give equal results.
+fixed order, so equal calls give equal results. Tangents (forward-mode derivatives) are refused.
 """
 
 from __future__ import annotations
@@ -22,7 +22,7 @@ from typing import Tuple
 import torch
 
 from reframework_amd import _capi
-from reframework_amd.grad import once_differentiable
+from reframework_amd.grad import once_differentiable, records
 
 
 class TokenOrder:
@@ -145,7 +145,7 @@ def permute_tokens(hidden_states: torch.Tensor, topk_ids: torch.Tensor,
     _capi.dtype_code(x.dtype)
     order = token_order(topk_ids, num_experts)
     x = x.contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
+    if records(x):
         return _PermuteFn.apply(x, order), order
     return _permute(x, order), order
 
@@ -169,7 +169,7 @@ def combine_tokens(rows: torch.Tensor, order: TokenOrder,
     rows = rows.contiguous()
     w = topk_weights if topk_weights.dtype == torch.float32 else topk_weights.float()
     w = w.contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or w.requires_grad):
+    if records(rows, w):
         return _CombineFn.apply(rows, w, order)
     out = torch.empty(M, rows.shape[1], dtype=rows.dtype, device=rows.device)
     _capi.combine_rows(rows, w, order.slot_to_row, out)

@@ -442,3 +442,31 @@ def test_no_second_derivatives(dev):
         assert torch.equal(first, again)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             again.sum().backward()
+
+
+def test_no_derivatives_forwards(dev):
+    """A tangent would be lost: refused, where nothing asks for a gradient too."""
+    from torch.autograd import forward_ad
+
+    banner("no derivatives forwards")
+    norm = LayerNorm(256, 1e-5).to(dev).requires_grad_(False)
+    x, t = torch.randn(9, 256, device=dev), torch.randn(9, 256, device=dev)
+    ids = torch.tensor([[0, 1]] * 9, device=dev)
+    weight = Fp8Weight.quantize(torch.randn(128, 256, device=dev), transposed=True)
+    rows, order = permute_tokens(x, ids, 2)
+    w = torch.rand(9, 2, device=dev)
+    calls = [(norm, x), (lambda v: norm.forward_add_residual(x, v), x), (lambda v: permute_tokens(v, ids, 2), x),
+             (lambda v: combine_tokens(v, order, w), rows), (lambda v: combine_tokens(rows, order, v), w),
+             (lambda v: matmul_fp8(v, weight), x)]
+    for f, v in calls:
+        f(v)
+        with forward_ad.dual_level():
+            f(v)  # without a tangent
+            dual = forward_ad.make_dual(v, torch.ones_like(v))
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                f(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
+                f(dual)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward_inplace"):
+            norm.forward_inplace(forward_ad.make_dual(x.clone(), t))
