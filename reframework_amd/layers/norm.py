@@ -28,6 +28,12 @@ from reframework_amd.layers.base import BaseOP
 from reframework_amd.mx import BLOCK, Mxfp8Rows
 
 
+def _written(x: torch.Tensor) -> None:
+    """Tells autograd, which does not see the kernels' writes, that ``x`` was overwritten: a recorded
+    call that keeps it for its gradient then raises instead of taking the new values."""
+    torch.autograd.graph.increment_version(x)
+
+
 class RMSNorm(BaseOP):
     def __init__(self, size: int, eps: float, bias: bool = False) -> None:
         super().__init__()
@@ -64,6 +70,7 @@ class RMSNorm(BaseOP):
             x.copy_(self.forward(x))
             return
         self._run(x, None, x, None)
+        _written(x)
 
     def forward_add_residual(self, x: torch.Tensor,
                              residual: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -210,6 +217,7 @@ class LayerNorm(BaseOP):
                 x.copy_(self.forward(x))
             return
         _capi.layer_norm(x.numel() // self.size, self.size, x, None, None, w, b, self.eps, x)
+        _written(x)
 
     def forward_add_residual(self, x: torch.Tensor,
                              residual: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

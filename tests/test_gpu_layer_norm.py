@@ -16,7 +16,7 @@ import pytest
 import torch
 
 from _helpers import DT, banner
-from reframework_amd.layers import LayerNorm
+from reframework_amd.layers import LayerNorm, RMSNorm
 from reframework_amd.moe import FusedMoE
 
 pytestmark = pytest.mark.gpu
@@ -305,3 +305,25 @@ def test_before_an_expert_layer_in_any_shape(dt, dev):
     x = torch.randn(2, 5, H, device=dev).to(DT[dt])
     out, new_res = moe.forward_with_norm(x, x.reshape(10, H), norm)  # the residual in rows
     assert out.shape == x.shape and new_res.shape == x.shape
+
+
+def test_an_overwritten_input_is_noticed(dev):
+    """forward_inplace overwrites what an earlier call keeps for its gradient."""
+    banner("layer_norm in place behind a recorded call")
+    norm, x, *_ = make(9, 256, torch.bfloat16, torch.bfloat16, dev)
+    out = norm(x)  # keeps x for the weight's gradient
+    norm.forward_inplace(x)
+    assert torch.equal(x, out.detach())
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.float().sum().backward()
+    rms = RMSNorm(256, EPS).to(dev)
+    out = norm(x)
+    rms.forward_inplace(x)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.float().sum().backward()
+    for n in (norm, rms):
+        with torch.inference_mode():
+            y = torch.randn(9, 256, device=dev).bfloat16()
+            want = n(y)
+            n.forward_inplace(y)
+            assert torch.equal(y, want)
