@@ -209,11 +209,11 @@ class Fp8Weight(_Codes):
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor,
                    transposed: bool = False) -> "Fp8Weight":
         """From a checkpoint's codes (float8_e4m3fn, or their bytes) [N, K] or [E, N, K] and
-        scales float32 [(E,) ceil(N/128), ceil(K/128)], on the GPU."""
+        scales float32 [(E,) ceil(N/128), ceil(K/128)], on the GPU; both are copied."""
         if codes.dim() == 2 and scales.dim() == 2:
             codes, scales = codes[None], scales[None]
         _check_codes(codes, scales, "weights")
-        return cls(_pack(codes), scales, *codes.shape[1:], transposed)
+        return cls(_pack(codes), scales.clone(), *codes.shape[1:], transposed)
 
     @property
     def device(self) -> torch.device:
@@ -224,9 +224,9 @@ class Fp8Weight(_Codes):
         return "wt" in self._buffers
 
     def codes(self) -> Tuple[torch.Tensor, torch.Tensor]:
-        """(codes [E, N, K], scales) as from_codes takes them."""
+        """(codes [E, N, K], scales) as from_codes takes them, copies."""
         cells, scales = self._held("w")
-        return _unpack(cells, self.rows, self.columns).view(E4M3), scales.view(torch.float32)
+        return _unpack(cells, self.rows, self.columns).view(E4M3), scales.view(torch.float32).clone()
 
     def dequantize(self) -> torch.Tensor:
         """[E, N, K] in fp32."""
@@ -277,29 +277,29 @@ class Fp8Experts(_Codes):
                    w2_scales: torch.Tensor) -> "Fp8Experts":
         """From a checkpoint's codes (float8_e4m3fn, or their bytes) [E, 2I, H] and [E, H, I]
         with float32 scales [E, 2 ceil(I/128), ceil(H/128)] (gate blocks first) and
-        [E, ceil(H/128), ceil(I/128)], on the GPU."""
+        [E, ceil(H/128), ceil(I/128)], on the GPU; all are copied."""
         if w1.dim() != 3 or w2.dim() != 3:
             raise ValueError("codes are stacked [E, rows, columns]")
         E, I, H = cls._check_sizes(w1, w2)
         _check_codes(w1, w1_scales, "w1", 2 * blocks(I))
         _check_codes(w2, w2_scales, "w2")
         halves = w1.detach().contiguous().reshape(2 * E, I, H)
-        return cls((_pack(halves), w1_scales.reshape(2 * E, blocks(I), -1)), (_pack(w2), w2_scales),
-                   H, I)
+        return cls((_pack(halves), w1_scales.clone().reshape(2 * E, blocks(I), -1)),
+                   (_pack(w2), w2_scales.clone()), H, I)
 
     @property
     def device(self) -> torch.device:
         return self._buffers["w1"].device
 
     def codes(self, name: str) -> Tuple[torch.Tensor, torch.Tensor]:
-        """``"w1"`` or ``"w2"`` as from_codes takes it: (codes, scales)."""
+        """``"w1"`` or ``"w2"`` as from_codes takes it: (codes, scales), copies."""
         cells, scales = self._held(name)
         H, I = self.hidden_size, self.intermediate_size
         if name == "w2":
-            return _unpack(cells, H, I).view(E4M3), scales.view(torch.float32)
+            return _unpack(cells, H, I).view(E4M3), scales.view(torch.float32).clone()
         halves = cells.reshape(2 * self.num_experts, blocks(I), *cells.shape[2:])
         codes = _unpack(halves, I, H).reshape(self.num_experts, 2 * I, H)
-        return codes.view(E4M3), scales.view(torch.float32)
+        return codes.view(E4M3), scales.view(torch.float32).clone()
 
     def dequantize(self, name: str) -> torch.Tensor:
         """``"w1"`` [E, 2I, H] or ``"w2"`` [E, H, I] in fp32."""

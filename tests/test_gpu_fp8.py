@@ -470,3 +470,27 @@ def test_no_derivatives_forwards(dev):
     with forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward_inplace"):
             norm.forward_inplace(forward_ad.make_dual(x.clone(), t))
+
+
+def test_weights_do_not_follow_the_tensors_they_came_from(dev):
+    """A loader may fill the next layer into the buffers of the last one."""
+    banner("fp8 weights are copies")
+    g = torch.Generator(device=dev).manual_seed(12)
+    codes = torch.randn(2, 160, 256, generator=g, device=dev).to(E4M3)
+    scales = torch.rand(2, 2, 2, generator=g, device=dev) + 0.5
+    want = codes.float() * scales.repeat_interleave(128, 1)[:, :160].repeat_interleave(128, 2)
+    weight = Fp8Weight.from_codes(codes, scales, transposed=True)
+    again = Fp8Weight.from_codes(*weight.codes(), transposed=True)
+    w1, w2 = torch.randn(2, 64, 256, device=dev).to(E4M3), torch.randn(2, 256, 32, device=dev).to(E4M3)
+    s1, s2 = torch.rand(2, 2, 2, device=dev), torch.rand(2, 2, 1, device=dev)
+    experts = Fp8Experts.from_codes(w1, s1, w2, s2)
+    held = [experts.dequantize(n).clone() for n in ("w1", "w2")]
+    for t in (scales, s1, s2):
+        t.zero_()
+    weight.codes()[1].zero_()
+    for t in (codes, w1, w2):
+        t.view(torch.uint8).zero_()
+    assert torch.equal(weight.dequantize(), want) and torch.equal(again.dequantize(), want)
+    assert all(torch.equal(experts.dequantize(n), h) for n, h in zip(("w1", "w2"), held))
+    experts.codes("w1")[1].zero_(), experts.codes("w2")[1].zero_()
+    assert all(torch.equal(experts.dequantize(n), h) for n, h in zip(("w1", "w2"), held))
