@@ -483,8 +483,8 @@ int moe355_token_order(const void* topk_ids, int ids_int64, int T, int K, int E,
  *   combine_rows_bwd   drows[slot_to_row[t,k]] = topk_w[t,k] * dout[t], zeros from
  *                  offsets[E] on; dw[t,k] = dot(dout[t], rows[slot_to_row[t,k]]) in
  *                  fp32, 0 for a slot without a row; either may be NULL
- * Slots whose row lies outside [0, T*K) have none. A call takes less than 2^26 tokens of
- * less than 2^24 values.
+ * Slots whose row lies outside [0, T*K) have none. A call takes up to 2^26 - 4 tokens (token_order
+ * less than 2^26) of less than 2^24 values.
  */
 int moe355_permute_rows(const void* x, const int32_t* offsets, const int32_t* slot_to_row, int T,
                         int H, int K, int E, int dtype, void* rows, void* stream);
@@ -503,7 +503,7 @@ int moe355_combine_rows_bwd(const void* dout, const void* rows, const float* top
  * With m a block's largest finite magnitude, at least 448 * 2^-126, the scale is m / 448 and
  * a code v * 448 / m rounded to nearest even; infinities and NaN become NaN. The reference has
  * no such format (its quantised experts are int8 on the host, reframework/moe/fused.py:140-197).
- * fp8_pack lays codes [N, K] out as cells.
+ * fp8_pack lays codes [N, K] out as cells. fp8_quantize takes up to 2^28 - 16 blocks a call.
  */
 int moe355_fp8_quantize(const void* x, int M, int K, int dtype, void* codes, float* scales,
                         void* stream);

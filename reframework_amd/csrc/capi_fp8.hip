@@ -163,9 +163,10 @@ int moe355_fp8_quantize(const void* x, int M, int K, int dtype, void* codes, flo
                         void* stream) {
   if (int rc = check_matrix(M, K)) return rc;
   if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
-  // a launch holds less than 2^32 threads, 16 a block
-  if (static_cast<long long>(M) * f8_blocks(K) >= 1 << 28)
-    return fail(MOE355_EUNSUPPORTED, "M=%d rows of K=%d: a call takes less than 2^28 blocks", M, K);
+  // a launch holds less than 2^32 threads, 256 for 16 blocks or the rest of them
+  if (static_cast<long long>(M) * f8_blocks(K) > (1 << 28) - 16)
+    return fail(MOE355_EUNSUPPORTED, "M=%d rows of K=%d: a call takes less than 2^28 blocks, 2^28 - 16 at most",
+                M, K);
   if (M == 0) return MOE355_OK;
   if (!x || !codes || !scales) return fail(MOE355_EINVAL, "NULL tensor argument");
   if (reinterpret_cast<uintptr_t>(x) % elem_size(dtype) || !aligned16(codes) || !aligned4(scales))

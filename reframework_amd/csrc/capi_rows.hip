@@ -28,13 +28,19 @@ int check_slots(int T, int K, int E, int H, int dtype) {
   if (T < 0 || K < 1) return fail(MOE355_EINVAL, "bad sizes T=%d K=%d", T, K);
   if (E < 1 || E > MOE355_MAX_EXPERTS)
     return fail(MOE355_EUNSUPPORTED, "E=%d outside [1, %d]", E, MOE355_MAX_EXPERTS);
-  // a launch holds less than 2^32 threads, 64 a token
   if (T >= 1 << 26) return fail(MOE355_EUNSUPPORTED, "T=%d: a call takes less than 2^26 tokens", T);
   if (static_cast<long long>(T) * K > INT_MAX / 2)
     return fail(MOE355_EUNSUPPORTED, "T*K=%lld too large", static_cast<long long>(T) * K);
   if (H <= 0) return fail(MOE355_EINVAL, "bad H=%d", H);
   if (H >= 1 << 24) return fail(MOE355_EUNSUPPORTED, "H=%d: rows are less than 2^24 wide", H);
   if (!valid_dtype(dtype)) return fail(MOE355_EINVAL, "unknown dtype %d", dtype);
+  return MOE355_OK;
+}
+
+int check_moves(int T, int K, int E, int H, int dtype) {
+  if (int rc = check_slots(T, K, E, H, dtype)) return rc;
+  // a launch holds less than 2^32 threads, 256 for four tokens or the rest of them
+  if (T > (1 << 26) - 4) return fail(MOE355_EUNSUPPORTED, "T=%d: a call moves 2^26 - 4 tokens at most", T);
   return MOE355_OK;
 }
 
@@ -141,7 +147,7 @@ int moe355_token_order(const void* topk_ids, int ids_int64, int T, int K, int E,
 
 int moe355_permute_rows(const void* x, const int32_t* offsets, const int32_t* slot_to_row, int T,
                         int H, int K, int E, int dtype, void* rows, void* stream) {
-  if (int rc = check_slots(T, K, E, H, dtype)) return rc;
+  if (int rc = check_moves(T, K, E, H, dtype)) return rc;
   if (T == 0) return MOE355_OK;
   if (!x || !offsets || !slot_to_row || !rows) return fail(MOE355_EINVAL, "NULL tensor argument");
   if (bad_element(x, dtype) || bad_element(rows, dtype))
@@ -154,7 +160,7 @@ int moe355_permute_rows(const void* x, const int32_t* offsets, const int32_t* sl
 
 int moe355_combine_rows(const void* rows, const float* topk_w, const int32_t* slot_to_row, int T,
                         int H, int K, int dtype, void* out, void* stream) {
-  if (int rc = check_slots(T, K, 1, H, dtype)) return rc;
+  if (int rc = check_moves(T, K, 1, H, dtype)) return rc;
   if (T == 0) return MOE355_OK;
   if (!rows || !slot_to_row || !out) return fail(MOE355_EINVAL, "NULL tensor argument");
   if (bad_element(rows, dtype) || bad_element(out, dtype))
@@ -168,7 +174,7 @@ int moe355_combine_rows(const void* rows, const float* topk_w, const int32_t* sl
 int moe355_combine_rows_bwd(const void* dout, const void* rows, const float* topk_w,
                             const int32_t* offsets, const int32_t* slot_to_row, int T, int H, int K,
                             int E, int dtype, void* drows, float* dw, void* stream) {
-  if (int rc = check_slots(T, K, E, H, dtype)) return rc;
+  if (int rc = check_moves(T, K, E, H, dtype)) return rc;
   if (T == 0 || (!drows && !dw)) return MOE355_OK;
   if (!dout || !topk_w || !offsets || !slot_to_row || (dw && !rows))
     return fail(MOE355_EINVAL, "NULL tensor argument");

@@ -271,3 +271,20 @@ def test_parts_of_an_item_cover_its_steps_once(steps):
             ends = [(p * steps // split, (p + 1) * steps // split) for p in range(split)]
             assert ends[0][0] == 0 and ends[-1][1] == steps
             assert all(a < b for a, b in ends) and all(x[1] == y[0] for x, y in zip(ends, ends[1:]))
+
+
+def test_sizes_past_a_launch_are_refused():
+    """A launch holds less than 2^32 threads: 256 for every four tokens, or every 16 blocks,
+    begun."""
+    for T in ((1 << 26) - 3, (1 << 26) - 1):
+        for name, defaults in (
+                ("moe355_permute_rows", dict(x=P, offsets=P, slots=P, T=T, H=1, K=1, E=1, dtype=1, rows=P)),
+                ("moe355_combine_rows", dict(rows=P, w=None, slots=P, T=T, H=1, K=1, dtype=1, out=P)),
+                ("moe355_combine_rows_bwd", dict(dout=P, rows=P, w=P, offsets=P, slots=P, T=T, H=1, K=1, E=1,
+                                                 dtype=1, drows=P, dw=P))):
+            _check(name, defaults, {}, -2, "2^26 - 4")
+    quantize = dict(x=P, M=1, K=128, dtype=1, codes=P, scales=P)
+    for M, K in (((1 << 28) - 15, 1), ((1 << 28) - 1, 128), (1 << 24, 2000)):
+        _check("moe355_fp8_quantize", quantize, {"M": M, "K": K}, -2, "2^28 - 16")
+    n = ctypes.c_size_t()  # the order itself takes three more
+    assert _rc("moe355_token_order_workspace_bytes", (1 << 26) - 1, 1, 1, ctypes.byref(n))[0] == 0
