@@ -36,54 +36,6 @@ int check_rows(int M, int dtype) {
   return MOE355_OK;
 }
 
-// Which kernels run a product of M rows of E matrices of N x Kp (gate_up: N of both): tile_rows
-// 0 streams the weights past 16-row tiles; max_parts: parts of items that the 256-row tiles may
-// leave in memory.
-struct F8Path {
-  int tile_rows, max_parts;
-  size_t part_bytes;
-};
-
-// By rows per matrix that has any, on average; random routing gives some matrices a tile more.
-// Whole expert calls in us, A: 8 experts of H 4096, I 14336 (2 slots), B: 64 of H 2048, I 1408
-// (6), C: 32 of H 1280, I 3328 (4), D: 16 of H 4096, I 6400 (2).
-// Streaming / 32-row tiles: A at 1 row 112 / 165, 3 rows 228 / 247; B at 1 row 80 / 91, 2 rows 103 /
-// 96, 6 rows 118 / 106; C at 4 rows 88 / 96, 12 rows 95 / 100; D at 4 rows 214 / 232. Where the tiles of
-// 256 weight rows are fewer than would keep the CUs busy, or have few steps, streaming pays longer;
-// products, streaming / 64 rows: one matrix of 28672 x 4096 at 8 rows 24 / 33, of 4096 x 4096
-// at 12 rows 7.5 / 26; 8 of 4096 x 14336 at 8 rows 83 / 106, 12 rows to fp32 89 / 102; 32 of 6656 x 1280 at
-// 8 rows 43 / 53; but 8 of 14336 x 4096 (448 such tiles) at 8 rows 83 / 75.
-// 32 / 64: A at 12 rows 267 / 273; B at 12 rows 123 / 116; D at 25 rows 254 / 276; A at 64 rows
-// 479 / 417.
-// 64 / 128: A at 32 rows 302 / 290, 64 rows 398 / 320; B at 36 rows 157 / 157, 65 rows 212 / 178;
-// C at 64 rows 167 / 135.
-// 128 / 256: A at 120 rows 390 / 523, 140 rows 492 / 461; B at 96 rows 195 / 219, 122 rows 221 /
-// 224; C at 106 rows 151 / 186, 128 rows 204 / 195, 150 rows 234 / 184; 4 experts of H 1024, I
-// 1024 at 1000 rows, 128 items, 59 / 77. Exact products of f16 (8 of H 2048, I 4096; 256: the
-// weights through LDS, a kernel since removed) at 512 rows 298 / 360, 1024 rows 560 / 561.
-constexpr int kF8StreamRows = 5, kF8StreamRowsFew = 12;
-
-F8Path f8_path(int M, int N, int Kp, int E, bool exact) {
-  F8Path p{};
-  const int active = std::max(1, std::min(M, E)), rows = M / active;
-  const long long wide = static_cast<long long>(active) * ((N + 255) / 256);
-  const bool few = 2 * wide < 3 * device_cu_count() || Kp / kF8Block < 16;
-  if (rows <= (few ? kF8StreamRowsFew : kF8StreamRows)) return p;
-  // Very few wide tiles leave most CUs idle. One matrix, streaming / tiled, of 4096 x 4096 at 16 rows
-  // 7.9 / 24, 100 rows 16 / 34, of 8192 x 8192 at 64 rows 41 / 56, of 28672 x 4096 at 16 rows 26 / 32; but of
-  // 16384 x 4096 at 64 rows 42 / 32, of 32768 x 4096 at 32 rows 41 / 33.
-  const int cus = device_cu_count();
-  if (rows < 128 && (8 * wide <= cus || (rows <= kF8StreamTile && 2 * wide <= cus))) return p;
-  const long long items = (static_cast<long long>(M) / 256 + active / 2) * ((N + 255) / 256);
-  p.tile_rows = rows <= 26 ? (rows >= 16 ? 32 : 64)
-                : rows < 128 || exact || items < device_cu_count() ? 128
-                                                                   : 256;
-  // cutting items of few steps saves less than the second launch takes
-  if (p.tile_rows == 256 && Kp / kF8Block >= 16) p.max_parts = device_cu_count();
-  p.part_bytes = static_cast<size_t>(p.max_parts) * f8_part_floats() * 4;
-  return p;
-}
-
 hipError_t launch_matmul(const F8Path& p, const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
   return p.tile_rows ? launch_f8_tiled(a, gate_up, p.tile_rows, s) : launch_f8_stream(a, gate_up, s);
 }
@@ -91,8 +43,7 @@ hipError_t launch_matmul(const F8Path& p, const F8MatmulArgs& a, bool gate_up, h
 // Where the data of an expert call lies in the workspace.
 struct F8Plan {
   int rows, n_blocks, max_tiles;
-  F8Path up, down;
-  bool exact_up, exact_down, narrow;
+  F8Experts path;
   size_t block_counts, offsets, slot_to_row, row_src, tile_map, xq, xq_scales, inter, inter_scales,
       y, y_scales, parts, bytes;
 };
@@ -114,21 +65,7 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->rows = static_cast<int>(R);
   p->n_blocks = R <= kPermuteSingleMax ? 1 : static_cast<int>((R + kPermuteChunk - 1) / kPermuteChunk);
   p->max_tiles = E + p->rows / kF8StreamTile;
-  // Where the weights' stream bounds the call exact products cost little (us, scaled / exact: A
-  // of f8_path at 32 rows 290 / 295, 64 rows 320 / 342, 100 rows 348 / 403; B at 36 rows 157 /
-  // 161, 96 rows 194 / 229). A bf16 result of few tokens is off by up to 0.0025 of its size
-  // with the scaled ones, by 0.0017 with these.
-  const int rows = static_cast<int>(R) / std::max(1, std::min(static_cast<int>(R), E));
-  p->exact_up = dtype != MOE355_BF16 || rows <= 40;
-  p->exact_down = dtype == MOE355_F32;
-  p->up = f8_path(p->rows, 2 * I, f8_pad(H), E, p->exact_up);
-  if (p->up.tile_rows == 0) p->exact_up = true;  // the only gate_up that streams
-  p->down = f8_path(p->rows, H, f8_pad(I), E, p->exact_down);
-  // Results of a bf16 call's slots wait in 16 bits until they are weighed and added: f16 with a
-  // power of two per 64 columns, whose 11 bits add little to the 8 of the result (4096 tokens of
-  // 2 of 8 experts, H 4096, I 14336 1554 us, so 1539; 2048 of 6 of 64, H 2048, I 1408 238, so 225).
-  // f16 results, whose own rounding is no finer, and a single slot keep fp32.
-  p->narrow = dtype == MOE355_BF16 && K > 1 && p->down.tile_rows == 256;
+  p->path = f8_experts(p->rows, H, I, E, K, dtype, device_cu_count());
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -144,9 +81,9 @@ int f8_plan(int T, int H, int I, int E, int K, int dtype, F8Plan* p) {
   p->xq_scales = take(static_cast<size_t>(T) * f8_blocks(H) * 4);
   p->inter = take(static_cast<size_t>(R) * f8_pad(I));
   p->inter_scales = take(static_cast<size_t>(R) * f8_blocks(I) * 4);
-  p->y = take(static_cast<size_t>(R) * H * (p->narrow ? 2 : 4));
-  p->y_scales = take(p->narrow ? static_cast<size_t>(R) * y_blocks(H) : 0);
-  p->parts = take(std::max(p->up.part_bytes, p->down.part_bytes));
+  p->y = take(static_cast<size_t>(R) * H * (p->path.narrow ? 2 : 4));
+  p->y_scales = take(p->path.narrow ? static_cast<size_t>(R) * y_blocks(H) : 0);
+  p->parts = take(std::max(p->path.up.part_bytes, p->path.down.part_bytes));
   p->bytes = off;
   return MOE355_OK;
 }
@@ -199,7 +136,7 @@ int moe355_fp8_matmul_workspace_bytes(int M, int N, int K, int E, int dtype, siz
   if (!bytes) return fail(MOE355_EINVAL, "NULL result");
   if (int rc = check_weights(N, K, E)) return rc;
   if (int rc = check_rows(M, dtype)) return rc;
-  *bytes = M == 0 ? 0 : f8_path(M, N, f8_pad(K), E, dtype == MOE355_F32).part_bytes;
+  *bytes = M == 0 ? 0 : f8_path(M, N, f8_pad(K), E, dtype == MOE355_F32, device_cu_count()).part_bytes;
   return MOE355_OK;
 }
 
@@ -214,7 +151,7 @@ int moe355_fp8_matmul(const void* x, const float* x_scales, const void* w, const
   if (!aligned16(x) || !aligned16(w) || !aligned4(x_scales) || !aligned4(w_scales) ||
       !aligned4(offsets) || !aligned16(out) || !aligned16(workspace))
     return fail(MOE355_EINVAL, "x/w/scales/offsets/out/workspace not aligned");
-  const F8Path p = f8_path(M, N, f8_pad(K), E, dtype == MOE355_F32);
+  const F8Path p = f8_path(M, N, f8_pad(K), E, dtype == MOE355_F32, device_cu_count());
   if (p.part_bytes > 0 && (!workspace || workspace_bytes < p.part_bytes))
     return fail(MOE355_EWORKSPACE, "workspace of %zu bytes, the call needs %zu", workspace_bytes,
                 p.part_bytes);
@@ -299,23 +236,23 @@ int moe355_fp8_fused_experts(const void* x, const float* x_scales, const void* w
     a.out_codes = at<uint8_t>(workspace, p.inter);
     a.out_scales = at<float>(workspace, p.inter_scales);
     a.M = p.rows; a.N = 2 * I; a.Kp = Hp; a.E = E; a.act = act;
-    a.parts = at<float>(workspace, p.parts); a.max_parts = p.up.max_parts; a.exact = p.exact_up;
-    if (int rc = check_hip(launch_matmul(p.up, a, true, s), "fp8 gate_up launch")) return rc;
+    a.parts = at<float>(workspace, p.parts); a.max_parts = p.path.up.max_parts; a.exact = p.path.exact_up;
+    if (int rc = check_hip(launch_matmul(p.path.up, a, true, s), "fp8 gate_up launch")) return rc;
 
     F8MatmulArgs d{};
     d.x = a.out_codes; d.x_scales = a.out_scales; d.offsets = pa.offsets;
     d.w = static_cast<const uint8_t*>(w2); d.w_scales = w2_scales;
     d.out = at<void>(workspace, p.y);
     d.M = p.rows; d.N = H; d.Kp = f8_pad(I); d.E = E; d.out_dtype = MOE355_F32;
-    if (p.narrow) d.slot_scales = at<uint8_t>(workspace, p.y_scales);
-    d.parts = a.parts; d.max_parts = p.down.max_parts; d.exact = p.exact_down;
-    if (int rc = check_hip(launch_matmul(p.down, d, false, s), "fp8 down launch")) return rc;
+    if (p.path.narrow) d.slot_scales = at<uint8_t>(workspace, p.y_scales);
+    d.parts = a.parts; d.max_parts = p.path.down.max_parts; d.exact = p.path.exact_down;
+    if (int rc = check_hip(launch_matmul(p.path.down, d, false, s), "fp8 down launch")) return rc;
 
     CombineArgs c{};
     c.y = d.out; c.topk_w = weights; c.slot_to_row = pa.slot_to_row;
     c.out = static_cast<char*>(out) + first * H * esz;
     c.T = n; c.K = K; c.H = H; c.R = p.rows; c.splits = 1;
-    c.y16 = p.narrow; c.y_scales = d.slot_scales; c.y_blocks = y_blocks(H);
+    c.y16 = p.path.narrow; c.y_scales = d.slot_scales; c.y_blocks = y_blocks(H);
     if (int rc = check_hip(launch_combine(c, dtype, s), "combine launch")) return rc;
   }
   return MOE355_OK;

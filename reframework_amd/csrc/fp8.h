@@ -15,14 +15,9 @@
 #pragma once
 
 #include "common.h"
+#include "fp8_path.h"
 
 namespace moe355 {
-
-constexpr int kF8Block = 128;
-constexpr int kF8StreamTile = 16;  // token rows of a tile of the weight-streaming kernel
-
-__host__ __device__ constexpr int f8_blocks(int n) { return (n + kF8Block - 1) / kF8Block; }
-__host__ __device__ constexpr int f8_pad(int n) { return f8_blocks(n) * kF8Block; }
 
 // What a value times 448 is divided by, of a block's largest finite magnitude. Where the
 // product could overflow (of fp32 values) both are brought down by 2^-64.
@@ -117,9 +112,7 @@ hipError_t launch_f8_pack(const F8PackArgs& a, hipStream_t s);
 // gate_up: out_codes, out_scales = act(gate) * up in 8 bits, of gate rows 0 .. I - 1 and up
 // rows I .. 2 I - 1; else out.
 hipError_t launch_f8_stream(const F8MatmulArgs& a, bool gate_up, hipStream_t s);
-// tile_rows: 32, 64, 128 or 256 (not of exact products). Room of one part of an item of 256
-// rows, in floats.
-size_t f8_part_floats();
+// tile_rows: 32, 64, 128 or 256 (not of exact products).
 hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, hipStream_t s);
 
 }  // namespace moe355

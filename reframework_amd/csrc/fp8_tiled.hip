@@ -875,6 +875,7 @@ long long row_tiles(const F8MatmulArgs& a, int rows) {
 template <bool kGateUp, typename OutT>
 hipError_t launch_turns(const F8MatmulArgs& a, hipStream_t s) {
   constexpr int BM = 256, WM = 4;
+  static_assert(Shape<BM, WM>::kPartTile == kF8PartFloats, "room of a part");
   const int cell_rows = f8_cell_rows(a.N, kGateUp);
   const long long nw = kGateUp ? cell_rows / 2 : (cell_rows + 1) / 2;
   const long long total = row_tiles(a, BM) * nw;
@@ -915,8 +916,6 @@ hipError_t launch_rows_of(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
 }
 
 }  // namespace
-
-size_t f8_part_floats() { return 256 * kBN; }
 
 hipError_t launch_f8_tiled(const F8MatmulArgs& a, bool gate_up, int tile_rows, hipStream_t s) {
   if (a.M == 0) return hipSuccess;
