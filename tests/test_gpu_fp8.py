@@ -494,3 +494,27 @@ def test_weights_do_not_follow_the_tensors_they_came_from(dev):
     assert all(torch.equal(experts.dequantize(n), h) for n, h in zip(("w1", "w2"), held))
     experts.codes("w1")[1].zero_(), experts.codes("w2")[1].zero_()
     assert all(torch.equal(experts.dequantize(n), h) for n, h in zip(("w1", "w2"), held))
+
+
+def test_differences_of_the_product_itself(dev):
+    """matmul_fp8 at x + a and x - a, both on codes: whole numbers beside a 448 in every block. Sums
+    are exact then, and so is half their difference against the gradient."""
+    banner("fp8 matmul, differences of the calls")
+    gen = torch.Generator(device=dev).manual_seed(13)
+    M, N, K, E = 90, 300, 400, 3
+    weight = Fp8Weight.from_codes(whole((E, N, K), gen, dev).to(E4M3), pow2((E, blocks(N), blocks(K)), gen, dev),
+                                  transposed=True)
+    offsets = torch.tensor([4, 33, 33, 87], dtype=torch.int32, device=dev)
+    x, d = whole((M, K), gen, dev, 8), whole((M, N), gen, dev, 8)
+    x[:, ::128], d[:, ::128] = 448.0, 448.0
+    leaf = x.clone().requires_grad_()
+    out = matmul_fp8(leaf, weight, offsets)
+    dx = torch.autograd.grad(out, leaf, d)[0].double()
+    for _ in range(4):
+        a = whole((M, K), gen, dev, 1)
+        a[:, ::128] = 0.0  # the blocks' largest stay
+        up, down = (matmul_fp8(x + s * a, weight, offsets).double() for s in (1.0, -1.0))
+        assert torch.equal((up + down) / 2, out.detach().double())
+        rows = ((up - down) / 2 * d.double()).sum(1)
+        assert torch.equal(rows, (dx * a.double()).sum(1)) and rows[4:87].abs().min() > 0
+        assert not rows[:4].any() and not rows[87:].any()
