@@ -33,7 +33,7 @@ __device__ __forceinline__ f32x4 mma_f8(const u32x4* w, const u32x4* x) {
 
 // The same product in bf16, which holds every code exactly, as are the products then, summed in
 // fp32: four instructions of 32 columns at half the rate, and the conversions. For fp32 results,
-// and for gate_up of tokens that are not bf16 or few (f8_plan): a sum that is off moves an intermediate
+// and for gate_up of tokens that are not bf16 or few (f8_experts): a sum that is off moves an intermediate
 // across a border of its 8-bit code, which is off by a 16th then. Of f16 results that would be
 // most of the error (0.001 to 0.0014 of the results' size instead of 0.0002), of bf16 ones it
 // is not (0.0021 instead of 0.0017).

@@ -25,6 +25,9 @@ struct F8Path {
 };
 
 // By rows per matrix that has any, on average; random routing gives some matrices a tile more.
+// Skewed routing is on one matrix's wrong side: experts in proportion to 1 / rank, us, even / skewed
+// (most rows), B at 12 rows 112 / 124 (100), 36 rows 161 / 175 (303), 96 rows 196 / 217 (796); A at 12 rows
+// 254 / 267 (34), 64 rows 321 / 370 (173), 125 rows 420 / 376 (314).
 // Whole expert calls in us, A: 8 experts of H 4096, I 14336 (2 slots), B: 64 of H 2048, I 1408
 // (6), C: 32 of H 1280, I 3328 (4), D: 16 of H 4096, I 6400 (2).
 // Streaming / 32-row tiles: A at 1 row 112 / 165, 3 rows 228 / 247; B at 1 row 80 / 91, 2 rows 103 /
@@ -40,7 +43,8 @@ struct F8Path {
 // 128 / 256: A at 120 rows 390 / 523, 140 rows 492 / 461; B at 96 rows 195 / 219, 122 rows 221 /
 // 224; C at 106 rows 151 / 186, 128 rows 204 / 195, 150 rows 234 / 184; 4 experts of H 1024, I
 // 1024 at 1000 rows, 128 items, 59 / 77. Exact products of f16 (8 of H 2048, I 4096; 256: the
-// weights through LDS, a kernel since removed) at 512 rows 298 / 360, 1024 rows 560 / 561.
+// weights through LDS, a kernel since removed) at 512 rows 298 / 360, 1024 rows 560 / 561
+// (now 463, fp32 545; bf16 on 256 rows 310).
 constexpr int kF8StreamRows = 5, kF8StreamRowsFew = 12;
 
 inline F8Path f8_path(int M, int N, int Kp, int E, bool exact, int cus) {

@@ -163,7 +163,8 @@ struct Loader {
   __amdgpu_buffer_rsrc_t xsrc, xssrc, wsrc;
   uint32_t xoff[S::kTokLoads], cell[2], soff;
   // Token rows of the next item whose codes and scales this lane loads, as rows of x; -1 past
-  // the tile's last row.
+  // the tile's last row. (gate_up reads them under branches, where the compiler waits for all
+  // loads in flight: once an item.)
   int src[S::kTokLoads + 1];
   int item = 0, step = 0, end = 0, loaded = 0;  // loaded: steps of all items
 
@@ -320,7 +321,8 @@ __device__ __forceinline__ void weight_scales(const F8MatmulArgs& a, const Item&
 
 // The epilogues take kM of a wave's kMT tile rows, from m0 on.
 // gate_up's, first part: gate's place takes act(gate) * up; the largest of each token's
-// features in this wave goes to `most` [waves over weights][BM].
+// features in this wave goes to `most` [waves over weights][BM]. The result goes to 8 bits, so the
+// hardware's sigmoid (off by 3e-7) does in every type.
 template <typename S, int BM, int WM, int kM>
 __device__ __forceinline__ void activate(const F8MatmulArgs& a, const Item& it, f32x4 (&acc)[kM][S::kNT],
                                          int wm, int wn, int m0, float (*most)[BM]) {
@@ -540,10 +542,15 @@ __device__ __forceinline__ f32x4 product(const Bf16Row& w, const Bf16Row& x) { r
 
 // Up to 128 token rows, where the weights' stream counts: a workgroup multiplies BM rows by 256
 // weight rows, a wave by 32 of them, whose tiles it alone needs: they go straight to its
-// registers, kAhead steps ahead, 1 KB a load. The tokens, which all waves need, go through LDS,
-// kAhead steps at a time, so that the waves meet once in as many steps. Two workgroups share a
-// CU where 128 registers do. (With the weights in LDS every step waits for all waves: 394 rows
-// of 16 matrices of 12800 x 4096 179 us, so 157, 5.35 TB/s of weights.)
+// registers, 1 KB a load, asked for while the group of kAhead steps before is multiplied. The
+// tokens, which all waves need, go through LDS, a group at a time, so that the waves meet once in
+// as many steps. (With the weights in LDS every step waits for all waves: 394 rows of 16 matrices
+// of 12800 x 4096 179 us, so 157, 5.35 TB/s of weights. Of 4096 x 6400 93 us, 4.5 TB/s.)
+// A group does not overlap the next one's tokens: the compiler, which cannot tell the two buffers
+// apart, takes its LDS reads to depend on the loads just asked for and waits for them, and so for
+// all weights before them, behind each barrier. Two workgroups share a CU where 128 registers
+// do; scaled products of 64 rows do not quite fit there (19 registers spilled, 48 bytes).
+// tests/test_token_loads.py holds that enough loads stay behind the tokens' for the wait below.
 template <bool kGateUp, int BM, bool kExact, typename OutT>
 __global__ __launch_bounds__(kThreads, kExact || BM > 64 ? 2 : 4) void rows_kernel(const F8MatmulArgs a) {
   constexpr int WM = 1, kAhead = kExact || BM > 64 ? 3 : 2;
@@ -907,7 +914,7 @@ hipError_t launch_rows(const F8MatmulArgs& a, hipStream_t s) {
 template <int BM>
 hipError_t launch_rows_of(const F8MatmulArgs& a, bool gate_up, hipStream_t s) {
   if (gate_up && a.exact) return launch_rows<true, BM, true, float>(a, s);
-  if (gate_up)  // not where exact products cost next to nothing (f8_plan)
+  if (gate_up)  // not where exact products cost next to nothing (f8_experts)
     return BM == 128 ? launch_rows<true, 128, false, float>(a, s) : hipErrorInvalidValue;
   if (a.exact) return launch_rows<false, BM, true, float>(a, s);
   if (a.out_dtype == MOE355_F32) return launch_rows<false, BM, false, float>(a, s);

@@ -94,7 +94,7 @@ def _quantize(x: torch.Tensor) -> Fp8Rows:
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
     """``x`` [..., K] (float32, bfloat16 or float16 on the GPU) as 8-bit rows, one per row of
-    ``x``."""
+    ``x``, without gradients."""
     _require_gpu(x, "x")
     _capi.dtype_code(x.dtype)
     if x.dim() == 0 or x.shape[-1] == 0:
